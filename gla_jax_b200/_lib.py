@@ -45,6 +45,7 @@ SIGNATURES = {
     "gla_launch_count": (ctypes.c_longlong, []),
     "gla_device_wait_timeouts": (ctypes.c_uint, []),
     "gla_device_bad_offsets": (ctypes.c_uint, []),
+    "gla_device_bad_parents": (ctypes.c_uint, []),
     "gla_profile_enable": (None, [c_int]),
     "gla_profile_report": (c_size_t, [c_char_p, c_size_t]),
     "gla_cumsum": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int]),
@@ -118,6 +119,14 @@ SIGNATURES = {
                                c_void_p, c_int, c_int]),
     "gla_sp_combine2": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                 c_void_p, c_int, c_void_p, c_void_p, c_int, c_int]),
+    "gla_decay_workspace_bytes": (c_size_t, [c_int64] * 6 + [c_int, c_int, c_int64, c_int]),
+    "gla_decay_fwd": (c_int, [c_void_p] + [c_int64] * 6 + [c_int, c_int, c_int64] + [c_void_p] * 3 + [c_int] + [c_void_p] * 7 + [c_size_t]),
+    "gla_decay_bwd": (c_int, [c_void_p] + [c_int64] * 6 + [c_int, c_int, c_int64] + [c_void_p] * 3 + [c_int] + [c_void_p] * 12 + [c_size_t]),
+    "gla_decay_step": (c_int, [c_void_p] + [c_int64] * 5 + [c_int] + [c_void_p] * 6 + [c_int, c_void_p, c_int64]),
+    "gla_decode_step_beams": (c_int, [c_void_p] + [c_int64] * 3 + [c_int] + [c_void_p] * 6 + [c_int, c_void_p, c_int64]),
+    "gla_reorder_states": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p]),
+    "gla_beam_select_workspace_bytes": (c_size_t, [c_int64] * 4 + [c_int]),
+    "gla_beam_select": (c_int, [c_void_p] + [c_int64] * 4 + [c_int] + [c_void_p] * 3 + [c_int64] + [c_void_p] * 4 + [c_size_t]),
 }
 
 
@@ -179,21 +188,23 @@ def stream_of(dev) -> int:
     return torch.cuda.current_stream(dev).cuda_stream
 
 
-_seen = {"waits": 0, "offsets": 0}
+_seen = {"waits": 0, "offsets": 0, "parents": 0}
 
 
 def check_device() -> None:
     """Synchronise the current device and raise GlaError if, since the previous call of this function, a bounded
-    device-side wait gave up (the outputs written meanwhile are incomplete) or a packed-sequence call was given
-    offsets that had to be clamped.  The entry points themselves return before their kernels run and cannot
+    device-side wait gave up (the outputs written meanwhile are incomplete), a packed-sequence call was given
+    offsets that had to be clamped or a beam search parents that name no beam.  The entry points themselves return before their kernels run and cannot
     report either."""
     lib = load()
     waits, offs = int(lib.gla_device_wait_timeouts()), int(lib.gla_device_bad_offsets())
     new_w, new_o = waits - _seen["waits"], offs - _seen["offsets"]
     _seen["waits"], _seen["offsets"] = waits, offs
-    if new_w or new_o:
+    new_p = int(lib.gla_device_bad_parents()) - _seen["parents"]
+    _seen["parents"] += new_p
+    if new_w or new_o or new_p:
         raise GlaError(f"device-side errors since the last check: {new_w} wait(s) gave up, {new_o} sequence(s) with "
-                       "invalid packed offsets")
+                       f"invalid packed offsets" + (f", {new_p} parent(s) outside the beams" if new_p else ""))
 
 
 def check(status: int, what: str) -> None:

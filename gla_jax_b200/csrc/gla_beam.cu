@@ -1,0 +1,643 @@
+// Decoding over recurrent states: the single-token step of attention with one decay per head, steps and copies that follow a
+// beam search's parents, and the selection of the next beams.
+//
+// What a beam carries in a recurrent model is its state, so that going on with a beam means having its state: rows of a
+// state tensor are (request, beam), and parents (requests, beams) names for each beam of a request the beam it goes on from.
+#include <math_constants.h>
+#include "gla_common.cuh"
+#include "gla_decay.cuh"
+
+namespace gla {
+namespace beam {
+
+using decay::cp16;
+using decay::cp_commit;
+using decay::cp_wait;
+using decay::sm32;
+
+static __device__ unsigned int g_bad_parents = 0;
+
+// parents[j] of a request of K beams, held inside [0, K); `count`: whether this thread reports one that was not
+__device__ __forceinline__ int parent_of(const int* parents, int64_t n, int K, int j, bool count) {
+  const int x = parents[n * K + j];
+  if (count && (x < 0 || x >= K)) atomicAdd(&g_bad_parents, 1u);
+  return x < 0 ? 0 : x >= K ? K - 1 : x;
+}
+
+// ---- single-token steps ----------------------------------------------------------------------------------------------------
+// S <- f S + k (x) v and o = q S for a row (request or beam) and head, f one number (KEYED = false) or one per key feature.
+// A block owns W value columns: W / 4 lanes of four columns, 128 / (W / 4) row lanes.  The state is read and written once,
+// which is all that counts (8 Dk Dv bytes against a few hundred).
+struct Step {
+  float* S;
+  const float* g;                 // (rows, H) or (rows, H, Dk)
+  const void *v, *k, *q;          // (rows, H, Dv), (rows, Hk, Dk)
+  void* out;
+  const int* parents;             // (rows / K, K) or NULL (K = 1)
+  int H, share, Dk, Dv, K, bf, out_bf;
+};
+constexpr int SNT = 128;
+
+// One row per block, its loads all in flight before the first is used.
+template <int W, int RPT>
+__global__ void __launch_bounds__(SNT) step_kernel(const Step p) {
+  constexpr int CL = W / 4, RL = SNT / CL;
+  __shared__ float red[4][W];
+  const int cl = threadIdx.x % CL, rl = threadIdx.x / CL;
+  const int64_t row = blockIdx.y;                                 // (request, head)
+  const int64_t b = row / p.H, h = row % p.H, kv = b * (p.H / p.share) + h / p.share;
+  const int c0 = blockIdx.x * W + 4 * cl;
+  const bool on = c0 < p.Dv;
+  float* Sp = p.S + (row * p.Dk + rl) * (int64_t)p.Dv + c0;
+  grid_dep_wait();
+  grid_dep_launch();
+  float4 s[RPT];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i)
+    if (on && rl + i * RL < p.Dk) s[i] = *reinterpret_cast<const float4*>(Sp + (int64_t)i * RL * p.Dv);
+  const float f = expf(p.g[row]);
+  float4 vv = make_float4(0.f, 0.f, 0.f, 0.f), acc = vv;
+  if (on) {
+    const int64_t at = row * p.Dv + c0;
+    vv = make_float4(ld_any(p.v, p.bf, at), ld_any(p.v, p.bf, at + 1), ld_any(p.v, p.bf, at + 2), ld_any(p.v, p.bf, at + 3));
+  }
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = rl + i * RL;
+    if (!on || r >= p.Dk) continue;
+    const float kr = ld_any(p.k, p.bf, kv * p.Dk + r), qr = ld_any(p.q, p.bf, kv * p.Dk + r);
+    float4 n;
+    n.x = fmaf(f, s[i].x, kr * vv.x); n.y = fmaf(f, s[i].y, kr * vv.y);
+    n.z = fmaf(f, s[i].z, kr * vv.z); n.w = fmaf(f, s[i].w, kr * vv.w);
+    *reinterpret_cast<float4*>(Sp + (int64_t)i * RL * p.Dv) = n;
+    acc.x = fmaf(qr, n.x, acc.x); acc.y = fmaf(qr, n.y, acc.y); acc.z = fmaf(qr, n.z, acc.z); acc.w = fmaf(qr, n.w, acc.w);
+  }
+#pragma unroll
+  for (int d = CL; d < 32; d <<= 1) {
+    acc.x += __shfl_xor_sync(0xffffffffu, acc.x, d); acc.y += __shfl_xor_sync(0xffffffffu, acc.y, d);
+    acc.z += __shfl_xor_sync(0xffffffffu, acc.z, d); acc.w += __shfl_xor_sync(0xffffffffu, acc.w, d);
+  }
+  if (threadIdx.x % 32 < CL) *reinterpret_cast<float4*>(&red[threadIdx.x / 32][4 * cl]) = acc;
+  __syncthreads();
+  const int c = blockIdx.x * W + threadIdx.x;
+  if (threadIdx.x < W && c < p.Dv)
+    st_any(p.out, p.out_bf, row * p.Dv + c, (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]));
+}
+
+// All K beams of a request per block: every beam's old columns go into shared memory (a thread's own elements, which it
+// alone reads again), then each beam is stepped from its parent's and written to its own place.  Nothing is read after it
+// was overwritten, so the step needs no second set of states, and moving states costs no pass of its own: a beam that
+// nobody goes on from is not even read.
+template <int W, bool KEYED>
+__global__ void __launch_bounds__(SNT) step_beams_kernel(const Step p) {
+  constexpr int CL = W / 4, RL = SNT / CL;
+  extern __shared__ __align__(16) uint8_t sm[];
+  const int rpt = (p.Dk + RL - 1) / RL;
+  float4* old = reinterpret_cast<float4*>(sm);                                        // [K][rpt][SNT]
+  float* red = reinterpret_cast<float*>(sm + (size_t)p.K * rpt * SNT * 16);           // [K][4][W]
+  const int cl = threadIdx.x % CL, rl = threadIdx.x / CL, warp = threadIdx.x / 32;
+  const int64_t n = blockIdx.y / p.H, h = blockIdx.y % p.H;
+  const int c0 = blockIdx.x * W + 4 * cl;
+  const bool on = c0 < p.Dv;
+  grid_dep_wait();
+  grid_dep_launch();
+  unsigned int used = 0;                                                              // beams that are somebody's parent
+  for (int j = 0; j < p.K; ++j) used |= 1u << parent_of(p.parents, n, p.K, j, blockIdx.x == 0 && h == 0 && threadIdx.x == 0);
+  for (int j = 0; j < p.K; ++j) {
+    if (!((used >> j) & 1u)) continue;
+    const float* Sp = p.S + (((n * p.K + j) * p.H + h) * p.Dk + rl) * (int64_t)p.Dv + c0;
+    for (int i = 0; i < rpt; ++i)
+      if (on && rl + i * RL < p.Dk) cp16(sm32(old + (j * rpt + i) * SNT + threadIdx.x), Sp + (int64_t)i * RL * p.Dv, true);
+  }
+  cp_commit();
+  cp_wait<0>();
+  for (int j = 0; j < p.K; ++j) {
+    const int from = parent_of(p.parents, n, p.K, j, false);
+    const int64_t b = n * p.K + j, row = b * p.H + h, kv = b * (p.H / p.share) + h / p.share;
+    float* Sp = p.S + (row * p.Dk + rl) * (int64_t)p.Dv + c0;
+    const float f1 = KEYED ? 0.f : expf(p.g[row]);
+    float4 vv = make_float4(0.f, 0.f, 0.f, 0.f), acc = vv;
+    if (on) {
+      const int64_t at = row * p.Dv + c0;
+      vv = make_float4(ld_any(p.v, p.bf, at), ld_any(p.v, p.bf, at + 1), ld_any(p.v, p.bf, at + 2), ld_any(p.v, p.bf, at + 3));
+    }
+    for (int i = 0; i < rpt; ++i) {
+      const int r = rl + i * RL;
+      if (!on || r >= p.Dk) continue;
+      const float f = KEYED ? expf(p.g[row * p.Dk + r]) : f1;
+      const float kr = ld_any(p.k, p.bf, kv * p.Dk + r), qr = ld_any(p.q, p.bf, kv * p.Dk + r);
+      const float4 s = old[(from * rpt + i) * SNT + threadIdx.x];
+      float4 x;
+      x.x = fmaf(f, s.x, kr * vv.x); x.y = fmaf(f, s.y, kr * vv.y);
+      x.z = fmaf(f, s.z, kr * vv.z); x.w = fmaf(f, s.w, kr * vv.w);
+      *reinterpret_cast<float4*>(Sp + (int64_t)i * RL * p.Dv) = x;
+      acc.x = fmaf(qr, x.x, acc.x); acc.y = fmaf(qr, x.y, acc.y); acc.z = fmaf(qr, x.z, acc.z); acc.w = fmaf(qr, x.w, acc.w);
+    }
+#pragma unroll
+    for (int d = CL; d < 32; d <<= 1) {
+      acc.x += __shfl_xor_sync(0xffffffffu, acc.x, d); acc.y += __shfl_xor_sync(0xffffffffu, acc.y, d);
+      acc.z += __shfl_xor_sync(0xffffffffu, acc.z, d); acc.w += __shfl_xor_sync(0xffffffffu, acc.w, d);
+    }
+    if (threadIdx.x % 32 < CL) *reinterpret_cast<float4*>(red + (j * 4 + warp) * W + 4 * cl) = acc;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.K * W; i += SNT) {
+    const int j = i / W, c = i % W;
+    if (blockIdx.x * W + c >= p.Dv) continue;
+    const float* x = red + j * 4 * W + c;
+    st_any(p.out, p.out_bf, ((n * p.K + j) * p.H + h) * p.Dv + blockIdx.x * W + c, (x[0] + x[W]) + (x[2 * W] + x[3 * W]));
+  }
+}
+
+template <int RPT>
+static int launch_step(cudaStream_t st, const Step& p, int64_t rows) {
+  ProfScope ps("decay_step_kernel", st);
+  GLA_LAUNCHED(launch_overlapped(step_kernel<32, RPT>, dim3((unsigned)((p.Dv + 31) / 32), (unsigned)rows), dim3(SNT), 0, st, p));
+  return GLA_OK;
+}
+template <int W, bool KEYED>
+static int launch_beams(cudaStream_t st, const Step& p, int64_t groups) {
+  constexpr int RL = SNT / (W / 4);
+  const size_t smem = (size_t)p.K * ((p.Dk + RL - 1) / RL) * SNT * 16 + (size_t)p.K * 4 * W * 4;
+  static SmemAttrOnce attr;
+  GLA_TRY(attr.ensure(step_beams_kernel<W, KEYED>, 200 << 10));
+  ProfScope ps("step_beams_kernel", st);
+  GLA_LAUNCHED(launch_overlapped(step_beams_kernel<W, KEYED>, dim3((unsigned)((p.Dv + W - 1) / W), (unsigned)groups), dim3(SNT), smem, st, p));
+  return GLA_OK;
+}
+// Columns per block: the widest whose K beams fit 64 KB (three blocks per SM), narrower with more beams and features; below
+// 16 the rows of a block no longer fill 64 bytes.
+template <bool KEYED>
+static int step_beams(cudaStream_t st, const Step& p, int64_t groups) {
+  const int64_t col = (int64_t)p.K * (p.Dk + 31) / 32 * 32 * 4;      // bytes of a column
+  if (col * 32 <= 64 << 10) return launch_beams<32, KEYED>(st, p, groups);
+  if (col * 16 <= 96 << 10) return launch_beams<16, KEYED>(st, p, groups);
+  return launch_beams<4, KEYED>(st, p, groups);
+}
+
+// ---- moving states -------------------------------------------------------------------------------------------------------
+constexpr int RT = 64;                 // tensors per launch
+struct Tensors {
+  uint8_t* p[RT];
+  int64_t bytes[RT];                   // of a row
+  unsigned int start[RT + 1];          // first block of each tensor
+  int n, K, unit;                      // beams; bytes of an access
+  const int* parents;
+};
+constexpr int MNT = 256;
+
+// A thread owns one `unit` (16 bytes where the rows allow) of all K rows of a request: those that others go on from are
+// read, then those that change are written.
+template <typename T>
+__global__ void __launch_bounds__(MNT) reorder_kernel(const Tensors t) {
+  extern __shared__ __align__(16) uint8_t sm[];
+  T* old = reinterpret_cast<T*>(sm);                                   // [K][MNT]
+  int i = 0, j = t.n;                                                  // the tensor of this block
+  while (j - i > 1) {
+    const int m = (i + j) / 2;
+    if (t.start[m] <= blockIdx.x) i = m; else j = m;
+  }
+  const int64_t units = t.bytes[i] / (int64_t)sizeof(T), per = (units + MNT - 1) / MNT;
+  const int64_t blk = blockIdx.x - t.start[i], n = blk / per, u = blk % per * MNT + threadIdx.x;
+  T* base = reinterpret_cast<T*>(t.p[i]) + n * t.K * units + u;
+  const bool count = i == 0 && blk % per == 0 && threadIdx.x == 0;
+  unsigned int taken = 0, moved = 0;
+  for (int b = 0; b < t.K; ++b) {
+    const int from = parent_of(t.parents, n, t.K, b, count);
+    if (from != b) { moved |= 1u << b; taken |= 1u << from; }
+  }
+  if (!moved || u >= units) return;
+  if constexpr (sizeof(T) == 16) {
+    for (int b = 0; b < t.K; ++b)
+      if ((taken >> b) & 1u) cp16(sm32(old + b * MNT + threadIdx.x), base + b * units, true);
+    cp_commit();
+    cp_wait<0>();
+  } else {
+    for (int b = 0; b < t.K; ++b)
+      if ((taken >> b) & 1u) old[b * MNT + threadIdx.x] = base[b * units];
+  }
+  for (int b = 0; b < t.K; ++b)
+    if ((moved >> b) & 1u) base[b * units] = old[parent_of(t.parents, n, t.K, b, false) * MNT + threadIdx.x];
+}
+template <typename T>
+static int launch_reorder(cudaStream_t st, const Tensors& t) {
+  static SmemAttrOnce attr;
+  GLA_TRY(attr.ensure(reorder_kernel<T>, 32 * MNT * sizeof(T)));
+  ProfScope ps("reorder_kernel", st);
+  reorder_kernel<T><<<t.start[t.n], MNT, (size_t)t.K * MNT * sizeof(T), st>>>(t);
+  GLA_CHECK_LAUNCH();
+  return GLA_OK;
+}
+
+// ---- selection -------------------------------------------------------------------------------------------------------------
+// For each request the M best of its K V continuations by score[k] + log_softmax(logits[k])[v], the largest first, the
+// lowest (beam, token) first among equal ones.
+//
+// One pass over the logits: a block streams a part of a row, keeps the running maximum and sum of exponentials of the
+// softmax per thread, and the part's M largest logits.  Within a row the order of the totals is that of the logits, so that
+// nothing but M candidates per part and its (maximum, sum) leaves the pass; a second kernel forms the totals of the
+// candidates in 64 bits and orders them.
+// The candidates of a part: a threshold below which nothing can be among the M any more (M larger ones have been seen).
+// Values above it go to a list in shared memory, which is cut to its M largest when it has grown (each counts how many are
+// larger) and raises the threshold.  Where many threads have one, as in the first tile, the M-th largest of a warp's 32
+// largest raises it first, so that a tile never adds more than a few of each warp.
+// A key is (order of the value, lowest index first), 0: none.
+typedef unsigned long long u64;
+__device__ __forceinline__ unsigned int order_of(float x) {
+  const unsigned int u = __float_as_uint(x + 0.f);                      // -0 is 0
+  return (u >> 31) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(unsigned int o) { return __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o); }
+__device__ __forceinline__ u64 key_of(float x, unsigned int i) { return ((u64)order_of(x) << 32) | (unsigned int)~i; }
+// what a logit counts as: not-a-number as one that is masked, +inf as the largest finite number
+__device__ __forceinline__ float clean(float x) { return x != x ? -CUDART_INF_F : fminf(x, 3.402823466e38f); }
+
+__device__ __forceinline__ u64 warp_sorted(u64 x, int lane) {           // descending over the lanes
+#pragma unroll
+  for (int k = 2; k <= 32; k <<= 1)
+#pragma unroll
+    for (int j = k >> 1; j; j >>= 1) {
+      const u64 y = __shfl_xor_sync(0xffffffffu, x, j);
+      const bool keep_max = ((lane & j) == 0) == ((lane & k) == 0);
+      x = keep_max ? (x > y ? x : y) : (x > y ? y : x);
+    }
+  return x;
+}
+
+constexpr int QNT = 256, QV = 16, TILE = QNT * QV;                      // threads, logits per thread and tile
+constexpr int QCAP = 32 * 8 * QV + 512;                                 // list: what a tile adds at most, and what may be left over
+struct Select {
+  const void* logits;
+  const float* scores;
+  const unsigned char* finished;
+  int64_t V;
+  int K, M, bf, parts;
+  int64_t part;                     // logits of a part, a multiple of TILE
+  int64_t pad;
+  u64* cand;                        // [row][part][M]
+  double2* sums;                    // [row][part]: maximum, sum of exponentials
+  float* out_scores;
+  long long* tokens;
+  int* parents;
+};
+
+// the list's M largest, in order, to its front (0 behind them); cnt becomes their number, returns the M-th (0: fewer)
+__device__ __forceinline__ u64 cut_list(u64* list, u64* best, int* cnt, int M) {
+  __syncthreads();
+  const int n = *cnt;
+  for (int i = threadIdx.x; i < M; i += QNT) best[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += QNT) {
+    const u64 x = list[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += list[j] > x;
+    if (rank < M) best[rank] = x;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < M; i += QNT) list[i] = best[i];
+  if (threadIdx.x == 0) *cnt = n < M ? n : M;
+  __syncthreads();
+  return list[M - 1];
+}
+
+template <bool BF>
+__global__ void __launch_bounds__(QNT) select_parts_kernel(const Select p) {
+  __shared__ u64 list[QCAP], best[32], wtau[8];
+  __shared__ float wm[8];
+  __shared__ double ws[8];
+  __shared__ int cnt;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  const int64_t row = blockIdx.y, V = p.V;
+  u64* cand = p.cand + (row * p.parts + blockIdx.x) * p.M;
+  const float score = p.scores[row];
+  const bool dead = !(score > -CUDART_INF_F), done = p.finished && p.finished[row];
+  if (dead || done) {
+    // a beam that has ended has one continuation, one without a score has none: the others rank by their number alone
+    if (tid < p.M) {
+      u64 x = 0;
+      if (blockIdx.x == 0) {
+        const bool one = done && !dead;
+        const int64_t i = !one ? tid : tid == 0 ? p.pad : tid - 1 < p.pad ? tid - 1 : tid;
+        if (i < V) x = key_of(one && tid == 0 ? 0.f : -CUDART_INF_F, (unsigned int)i);
+      }
+      cand[tid] = x;
+    }
+    if (tid == 0) p.sums[row * p.parts + blockIdx.x] = blockIdx.x == 0 ? make_double2(0.0, 1.0) : make_double2(-CUDART_INF, 0.0);
+    return;
+  }
+  // A thread's logits are the same whatever a row's address, so that equal rows have equal sums to the last bit and their
+  // totals tie.  Rows that do not start on 16 bytes are put together from two aligned accesses.
+  constexpr int E = BF ? 8 : 4, NV = QV / E, ES = BF ? 2 : 4;         // logits per 16 bytes, accesses per tile
+  const char* base = (const char*)p.logits + row * V * ES;
+  const int shift = (int)((uintptr_t)base & 15) / ES;
+  const int64_t lo = blockIdx.x * p.part, hi = lo + p.part < V ? lo + p.part : V;
+  if (tid == 0) cnt = 0;
+  float m = -CUDART_INF_F, s = 0.f;
+  u64 tau = 0;
+  __syncthreads();
+  for (int64_t t0 = lo; t0 < hi; t0 += TILE) {
+    float x[QV];
+    unsigned int has = 0;
+#pragma unroll
+    for (int w = 0; w < NV; ++w) {
+      const int64_t e = t0 + (int64_t)(w * QNT + tid) * E;
+      if (shift ? e >= shift && e - shift + 2 * E <= V : e + E <= V) {
+        uint4 u = __ldg((const uint4*)(base + (e - shift) * ES));
+        if (shift) {
+          const uint4 n = __ldg((const uint4*)(base + (e - shift + E) * ES));
+          const unsigned int z[8] = {u.x, u.y, u.z, u.w, n.x, n.y, n.z, n.w};
+          unsigned int y[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            // 32 bits from byte 4 i + shift ES on: words by a chain of selects, bytes by a funnel shift
+            unsigned int a = z[i], b = z[i + 1];
+#pragma unroll
+            for (int j = 1; j < 4; ++j)
+              if (shift * ES / 4 == j) { a = z[i + j]; b = i + j + 1 < 8 ? z[i + j + 1 < 8 ? i + j + 1 : 7] : 0; }
+            y[i] = __funnelshift_r(a, b, shift * ES % 4 * 8);
+          }
+          u = make_uint4(y[0], y[1], y[2], y[3]);
+        }
+        const unsigned int y[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (BF) { x[w * E + 2 * i] = __uint_as_float(y[i] << 16); x[w * E + 2 * i + 1] = __uint_as_float(y[i] & 0xffff0000u); }
+          else x[w * E + i] = __uint_as_float(y[i]);
+        }
+        has |= ((1u << E) - 1) << (w * E);
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+          x[w * E + i] = -CUDART_INF_F;
+          if (e + i < V) {
+            x[w * E + i] = BF ? __bfloat162float(((const bf16*)base)[e + i]) : ((const float*)base)[e + i];
+            has |= 1u << (w * E + i);
+          }
+        }
+      }
+    }
+    float top = -CUDART_INF_F;
+#pragma unroll
+    for (int i = 0; i < QV; ++i) { x[i] = clean(x[i]); top = fmaxf(top, x[i]); }
+    if (top > m) { s *= exp2f((m - top) * 1.4426950408889634f); m = top; }
+    if (m > -CUDART_INF_F) {
+#pragma unroll
+      for (int i = 0; i < QV; ++i) s += expf(x[i] - m);
+    }
+    // the thread's largest key
+    u64 first = 0;
+    if (order_of(top) >= (unsigned int)(tau >> 32)) {
+#pragma unroll
+      for (int i = QV - 1; i >= 0; --i) {
+        const int64_t e = t0 + (int64_t)(i / E * QNT + tid) * E + i % E;
+        if (((has >> i) & 1u) && x[i] == top) first = key_of(x[i], (unsigned int)e);
+      }
+    }
+    const int many = __syncthreads_count(first > tau);
+    if (many > 64) {
+      const u64 o = warp_sorted(first, lane);
+      const u64 mth = __shfl_sync(0xffffffffu, o, p.M - 1);
+      if (lane == 0) wtau[warp] = mth;
+      __syncthreads();
+      u64 y = tau;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) y = wtau[w] > y ? wtau[w] : y;
+      tau = y > 0 ? y - 1 : 0;                                // (the M-th itself stays in)
+    }
+    if (first > tau) {
+#pragma unroll
+      for (int i = 0; i < QV; ++i) {
+        const int64_t e = t0 + (int64_t)(i / E * QNT + tid) * E + i % E;
+        const u64 y = ((has >> i) & 1u) ? key_of(x[i], (unsigned int)e) : 0;
+        if (y > tau) list[atomicAdd(&cnt, 1)] = y;
+      }
+    }
+    if (many) {
+      __syncthreads();
+      if (cnt > 256 || many > 64) {
+        const u64 y = cut_list(list, best, &cnt, p.M);
+        tau = y > tau ? y : tau;
+      }
+    }
+    __syncthreads();
+  }
+  cut_list(list, best, &cnt, p.M);
+  if (tid < p.M) cand[tid] = list[tid];
+  // (maximum, sum) of the part
+  float top = m;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  if (lane == 0) wm[warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = fmaxf(top, wm[w]);
+  double sum = m > -CUDART_INF_F ? (double)s * expf(m - top) : 0.0;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  if (lane == 0) ws[warp] = sum;
+  __syncthreads();
+  if (tid == 0) {
+    sum = 0.0;
+    for (int w = 0; w < 8; ++w) sum += ws[w];
+    p.sums[row * p.parts + blockIdx.x] = make_double2(top, sum);
+  }
+}
+
+// order of a 64-bit total, and the totals' candidates: (total, beam and token)
+__device__ __forceinline__ u64 order_of(double x) {
+  const long long u = __double_as_longlong(x + 0.0);
+  return u < 0 ? ~(u64)u : (u64)u | 0x8000000000000000ull;
+}
+constexpr int SCAP = 1024;              // candidates of a request: K parts M, at most
+__global__ void __launch_bounds__(QNT) select_beams_kernel(const Select p) {
+  __shared__ u64 key[SCAP];
+  __shared__ u64 where[SCAP];           // (beam, token)
+  __shared__ double base[64][2];        // per beam: maximum, log of the sum
+  __shared__ double tot[SCAP];
+  const int tid = threadIdx.x, K = p.K, M = p.M, per = p.parts * M, n = K * per;
+  const int64_t req = blockIdx.x;
+  for (int k = tid; k < K; k += QNT) {
+    const double2* sm = p.sums + (req * K + k) * p.parts;
+    double top = -CUDART_INF, s = 0.0;
+    for (int i = 0; i < p.parts; ++i) top = fmax(top, sm[i].x);
+    for (int i = 0; i < p.parts; ++i)
+      if (sm[i].x > -CUDART_INF) s += sm[i].y * exp(sm[i].x - top);
+    base[k][0] = top;
+    base[k][1] = log(s);
+  }
+  __syncthreads();
+  const u64* cand = p.cand + req * n;
+  for (int i = tid; i < n; i += QNT) {
+    const u64 c = cand[i];
+    const int k = i / per;
+    double t = -CUDART_INF;
+    u64 o = 0;
+    if (c) {
+      const float x = value_of((unsigned int)(c >> 32));
+      if (x > -CUDART_INF_F && base[k][0] > -CUDART_INF) t = (double)p.scores[req * K + k] + (((double)x - base[k][0]) - base[k][1]);
+      if (!(t > -CUDART_INF)) t = -CUDART_INF;
+      o = order_of(t);
+    }
+    key[i] = o;
+    tot[i] = t;
+    where[i] = ((u64)k << 32) | (unsigned int)~(unsigned int)c;
+  }
+  __syncthreads();
+  for (int i = tid; i < n; i += QNT) {
+    const u64 x = key[i];
+    if (!x) continue;
+    const u64 at = where[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += key[j] > x || (key[j] == x && where[j] < at);
+    if (rank < M) {
+      p.out_scores[req * M + rank] = (float)tot[i];
+      p.tokens[req * M + rank] = (long long)(at & 0xffffffffu);
+      p.parents[req * M + rank] = (int)(at >> 32);
+    }
+  }
+}
+
+// Parts of a row: enough blocks for the device (six per SM), few enough that a request's candidates fit.
+static void plan(int64_t rows, int64_t V, int K, int M, int bf, int* parts, int64_t* part) {
+  const int64_t tiles = (V + TILE - 1) / TILE;
+  int64_t n = (6 * 148 + rows - 1) / rows;
+  if (n > tiles) n = tiles;
+  if (n > SCAP / (K * M)) n = SCAP / (K * M);
+  if (n < 1) n = 1;
+  *part = (tiles + n - 1) / n * TILE;
+  *parts = (int)((V + *part - 1) / *part);
+}
+
+}  // namespace beam
+unsigned int beam_bad_parents() {
+  unsigned int v = 0;
+  cudaMemcpyFromSymbol(&v, beam::g_bad_parents, sizeof(v));
+  return v;
+}
+}  // namespace gla
+
+using namespace gla;
+
+extern "C" {
+
+unsigned int gla_device_bad_parents(void) { return beam_bad_parents(); }
+
+static int step_check(int64_t B, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype, int out_dtype, const int32_t* parents, int64_t K) {
+  if (B <= 0 || H <= 0 || Hk <= 0 || Dk <= 0 || Dv <= 0 || H % Hk) return GLA_ERR_BAD_DIMS;
+  if (parents && (K <= 0 || B % K)) return GLA_ERR_BAD_DIMS;
+  if ((dtype != GLA_F32 && dtype != GLA_BF16) || (out_dtype != GLA_F32 && out_dtype != GLA_BF16)) return GLA_ERR_UNSUPPORTED;
+  if (Dk % 8 || Dv % 8 || Dk > 256 || Dv > 256 || (parents && K > 32)) return GLA_ERR_UNSUPPORTED;
+  if (B * H / (parents ? K : 1) > 65535) return GLA_ERR_TOO_LARGE;
+  return GLA_OK;
+}
+
+int gla_decay_step(void* stream, int64_t B, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype, float* state, const float* log_decay,
+                   const void* value, const void* key, const void* query, void* out, int out_dtype, const int32_t* parents, int64_t beams) {
+  if (!state || !log_decay || !value || !key || !query || !out) return GLA_ERR_NULL_POINTER;
+  GLA_TRY(step_check(B, H, Hk, Dk, Dv, dtype, out_dtype, parents, beams));
+  if (!aligned16(state)) return GLA_ERR_ALIGNMENT;
+  beam::Step p{state, log_decay, value, key, query, out, parents, (int)H, (int)(H / Hk), (int)Dk, (int)Dv, parents ? (int)beams : 1,
+               dtype == GLA_BF16, out_dtype == GLA_BF16};
+  cudaStream_t st = (cudaStream_t)stream;
+  if (parents) return beam::step_beams<false>(st, p, B / beams * H);
+  if (Dk <= 64) return beam::launch_step<4>(st, p, B * H);
+  if (Dk <= 128) return beam::launch_step<8>(st, p, B * H);
+  return beam::launch_step<16>(st, p, B * H);
+}
+
+int gla_decode_step_beams(void* stream, int64_t B, int64_t H, int64_t D, int dtype, float* state, const float* log_fgate, const void* value,
+                          const void* key, const void* query, void* out, int out_dtype, const int32_t* parents, int64_t beams) {
+  if (!state || !log_fgate || !value || !key || !query || !out || !parents) return GLA_ERR_NULL_POINTER;
+  GLA_TRY(step_check(B, H, H, D, D, dtype, out_dtype, parents, beams));
+  if (D != 32 && D != 64 && D != 128 && D != 256) return GLA_ERR_UNSUPPORTED;
+  if (!aligned16(state)) return GLA_ERR_ALIGNMENT;
+  beam::Step p{state, log_fgate, value, key, query, out, parents, (int)H, 1, (int)D, (int)D, (int)beams, dtype == GLA_BF16, out_dtype == GLA_BF16};
+  return beam::step_beams<true>((cudaStream_t)stream, p, B / beams * H);
+}
+
+int gla_reorder_states(void* stream, int64_t count, void* const* tensors, const int64_t* row_bytes, int64_t requests, int64_t beams,
+                       const int32_t* parents) {
+  if (!tensors || !row_bytes || !parents) return GLA_ERR_NULL_POINTER;
+  if (count < 0 || requests <= 0 || beams <= 0) return GLA_ERR_BAD_DIMS;
+  if (beams > 32) return GLA_ERR_UNSUPPORTED;
+  for (int64_t i = 0; i < count; ++i) {
+    if (!tensors[i]) return GLA_ERR_NULL_POINTER;
+    if (row_bytes[i] <= 0) return GLA_ERR_BAD_DIMS;
+  }
+  // tensors by the widest access that their address and rows allow, RT of them a launch
+  for (int unit = 16; unit; unit = unit == 16 ? 4 : unit == 4 ? 1 : 0) {
+    beam::Tensors t{};
+    t.K = (int)beams; t.unit = unit; t.parents = parents;
+    unsigned int blocks = 0;
+    const auto flush = [&]() -> int {
+      if (!t.n) return GLA_OK;
+      t.start[t.n] = blocks;
+      const int s = unit == 16 ? beam::launch_reorder<uint4>((cudaStream_t)stream, t)
+                    : unit == 4 ? beam::launch_reorder<uint32_t>((cudaStream_t)stream, t) : beam::launch_reorder<uint8_t>((cudaStream_t)stream, t);
+      t.n = 0; blocks = 0;
+      return s;
+    };
+    for (int64_t i = 0; i < count; ++i) {
+      const uintptr_t both = (uintptr_t)tensors[i] | (uintptr_t)row_bytes[i];
+      const int own = (both & 15) == 0 ? 16 : (both & 3) == 0 ? 4 : 1;
+      if (own != unit) continue;
+      const int64_t per = (row_bytes[i] / unit + beam::MNT - 1) / beam::MNT * requests;
+      if (per > 1 << 30) return GLA_ERR_TOO_LARGE;
+      if (t.n == beam::RT || (int64_t)blocks + per > 1 << 30) GLA_TRY(flush());
+      t.p[t.n] = (uint8_t*)tensors[i];
+      t.bytes[t.n] = row_bytes[i];
+      t.start[t.n++] = blocks;
+      blocks += (unsigned int)per;
+    }
+    GLA_TRY(flush());
+  }
+  return GLA_OK;
+}
+
+static int select_check(int64_t N, int64_t K, int64_t V, int64_t M, int dtype, int64_t pad) {
+  if (N <= 0 || K <= 0 || V <= 0 || M <= 0 || M > K * V || pad < 0 || pad >= V) return GLA_ERR_BAD_DIMS;
+  if (dtype != GLA_F32 && dtype != GLA_BF16) return GLA_ERR_UNSUPPORTED;
+  if (K > 32 || M > 32) return GLA_ERR_UNSUPPORTED;
+  if (N * K > 65535 || V > 1 << 30) return GLA_ERR_TOO_LARGE;
+  return GLA_OK;
+}
+static size_t select_bytes(int64_t N, int64_t K, int64_t M, int parts) {
+  return align_up((size_t)(N * K * parts * M) * 8, 256) + align_up((size_t)(N * K * parts) * 16, 256);
+}
+
+size_t gla_beam_select_workspace_bytes(int64_t N, int64_t K, int64_t V, int64_t M, int dtype) {
+  if (select_check(N, K, V, M, dtype, 0) != GLA_OK) return 0;
+  int parts; int64_t part;
+  beam::plan(N * K, V, (int)K, (int)M, dtype == GLA_BF16, &parts, &part);
+  return select_bytes(N, K, M, parts);
+}
+
+int gla_beam_select(void* stream, int64_t N, int64_t K, int64_t V, int64_t M, int dtype, const void* logits, const float* scores,
+                    const unsigned char* finished, int64_t pad_token, float* out_scores, int64_t* tokens, int32_t* parents, void* workspace,
+                    size_t workspace_bytes) {
+  if (!logits || !scores || !out_scores || !tokens || !parents) return GLA_ERR_NULL_POINTER;
+  GLA_TRY(select_check(N, K, V, M, dtype, pad_token));
+  if ((uintptr_t)logits % (dtype == GLA_BF16 ? 2 : 4)) return GLA_ERR_ALIGNMENT;
+  beam::Select p{};
+  p.logits = logits; p.scores = scores; p.finished = finished; p.V = V; p.K = (int)K; p.M = (int)M; p.bf = dtype == GLA_BF16; p.pad = pad_token;
+  beam::plan(N * K, V, p.K, p.M, p.bf, &p.parts, &p.part);
+  if (!workspace || workspace_bytes < select_bytes(N, K, M, p.parts)) return GLA_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return GLA_ERR_ALIGNMENT;
+  p.cand = (unsigned long long*)workspace;
+  p.sums = (double2*)((char*)workspace + align_up((size_t)(N * K * p.parts * M) * 8, 256));
+  p.out_scores = out_scores; p.tokens = (long long*)tokens; p.parents = parents;
+  cudaStream_t st = (cudaStream_t)stream;
+  {
+    ProfScope ps("select_parts_kernel", st);
+    const dim3 grid((unsigned)p.parts, (unsigned)(N * K));
+    if (p.bf) beam::select_parts_kernel<true><<<grid, beam::QNT, 0, st>>>(p);
+    else beam::select_parts_kernel<false><<<grid, beam::QNT, 0, st>>>(p);
+    GLA_CHECK_LAUNCH();
+  }
+  ProfScope ps("select_beams_kernel", st);
+  beam::select_beams_kernel<<<(unsigned)N, beam::QNT, 0, st>>>(p);
+  GLA_CHECK_LAUNCH();
+  return GLA_OK;
+}
+
+}  // extern "C"

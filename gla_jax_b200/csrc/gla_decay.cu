@@ -1,0 +1,309 @@
+// Linear attention with one decay per head: what runs around the walks of gla_decay.cuh (runs of a sequence and their
+// states, sums over shared heads, the gradient of the decays), forward and backward.
+#include "gla_decay.cuh"
+
+namespace gla {
+namespace decay {
+namespace {
+
+// The state that enters each run of a sequence, from what each run adds: element by element, in place.
+__global__ void __launch_bounds__(256) entering_kernel(const Walk p) {
+  const int64_t s = blockIdx.z, h = blockIdx.y, e = blockIdx.x * 256ll + threadIdx.x, dd = (int64_t)p.kd * p.vd;
+  if (e >= dd) return;
+  const int64_t c = e / p.kd, k = e % p.kd;
+  float x = ld_any(p.init, !p.init_f32, (s * p.H + h) * dd + k * p.ik + c * p.ic);
+  int64_t n = 1;
+  slot_of(p, s, 0, n);
+  for (int64_t i = 0; i < n; ++i) {
+    const int64_t at = slot_of(p, s, p.rev ? n - 1 - i : i, n) * p.H + h;
+    if (at / p.H >= p.nslots) return;
+    float* u = p.seg_state + at * dd + e;
+    const bool more = i + 1 < n;
+    const float add = more ? *u : 0.f;
+    *u = x;
+    if (more) x = fmaf((float)exp2(p.seg_total[at]), x, add);
+  }
+}
+
+// out[row][hk][d] = sum over the heads that share hk of x[row][h][d], in order
+template <typename T>
+__global__ void __launch_bounds__(256) share_sum_kernel(const float* x, T* out, int64_t n, int share, int d) {
+  const int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4;
+  if (i >= n) return;
+  const int64_t row = i / d, c = i % d;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int j = 0; j < share; ++j) {
+    const float4 y = *reinterpret_cast<const float4*>(x + (row * share + j) * d + c);
+    a.x += y.x; a.y += y.y; a.z += y.z; a.w += y.w;
+  }
+  st_f(out, i, a.x); st_f(out, i + 1, a.y); st_f(out, i + 2, a.z); st_f(out, i + 3, a.w);
+}
+
+// dg_t = sum over i >= t of (q dq - k dk) + <S_T, dS_T>: a block per sequence and head, from the end, the running sum in
+// 64 bits
+struct Gate {
+  const float *rq, *rk;             // [tiles][token][H]
+  int nq, nk;
+  const int* cu;
+  int64_t T, nseq, rows;
+  int H;
+  const float* S;                   // [s][h] final state, float32
+  const void* dS;
+  int dS_f32;
+  int64_t dd;
+  float* dg;
+};
+__global__ void __launch_bounds__(512) gate_grad_kernel(const Gate p) {
+  __shared__ double part[16];
+  __shared__ double carry;
+  const int64_t s = blockIdx.x, h = blockIdx.y;
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  int64_t a = s * p.T, b = a + p.T;
+  if (p.cu) {
+    const auto at = [&](int64_t i) { const int64_t x = p.cu[i]; return x < 0 ? (int64_t)0 : x > p.T ? p.T : x; };
+    a = at(s); b = at(s + 1);
+    if (b < a) b = a;
+    if (s == p.nseq - 1)
+      for (int64_t t = b + tid; t < p.T; t += 512) p.dg[t * p.H + h] = 0.f;
+  }
+  double dot = 0.0;
+  for (int64_t e = tid; e < p.dd; e += 512) dot += (double)p.S[(s * p.H + h) * p.dd + e] * ld_any(p.dS, !p.dS_f32, (s * p.H + h) * p.dd + e);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+  if (lane == 0) part[warp] = dot;
+  __syncthreads();
+  if (tid == 0) {
+    double x = 0.0;
+    for (int w = 0; w < 16; ++w) x += part[w];
+    carry = x;
+  }
+  __syncthreads();
+  for (int64_t end = b; end > a; end -= 512) {
+    const int64_t t = end - 1 - tid;
+    double x = 0.0;
+    if (t >= a) {
+      for (int i = 0; i < p.nq; ++i) x += p.rq[(i * p.rows + t) * p.H + h];
+      for (int i = 0; i < p.nk; ++i) x -= p.rk[(i * p.rows + t) * p.H + h];
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (lane == 31) part[warp] = x;
+    __syncthreads();
+    double before = carry;
+    for (int w = 0; w < warp; ++w) before += part[w];
+    x += before;
+    if (t >= a) p.dg[t * p.H + h] = (float)x;
+    __syncthreads();
+    if (tid == 511) carry = x;
+    __syncthreads();
+  }
+}
+
+int sm_count() {
+  static int sms[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!sms[dev] && cudaDeviceGetAttribute(&sms[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  return sms[dev];
+}
+
+// Tokens of a run.  A walk has a block per run, head and tile of value columns; with fewer blocks than the device holds
+// (two per SM) sequences are cut into runs, at the price of reading k and v twice.  Runs shorter than 256 tokens do not pay.
+int64_t run_tokens(int64_t T, int64_t nseq, int64_t H, int64_t vd, bool packed) {
+  const int64_t blocks = H * ((vd + 127) / 128) * nseq, want = 2 * (int64_t)sm_count();
+  int64_t n = packed ? want / (H * ((vd + 127) / 128)) : want / blocks;      // runs: of the packed axis, of each sequence
+  if (blocks * 2 > want) n = 1;
+  if (n > T / 256) n = T / 256;
+  if (n <= 1) return align_up(T, 64);
+  return align_up((T + n - 1) / n, 64);
+}
+
+}  // namespace
+
+struct Dims {
+  int64_t B, T, H, Hk, Dk, Dv, nseq;   // nseq > 0: packed, one axis of T tokens
+  int bf, hid_f32;
+  int64_t seqs() const { return nseq ? nseq : B; }
+  int64_t rows() const { return B * T; }
+  int64_t seg(int64_t vd) const { return run_tokens(T, seqs(), H, vd, nseq > 0); }
+  int64_t slots(int64_t s) const { const int64_t n = (T + s - 1) / s; return nseq ? nseq + n : B * n; }
+  bool cut(int64_t s) const { return s < T; }
+  size_t seg_bytes(int64_t vd) const {
+    const int64_t s = seg(vd);
+    return cut(s) ? align_up((size_t)(slots(s) * H * Dk * Dv) * 4, 256) + align_up((size_t)(slots(s) * H) * 8, 256) : 0;
+  }
+};
+
+static int walk(cudaStream_t st, int mode, const Walk& p, bool out, const char* name) {
+  switch (mode) {
+    case M_ONE: return walk_one(st, p, out, name);
+    case M_STATE: return walk_state(st, p, out, name);
+    case M_FINE: return walk_fine(st, p, out, name);
+    default: return walk_full(st, p, out, name);
+  }
+}
+// A whole walk: the runs' sums and their entering states first where sequences are cut.
+static int run_walk(cudaStream_t st, const Dims& d, int mode, Walk p, void* ws, const char* first, const char* name) {
+  p.H = (int)d.H; p.T = d.T; p.nseq = d.seqs();
+  p.seg = d.seg(p.vd);
+  p.nslots = d.slots(p.seg);
+  if (p.nslots > 2147483647LL || d.H * ((p.vd + 63) / 64) > 65535 || p.nseq > 65535 * 32767LL) return GLA_ERR_TOO_LARGE;
+  if (d.cut(p.seg)) {
+    if (p.nseq > 65535) return GLA_ERR_TOO_LARGE;
+    p.seg_state = (float*)ws;
+    p.seg_total = (double*)((char*)ws + align_up((size_t)(p.nslots * d.H * d.Dk * d.Dv) * 4, 256));
+    GLA_TRY(walk(st, mode, p, false, first));
+    ProfScope ps("decay_entering_kernel", st);
+    entering_kernel<<<dim3((unsigned)((d.Dk * d.Dv + 255) / 256), (unsigned)d.H, (unsigned)p.nseq), 256, 0, st>>>(p);
+    GLA_CHECK_LAUNCH();
+  }
+  return walk(st, mode, p, true, name);
+}
+
+size_t fwd_ws_bytes(const Dims& d) { return d.seg_bytes(d.Dv); }
+int fwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const float* g, int64_t gt, const void* v, const void* k,
+        const void* q, void* hf, void* out, float* fin32, void* ws) {
+  Walk p{};
+  p.q = q; p.k = k; p.v = v;
+  p.gq = p.gk = (int)(d.H / d.Hk); p.gv = 1;
+  p.kd = (int)d.Dk; p.vd = (int)d.Dv;
+  p.g = g; p.gt = gt; p.cu = cu; p.count_bad = cu != nullptr;
+  p.init = h0; p.fin = hf; p.fin32 = fin32; p.ik = d.Dv; p.ic = 1; p.init_f32 = p.fin_f32 = d.hid_f32;
+  p.out = out; p.out_f32 = !d.bf;
+  return run_walk(st, d, !d.bf ? M_FULL : d.hid_f32 ? M_STATE : M_ONE, p, ws, "decay_runs_kernel", "decay_walk_kernel");
+}
+
+static size_t bwd_parts(const Dims& d, bool gate, size_t (&at)[5]) {
+  const int64_t share = d.H / d.Hk, tiles = (d.Dk + 127) / 128;
+  const size_t seg = d.seg_bytes(d.Dv) > d.seg_bytes(d.Dk) ? d.seg_bytes(d.Dv) : d.seg_bytes(d.Dk);
+  const size_t dots = gate ? align_up((size_t)(tiles * d.rows() * d.H) * 4, 256) : 0;
+  at[0] = seg;
+  at[1] = at[0] + dots;
+  at[2] = at[1] + dots;
+  at[3] = at[2] + (share > 1 ? align_up((size_t)(d.rows() * d.H * d.Dk) * 4, 256) : 0);
+  return at[3];
+}
+size_t bwd_ws_bytes(const Dims& d, bool gate) {
+  size_t at[5];
+  return bwd_parts(d, gate, at);
+}
+static int share_sum(cudaStream_t st, const Dims& d, const float* x, void* out) {
+  const int64_t n = d.rows() * d.Hk * d.Dk;
+  const unsigned blocks = (unsigned)((n / 4 + 255) / 256);
+  ProfScope ps("decay_share_sum_kernel", st);
+  if (d.bf) share_sum_kernel<bf16><<<blocks, 256, 0, st>>>(x, (bf16*)out, n, (int)(d.H / d.Hk), (int)d.Dk);
+  else share_sum_kernel<float><<<blocks, 256, 0, st>>>(x, (float*)out, n, (int)(d.H / d.Hk), (int)d.Dk);
+  GLA_CHECK_LAUNCH();
+  return GLA_OK;
+}
+int bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const float* g, int64_t gt, const void* v, const void* k,
+        const void* q, const float* fin32, const void* dhf, const void* dout, void* dh, float* dg, void* dv, void* dk, void* dq, void* ws) {
+  size_t at[5];
+  bwd_parts(d, dg != nullptr, at);
+  float *rq = (float*)((char*)ws + at[0]), *rk = (float*)((char*)ws + at[1]), *wide = (float*)((char*)ws + at[2]);
+  const int share = (int)(d.H / d.Hk), mode = d.bf ? M_FINE : M_FULL;
+  Walk p{};
+  p.g = g; p.gt = gt; p.cu = cu;
+  p.init_f32 = p.fin_f32 = d.hid_f32;
+  // dq, forwards over the states of the forward, transposed
+  p.q = dout; p.k = v; p.v = k; p.gq = p.gk = 1; p.gv = share; p.kd = (int)d.Dv; p.vd = (int)d.Dk;
+  p.init = h0; p.ik = 1; p.ic = d.Dv;
+  p.out = share > 1 ? (void*)wide : dq; p.out_f32 = share > 1 || !d.bf;
+  p.r = dg ? q : nullptr; p.gr = share; p.rdot = rq;
+  GLA_TRY(run_walk(st, d, mode, p, ws, "decay_runs_kernel", "decay_dq_kernel"));
+  if (share > 1) GLA_TRY(share_sum(st, d, wide, dq));
+  // dk, backwards
+  p.rev = 1;
+  p.q = v; p.k = dout; p.v = q;
+  p.init = dhf;
+  p.out = share > 1 ? (void*)wide : dk;
+  p.r = dg ? k : nullptr; p.rdot = rk;
+  GLA_TRY(run_walk(st, d, mode, p, ws, "decay_runs_kernel", "decay_dk_kernel"));
+  if (share > 1) GLA_TRY(share_sum(st, d, wide, dk));
+  // dv and the gradient of the first state, backwards
+  p.q = k; p.k = q; p.v = dout; p.gq = p.gk = share; p.gv = 1; p.kd = (int)d.Dk; p.vd = (int)d.Dv;
+  p.ik = d.Dv; p.ic = 1; p.fin = dh;
+  p.out = dv; p.out_f32 = !d.bf; p.r = nullptr; p.rdot = nullptr;
+  GLA_TRY(run_walk(st, d, mode, p, ws, "decay_runs_kernel", "decay_dv_kernel"));
+  if (dg) {
+    Gate w{};
+    w.rq = rq; w.rk = rk; w.nq = w.nk = (int)((d.Dk + 127) / 128);
+    w.cu = cu; w.T = d.T; w.nseq = d.seqs(); w.rows = d.rows(); w.H = (int)d.H;
+    w.S = fin32; w.dS = dhf; w.dS_f32 = d.hid_f32; w.dd = d.Dk * d.Dv; w.dg = dg;
+    ProfScope ps("decay_gate_grad_kernel", st);
+    gate_grad_kernel<<<dim3((unsigned)w.nseq, (unsigned)d.H), 512, 0, st>>>(w);
+    GLA_CHECK_LAUNCH();
+  }
+  return GLA_OK;
+}
+unsigned int read_all_bad_offsets() { return bad_offsets_one() + bad_offsets_state() + bad_offsets_fine() + bad_offsets_full(); }
+
+// What the entry points share: sizes, types, alignment, workspace.
+static int check(const Dims& d, int dtype, int hidden_dtype, const int* cu) {
+  if (d.B <= 0 || d.T <= 0 || d.H <= 0 || d.Hk <= 0 || d.Dk <= 0 || d.Dv <= 0 || d.nseq < 0 || d.H % d.Hk) return GLA_ERR_BAD_DIMS;
+  if ((d.nseq > 0) != (cu != nullptr) || (d.nseq > 0 && (d.B != 1 || d.T > 2147483647LL))) return GLA_ERR_BAD_DIMS;
+  if ((dtype != GLA_F32 && dtype != GLA_BF16) || (hidden_dtype != GLA_F32 && hidden_dtype != dtype)) return GLA_ERR_UNSUPPORTED;
+  if (d.Dk % 8 || d.Dv % 8 || d.Dk > 256 || d.Dv > 256) return GLA_ERR_UNSUPPORTED;
+  if (d.H > 65535 / 4 || d.seqs() > 65535 || d.T > (int64_t)1 << 40) return GLA_ERR_TOO_LARGE;
+  return GLA_OK;
+}
+
+}  // namespace decay
+}  // namespace gla
+
+using namespace gla;
+using decay::Dims;
+
+extern "C" {
+
+static Dims dims_of(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype, int hidden_dtype, int64_t nseq) {
+  return Dims{B, T, H, Hk, Dk, Dv, nseq, dtype == GLA_BF16, hidden_dtype == GLA_F32};
+}
+
+size_t gla_decay_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype, int hidden_dtype,
+                                 int64_t nseq, int backward) {
+  const Dims d = dims_of(B, T, H, Hk, Dk, Dv, dtype, hidden_dtype, nseq);
+  static const int some = 0;
+  if (decay::check(d, dtype, hidden_dtype, nseq > 0 ? &some : nullptr) != GLA_OK) return 0;
+  return backward ? decay::bwd_ws_bytes(d, backward > 1) : decay::fwd_ws_bytes(d);
+}
+
+int gla_decay_fwd(void* stream, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype, int hidden_dtype,
+                  int64_t nseq, const int32_t* cu_seqlens, const void* hidden_init, const float* log_decay, int per_token,
+                  const void* value, const void* key, const void* query, void* hidden_final, void* out, float* final32,
+                  void* workspace, size_t workspace_bytes) {
+  if (!hidden_init || !log_decay || !value || !key || !query || !hidden_final || !out) return GLA_ERR_NULL_POINTER;
+  const Dims d = dims_of(B, T, H, Hk, Dk, Dv, dtype, hidden_dtype, nseq);
+  GLA_TRY(decay::check(d, dtype, hidden_dtype, cu_seqlens));
+  for (const void* p : {value, key, query, (const void*)out})
+    if (!aligned16(p)) return GLA_ERR_ALIGNMENT;
+  const size_t need = decay::fwd_ws_bytes(d);
+  if (need && (!workspace || workspace_bytes < need)) return GLA_ERR_WORKSPACE;
+  if (need && !aligned16(workspace)) return GLA_ERR_ALIGNMENT;
+  return decay::fwd((cudaStream_t)stream, d, cu_seqlens, hidden_init, log_decay, per_token ? H : 0, value, key, query, hidden_final, out,
+                    final32, workspace);
+}
+
+int gla_decay_bwd(void* stream, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype, int hidden_dtype,
+                  int64_t nseq, const int32_t* cu_seqlens, const void* hidden_init, const float* log_decay, int per_token,
+                  const void* value, const void* key, const void* query, const float* final32, const void* dhidden_final,
+                  const void* dout, void* dhidden_init, float* dlog_decay, void* dvalue, void* dkey, void* dquery, void* workspace,
+                  size_t workspace_bytes) {
+  if (!hidden_init || !log_decay || !value || !key || !query || !dhidden_final || !dout || !dhidden_init || !dvalue || !dkey || !dquery ||
+      (dlog_decay && !final32))
+    return GLA_ERR_NULL_POINTER;
+  const Dims d = dims_of(B, T, H, Hk, Dk, Dv, dtype, hidden_dtype, nseq);
+  GLA_TRY(decay::check(d, dtype, hidden_dtype, cu_seqlens));
+  for (const void* p : {value, key, query, dout, (const void*)dvalue, (const void*)dkey, (const void*)dquery})
+    if (!aligned16(p)) return GLA_ERR_ALIGNMENT;
+  const size_t need = decay::bwd_ws_bytes(d, dlog_decay != nullptr);
+  if (need && (!workspace || workspace_bytes < need)) return GLA_ERR_WORKSPACE;
+  if (need && !aligned16(workspace)) return GLA_ERR_ALIGNMENT;
+  return decay::bwd((cudaStream_t)stream, d, cu_seqlens, hidden_init, log_decay, per_token ? H : 0, value, key, query, final32, dhidden_final,
+                    dout, dhidden_init, dlog_decay, dvalue, dkey, dquery, workspace);
+}
+
+}  // extern "C"

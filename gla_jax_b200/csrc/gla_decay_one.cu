@@ -1,0 +1,9 @@
+// The walks of gla_decay.cuh in mode "one" (a file each, so that they compile side by side).
+#include "gla_decay.cuh"
+
+namespace gla {
+namespace decay {
+int walk_one(cudaStream_t stream, const Walk& p, bool out, const char* name) { return walk_mode<M_ONE>(stream, p, out, name); }
+unsigned int bad_offsets_one() { return read_bad_offsets(); }
+}  // namespace decay
+}  // namespace gla

@@ -9,6 +9,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAFunctions.h>
+#include <algorithm>
 #include <cmath>
 #include "../../include/gla_b200.h"
 
@@ -290,9 +291,181 @@ std::optional<std::tuple<Tensor, Tensor>> chunk_gla_packed(const Tensor& h, cons
   return std::make_tuple(r[0], r[1]);
 }
 
+// ---- attention with one decay per head ---------------------------------------------------------------------------------
+// (T, H, Dv) or (B, T, H, Dv) values, (.., Hk, Dk) keys and queries, decays (.., H) or (H), states (B, H, Dk, Dv) in the
+// values' type or float32; cu: packed sequences on one axis
+struct DecayDims {
+  int64_t B, T, H, Hk, Dk, Dv, nseq;
+  int dt, hdt;
+  int per_token;
+  std::vector<int64_t> list() const { return {B, T, H, Hk, Dk, Dv, nseq, dt, hdt, per_token}; }
+  static DecayDims of(const std::vector<int64_t>& a) {
+    return {a[0], a[1], a[2], a[3], a[4], a[5], a[6], (int)a[7], (int)a[8], (int)a[9]};
+  }
+};
+bool decay_dims(const Tensor& h, const Tensor& g, const Tensor& v, const Tensor& k, const Tensor& q, const Tensor& cu, DecayDims& d) {
+  if (!v.defined() || !here(v)) return false;
+  for (const Tensor* t : {&h, &g, &k, &q}) if (!t->defined() || t->device() != v.device()) return false;
+  const bool packed = cu.defined();
+  const int b = v.dim() == 4;
+  if ((v.dim() != 3 && !b) || (packed && b) || k.dim() != v.dim() || k.sizes() != q.sizes()) return false;
+  if (k.size(b) != v.size(b) || (b && k.size(0) != v.size(0))) return false;
+  d.B = b ? v.size(0) : 1; d.T = v.size(b); d.H = v.size(b + 1); d.Dv = v.size(b + 2);
+  d.Hk = k.size(b + 1); d.Dk = k.size(b + 2);
+  d.nseq = packed ? cu.numel() - 1 : 0;
+  d.dt = dt_of(v);
+  d.hdt = dt_of(h);
+  if (d.dt < 0 || (d.hdt != d.dt && d.hdt != GLA_F32) || k.scalar_type() != v.scalar_type() || q.scalar_type() != v.scalar_type()) return false;
+  if (packed && (cu.dim() != 1 || cu.numel() < 2 || cu.device() != v.device() || cu.scalar_type() != torch::kInt32)) return false;
+  d.per_token = g.dim() != 1;
+  if (d.per_token ? g.dim() != v.dim() - 1 || g.size(b) != d.T || g.size(b + 1) != d.H || (b && g.size(0) != d.B) : g.size(0) != d.H) return false;
+  if (g.is_complex()) return false;
+  const int hb = b || packed;
+  if (h.dim() != 3 + hb || (hb && h.size(0) != (packed ? d.nseq : d.B))) return false;
+  if (h.size(hb) != d.H || h.size(hb + 1) != d.Dk || h.size(hb + 2) != d.Dv) return false;
+  return d.B > 0 && d.H > 0 && d.Hk > 0 && d.H % d.Hk == 0 && d.Dk > 0 && d.Dv > 0;
+}
+std::string decay_text(const DecayDims& d) {
+  return "T=" + std::to_string(d.T) + " H=" + std::to_string(d.H) + " Hk=" + std::to_string(d.Hk) + " Dk=" + std::to_string(d.Dk) +
+         " Dv=" + std::to_string(d.Dv) + " (head sizes are multiples of 8 up to 256)";
+}
+struct DecayFn : torch::autograd::Function<DecayFn> {
+  static variable_list run(const DecayDims& d, const Tensor& h, const Tensor& g, const Tensor& v, const Tensor& k, const Tensor& q,
+                           const Tensor& cu, bool final32) {
+    Tensor hf = torch::empty_like(h), out = torch::empty_like(v), f32 = final32 ? torch::empty(h.sizes(), h.options().dtype(torch::kFloat32)) : Tensor();
+    const size_t n = gla_decay_workspace_bytes(d.B, d.T, d.H, d.Hk, d.Dk, d.Dv, d.dt, d.hdt, d.nseq, 0);
+    Tensor ws = bytes(v, n);
+    const int st = gla_decay_fwd(stream_of(v), d.B, d.T, d.H, d.Hk, d.Dk, d.Dv, d.dt, d.hdt, d.nseq, (const int32_t*)ptr(cu), ptr(h),
+                                 (const float*)ptr(g), d.per_token, ptr(v), ptr(k), ptr(q), ptr(hf), ptr(out), (float*)ptr(f32), ptr(ws), n);
+    if (st == GLA_ERR_UNSUPPORTED) raise("chunk_decay_attention: unsupported configuration " + decay_text(d));
+    check(st, "gla_decay_fwd");
+    return {hf, out, f32};
+  }
+  static variable_list forward(AutogradContext* ctx, const Tensor& h0, const Tensor& g0, const Tensor& v0, const Tensor& k0, const Tensor& q0,
+                               const Tensor& cu0, std::vector<int64_t> dims) {
+    const DecayDims d = DecayDims::of(dims);
+    const Tensor cu = d.nseq ? cu0 : Tensor();
+    Tensor h = h0.contiguous(), g = f32(g0), v = v0.contiguous(), k = k0.contiguous(), q = q0.contiguous();
+    const bool gate = g0.requires_grad();
+    variable_list r = run(d, h, g, v, k, q, cu, gate);
+    ctx->save_for_backward({h, g, v, k, q, r[2], cu});
+    ctx->set_materialize_grads(false);
+    dims.push_back(gate);
+    dims.push_back((int64_t)g0.scalar_type());
+    ctx->saved_data["d"] = dims;
+    return {r[0], r[1]};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto a = ctx->saved_data["d"].toIntVector();
+    const DecayDims d = DecayDims::of(a);
+    const variable_list s = ctx->get_saved_variables();
+    const Tensor &h = s[0], &g = s[1], &v = s[2], &k = s[3], &q = s[4], &cu = s[6];
+    const bool gate = a[10];
+    Tensor dhf = grad_or_zeros(grads[0], h), dout = grad_or_zeros(grads[1], v);
+    Tensor dh = torch::empty_like(h), dg = gate ? torch::empty_like(g) : Tensor(), dv = torch::empty_like(v), dk = torch::empty_like(k),
+           dq = torch::empty_like(q);
+    const size_t n = gla_decay_workspace_bytes(d.B, d.T, d.H, d.Hk, d.Dk, d.Dv, d.dt, d.hdt, d.nseq, gate ? 2 : 1);
+    Tensor ws = bytes(v, n);
+    check(gla_decay_bwd(stream_of(v), d.B, d.T, d.H, d.Hk, d.Dk, d.Dv, d.dt, d.hdt, d.nseq, (const int32_t*)ptr(cu), ptr(h), (const float*)ptr(g),
+                        d.per_token, ptr(v), ptr(k), ptr(q), (const float*)ptr(s[5]), ptr(dhf), ptr(dout), ptr(dh), (float*)ptr(dg), ptr(dv),
+                        ptr(dk), ptr(dq), ptr(ws), n), "gla_decay_bwd");
+    const auto gt = (torch::ScalarType)a[11];
+    return {dh, gate && gt != torch::kFloat32 ? dg.to(gt) : dg, dv, dk, dq, Tensor(), Tensor()};
+  }
+};
+std::optional<std::tuple<Tensor, Tensor>> chunk_decay(const Tensor& h, const Tensor& g0, const Tensor& v, const Tensor& k, const Tensor& q,
+                                                      const std::optional<Tensor>& cu0) {
+  DecayDims d;
+  Tensor cu = cu0.has_value() ? cu0->contiguous() : Tensor();
+  if (!decay_dims(h, g0, v, k, q, cu, d)) return std::nullopt;
+  no_forward_mode("chunk_decay_attention", {&h, &g0, &v, &k, &q});
+  // no tokens: the state goes through
+  if (d.T == 0) return std::make_tuple(h.clone(), torch::empty_like(v));
+  const bool grad = wants_grad({&h, &g0, &v, &k, &q});
+  Tensor g = g0;
+  if (grad && !d.per_token && g0.requires_grad()) {
+    // the gradient of a decay that every token has is the sum over the tokens
+    g = v.dim() == 4 ? g0.expand({d.B, d.T, d.H}) : g0.expand({d.T, d.H});
+    d.per_token = 1;
+  }
+  // (a node takes no undefined tensor)
+  variable_list r = grad ? DecayFn::apply(h, g, v, k, q, d.nseq ? cu : v.detach(), d.list())
+                         : DecayFn::run(d, h.contiguous(), f32(g), v.contiguous(), k.contiguous(), q.contiguous(), cu, false);
+  return std::make_tuple(r[0], r[1]);
+}
+
+// ---- beam search over recurrent states ---------------------------------------------------------------------------------
+// parents (requests, beams) of `rows` rows, as the library takes them; nullopt: not of that form
+std::optional<Tensor> parents_of(const std::optional<Tensor>& p, int64_t rows, const Tensor& like) {
+  if (!p.has_value()) return Tensor();
+  if (p->dim() != 2 || p->size(0) * p->size(1) != rows || p->device() != like.device()) return std::nullopt;
+  if (p->scalar_type() != torch::kInt32 && p->scalar_type() != torch::kInt64) return std::nullopt;
+  return p->to(torch::kInt32).contiguous();
+}
+std::optional<Tensor> decay_step(Tensor state, const Tensor& g, const Tensor& v, const Tensor& k, const Tensor& q,
+                                 std::optional<torch::ScalarType> out_dtype, const std::optional<Tensor>& parents0) {
+  if (!state.defined() || !here(state) || state.dim() != 4 || state.scalar_type() != torch::kFloat32 || !state.is_contiguous()) return std::nullopt;
+  const int64_t B = state.size(0), H = state.size(1), Dk = state.size(2), Dv = state.size(3);
+  if (v.dim() != 3 || v.size(0) != B || v.size(1) != H || v.size(2) != Dv || k.dim() != 3 || k.size(0) != B || k.size(2) != Dk || k.sizes() != q.sizes() ||
+      g.dim() != 2 || g.size(0) != B || g.size(1) != H || k.size(1) == 0 || H % k.size(1))
+    return std::nullopt;
+  for (const Tensor* t : {&g, &v, &k, &q}) if (t->device() != state.device()) return std::nullopt;
+  if (dt_of(v) < 0 || k.scalar_type() != v.scalar_type() || q.scalar_type() != v.scalar_type() || g.is_complex()) return std::nullopt;
+  const auto od = out_dtype.value_or(v.scalar_type());
+  if (od != torch::kFloat32 && od != torch::kBFloat16) return std::nullopt;
+  torch::NoGradGuard no_grad;
+  const auto par = parents_of(parents0, B, state);
+  if (!par.has_value()) return std::nullopt;
+  Tensor g32 = f32(g), vc = v.contiguous(), kc = k.contiguous(), qc = q.contiguous(), out = torch::empty({B, H, Dv}, v.options().dtype(od));
+  if (B == 0) return out;
+  check(gla_decay_step(stream_of(v), B, H, k.size(1), Dk, Dv, dt_of(v), (float*)ptr(state), (const float*)ptr(g32), ptr(vc), ptr(kc), ptr(qc),
+                       ptr(out), dt_of(out), (const int32_t*)ptr(*par), par->defined() ? par->size(1) : 1), "gla_decay_step");
+  return out;
+}
+bool reorder_states(const std::vector<Tensor>& states, const Tensor& parents) {
+  if (!parents.defined() || !here(parents) || parents.dim() != 2 || parents.numel() == 0) return false;
+  const auto par = parents_of(parents, parents.numel(), parents);
+  if (!par.has_value()) return false;
+  const int64_t rows = parents.numel();
+  std::vector<void*> p;
+  std::vector<int64_t> n;
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;
+  for (const Tensor& t : states) {
+    if (!t.defined() || t.device() != parents.device() || t.dim() < 1 || t.size(0) != rows || !t.is_contiguous()) return false;
+    if (t.requires_grad() && torch::GradMode::is_enabled()) return false;
+    if (t.numel() == 0) continue;
+    p.push_back(t.data_ptr());
+    n.push_back((int64_t)t.nbytes() / rows);
+    spans.emplace_back((uintptr_t)t.data_ptr(), (uintptr_t)t.data_ptr() + t.nbytes());
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i) if (spans[i].first < spans[i - 1].second) return false;
+  check(gla_reorder_states(stream_of(parents), (int64_t)p.size(), p.data(), n.data(), parents.size(0), parents.size(1), (const int32_t*)ptr(*par)),
+        "gla_reorder_states");
+  return true;
+}
+std::optional<std::tuple<Tensor, Tensor, Tensor>> beam_select(const Tensor& logits, const Tensor& scores, int64_t M, const std::optional<Tensor>& finished,
+                                                              int64_t pad) {
+  if (!logits.defined() || !here(logits) || logits.dim() != 3 || dt_of(logits) < 0) return std::nullopt;
+  const int64_t N = logits.size(0), K = logits.size(1), V = logits.size(2);
+  if (scores.dim() != 2 || scores.size(0) != N || scores.size(1) != K || scores.device() != logits.device() || !scores.is_floating_point()) return std::nullopt;
+  if (finished.has_value() && (finished->sizes() != scores.sizes() || finished->device() != logits.device() || finished->scalar_type() != torch::kBool))
+    return std::nullopt;
+  if (N < 1 || M < 1 || K < 1 || V < 1 || M > K * V || pad < 0 || pad >= V || K > 32 || M > 32) return std::nullopt;
+  torch::NoGradGuard no_grad;
+  Tensor x = logits.contiguous(), s = f32(scores), f = finished.has_value() ? finished->contiguous() : Tensor();
+  Tensor best = torch::empty({N, M}, s.options().requires_grad(false)), tokens = torch::empty({N, M}, best.options().dtype(torch::kInt64)),
+         parents = torch::empty({N, M}, best.options().dtype(torch::kInt32));
+  const size_t n = gla_beam_select_workspace_bytes(N, K, V, M, dt_of(x));
+  Tensor ws = bytes(x, n);
+  check(gla_beam_select(stream_of(x), N, K, V, M, dt_of(x), ptr(x), (const float*)ptr(s), (const unsigned char*)ptr(f), pad, (float*)ptr(best),
+                        tokens.data_ptr<int64_t>(), parents.data_ptr<int32_t>(), ptr(ws), n), "gla_beam_select");
+  return std::make_tuple(best, tokens, parents);
+}
+
 // ---- decode step ---------------------------------------------------------------------------------------------------
 std::optional<Tensor> decode_step(Tensor state, const Tensor& g, const Tensor& v, const Tensor& k, const Tensor& q,
-                                  std::optional<torch::ScalarType> out_dtype) {
+                                  std::optional<torch::ScalarType> out_dtype, const std::optional<Tensor>& parents0) {
   if (!state.defined() || !here(state) || state.dim() != 4 || state.scalar_type() != torch::kFloat32 || !state.is_contiguous()) return std::nullopt;
   const int64_t B = state.size(0), H = state.size(1), D = state.size(2);
   if (state.size(3) != D || v.dim() != 3 || v.size(0) != B || v.size(1) != H || v.size(2) != D) return std::nullopt;
@@ -302,7 +475,14 @@ std::optional<Tensor> decode_step(Tensor state, const Tensor& g, const Tensor& v
   const auto od = out_dtype.value_or(v.scalar_type());
   if (od != torch::kFloat32 && od != torch::kBFloat16) return std::nullopt;
   torch::NoGradGuard no_grad;
+  const auto par = parents_of(parents0, B, state);
+  if (!par.has_value()) return std::nullopt;
   Tensor g32 = f32(g), vc = v.contiguous(), kc = k.contiguous(), qc = q.contiguous(), out = torch::empty({B, H, D}, v.options().dtype(od));
+  if (par->defined()) {
+    check(gla_decode_step_beams(stream_of(v), B, H, D, dt_of(v), (float*)ptr(state), (const float*)ptr(g32), ptr(vc), ptr(kc), ptr(qc), ptr(out),
+                                dt_of(out), (const int32_t*)ptr(*par), par->size(1)), "gla_decode_step_beams");
+    return out;
+  }
   check(gla_decode_step(stream_of(v), B, H, D, dt_of(v), (float*)ptr(state), (const float*)ptr(g32), ptr(vc), ptr(kc), ptr(qc), ptr(out),
                         dt_of(out)), "gla_decode_step");
   return out;
@@ -503,6 +683,10 @@ PYBIND11_MODULE(gla_b200_host, m) {
   m.def("chunk_gla_packed", &chunk_gla_packed, release());
   m.def("gla_layer", &gla_layer, release());
   m.def("decode_step", &decode_step, release());
+  m.def("chunk_decay", &chunk_decay, release());
+  m.def("decay_step", &decay_step, release());
+  m.def("reorder_states", &reorder_states, release());
+  m.def("beam_select", &beam_select, release());
   m.def("scan", &scan, release());
   m.def("rnn", &rnn, release());
 }

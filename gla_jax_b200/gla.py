@@ -183,15 +183,30 @@ def chunk_gla_packed(hidden_init, log_fgate, value, key, query, cu_seqlens, chun
     raise TypeError("chunk_gla_packed: bfloat16 arrays, all on one device, are required")
 
 
-def decode_step(state, log_fgate, value, key, query, out_dtype=None):
+def _refuse_parents(what, parents, state):
+    """Raise the error for parents that are not (requests, beams) integers beside the rows of ``state``."""
+    if parents is None:
+        return
+    if parents.dim() != 2 or parents.numel() != state.shape[0]:
+        raise ValueError(f"{what}: parents must be (requests, beams) with requests * beams = {state.shape[0]}, got {tuple(parents.shape)}")
+    if parents.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"{what}: parents must be int32 or int64, got {parents.dtype}")
+    if parents.device != state.device:
+        raise ValueError(f"{what}: parents must be on {state.device}, got {parents.device}")
+
+
+def decode_step(state, log_fgate, value, key, query, out_dtype=None, parents=None):
     """One token of the recurrence (reference: the loop body of gla.py:26-47) for a batch of requests.
 
     ``state`` (B, H, D, D) float32 CUDA tensor is updated IN PLACE
     (``S <- exp(log_fgate)[..., None] * S + key[..., None] * value[..., None, :]``); returns
     ``out = query @ S`` of shape (B, H, D) in ``out_dtype`` (default: value's dtype).  ``log_fgate``,
     ``value``, ``key``, ``query`` are (B, H, D).  T calls equal one ``recurrent_gla`` over T tokens
-    (``hidden_init`` -> ``hidden_final`` chaining, gla.py:720-723).  Not differentiable (serving path)."""
-    out = _lib.native().decode_step(state, log_fgate, value, key, query, out_dtype)
+    (``hidden_init`` -> ``hidden_final`` chaining, gla.py:720-723).  Not differentiable (serving path).
+
+    ``parents`` (requests, beams), with ``B = requests * beams``: every row goes on from the state of the row of its
+    request that ``parents`` names (see ``beam.reorder_states``), in the same pass."""
+    out = _lib.native().decode_step(state, log_fgate, value, key, query, out_dtype, parents)
     if out is not None:
         return out
     if state.dtype != torch.float32 or not state.is_contiguous() or state.dim() != 4:
@@ -202,6 +217,7 @@ def decode_step(state, log_fgate, value, key, query, out_dtype=None):
         raise ValueError("decode_step: expected state (B, H, D, D) and log_fgate, value, key, query (B, H, D)")
     if key.dtype != value.dtype or query.dtype != value.dtype or value.dtype not in _DT or (out_dtype or value.dtype) not in _DT:
         raise TypeError("decode_step: value, key, query must share a dtype, float32 or bfloat16")
+    _refuse_parents("decode_step", parents, state)
     _stream(value.device)
     raise RuntimeError("decode_step needs CUDA tensors on one device; there is no CPU fallback")
 

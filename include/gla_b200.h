@@ -134,6 +134,10 @@ GLA_API unsigned int gla_device_wait_timeouts(void);
  * array seen so far was valid.  No counterpart in the reference. */
 GLA_API unsigned int gla_device_bad_offsets(void);
 
+/* The same for the parents of gla_decay_step, gla_decode_step_beams and gla_reorder_states: the number of entries outside
+ * [0, beams) since the library was loaded, each of which was taken as the nearest beam there is. */
+GLA_API unsigned int gla_device_bad_parents(void);
+
 /* Per-kernel device timing for benchmarks (diagnostic; no counterpart in the reference, whose
  * harness times whole calls with timeit, gla.py:1430-1434).  While enabled on the calling
  * thread, each internal kernel launch is bracketed by CUDA events on its stream;
@@ -500,6 +504,72 @@ GLA_API int gla_sp_combine(void* stream, int64_t R, int64_t rank, int64_t BH, in
 GLA_API int gla_sp_combine2(void* stream, int64_t R, int64_t rank, int64_t BH, int64_t D,
                     const float* all_G, int64_t g_rank_stride, const float* all_S, int64_t s_rank_stride,
                     const void* init, int init_dtype, float* entering, void* total, int total_dtype, int reverse);
+
+/* ------------------------------------------------------------------------------------
+ * attention with one decay per head - the sibling of chunk_gla whose gate is a number per token and head (or per head)
+ * instead of one per key feature; no counterpart in the reference.
+ *     S_t = exp(g_t) S_{t-1} + key_t (x) value_t        out_t = query_t S_t
+ *   value, out (B, T, H, Dv); key, query (B, T, Hk, Dk), head h using key/query head h / (H / Hk); hidden (B, H, Dk, Dv)
+ *   log_decay (B, T, H) float32 with per_token != 0, else (H) float32.  -inf resets the state.
+ *   nseq > 0: packed.  B = 1; the axis of T tokens holds nseq sequences, sequence s the tokens [cu_seqlens[s],
+ *   cu_seqlens[s + 1]) (DEVICE, int32, rising from 0, any length, 0 included); hidden is (nseq, H, Dk, Dv).  Tokens behind the last
+ *   sequence give zeros.  Offsets that fall or leave [0, T] are held inside and counted (gla_device_bad_offsets).
+ * Dk and Dv multiples of 8 up to 256; any T > 0; H a multiple of Hk.  `dtype` is that of value, key, query, out and their
+ * gradients; hidden_dtype that of hidden_init, hidden_final and their gradients: dtype or GLA_F32.  value, key, query, out and
+ * gradients 16-byte aligned.  final32, if not NULL, receives the final state in float32, which the backward needs
+ * for dlog_decay (in layout (B or nseq, H, Dk, Dv)).
+ * bf16 forward: scores, the state as an operand and decayed values are rounded to bf16 once (the state from three
+ * bf16 planes of the values where it leaves in float32); sums, states and decays in float32 and more.
+ * bf16 backward: the same operands in two planes.  float32: three planes everywhere.
+ * Backward: dlog_decay (B, T, H) float32 or NULL; dhidden_init as hidden_init.
+ * Workspace: gla_decay_workspace_bytes with backward = 0 (forward), 1 (backward without dlog_decay), 2 (with it); 0 bytes
+ * may be needed, or the sizes may be unsupported (the calls say which).
+ * ---------------------------------------------------------------------------------- */
+GLA_API size_t gla_decay_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype,
+                             int hidden_dtype, int64_t nseq, int backward);
+GLA_API int gla_decay_fwd(void* stream, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype,
+                      int hidden_dtype, int64_t nseq, const int32_t* cu_seqlens,
+                      const void* hidden_init, const float* log_decay, int per_token,
+                      const void* value, const void* key, const void* query,
+                      void* hidden_final, void* out, float* final32, void* workspace, size_t workspace_bytes);
+GLA_API int gla_decay_bwd(void* stream, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype,
+                      int hidden_dtype, int64_t nseq, const int32_t* cu_seqlens,
+                      const void* hidden_init, const float* log_decay, int per_token,
+                      const void* value, const void* key, const void* query, const float* final32,
+                      const void* dhidden_final, const void* dout,
+                      void* dhidden_init, float* dlog_decay, void* dvalue, void* dkey, void* dquery,
+                      void* workspace, size_t workspace_bytes);
+
+/* ------------------------------------------------------------------------------------
+ * Beam search over recurrent states (no counterpart in the reference).  What a beam carries is its state: rows of a state
+ * tensor are (request, beam), and `parents` (requests, beams) int32 on the device names for each beam the beam of its
+ * request that it goes on from (several may have the same one).  Up to 32 beams.
+ *   gla_decay_step         one token of the recurrence above, state (B, H, Dk, Dv) float32 in place (16-byte aligned), log_decay (B, H)
+ *                          float32, value (B, H, Dv), key and query (B, Hk, Dk), out (B, H, Dv) in out_dtype.  With parents
+ *                          (B = requests * beams) every row is stepped from its parent's state; the moves cost no pass.
+ *   gla_decode_step_beams  gla_decode_step (a decay per key feature) with parents.
+ *   gla_reorder_states     rows of `count` tensors (HOST arrays of device addresses and of bytes per row) moved to where
+ *                          the parents say, in place; rows that stay are not touched.  The tensors must not overlap.
+ *   gla_beam_select        logits (N, K, V) in dtype, scores (N, K) float32 (finite or -inf): the M best of each request's K V
+ *                          totals scores[k] + log_softmax(logits[k])[v], largest first, the lowest (k, v) first among equal
+ *                          ones; totals in 64 bits.  A logit of -inf or NaN is masked (a row of them has no continuation:
+ *                          totals of -inf), +inf counts as the largest finite number.  A beam with a score of -inf or NaN has totals of
+ *                          -inf.  finished (N, K) bytes or NULL: such a beam continues with pad_token alone, at its score,
+ *                          and its logits are not read.  out_scores (N, M) float32, tokens (N, M), parents (N, M).  K, M <= 32,
+ *                          M <= K V, V <= 2^30.
+ * ---------------------------------------------------------------------------------- */
+GLA_API int gla_decay_step(void* stream, int64_t B, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype,
+                   float* state, const float* log_decay, const void* value, const void* key, const void* query,
+                   void* out, int out_dtype, const int32_t* parents, int64_t beams);
+GLA_API int gla_decode_step_beams(void* stream, int64_t B, int64_t H, int64_t D, int dtype,
+                   float* state, const float* log_fgate, const void* value, const void* key, const void* query,
+                   void* out, int out_dtype, const int32_t* parents, int64_t beams);
+GLA_API int gla_reorder_states(void* stream, int64_t count, void* const* tensors, const int64_t* row_bytes,
+                   int64_t requests, int64_t beams, const int32_t* parents);
+GLA_API size_t gla_beam_select_workspace_bytes(int64_t N, int64_t K, int64_t V, int64_t M, int dtype);
+GLA_API int gla_beam_select(void* stream, int64_t N, int64_t K, int64_t V, int64_t M, int dtype,
+                   const void* logits, const float* scores, const unsigned char* finished, int64_t pad_token,
+                   float* out_scores, int64_t* tokens, int32_t* parents, void* workspace, size_t workspace_bytes);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,250 @@
+"""Beam search over recurrent states: selection, moving of states, steps that follow parents, and a whole search."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def selected(logits, scores, M, finished=None, pad=0):
+    """The definition in 64 bits: a stable sort of all totals."""
+    x = logits.double().nan_to_num(nan=-math.inf, posinf=3.4028234663852886e38, neginf=-math.inf)
+    top = x.amax(-1, keepdim=True)
+    # (rows padded to one alignment: torch's sum of a row goes by its address, and equal rows have to have equal sums)
+    e = torch.nn.functional.pad((x - top).exp(), (0, -x.shape[-1] % 64))
+    p = (x - top) - e.sum(-1, keepdim=True).log()
+    p = torch.where(top > -math.inf, p, torch.full_like(p, -math.inf))
+    if finished is not None:
+        only = torch.full_like(p, -math.inf)
+        only[..., pad] = 0.0
+        p = torch.where(finished[..., None], only, p)
+    total = (scores.double()[..., None] + p).nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf).flatten(1)
+    best, at = total.sort(dim=1, descending=True, stable=True)
+    V = logits.shape[-1]
+    return best[:, :M], at[:, :M] % V, at[:, :M] // V
+
+
+def same(got, want):
+    scores, tokens, parents = got
+    assert torch.equal(tokens, want[1]) and torch.equal(parents.long(), want[2])
+    fin = torch.isfinite(want[0])
+    assert torch.equal(torch.isfinite(scores), fin)
+    # the total rounded once, and a logarithm of a float32 sum of exponentials: 2^-24 of the total and 2^-20
+    assert ((scores.double() - want[0])[fin].abs() <= 2.0 ** -24 * want[0][fin].abs() + 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,K,V,M", [(1, 1, 1, 1), (2, 3, 2, 6), (3, 4, 17, 8), (2, 5, 4095, 5), (1, 4, 4097, 32), (3, 2, 33333, 4),
+                                     (2, 32, 1000, 32), (1, 8, 100003, 16), (70, 2, 777, 4)])
+def test_selection(cuda_device, N, K, V, M, dtype):
+    from gla_jax_b200 import beam_select
+    gen = torch.Generator(device=cuda_device).manual_seed(N * V + M)
+    logits = (3 * torch.randn(N, K, V, generator=gen, device=cuda_device)).to(dtype)
+    scores = -10 * torch.rand(N, K, generator=gen, device=cuda_device)
+    same(beam_select(logits, scores, M), selected(logits, scores, M))
+    if K > 1 and V > 2:
+        fin = torch.rand(N, K, generator=gen, device=cuda_device) < 0.5
+        same(beam_select(logits, scores, M, finished=fin, pad_token=2), selected(logits, scores, M, fin, 2))
+        scores[:, 1:] = -math.inf                                    # the first token of a search
+        same(beam_select(logits, scores, M), selected(logits, scores, M))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_selection_of_ties_masks_and_odd_values(cuda_device, dtype):
+    from gla_jax_b200 import beam_select
+    N, K, V, M = 2, 3, 9001, 12
+    z = torch.zeros(N, K, V, device=cuda_device, dtype=dtype)
+    s = torch.zeros(N, K, device=cuda_device)
+    low = torch.finfo(dtype).min
+    ramp = torch.arange(V, device=cuda_device, dtype=torch.float32).to(dtype).expand(N, K, V).contiguous()
+    late = torch.full_like(z, -math.inf)
+    late[..., 5000:] = 1.0
+    one = torch.full_like(z, -math.inf)
+    one[:, 1, 77] = 3.0
+    lowest = torch.full_like(z, low)
+    lowest[..., 8000] = 0
+    odd = torch.randn(N, K, V, device=cuda_device).to(dtype)
+    odd[0, 0, 5], odd[0, 1, 3], odd[1, 2, 8999], odd[1, 0] = math.nan, math.inf, math.inf, math.nan
+    steps = (torch.randn(N, K, V, device=cuda_device) * 2).round().to(dtype)                # many equal logits
+    sign = z.clone()
+    sign[..., ::2] = -0.0
+    for x in (z, ramp, ramp.flip(-1), late, one, lowest, odd, steps, sign, torch.full_like(z, -math.inf), torch.full_like(z, math.nan)):
+        for m in (1, M, 32):
+            same(beam_select(x, s, m), selected(x, s, m))
+    s2 = torch.tensor([[0.0, -math.inf, math.nan], [-math.inf] * 3], device=cuda_device)
+    want = selected(steps, s2.nan_to_num(nan=-math.inf, neginf=-math.inf), M)
+    same(beam_select(steps, s2, M), want)
+    # rows that start anywhere
+    big = torch.randn(N * K * V + 3, device=cuda_device).to(dtype)
+    for off in (1, 3):
+        x = big[off:off + N * K * V].view(N, K, V)
+        same(beam_select(x, s, M), selected(x, s, M))
+
+
+@pytest.mark.parametrize("N,K", [(1, 1), (3, 4), (2, 32), (5, 7)])
+def test_reorder(cuda_device, N, K):
+    from gla_jax_b200 import reorder_states
+    gen = torch.Generator(device=cuda_device).manual_seed(K)
+    for parents in (torch.randint(0, K, (N, K), generator=gen, device=cuda_device), torch.arange(K, device=cuda_device).roll(1).expand(N, K).contiguous(),
+                    torch.arange(K, device=cuda_device).expand(N, K), torch.full((N, K), K - 1, device=cuda_device)):
+        row = (torch.arange(N, device=cuda_device)[:, None] * K + parents).flatten()
+        states = [torch.randn(N * K, 2, 64, 64, device=cuda_device), torch.randn(N * K, 3, 5, device=cuda_device).bfloat16(),
+                  torch.randint(0, 9, (N * K, 7), device=cuda_device), torch.randint(0, 2, (N * K,), device=cuda_device).bool(),
+                  torch.randn(N * K + 1, 5, device=cuda_device)[1:], torch.randn(N * K, 0, device=cuda_device)]
+        states += [torch.randn(N * K, 33 + i, device=cuda_device) for i in range(70)]       # more than a launch takes
+        want = [s[row] for s in states]
+        reorder_states(states, parents.to(torch.int32))
+        for a, b in zip(states, want):
+            assert torch.equal(a, b)
+    one = torch.randn(N * K, 12, device=cuda_device)
+    want = one[row]
+    reorder_states(one, parents)                                                            # int64
+    assert torch.equal(one, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("N,K,H,Hk,Dk,Dv", [(3, 1, 2, 2, 64, 64), (2, 4, 4, 2, 128, 64), (1, 5, 2, 1, 80, 96), (2, 8, 2, 2, 128, 128),
+                                            (1, 32, 1, 1, 256, 40), (1, 16, 2, 2, 256, 256)])
+def test_steps_follow_parents(cuda_device, N, K, H, Hk, Dk, Dv, dtype):
+    from gla_jax_b200 import decay_attention_step, decode_step
+    gen = torch.Generator(device=cuda_device).manual_seed(Dk + K)
+    n = lambda *s: torch.randn(*s, generator=gen, device=cuda_device)  # noqa: E731
+    B = N * K
+    parents = torch.randint(0, K, (N, K), generator=gen, device=cuda_device, dtype=torch.int32)
+    row = (torch.arange(N, device=cuda_device)[:, None] * K + parents).flatten()
+    state, g = n(B, H, Dk, Dv), -n(B, H).abs()
+    v, k, q = n(B, H, Dv).to(dtype), n(B, Hk, Dk).to(dtype), n(B, Hk, Dk).to(dtype)
+    a, b = state.clone(), state[row].contiguous()
+    o1 = decay_attention_step(a, g, v, k, q, parents=parents)
+    o2 = decay_attention_step(b, g, v, k, q)
+    assert torch.equal(a, b)
+    # the sums over features are added in another order: 16 additions of Dk terms
+    unit = (q.float().abs().repeat_interleave(H // Hk, 1)[..., None] * b.abs()).sum(-2)
+    tol = 2.0 ** -19 + (2.0 ** -7 if dtype == torch.bfloat16 else 0)
+    assert ((o1.float() - o2.float()).abs() <= tol * unit).all()
+    if Dk == Dv and Hk == H:
+        f = -n(B, H, Dk).abs()
+        a, b = state.clone(), state[row].contiguous()
+        o1, o2 = decode_step(a, f, v, k, q, parents=parents), decode_step(b, f, v, k, q)
+        assert torch.equal(a, b) and ((o1.float() - o2.float()).abs() <= tol * (q.float().abs()[..., None] * b.abs()).sum(-2)).all()
+
+
+def test_bad_parents_are_reported(cuda_device):
+    from gla_jax_b200 import check_device, decay_attention_step, reorder_states
+    from gla_jax_b200._lib import GlaError
+    check_device()
+    bad = torch.tensor([[0, 7], [-4, 1]], dtype=torch.int32, device=cuda_device)
+    x = torch.randn(4, 2, 64, 64, device=cuda_device)
+    want = x[torch.tensor([0, 1, 2, 3], device=cuda_device)].clone()
+    reorder_states(x, bad)                                       # held inside: 7 is 1, -4 is 0
+    assert torch.equal(x, want)
+    with pytest.raises(GlaError, match="2 parent"):
+        check_device()
+    z = torch.zeros(4, 2, 64, device=cuda_device)
+    decay_attention_step(x, torch.zeros(4, 2, device=cuda_device), z, z, z, parents=bad)
+    assert torch.equal(x, want)
+    with pytest.raises(GlaError, match="2 parent"):
+        check_device()
+    check_device()
+
+
+def test_a_search(cuda_device):
+    """A prompt, its state given to all beams, and ten tokens of search, against the same in 64 bits."""
+    from gla_jax_b200 import beam_select, chunk_decay_attention, decay_attention_step, reorder_states
+    gen = torch.Generator(device=cuda_device).manual_seed(5)
+    n = lambda *s: torch.randn(*s, generator=gen, device=cuda_device)  # noqa: E731
+    N, K, H, D, V, T, steps, eos = 2, 4, 2, 32, 61, 19, 10, 3
+    emb, wo = n(V, H, 3, D) * 0.5, n(H * D, V) * 0.6
+    g = torch.tensor([-0.1, -0.6], device=cuda_device)
+    prompt = torch.randint(4, V, (N, T), generator=gen, device=cuda_device)
+    x = emb[prompt]
+    h0 = torch.zeros(N, H, D, D, device=cuda_device)
+    state, out = chunk_decay_attention(h0, g, *(x[:, :, :, i] for i in range(3)))
+    state64 = torch.zeros(N, H, D, D, device=cuda_device, dtype=torch.float64)
+    for t in range(T):
+        state64 = g.double().exp()[:, None, None] * state64 + x[:, t, :, 1, :, None].double() * x[:, t, :, 0, None, :].double()
+    state, state64 = state.repeat_interleave(K, 0), state64.repeat_interleave(K, 0)
+    history = torch.zeros(N * K, steps, dtype=torch.int64, device=cuda_device)
+    history64 = history.clone()
+    scores = torch.full((N, K), -math.inf, device=cuda_device)
+    scores[:, 0] = 0
+    scores64, tokens64 = scores.double(), None
+    tokens = prompt[:, -1:].expand(N, K)
+    tokens64 = tokens
+    parents = torch.arange(K, device=cuda_device, dtype=torch.int32).expand(N, K).contiguous()
+    parents64 = parents.long()
+    finished = finished64 = torch.zeros(N, K, dtype=torch.bool, device=cuda_device)
+    base = torch.arange(N, device=cuda_device)[:, None] * K
+    for t in range(steps):
+        e = emb[tokens.flatten()]
+        out = decay_attention_step(state, g.expand(N * K, H), e[:, :, 0], e[:, :, 1], e[:, :, 2], parents=parents)
+        scores, tokens, parents = beam_select((out.flatten(1) @ wo).view(N, K, V), scores, finished=finished, pad_token=eos)
+        finished = finished.gather(1, parents.long()) | (tokens == eos)
+        reorder_states(history, parents)
+        history[:, t] = tokens.flatten()
+        e = emb[tokens64.flatten()].double()
+        state64 = state64[(base + parents64).flatten()]
+        state64 = g.double().exp()[:, None, None] * state64 + e[:, :, 1, :, None] * e[:, :, 0, None, :]
+        o = (e[:, :, 2, :, None] * state64).sum(-2)
+        scores64, tokens64, parents64 = selected((o.flatten(1) @ wo.double()).view(N, K, V), scores64, K, finished64, eos)
+        finished64 = finished64.gather(1, parents64) | (tokens64 == eos)
+        history64 = history64[(base + parents64).flatten()]
+        history64[:, t] = tokens64.flatten()
+    assert torch.equal(history, history64)
+    torch.testing.assert_close(scores.double(), scores64, rtol=1e-4, atol=1e-4)
+
+
+def test_in_a_graph(cuda_device):
+    from gla_jax_b200 import beam_select, decay_attention_step, reorder_states
+    N, K, V = 2, 4, 5000
+    logits, scores = torch.randn(N, K, V, device=cuda_device), torch.randn(N, K, device=cuda_device)
+    state, extra = torch.randn(N * K, 2, 64, 64, device=cuda_device), torch.randn(N * K, 40, device=cuda_device)
+    x = torch.randn(N * K, 2, 64, device=cuda_device)
+
+    def once():
+        s, t, p = beam_select(logits, scores)
+        reorder_states([extra], p)
+        return s, t, p, decay_attention_step(state, x[..., 0], x, x, x, parents=p)
+
+    once()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = once()
+    logits.copy_(torch.randn_like(logits))
+    a, b = state.clone(), extra.clone()
+    graph.replay()
+    s1, e1, g1 = state.clone(), extra.clone(), [y.clone() for y in got]
+    state.copy_(a)
+    extra.copy_(b)
+    for y, z in zip(once(), g1):
+        assert torch.equal(y, z)
+    assert torch.equal(state, s1) and torch.equal(extra, e1)
+
+
+def test_refusals(cuda_device):
+    from gla_jax_b200 import beam_select, reorder_states
+    x, s = torch.randn(2, 3, 10, device=cuda_device), torch.randn(2, 3, device=cuda_device)
+    for bad in (dict(num_select=0), dict(num_select=33), dict(pad_token=10), dict(finished=torch.zeros(2, 3, device=cuda_device)),
+                dict(finished=torch.zeros(2, 2, dtype=torch.bool, device=cuda_device))):
+        with pytest.raises(ValueError):
+            beam_select(x, s, **bad)
+    with pytest.raises(ValueError):
+        beam_select(x, s[:1])
+    with pytest.raises(TypeError):
+        beam_select(x.half(), s)
+    with pytest.raises(ValueError):
+        beam_select(torch.randn(1, 33, 10, device=cuda_device), torch.randn(1, 33, device=cuda_device))
+    p = torch.zeros(2, 3, dtype=torch.int32, device=cuda_device)
+    y = torch.randn(6, 8, device=cuda_device)
+    with pytest.raises(ValueError, match="overlap"):
+        reorder_states([y, y], p)
+    with pytest.raises(ValueError, match="rows"):
+        reorder_states([y[:5]], p)
+    with pytest.raises(ValueError, match="contiguous"):
+        reorder_states([y.t()[:6]], p)
+    with pytest.raises(TypeError):
+        reorder_states([y], p.float())
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        reorder_states([y.clone().requires_grad_(True)], p)
