@@ -120,6 +120,7 @@ SIGNATURES = {
     "gla_sp_combine2": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64,
                                 c_void_p, c_int, c_void_p, c_void_p, c_int, c_int]),
     "gla_decay_workspace_bytes": (c_size_t, [c_int64] * 6 + [c_int, c_int, c_int64, c_int]),
+    "gla_decay_saved_bytes": (c_size_t, [c_int64] * 6 + [c_int, c_int, c_int64]),
     "gla_decay_fwd": (c_int, [c_void_p] + [c_int64] * 6 + [c_int, c_int, c_int64] + [c_void_p] * 3 + [c_int] + [c_void_p] * 7 + [c_size_t]),
     "gla_decay_bwd": (c_int, [c_void_p] + [c_int64] * 6 + [c_int, c_int, c_int64] + [c_void_p] * 3 + [c_int] + [c_void_p] * 12 + [c_size_t]),
     "gla_decay_step": (c_int, [c_void_p] + [c_int64] * 5 + [c_int] + [c_void_p] * 6 + [c_int, c_void_p, c_int64]),

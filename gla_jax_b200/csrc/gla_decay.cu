@@ -1,27 +1,36 @@
 // Linear attention with one decay per head: what runs around the walks of gla_decay.cuh (runs of a sequence and their
 // states, sums over shared heads, the gradient of the decays), forward and backward.
-#include "gla_decay.cuh"
+#include "gla_decay_bf16.cuh"
 
 namespace gla {
 namespace decay {
 namespace {
 
-// The state that enters each run of a sequence, from what each run adds: element by element, in place.
-__global__ void __launch_bounds__(256) entering_kernel(const Walk p) {
-  const int64_t s = blockIdx.z, h = blockIdx.y, e = blockIdx.x * 256ll + threadIdx.x, dd = (int64_t)p.kd * p.vd;
+// The state that enters each run of a sequence, from what each run adds: element by element, in place.  Eight runs' sums
+// are requested before the first is used.
+__global__ void __launch_bounds__(128) entering_kernel(const Walk p) {
+  const int64_t s = blockIdx.z, h = blockIdx.y, e = blockIdx.x * 128ll + threadIdx.x, dd = (int64_t)p.kd * p.vd;
   if (e >= dd) return;
   const int64_t c = e / p.kd, k = e % p.kd;
-  float x = ld_any(p.init, !p.init_f32, (s * p.H + h) * dd + k * p.ik + c * p.ic);
   int64_t n = 1;
-  slot_of(p, s, 0, n);
-  for (int64_t i = 0; i < n; ++i) {
-    const int64_t at = slot_of(p, s, p.rev ? n - 1 - i : i, n) * p.H + h;
-    if (at / p.H >= p.nslots) return;
-    float* u = p.seg_state + at * dd + e;
-    const bool more = i + 1 < n;
-    const float add = more ? *u : 0.f;
-    *u = x;
-    if (more) x = fmaf((float)exp2(p.seg_total[at]), x, add);
+  const int64_t s0 = slot_of(p, s, 0, n);
+  if (s0 + n > p.nslots) return;
+  float x = ld_any(p.init, !p.init_f32, (s * p.H + h) * dd + k * p.ik + c * p.ic);
+  for (int64_t i0 = 0; i0 < n; i0 += 8) {
+    float add[8], f[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j + 1 < n) {
+        const int64_t at = (s0 + (p.rev ? n - 1 - i0 - j : i0 + j)) * p.H + h;
+        add[j] = p.seg_state[at * dd + e];
+        f[j] = exp2f((float)p.seg_total[at]);
+      }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i0 + j < n) {
+        p.seg_state[((s0 + (p.rev ? n - 1 - i0 - j : i0 + j)) * p.H + h) * dd + e] = x;
+        if (i0 + j + 1 < n) x = fmaf(f[j], x, add[j]);
+      }
   }
 }
 
@@ -157,21 +166,115 @@ static int run_walk(cudaStream_t st, const Dims& d, int mode, Walk p, void* ws, 
     p.seg_total = (double*)((char*)ws + align_up((size_t)(p.nslots * d.H * d.Dk * d.Dv) * 4, 256));
     GLA_TRY(walk(st, mode, p, false, first));
     ProfScope ps("decay_entering_kernel", st);
-    entering_kernel<<<dim3((unsigned)((d.Dk * d.Dv + 255) / 256), (unsigned)d.H, (unsigned)p.nseq), 256, 0, st>>>(p);
+    entering_kernel<<<dim3((unsigned)((d.Dk * d.Dv + 127) / 128), (unsigned)d.H, (unsigned)p.nseq), 128, 0, st>>>(p);
     GLA_CHECK_LAUNCH();
   }
   return walk(st, mode, p, true, name);
 }
 
-size_t fwd_ws_bytes(const Dims& d) { return d.seg_bytes(d.Dv); }
+// ---- bf16, head sizes up to 128: the walks of gla_decay_bf16.cuh ---------------------------------------------------------
+static bool fast(const Dims& d) { return d.bf && d.Dk <= 128 && d.Dv <= 128; }
+static size_t state_bytes(const Dims& d, int64_t n) { return align_up((size_t)(n * d.H * d.Dk * d.Dv) * 4, 256); }
+// saved: final states in float32 | states that enter the runs (where sequences are cut)
+size_t saved_bytes(const Dims& d) {
+  return state_bytes(d, d.seqs()) + (fast(d) && d.cut(d.seg(128)) ? state_bytes(d, d.slots(d.seg(128))) : 0);
+}
+static size_t fast_totals(const Dims& d) { return align_up((size_t)(d.slots(d.seg(128)) * d.H) * 8, 256); }
+static Walk fast_base(const Dims& d, const int* cu, const float* g, int64_t gt) {
+  Walk p{};
+  p.H = (int)d.H; p.T = d.T; p.nseq = d.seqs(); p.seg = d.seg(128); p.nslots = d.slots(p.seg);
+  p.g = g; p.gt = gt; p.cu = cu;
+  p.init_f32 = p.fin_f32 = d.hid_f32;
+  return p;
+}
+static int entering(cudaStream_t st, const Walk& p) {
+  ProfScope ps("decay_entering_kernel", st);
+  entering_kernel<<<dim3((unsigned)(((int64_t)p.kd * p.vd + 127) / 128), (unsigned)p.H, (unsigned)p.nseq), 128, 0, st>>>(p);
+  GLA_CHECK_LAUNCH();
+  return GLA_OK;
+}
+static int fast_fwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const float* g, int64_t gt, const void* v, const void* k,
+                    const void* q, void* hf, void* out, void* saved, void* ws) {
+  Walk p = fast_base(d, cu, g, gt);
+  p.q = q; p.k = k; p.v = v;
+  p.gq = p.gk = (int)(d.H / d.Hk); p.gv = 1;
+  p.kd = (int)d.Dk; p.vd = (int)d.Dv;
+  p.init = h0; p.ik = d.Dv; p.ic = 1;
+  p.count_bad = cu != nullptr;
+  if (d.cut(p.seg)) {
+    p.seg_total = (double*)ws;
+    p.seg_state = (float*)(saved ? (char*)saved + state_bytes(d, d.seqs()) : (char*)ws + fast_totals(d));
+    GLA_TRY(fast_walk(st, p, d.hid_f32 ? F_SUMS_STATE : F_SUMS, "decay_runs_kernel"));
+    GLA_TRY(entering(st, p));
+  }
+  p.sk = 1; p.sc = d.Dk;
+  p.fin = hf; p.fin32 = (float*)saved;
+  p.out = out;
+  return fast_walk(st, p, d.hid_f32 ? F_STATE : F_ONE, "decay_walk_kernel");
+}
+static int share_sum(cudaStream_t st, const Dims& d, const float* x, void* out);
+static size_t fast_bwd_parts(const Dims& d, bool gate, size_t (&at)[4]) {
+  const int64_t s = d.seg(128);
+  at[0] = d.cut(s) ? fast_totals(d) : 0;
+  at[1] = at[0] + (d.cut(s) ? state_bytes(d, d.slots(s)) : 0);
+  at[2] = at[1] + (gate ? align_up((size_t)(d.rows() * d.H) * 4, 256) : 0);
+  at[3] = at[2] + (d.H > d.Hk ? align_up((size_t)(d.rows() * d.H * d.Dk) * 4, 256) : 0);
+  return at[3];
+}
+static int fast_bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const float* g, int64_t gt, const void* v, const void* k,
+                    const void* q, const void* saved, const void* dhf, const void* dout, void* dh, float* dg, void* dv, void* dk, void* dq,
+                    void* ws) {
+  size_t at[4];
+  fast_bwd_parts(d, dg != nullptr, at);
+  const int share = (int)(d.H / d.Hk);
+  float *a = (float*)((char*)ws + at[1]), *wide = (float*)((char*)ws + at[2]);
+  Walk p = fast_base(d, cu, g, gt);
+  const bool cut = d.cut(p.seg);
+  float* runs = cut ? (float*)((char*)saved + state_bytes(d, d.seqs())) : nullptr;
+  // dq: the forward's walk with roles exchanged, over the forward's states
+  p.q = dout; p.k = v; p.v = k; p.gq = p.gk = 1; p.gv = share; p.kd = (int)d.Dv; p.vd = (int)d.Dk;
+  p.init = h0; p.ik = 1; p.ic = d.Dv;
+  p.seg_state = runs; p.sk = d.Dk; p.sc = 1;
+  p.out = share > 1 ? (void*)wide : dq; p.out_f32 = share > 1;
+  p.r = dg ? q : nullptr; p.gr = share; p.rdot = a;
+  GLA_TRY(fast_walk(st, p, dg ? F_FINE : F_ONE, "decay_dq_kernel"));
+  if (share > 1) GLA_TRY(share_sum(st, d, wide, dq));
+  // the rest, backwards
+  Back b{};
+  b.w = fast_base(d, cu, g, gt);
+  b.w.rev = 1;
+  b.w.kd = (int)d.Dk; b.w.vd = (int)d.Dv;
+  b.w.init = dhf; b.w.ik = d.Dv; b.w.ic = 1;
+  if (cut) {
+    b.w.seg_total = (double*)ws;
+    b.w.seg_state = (float*)((char*)ws + at[0]);
+    Walk r = b.w;
+    r.k = q; r.v = dout; r.gk = share; r.gv = 1; r.gq = 1;
+    GLA_TRY(fast_walk(st, r, F_SUMS, "decay_runs_kernel"));
+    GLA_TRY(entering(st, r));
+  }
+  b.w.q = q; b.w.k = k; b.w.v = v; b.w.gq = b.w.gk = share; b.w.gv = 1;
+  b.w.fin = dh;
+  b.dout = dout; b.a = a; b.S_runs = runs; b.S_end = (const float*)saved;
+  b.dk = share > 1 ? (void*)wide : dk; b.dk_f32 = share > 1; b.dv = dv; b.dg = dg;
+  GLA_TRY(fast_back(st, b, dg != nullptr));
+  return share > 1 ? share_sum(st, d, wide, dk) : GLA_OK;
+}
+
+size_t fwd_ws_bytes(const Dims& d, bool saved) {
+  if (!fast(d)) return d.seg_bytes(d.Dv);
+  const int64_t s = d.seg(128);
+  return d.cut(s) ? fast_totals(d) + (saved ? 0 : state_bytes(d, d.slots(s))) : 0;
+}
 int fwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const float* g, int64_t gt, const void* v, const void* k,
-        const void* q, void* hf, void* out, float* fin32, void* ws) {
+        const void* q, void* hf, void* out, void* saved, void* ws) {
+  if (fast(d)) return fast_fwd(st, d, cu, h0, g, gt, v, k, q, hf, out, saved, ws);
   Walk p{};
   p.q = q; p.k = k; p.v = v;
   p.gq = p.gk = (int)(d.H / d.Hk); p.gv = 1;
   p.kd = (int)d.Dk; p.vd = (int)d.Dv;
   p.g = g; p.gt = gt; p.cu = cu; p.count_bad = cu != nullptr;
-  p.init = h0; p.fin = hf; p.fin32 = fin32; p.ik = d.Dv; p.ic = 1; p.init_f32 = p.fin_f32 = d.hid_f32;
+  p.init = h0; p.fin = hf; p.fin32 = (float*)saved; p.ik = d.Dv; p.ic = 1; p.init_f32 = p.fin_f32 = d.hid_f32;
   p.out = out; p.out_f32 = !d.bf;
   return run_walk(st, d, !d.bf ? M_FULL : d.hid_f32 ? M_STATE : M_ONE, p, ws, "decay_runs_kernel", "decay_walk_kernel");
 }
@@ -187,8 +290,8 @@ static size_t bwd_parts(const Dims& d, bool gate, size_t (&at)[5]) {
   return at[3];
 }
 size_t bwd_ws_bytes(const Dims& d, bool gate) {
-  size_t at[5];
-  return bwd_parts(d, gate, at);
+  size_t at[5], fa[4];
+  return fast(d) ? fast_bwd_parts(d, gate, fa) : bwd_parts(d, gate, at);
 }
 static int share_sum(cudaStream_t st, const Dims& d, const float* x, void* out) {
   const int64_t n = d.rows() * d.Hk * d.Dk;
@@ -200,7 +303,8 @@ static int share_sum(cudaStream_t st, const Dims& d, const float* x, void* out) 
   return GLA_OK;
 }
 int bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const float* g, int64_t gt, const void* v, const void* k,
-        const void* q, const float* fin32, const void* dhf, const void* dout, void* dh, float* dg, void* dv, void* dk, void* dq, void* ws) {
+        const void* q, const void* saved, const void* dhf, const void* dout, void* dh, float* dg, void* dv, void* dk, void* dq, void* ws) {
+  if (fast(d)) return fast_bwd(st, d, cu, h0, g, gt, v, k, q, saved, dhf, dout, dh, dg, dv, dk, dq, ws);
   size_t at[5];
   bwd_parts(d, dg != nullptr, at);
   float *rq = (float*)((char*)ws + at[0]), *rk = (float*)((char*)ws + at[1]), *wide = (float*)((char*)ws + at[2]);
@@ -232,14 +336,14 @@ int bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const flo
     Gate w{};
     w.rq = rq; w.rk = rk; w.nq = w.nk = (int)((d.Dk + 127) / 128);
     w.cu = cu; w.T = d.T; w.nseq = d.seqs(); w.rows = d.rows(); w.H = (int)d.H;
-    w.S = fin32; w.dS = dhf; w.dS_f32 = d.hid_f32; w.dd = d.Dk * d.Dv; w.dg = dg;
+    w.S = (const float*)saved; w.dS = dhf; w.dS_f32 = d.hid_f32; w.dd = d.Dk * d.Dv; w.dg = dg;
     ProfScope ps("decay_gate_grad_kernel", st);
     gate_grad_kernel<<<dim3((unsigned)w.nseq, (unsigned)d.H), 512, 0, st>>>(w);
     GLA_CHECK_LAUNCH();
   }
   return GLA_OK;
 }
-unsigned int read_all_bad_offsets() { return bad_offsets_one() + bad_offsets_state() + bad_offsets_fine() + bad_offsets_full(); }
+unsigned int read_all_bad_offsets() { return bad_offsets_one() + bad_offsets_state() + bad_offsets_fine() + bad_offsets_full() + bad_offsets_fast(); }
 
 // What the entry points share: sizes, types, alignment, workspace.
 static int check(const Dims& d, int dtype, int hidden_dtype, const int* cu) {
@@ -264,45 +368,52 @@ static Dims dims_of(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int
 }
 
 size_t gla_decay_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype, int hidden_dtype,
-                                 int64_t nseq, int backward) {
+                                 int64_t nseq, int what) {
   const Dims d = dims_of(B, T, H, Hk, Dk, Dv, dtype, hidden_dtype, nseq);
   static const int some = 0;
   if (decay::check(d, dtype, hidden_dtype, nseq > 0 ? &some : nullptr) != GLA_OK) return 0;
-  return backward ? decay::bwd_ws_bytes(d, backward > 1) : decay::fwd_ws_bytes(d);
+  return what > 1 ? decay::bwd_ws_bytes(d, what == 3) : decay::fwd_ws_bytes(d, what == 1);
+}
+
+size_t gla_decay_saved_bytes(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype, int hidden_dtype, int64_t nseq) {
+  const Dims d = dims_of(B, T, H, Hk, Dk, Dv, dtype, hidden_dtype, nseq);
+  static const int some = 0;
+  return decay::check(d, dtype, hidden_dtype, nseq > 0 ? &some : nullptr) == GLA_OK ? decay::saved_bytes(d) : 0;
 }
 
 int gla_decay_fwd(void* stream, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype, int hidden_dtype,
                   int64_t nseq, const int32_t* cu_seqlens, const void* hidden_init, const float* log_decay, int per_token,
-                  const void* value, const void* key, const void* query, void* hidden_final, void* out, float* final32,
+                  const void* value, const void* key, const void* query, void* hidden_final, void* out, void* saved,
                   void* workspace, size_t workspace_bytes) {
   if (!hidden_init || !log_decay || !value || !key || !query || !hidden_final || !out) return GLA_ERR_NULL_POINTER;
   const Dims d = dims_of(B, T, H, Hk, Dk, Dv, dtype, hidden_dtype, nseq);
   GLA_TRY(decay::check(d, dtype, hidden_dtype, cu_seqlens));
   for (const void* p : {value, key, query, (const void*)out})
     if (!aligned16(p)) return GLA_ERR_ALIGNMENT;
-  const size_t need = decay::fwd_ws_bytes(d);
+  const size_t need = decay::fwd_ws_bytes(d, saved != nullptr);
+  if (!aligned16(saved)) return GLA_ERR_ALIGNMENT;
   if (need && (!workspace || workspace_bytes < need)) return GLA_ERR_WORKSPACE;
   if (need && !aligned16(workspace)) return GLA_ERR_ALIGNMENT;
   return decay::fwd((cudaStream_t)stream, d, cu_seqlens, hidden_init, log_decay, per_token ? H : 0, value, key, query, hidden_final, out,
-                    final32, workspace);
+                    saved, workspace);
 }
 
 int gla_decay_bwd(void* stream, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype, int hidden_dtype,
                   int64_t nseq, const int32_t* cu_seqlens, const void* hidden_init, const float* log_decay, int per_token,
-                  const void* value, const void* key, const void* query, const float* final32, const void* dhidden_final,
+                  const void* value, const void* key, const void* query, const void* saved, const void* dhidden_final,
                   const void* dout, void* dhidden_init, float* dlog_decay, void* dvalue, void* dkey, void* dquery, void* workspace,
                   size_t workspace_bytes) {
-  if (!hidden_init || !log_decay || !value || !key || !query || !dhidden_final || !dout || !dhidden_init || !dvalue || !dkey || !dquery ||
-      (dlog_decay && !final32))
+  if (!hidden_init || !log_decay || !value || !key || !query || !dhidden_final || !dout || !saved || !dhidden_init || !dvalue || !dkey ||
+      !dquery)
     return GLA_ERR_NULL_POINTER;
   const Dims d = dims_of(B, T, H, Hk, Dk, Dv, dtype, hidden_dtype, nseq);
   GLA_TRY(decay::check(d, dtype, hidden_dtype, cu_seqlens));
-  for (const void* p : {value, key, query, dout, (const void*)dvalue, (const void*)dkey, (const void*)dquery})
+  for (const void* p : {value, key, query, saved, dout, (const void*)dvalue, (const void*)dkey, (const void*)dquery})
     if (!aligned16(p)) return GLA_ERR_ALIGNMENT;
   const size_t need = decay::bwd_ws_bytes(d, dlog_decay != nullptr);
   if (need && (!workspace || workspace_bytes < need)) return GLA_ERR_WORKSPACE;
   if (need && !aligned16(workspace)) return GLA_ERR_ALIGNMENT;
-  return decay::bwd((cudaStream_t)stream, d, cu_seqlens, hidden_init, log_decay, per_token ? H : 0, value, key, query, final32, dhidden_final,
+  return decay::bwd((cudaStream_t)stream, d, cu_seqlens, hidden_init, log_decay, per_token ? H : 0, value, key, query, saved, dhidden_final,
                     dout, dhidden_init, dlog_decay, dvalue, dkey, dquery, workspace);
 }
 

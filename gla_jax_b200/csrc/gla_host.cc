@@ -331,15 +331,16 @@ std::string decay_text(const DecayDims& d) {
 }
 struct DecayFn : torch::autograd::Function<DecayFn> {
   static variable_list run(const DecayDims& d, const Tensor& h, const Tensor& g, const Tensor& v, const Tensor& k, const Tensor& q,
-                           const Tensor& cu, bool final32) {
-    Tensor hf = torch::empty_like(h), out = torch::empty_like(v), f32 = final32 ? torch::empty(h.sizes(), h.options().dtype(torch::kFloat32)) : Tensor();
-    const size_t n = gla_decay_workspace_bytes(d.B, d.T, d.H, d.Hk, d.Dk, d.Dv, d.dt, d.hdt, d.nseq, 0);
+                           const Tensor& cu, bool residuals) {
+    Tensor hf = torch::empty_like(h), out = torch::empty_like(v);
+    Tensor saved = residuals ? bytes(v, gla_decay_saved_bytes(d.B, d.T, d.H, d.Hk, d.Dk, d.Dv, d.dt, d.hdt, d.nseq)) : Tensor();
+    const size_t n = gla_decay_workspace_bytes(d.B, d.T, d.H, d.Hk, d.Dk, d.Dv, d.dt, d.hdt, d.nseq, residuals);
     Tensor ws = bytes(v, n);
     const int st = gla_decay_fwd(stream_of(v), d.B, d.T, d.H, d.Hk, d.Dk, d.Dv, d.dt, d.hdt, d.nseq, (const int32_t*)ptr(cu), ptr(h),
-                                 (const float*)ptr(g), d.per_token, ptr(v), ptr(k), ptr(q), ptr(hf), ptr(out), (float*)ptr(f32), ptr(ws), n);
+                                 (const float*)ptr(g), d.per_token, ptr(v), ptr(k), ptr(q), ptr(hf), ptr(out), ptr(saved), ptr(ws), n);
     if (st == GLA_ERR_UNSUPPORTED) raise("chunk_decay_attention: unsupported configuration " + decay_text(d));
     check(st, "gla_decay_fwd");
-    return {hf, out, f32};
+    return {hf, out, saved};
   }
   static variable_list forward(AutogradContext* ctx, const Tensor& h0, const Tensor& g0, const Tensor& v0, const Tensor& k0, const Tensor& q0,
                                const Tensor& cu0, std::vector<int64_t> dims) {
@@ -347,7 +348,7 @@ struct DecayFn : torch::autograd::Function<DecayFn> {
     const Tensor cu = d.nseq ? cu0 : Tensor();
     Tensor h = h0.contiguous(), g = f32(g0), v = v0.contiguous(), k = k0.contiguous(), q = q0.contiguous();
     const bool gate = g0.requires_grad();
-    variable_list r = run(d, h, g, v, k, q, cu, gate);
+    variable_list r = run(d, h, g, v, k, q, cu, true);
     ctx->save_for_backward({h, g, v, k, q, r[2], cu});
     ctx->set_materialize_grads(false);
     dims.push_back(gate);
@@ -364,10 +365,10 @@ struct DecayFn : torch::autograd::Function<DecayFn> {
     Tensor dhf = grad_or_zeros(grads[0], h), dout = grad_or_zeros(grads[1], v);
     Tensor dh = torch::empty_like(h), dg = gate ? torch::empty_like(g) : Tensor(), dv = torch::empty_like(v), dk = torch::empty_like(k),
            dq = torch::empty_like(q);
-    const size_t n = gla_decay_workspace_bytes(d.B, d.T, d.H, d.Hk, d.Dk, d.Dv, d.dt, d.hdt, d.nseq, gate ? 2 : 1);
+    const size_t n = gla_decay_workspace_bytes(d.B, d.T, d.H, d.Hk, d.Dk, d.Dv, d.dt, d.hdt, d.nseq, gate ? 3 : 2);
     Tensor ws = bytes(v, n);
     check(gla_decay_bwd(stream_of(v), d.B, d.T, d.H, d.Hk, d.Dk, d.Dv, d.dt, d.hdt, d.nseq, (const int32_t*)ptr(cu), ptr(h), (const float*)ptr(g),
-                        d.per_token, ptr(v), ptr(k), ptr(q), (const float*)ptr(s[5]), ptr(dhf), ptr(dout), ptr(dh), (float*)ptr(dg), ptr(dv),
+                        d.per_token, ptr(v), ptr(k), ptr(q), ptr(s[5]), ptr(dhf), ptr(dout), ptr(dh), (float*)ptr(dg), ptr(dv),
                         ptr(dk), ptr(dq), ptr(ws), n), "gla_decay_bwd");
     const auto gt = (torch::ScalarType)a[11];
     return {dh, gate && gt != torch::kFloat32 ? dg.to(gt) : dg, dv, dk, dq, Tensor(), Tensor()};

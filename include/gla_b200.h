@@ -516,26 +516,29 @@ GLA_API int gla_sp_combine2(void* stream, int64_t R, int64_t rank, int64_t BH, i
  *   sequence give zeros.  Offsets that fall or leave [0, T] are held inside and counted (gla_device_bad_offsets).
  * Dk and Dv multiples of 8 up to 256; any T > 0; H a multiple of Hk.  `dtype` is that of value, key, query, out and their
  * gradients; hidden_dtype that of hidden_init, hidden_final and their gradients: dtype or GLA_F32.  value, key, query, out and
- * gradients 16-byte aligned.  final32, if not NULL, receives the final state in float32, which the backward needs
- * for dlog_decay (in layout (B or nseq, H, Dk, Dv)).
- * bf16 forward: scores, the state as an operand and decayed values are rounded to bf16 once (the state from three
- * bf16 planes of the values where it leaves in float32); sums, states and decays in float32 and more.
- * bf16 backward: the same operands in two planes.  float32: three planes everywhere.
+ * gradients 16-byte aligned.
+ * A forward that will be differentiated gets `saved` (gla_decay_saved_bytes), which the backward reads: final states in
+ * float32 and, where few heads make the library cut sequences into runs, the states that enter the runs.  NULL otherwise.
+ * bf16, head sizes up to 128: scores and the state as an operand are rounded to bf16 once, decayed values to two bf16
+ * planes (three where hidden is float32; the state in two where dlog_decay is asked for); sums, states and decays in float32
+ * and more.  bf16 beyond: one plane of each in the forward, two in the backward.  float32: three planes everywhere.
  * Backward: dlog_decay (B, T, H) float32 or NULL; dhidden_init as hidden_init.
- * Workspace: gla_decay_workspace_bytes with backward = 0 (forward), 1 (backward without dlog_decay), 2 (with it); 0 bytes
- * may be needed, or the sizes may be unsupported (the calls say which).
+ * Workspace: gla_decay_workspace_bytes for the forward without (what = 0) and with `saved` (1), the backward without (2)
+ * and with dlog_decay (3); 0 bytes may be needed, or the sizes may be unsupported (the calls say which).
  * ---------------------------------------------------------------------------------- */
 GLA_API size_t gla_decay_workspace_bytes(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype,
-                             int hidden_dtype, int64_t nseq, int backward);
+                             int hidden_dtype, int64_t nseq, int what);
+GLA_API size_t gla_decay_saved_bytes(int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype,
+                             int hidden_dtype, int64_t nseq);
 GLA_API int gla_decay_fwd(void* stream, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype,
                       int hidden_dtype, int64_t nseq, const int32_t* cu_seqlens,
                       const void* hidden_init, const float* log_decay, int per_token,
                       const void* value, const void* key, const void* query,
-                      void* hidden_final, void* out, float* final32, void* workspace, size_t workspace_bytes);
+                      void* hidden_final, void* out, void* saved, void* workspace, size_t workspace_bytes);
 GLA_API int gla_decay_bwd(void* stream, int64_t B, int64_t T, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype,
                       int hidden_dtype, int64_t nseq, const int32_t* cu_seqlens,
                       const void* hidden_init, const float* log_decay, int per_token,
-                      const void* value, const void* key, const void* query, const float* final32,
+                      const void* value, const void* key, const void* query, const void* saved,
                       const void* dhidden_final, const void* dout,
                       void* dhidden_init, float* dlog_decay, void* dvalue, void* dkey, void* dquery,
                       void* workspace, size_t workspace_bytes);

@@ -42,7 +42,8 @@ def test_validation_without_gpu(lib):
     assert lib.gla_decay_workspace_bytes(1, 8, 2, 2, 64, 64, 1, 1, 0, 0) == 0
     need = lib.gla_decay_workspace_bytes(1, 65536, 2, 2, 64, 64, 1, 1, 0, 0)
     assert need > 0 and fwd(1, 65536, 2, 2, 64, 64, n=need - 1) == fwd(1, 65536, 2, 2, 64, 64, ws=None) == 5
-    assert lib.gla_decay_workspace_bytes(1, 65536, 2, 1, 64, 64, 1, 1, 0, 2) > lib.gla_decay_workspace_bytes(1, 65536, 2, 2, 64, 64, 1, 1, 0, 1) > 0
+    assert lib.gla_decay_workspace_bytes(1, 65536, 2, 1, 64, 64, 1, 1, 0, 3) > lib.gla_decay_workspace_bytes(1, 65536, 2, 2, 64, 64, 1, 1, 0, 2) > 0
+    assert lib.gla_decay_saved_bytes(1, 8, 2, 2, 64, 64, 1, 1, 0) >= 2 * 64 * 64 * 4 and lib.gla_decay_saved_bytes(1, 8, 3, 2, 64, 64, 1, 1, 0) == 0
     assert lib.gla_decay_workspace_bytes(1, 8, 2, 2, 60, 64, 1, 1, 0, 0) == 0
     step = lambda B=4, Dk=64, parents=None, beams=1, state=p: lib.gla_decay_step(  # noqa: E731
         None, B, 2, 2, Dk, 64, 1, state, p, p, p, p, p, 1, parents, beams)
