@@ -19,28 +19,32 @@ namespace decay {
 template <int PITCH> __device__ __forceinline__ uint32_t at16(uint32_t base, int r, int piece) {      // PITCH bytes a row
   return base + r * PITCH + ((piece ^ (r & 7)) << 4);
 }
+// Matrix loads of 16 x 16 at (row, column) of a tile, both multiples of 16: lane offsets of the two patterns, to which the
+// column is added by exclusive or and the row as it is.  lane_a: A [m][k] (ldsm), B [k][n] (ldsm_t); lane_b: A [k][m]
+// (ldsm_t), B [n][k] (ldsm).
+template <int PITCH> __device__ __forceinline__ uint32_t lane_a(int lane) { return (lane & 15) * PITCH + (((lane >> 4) ^ (lane & 7)) << 4); }
+template <int PITCH> __device__ __forceinline__ uint32_t lane_b(int lane) {
+  return ((lane & 7) + ((lane >> 4) & 1) * 8) * PITCH + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+}
+// A chunk of 64 rows into a tile: a thread's 16-byte pieces lie NT / (D / 8) rows apart.  src: row 0 of the chunk.
 template <int D, int NT>
-__device__ __forceinline__ void fetch_tile(uint32_t dst, const void* src, int64_t row0, int64_t step, int nv, int d) {
-  constexpr int C8 = D / 8;
+__device__ __forceinline__ void fetch_tile(uint32_t tile, const bf16* src, int64_t step, int nv, int d) {
+  constexpr int C8 = D / 8, RS = NT / C8;
+  static_assert(RS % 8 == 0, "the pieces of a thread lie at one place of their rows");
+  const int r0 = threadIdx.x / C8, c = threadIdx.x % C8;
+  const bf16* g = src + r0 * step + c * 8;
+  const uint32_t dst = at16<2 * D>(tile, r0, c);
+  const int n = c * 8 < d ? nv - r0 : 0;
 #pragma unroll
-  for (int j = 0; j < 64 * C8 / NT; ++j) {
-    const int i = threadIdx.x + NT * j, r = i / C8, c = i % C8;
-    const bool in = r < nv && c * 8 < d;
-    cp16(at16<2 * D>(dst, r, c), (const bf16*)src + (in ? row0 + r * step + c * 8 : 0), in);
+  for (int j = 0; j < 64 / RS; ++j) {
+    cp16(dst + j * RS * 2 * D, RS * j < n ? g : src, RS * j < n);
+    g += RS * step;
   }
 }
-// fragments: A [m][k], A [k][m], B [n][k] and B [k][n], 16 x 16 at (row, column) of a tile
-template <int PITCH> __device__ __forceinline__ void frag_a(uint32_t (&a)[4], uint32_t t, int m, int k, int lane) {
-  ldsm(a, at16<PITCH>(t, m + (lane & 15), k / 8 + (lane >> 4)));
-}
-template <int PITCH> __device__ __forceinline__ void frag_at(uint32_t (&a)[4], uint32_t t, int k, int m, int lane) {
-  ldsm_t(a, at16<PITCH>(t, k + (lane & 7) + ((lane >> 4) & 1) * 8, m / 8 + ((lane >> 3) & 1)));
-}
-template <int PITCH> __device__ __forceinline__ void frag_b(uint32_t (&b)[4], uint32_t t, int n, int k, int lane) {
-  ldsm(b, at16<PITCH>(t, n + (lane & 7) + ((lane >> 4) & 1) * 8, k / 8 + ((lane >> 3) & 1)));
-}
-template <int PITCH> __device__ __forceinline__ void frag_bt(uint32_t (&b)[4], uint32_t t, int k, int n, int lane) {
-  ldsm_t(b, at16<PITCH>(t, k + (lane & 15), n / 8 + (lane >> 4)));
+__device__ __forceinline__ float ex2(float x) {      // 2^-22 relative, 0 below 2^-126
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 // an A fragment times a weight per k (w[0], w[1]: k 2 tq, 2 tq + 1; w[2], w[3]: eight further), in NU planes
 template <int NU>
@@ -55,15 +59,20 @@ __device__ __forceinline__ void weighted(uint32_t (&z)[NU][4], const uint32_t (&
   }
 }
 
-// The gates of a chunk of 64 by one warp: two rows a lane.  lam: running sums, base 2, as two floats; wt: exp(lam_i) and
-// exp(lam_L - lam_i).  Returns the chunk's sum (base 2).
+// What a chunk of 64 needs of its gates, made by one warp, two rows a lane.  lam: running sums, base 2, as two floats;
+// wt: exp(lam_i) and exp(lam_L - lam_i).  The weight exp(lam_i - lam_j) of a score below the diagonal blocks of 16 x 16 is a
+// product rf_i cf_j over the last token before i's block, so that 160 exponentials make 1536 weights.
+struct Gates {
+  float2 lam[64], wt[64];
+  float rf[64], cf[3][64];           // cf[b - 1]: to the last token before row block b
+};
 __device__ __forceinline__ float2 gates_of(const Walk& p, int64_t t0, int nv, int h, int lane) {
   float2 g = make_float2(0.f, 0.f);
   if (2 * lane < nv) g.x = p.g[(t0 + 2 * lane) * p.gt + h];
   if (2 * lane + 1 < nv) g.y = p.g[(t0 + 2 * lane + 1) * p.gt + h];
   return g;
 }
-__device__ __forceinline__ double scan_gates(float2 g, float2* lam, float2* wt, int lane) {
+__device__ __forceinline__ double scan_gates(float2 g, Gates& s, int lane) {
   // exp of less than -200 is 0 either way; -inf would leave inf - inf
   const double a = (double)(g.x < -200.f ? -200.f : g.x) * 1.4426950408889634, b = (double)(g.y < -200.f ? -200.f : g.y) * 1.4426950408889634;
   double inc = a + b;
@@ -72,23 +81,99 @@ __device__ __forceinline__ double scan_gates(float2 g, float2* lam, float2* wt, 
     const double y = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += y;
   }
-  const double all = __shfl_sync(0xffffffffu, inc, 31);
+  const double all = __shfl_sync(0xffffffffu, inc, 31), own = __shfl_sync(0xffffffffu, inc, lane >= 8 ? lane / 8 * 8 - 1 : 0);
+  const double at[3] = {__shfl_sync(0xffffffffu, inc, 7), __shfl_sync(0xffffffffu, inc, 15), __shfl_sync(0xffffffffu, inc, 23)};
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const double v = i ? inc : inc - b;
     const float hi = (float)v;
-    lam[2 * lane + i] = make_float2(hi, (float)(v - hi));
-    wt[2 * lane + i] = make_float2(exp2f((float)v), exp2f((float)(all - v)));
+    const int r = 2 * lane + i;
+    s.lam[r] = make_float2(hi, (float)(v - hi));
+    s.wt[r] = make_float2(ex2(hi), ex2((float)(all - v)));
+    s.rf[r] = ex2((float)(v - own));
+#pragma unroll
+    for (int m = 0; m < 3; ++m)
+      if (lane < 8 * (m + 1)) s.cf[m][r] = ex2((float)(at[m] - v));
   }
   return all;
 }
-__device__ __forceinline__ float decay_of(float2 i, float2 j) { return exp2f((i.x - j.x) + (i.y - j.y)); }
+__device__ __forceinline__ float decay_of(float2 i, float2 j) { return ex2((i.x - j.x) + (i.y - j.y)); }
+// the weights of rows r, r + 8 (index / 2) and columns j, j + 1 of a block
+__device__ __forceinline__ void weights_of(float (&w)[4], const Gates& s, int mi, int nj, int r, int j) {
+  if (mi == nj) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int i = r + 8 * (e / 2), c = j + e % 2;
+      w[e] = c <= i ? decay_of(s.lam[i], s.lam[c]) : 0.f;
+    }
+  } else {
+    const float2 c = *reinterpret_cast<const float2*>(&s.cf[mi - 1][j]);
+    const float a = s.rf[r], b = s.rf[r + 8];
+    w[0] = a * c.x; w[1] = a * c.y; w[2] = b * c.x; w[3] = b * c.y;
+  }
+}
+// Whether a B fragment holds something that is not finite.  In a diagonal block it would meet the zeros of later (backwards:
+// earlier) tokens in the product, and 0 x inf is not a number; the recurrence has it at its own token and after only.
+__device__ __forceinline__ bool not_finite(const uint32_t (&b)[4]) {
+  bool x = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x = x || (b[i] & 0x7f80u) == 0x7f80u || (b[i] & 0x7f800000u) == 0x7f800000u;
+  return x;
+}
+__device__ __forceinline__ float lds_bf16(uint32_t a) {
+  uint16_t u;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(u) : "r"(a));
+  return __uint_as_float((uint32_t)u << 16);
+}
+// Such a block by the sums themselves: o (rows gr, gr + 8 of the block at r0, tiles of 8 columns from c0) += P V over the block's
+// own tokens, j <= i; UP: P^T V, over j >= i.
+template <int PITCH, int NT8, bool UP>
+__device__ __noinline__ void diagonal_sums(float (&o)[NT8][4], uint32_t tp, uint32_t tv, int r0, int c0, int gr, int tq) {
+#pragma unroll 1
+  for (int j = 0; j < 16; ++j) {
+    const int t = r0 + j;
+    float s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) s[u] = UP ? lds_bf16(at16<128>(tp, t, (r0 + gr + 8 * u) / 8) + gr * 2) : lds_bf16(at16<128>(tp, r0 + gr + 8 * u, t / 8) + t % 8 * 2);
+#pragma unroll
+    for (int n = 0; n < NT8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = gr + 8 * (e / 2), c = c0 + 8 * n + 2 * tq + e % 2;
+        if (UP ? j >= i : j <= i) o[n][e] = fmaf(s[e / 2], lds_bf16(at16<PITCH>(tv, t, c / 8) + c % 8 * 2), o[n][e]);
+      }
+  }
+}
+template <int PITCH, int NT8, bool UP>
+__device__ __forceinline__ void diagonal_by_sums(float (&o)[NT8][4], uint32_t tp, uint32_t tv, int r0, int c0, int gr, int tq) {
+  float x[NT8][4];                   // (a copy, so that o itself stays in registers)
+#pragma unroll
+  for (int n = 0; n < NT8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[n][e] = o[n][e];
+  diagonal_sums<PITCH, NT8, UP>(x, tp, tv, r0, c0, gr, tq);
+#pragma unroll
+  for (int n = 0; n < NT8; ++n)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[n][e] = x[n][e];
+}
+// 4 x 4 words across the four lanes of a row: lane tq is left with word tq of each
+__device__ __forceinline__ void transpose4(uint32_t (&v)[4], int tq) {
+#pragma unroll
+  for (int s = 1; s < 4; s <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (!(j & s)) {
+        const uint32_t y = __shfl_xor_sync(0xffffffffu, (tq & s) ? v[j] : v[j | s], s);
+        if (tq & s) v[j] = y; else v[j | s] = y;
+      }
+}
 
 template <int KD, int NC, bool OUT>
 struct FLay {
   static constexpr int VT = 64 * NC, NT = 128;
   static constexpr int PK = 128 * KD, PV = 128 * VT, STAGE = (OUT ? 2 : 1) * PK + PV;
-  static constexpr int P0 = 2 * STAGE, LAM = P0 + (OUT ? 8192 : 0), WT = LAM + 1024, RD = WT + 1024, END = RD + (OUT ? 1024 : 0);
+  static constexpr int P0 = 2 * STAGE, G0 = P0 + (OUT ? 8192 : 0), RD = G0 + 2 * (int)sizeof(Gates), END = RD + (OUT ? 1024 : 0);
 };
 
 // KD: features; NC: groups of 16 value columns of a warp; NU: planes of the weighted values (3: and exact additions); NS:
@@ -97,9 +182,8 @@ template <int KD, int NC, int NU, int NS, bool OUT>
 __global__ void __launch_bounds__(128, 2) fast_walk_kernel(const Walk p) {
   using Y = FLay<KD, NC, OUT>;
   constexpr int KT = KD / 8, QP = 2 * KD, VP = 2 * Y::VT;
-  extern __shared__ __align__(128) uint8_t sm[];
-  float2* lam_ = reinterpret_cast<float2*>(sm + Y::LAM);
-  float2* wt_ = reinterpret_cast<float2*>(sm + Y::WT);
+  extern __shared__ __align__(256) uint8_t sm[];
+  Gates* gates = reinterpret_cast<Gates*>(sm + Y::G0);
   float* rd = reinterpret_cast<float*>(sm + Y::RD);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, gr = lane / 4, tq = lane % 4;
   const int h = blockIdx.y % p.H, vt = blockIdx.y / p.H;
@@ -120,6 +204,33 @@ __global__ void __launch_bounds__(128, 2) fast_walk_kernel(const Walk p) {
   if (!OUT && (p.rev ? run.first : run.last)) return;
 
   const int64_t sh = run.s * p.H + h, dd = (int64_t)p.kd * p.vd, slot_h = (int64_t)blockIdx.x * p.H + h;
+  const int Hq = p.H / p.gq, Hk = p.H / p.gk, Hv = p.H / p.gv;
+  const int len = (int)(run.hi - run.lo), chunks = (len + 63) / 64;
+  const uint32_t base = sm32(sm);
+  const int64_t r0 = run.base + run.lo;                                   // the run's first token
+  const int64_t sk = (int64_t)Hk * p.kd, sv = (int64_t)Hv * p.vd, sq = (int64_t)Hq * p.kd;
+  const bf16* gk = (const bf16*)p.k + r0 * sk + h / p.gk * p.kd;
+  const bf16* gv = (const bf16*)p.v + r0 * sv + h / p.gv * p.vd + cbase;
+  const bf16* gq = OUT ? (const bf16*)p.q + r0 * sq + h / p.gq * p.kd : nullptr;
+  // chunk i of the walk; backwards in time (sums only) from the last one
+  const auto first_of = [&](int i) { return 64 * (p.rev ? chunks - 1 - i : i); };
+  const auto fetch = [&](int i) {
+    const int c0 = first_of(i), nv = len - c0 < 64 ? len - c0 : 64;
+    const uint32_t s = base + (i & 1) * Y::STAGE;
+    fetch_tile<KD, 128>(s, gk + c0 * sk, sk, nv, p.kd);
+    fetch_tile<Y::VT, 128>(s + Y::PK, gv + c0 * sv, sv, nv, p.vd - cbase);
+    if constexpr (OUT) fetch_tile<KD, 128>(s + Y::PK + Y::PV, gq + c0 * sq, sq, nv, p.kd);
+  };
+  double total = 0.0;
+  if (chunks) {
+    fetch(0);
+    if (warp == 0) {
+      const int c0 = first_of(0);
+      total += scan_gates(gates_of(p, r0 + c0, len - c0 < 64 ? len - c0 : 64, h, lane), gates[0], lane);
+    }
+  }
+  cp_commit();
+
   float st[NC][KT][4];
 #pragma unroll
   for (int n = 0; n < NC; ++n)
@@ -134,33 +245,12 @@ __global__ void __launch_bounds__(128, 2) fast_walk_kernel(const Walk p) {
         st[n][j][e] = x;
       }
 
-  const int Hq = p.H / p.gq, Hk = p.H / p.gk, Hv = p.H / p.gv, Hr = p.r ? p.H / p.gr : 1;
-  const int len = (int)(run.hi - run.lo), chunks = (len + 63) / 64;
-  const uint32_t base = sm32(sm);
-  // chunk i of the walk; backwards in time (sums only) from the last one
-  const auto first_of = [&](int i) { return 64 * (p.rev ? chunks - 1 - i : i); };
-  const auto fetch = [&](int i) {
-    const int c0 = first_of(i), nv = len - c0 < 64 ? len - c0 : 64;
-    const int64_t t0 = run.base + run.lo + c0;
-    const uint32_t s = base + (i & 1) * Y::STAGE;
-    fetch_tile<KD, 128>(s, p.k, (t0 * Hk + h / p.gk) * p.kd, (int64_t)Hk * p.kd, nv, p.kd);
-    fetch_tile<Y::VT, 128>(s + Y::PK, p.v, (t0 * Hv + h / p.gv) * p.vd + cbase, (int64_t)Hv * p.vd, nv, p.vd - cbase);
-    if constexpr (OUT) fetch_tile<KD, 128>(s + Y::PK + Y::PV, p.q, (t0 * Hq + h / p.gq) * p.kd, (int64_t)Hq * p.kd, nv, p.kd);
-  };
-  double total = 0.0;
-  if (chunks) {
-    fetch(0);
-    if (warp == 0) {
-      const int c0 = first_of(0);
-      total += scan_gates(gates_of(p, run.base + run.lo + c0, len - c0 < 64 ? len - c0 : 64, h, lane), lam_, wt_, lane);
-    }
-  }
-  cp_commit();
+  const uint32_t laq = lane_a<QP>(lane), lbq = lane_b<QP>(lane), lav = lane_a<VP>(lane) ^ (cl * 2), lbv = lane_b<VP>(lane) ^ (cl * 2), lap = lane_a<128>(lane);
   for (int i = 0; i < chunks; ++i) {
     const int c0 = first_of(i), nv = len - c0 < 64 ? len - c0 : 64;
-    const int64_t t0 = run.base + run.lo + c0;
+    const int64_t t0 = r0 + c0;
     const uint32_t uk = base + (i & 1) * Y::STAGE, uv = uk + Y::PK, uq = uv + Y::PV, up = base + Y::P0;
-    const float2 *lam = lam_ + 64 * (i & 1), *wt = wt_ + 64 * (i & 1);
+    const Gates& gs = gates[i & 1];
     cp_wait<0>();
     __syncthreads();                 // this chunk is here, and nobody reads the other stage any more
     float2 gn = make_float2(0.f, 0.f);
@@ -168,205 +258,190 @@ __global__ void __launch_bounds__(128, 2) fast_walk_kernel(const Walk p) {
       fetch(i + 1);
       if (warp == 0) {
         const int n0 = first_of(i + 1);
-        gn = gates_of(p, run.base + run.lo + n0, len - n0 < 64 ? len - n0 : 64, h, lane);
+        gn = gates_of(p, r0 + n0, len - n0 < 64 ? len - n0 : 64, h, lane);
       }
     }
     cp_commit();
     if constexpr (OUT) {
-      if (p.r && i > 0 && tid < 64) {
+      if (p.r && i > 0 && tid < 64)
         // the row sums of the chunk before (a whole one)
         p.rdot[(vt * (p.cu ? p.T : p.nseq * p.T) + t0 - 64 + tid) * p.H + h] = (rd[tid] + rd[64 + tid]) + (rd[128 + tid] + rd[192 + tid]);
-      }
-      // scores in blocks of 16 x 16: rows 48.. by two warps, 32.. by one, 16.. and 0.. by one
-      const auto scores = [&](auto nb, int mi, int nj) {
-        constexpr int NB = decltype(nb)::value;
-        float c[NB][2][4] = {};
+      // scores in blocks of 16 x 16: (3,0) (3,1) | (3,2) (3,3) | (2,0) (2,1) (2,2) | (1,0) (1,1) (0,0)
+#pragma unroll 1
+      for (int b = 0; b < (warp < 2 ? 2 : 3); ++b) {
+        const int mi = warp < 2 ? 3 : warp == 2 ? 2 : b < 2 ? 1 : 0, nj = warp == 1 ? 2 + b : warp == 3 && b == 2 ? 0 : b;
+        if (mi * 16 >= nv) continue;
+        float c[2][4] = {};
+        const uint32_t qa = uq + mi * 16 * QP, ka = uk + nj * 16 * QP;
 #pragma unroll
         for (int kk = 0; kk < KD / 16; ++kk) {
-          uint32_t a[4];
-          frag_a<QP>(a, uq, mi * 16, kk * 16, lane);
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
-            uint32_t x[4];
-            frag_b<QP>(x, uk, (nj + b) * 16, kk * 16, lane);
-            mma16(c[b][0], a, x[0], x[1]);
-            mma16(c[b][1], a, x[2], x[3]);
-          }
+          uint32_t a[4], x[4];
+          ldsm(a, qa + (laq ^ (kk * 32)));
+          ldsm(x, ka + (lbq ^ (kk * 32)));
+          mma16(c[0], a, x[0], x[1]);
+          mma16(c[1], a, x[2], x[3]);
         }
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int n = 0; n < 2; ++n) {
+          const int r = mi * 16 + gr, j = nj * 16 + n * 8 + 2 * tq;
+          float w[4];
+          weights_of(w, gs, mi, nj, r, j);
+          // (a score of a masked pair may be anything: 0 by selection)
+          const bool d = mi == nj;
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              const int r = mi * 16 + gr + 4 * e, j = (nj + b) * 16 + n * 8 + 2 * tq;
-              const float2 lr = lam[r];
-              const float x = j <= r ? c[b][n][e] * decay_of(lr, lam[j]) : 0.f, y = j + 1 <= r ? c[b][n][e + 1] * decay_of(lr, lam[j + 1]) : 0.f;
-              const uint32_t z = pack_bf16x2(x, y);
-              asm volatile("st.shared.b32 [%0], %1;" ::"r"(at16<128>(up, r, j / 8) + (j % 8) * 2), "r"(z) : "memory");
-            }
-      };
-      if (warp == 0) scores(std::integral_constant<int, 2>(), 3, 0);
-      else if (warp == 1) scores(std::integral_constant<int, 2>(), 3, 2);
-      else if (warp == 2) scores(std::integral_constant<int, 3>(), 2, 0);
-      else { scores(std::integral_constant<int, 2>(), 1, 0); scores(std::integral_constant<int, 1>(), 0, 0); }
+          for (int e = 0; e < 4; ++e) c[n][e] = d && j + e % 2 > r + 8 * (e / 2) ? 0.f : c[n][e] * w[e];
+          const uint32_t at = at16<128>(up, r, 2 * nj + n) + 4 * tq;
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(pack_bf16x2(c[n][0], c[n][1])) : "memory");
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(at + 8 * 128), "r"(pack_bf16x2(c[n][2], c[n][3])) : "memory");
+        }
+      }
     }
-    if (warp == 0 && i + 1 < chunks) total += scan_gates(gn, lam_ + 64 * ((i + 1) & 1), wt_ + 64 * ((i + 1) & 1), lane);
+    if (warp == 0 && i + 1 < chunks) total += scan_gates(gn, gates[(i + 1) & 1], lane);
     if constexpr (OUT) {
       __syncthreads();
 #pragma unroll 1
       for (int m = 0; m < 64 && m < nv; m += 32) {
-        float o[2][2 * NC][4];
-        const auto inter = [&](float (&x)[2][2 * NC][4]) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int n = 0; n < 2 * NC; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[r][n][e] = 0.f;
+          float o[2][2 * NC][4] = {};
 #pragma unroll
           for (int kk = 0; kk < KD / 16; ++kk) {
             uint32_t a[2][4];
-            frag_a<QP>(a[0], uq, m, kk * 16, lane);
-            frag_a<QP>(a[1], uq, m + 16, kk * 16, lane);
+            ldsm(a[0], uq + m * QP + (laq ^ (kk * 32)));
+            ldsm(a[1], uq + (m + 16) * QP + (laq ^ (kk * 32)));
+            uint32_t b[NC][4][NS];
 #pragma unroll
             for (int n = 0; n < NC; ++n) {
-              uint32_t b0[NS], b1[NS], b2[NS], b3[NS];
-              planes<NS>(st[n][2 * kk][0], st[n][2 * kk][1], b0);
-              planes<NS>(st[n][2 * kk + 1][0], st[n][2 * kk + 1][1], b1);
-              planes<NS>(st[n][2 * kk][2], st[n][2 * kk][3], b2);
-              planes<NS>(st[n][2 * kk + 1][2], st[n][2 * kk + 1][3], b3);
+              planes<NS>(st[n][2 * kk][0], st[n][2 * kk][1], b[n][0]);
+              planes<NS>(st[n][2 * kk + 1][0], st[n][2 * kk + 1][1], b[n][1]);
+              planes<NS>(st[n][2 * kk][2], st[n][2 * kk][3], b[n][2]);
+              planes<NS>(st[n][2 * kk + 1][2], st[n][2 * kk + 1][3], b[n][3]);
+            }
 #pragma unroll
-              for (int s = NS - 1; s >= 0; --s)
+            for (int s = NS - 1; s >= 0; --s)
+#pragma unroll
+              for (int n = 0; n < NC; ++n)
 #pragma unroll
                 for (int r = 0; r < 2; ++r) {
-                  mma16(x[r][2 * n], a[r], b0[s], b1[s]);
-                  mma16(x[r][2 * n + 1], a[r], b2[s], b3[s]);
+                  mma16(o[r][2 * n], a[r], b[n][0][s], b[n][1][s]);
+                  mma16(o[r][2 * n + 1], a[r], b[n][2][s], b[n][3][s]);
                 }
-            }
           }
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            const float w0 = wt[m + 16 * r + gr].x, w1 = wt[m + 16 * r + gr + 8].x;
+            const float w0 = gs.wt[m + 16 * r + gr].x, w1 = gs.wt[m + 16 * r + gr + 8].x;
 #pragma unroll
-            for (int n = 0; n < 2 * NC; ++n) { x[r][n][0] *= w0; x[r][n][1] *= w0; x[r][n][2] *= w1; x[r][n][3] *= w1; }
+            for (int n = 0; n < 2 * NC; ++n) { o[r][n][0] *= w0; o[r][n][1] *= w0; o[r][n][2] *= w1; o[r][n][3] *= w1; }
           }
-        };
-        inter(o);
-        if (p.r) {
-          // the rows' products with what comes from before the chunk
+          if (p.r) {
+            // the rows' products with what comes from before the chunk
+            const int Hr = p.H / p.gr;
 #pragma unroll
-          for (int r = 0; r < 2; ++r) {
-            float dot[2] = {0.f, 0.f};
+            for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int row = m + 16 * r + gr + 8 * half;
-              if (row < nv) {
-                const int64_t ra = ((t0 + row) * Hr + h / p.gr) * p.vd + cw + 2 * tq;
+              for (int half = 0; half < 2; ++half) {
+                const int row = m + 16 * r + gr + 8 * half;
+                float dot = 0.f;
+                if (row < nv) {
+                  const int64_t ra = ((t0 + row) * Hr + h / p.gr) * p.vd + cw + 2 * tq;
 #pragma unroll
-                for (int n = 0; n < 2 * NC; ++n)
-                  if (cw + 8 * n < p.vd) {
-                    const float2 x = pair_of(__ldg((const unsigned int*)((const bf16*)p.r + ra + 8 * n)));
-                    dot[half] = fmaf(o[r][n][2 * half], x.x, fmaf(o[r][n][2 * half + 1], x.y, dot[half]));
-                  }
+                  for (int n = 0; n < 2 * NC; ++n)
+                    if (cw + 8 * n < p.vd) {
+                      const float2 x = pair_of(__ldg((const unsigned int*)((const bf16*)p.r + ra + 8 * n)));
+                      dot = fmaf(o[r][n][2 * half], x.x, fmaf(o[r][n][2 * half + 1], x.y, dot));
+                    }
+                }
+                dot += __shfl_xor_sync(0xffffffffu, dot, 1);
+                dot += __shfl_xor_sync(0xffffffffu, dot, 2);
+                if (tq == 0) rd[warp * 64 + row] = dot;
               }
-              dot[half] += __shfl_xor_sync(0xffffffffu, dot[half], 1);
-              dot[half] += __shfl_xor_sync(0xffffffffu, dot[half], 2);
-              if (tq == 0) rd[warp * 64 + row] = dot[half];
+          }
+#pragma unroll 1
+          for (int kj = 0; kj <= m + 16; kj += 16) {
+            uint32_t a[2][4], b[NC][4];
+            bool odd = false;
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+              ldsm_t(b[n], uv + kj * VP + (lav ^ (n * 32)));
+              odd = odd || not_finite(b[n]);
+            }
+            odd = __any_sync(0xffffffffu, odd);
+            ldsm(a[1], up + (m + 16) * 128 + (lap ^ (kj * 2)));
+            if (odd && kj == m + 16) {
+              diagonal_by_sums<VP, 2 * NC, false>(o[1], up, uv, kj, cl, gr, tq);
+            } else {
+#pragma unroll
+              for (int n = 0; n < NC; ++n) { mma16(o[1][2 * n], a[1], b[n][0], b[n][1]); mma16(o[1][2 * n + 1], a[1], b[n][2], b[n][3]); }
+            }
+            if (kj <= m) {
+              ldsm(a[0], up + m * 128 + (lap ^ (kj * 2)));
+              if (odd && kj == m) {
+                diagonal_by_sums<VP, 2 * NC, false>(o[0], up, uv, kj, cl, gr, tq);
+              } else {
+#pragma unroll
+                for (int n = 0; n < NC; ++n) { mma16(o[0][2 * n], a[0], b[n][0], b[n][1]); mma16(o[0][2 * n + 1], a[0], b[n][2], b[n][3]); }
+              }
             }
           }
-        }
-        for (int kj = 0; kj <= m / 16 + 1; ++kj) {
-          uint32_t a[2][4], b[NC][4];
-#pragma unroll
-          for (int n = 0; n < NC; ++n) frag_bt<VP>(b[n], uv, kj * 16, cl + 16 * n, lane);
-          frag_a<128>(a[1], up, m + 16, kj * 16, lane);
-#pragma unroll
-          for (int n = 0; n < NC; ++n) { mma16(o[1][2 * n], a[1], b[n][0], b[n][1]); mma16(o[1][2 * n + 1], a[1], b[n][2], b[n][3]); }
-          if (kj <= m / 16) {
-            frag_a<128>(a[0], up, m, kj * 16, lane);
-#pragma unroll
-            for (int n = 0; n < NC; ++n) { mma16(o[0][2 * n], a[0], b[n][0], b[n][1]); mma16(o[0][2 * n + 1], a[0], b[n][2], b[n][3]); }
-          }
-        }
-        // A value that is not finite meets the zeros above the diagonal (0 x inf); the recurrence has it at its own token
-        // and after only, so what is not finite is summed again over j <= i
-        float bad = 0.f;
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int n = 0; n < 2 * NC; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) bad = fmaf(o[r][n][e], 0.f, bad);
-        if (__any_sync(0xffffffffu, bad != 0.f)) {
-          float keep[2][2 * NC][4];
-          inter(keep);
 #pragma unroll
           for (int r = 0; r < 2; ++r)
 #pragma unroll
-            for (int n = 0; n < 2 * NC; ++n)
+            for (int half = 0; half < 2; ++half) {
+              const int row = m + 16 * r + gr + 8 * half;
+              if (p.out_f32 || NC == 1) {
+                const int64_t at = ((t0 + row) * p.H + h) * p.vd + cw + 2 * tq;
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (!(fabsf(o[r][n][e]) <= 3.402823466e38f)) {
-                  const int row = m + 16 * r + gr + 8 * (e / 2), c = cl + 8 * n + 2 * tq + e % 2;
-                  float x = keep[r][n][e];
-#pragma unroll 1
-                  for (int j = 0; j <= row; ++j) {
-                    uint16_t s, v;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(s) : "r"(at16<128>(up, row, j / 8) + (j % 8) * 2));
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at16<VP>(uv, j, c / 8) + (c % 8) * 2));
-                    x = fmaf(__uint_as_float((uint32_t)s << 16), __uint_as_float((uint32_t)v << 16), x);
+                for (int n = 0; n < 2 * NC; ++n)
+                  if (row < nv && cw + 8 * n < p.vd) {
+                    const float x = o[r][n][2 * half], y = o[r][n][2 * half + 1];
+                    if (p.out_f32) *reinterpret_cast<float2*>((float*)p.out + at + 8 * n) = make_float2(x, y);
+                    else *reinterpret_cast<uint32_t*>((bf16*)p.out + at + 8 * n) = pack_bf16x2(x, y);
                   }
-                  o[r][n][e] = x;
-                }
-        }
-        __syncwarp();
+              } else {
+                uint32_t v[4];
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int row = m + 16 * r + gr + 8 * half;
-            if (row < nv) {
-              const int64_t at = ((t0 + row) * p.H + h) * p.vd + cw + 2 * tq;
-#pragma unroll
-              for (int n = 0; n < 2 * NC; ++n)
-                if (cw + 8 * n < p.vd) {
-                  const float x = o[r][n][2 * half], y = o[r][n][2 * half + 1];
-                  if (p.out_f32) *reinterpret_cast<float2*>((float*)p.out + at + 8 * n) = make_float2(x, y);
-                  else *reinterpret_cast<uint32_t*>((bf16*)p.out + at + 8 * n) = pack_bf16x2(x, y);
-                }
+                for (int n = 0; n < 4; ++n) v[n] = pack_bf16x2(o[r][n % (2 * NC)][2 * half], o[r][n % (2 * NC)][2 * half + 1]);
+                transpose4(v, tq);
+                if (row < nv && cw + 8 * tq < p.vd)
+                  *reinterpret_cast<uint4*>((bf16*)p.out + ((t0 + row) * p.H + h) * p.vd + cw + 8 * tq) = make_uint4(v[0], v[1], v[2], v[3]);
+              }
             }
-          }
       }
-    } else {
-      // (the gates of the next chunk are read behind the next barrier)
     }
     // the state: st = exp(lam_L) st + (w V)^T K, backwards in time with exp(lam_i) as weights
-    const float all = wt[63].x;
+    const float all = gs.wt[63].x;
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
       for (int j = 0; j < KT; ++j)
 #pragma unroll
         for (int e = 0; e < 4; ++e) st[n][j][e] *= all;
+    const float* ws = &gs.wt[0].x + (p.rev ? 0 : 1);
 #pragma unroll 1
     for (int kk = 0; kk < 64 && kk < nv; kk += 16) {
-      const int j = kk + 2 * tq;
-      const float w[4] = {p.rev ? wt[j].x : wt[j].y, p.rev ? wt[j + 1].x : wt[j + 1].y, p.rev ? wt[j + 8].x : wt[j + 8].y,
-                          p.rev ? wt[j + 9].x : wt[j + 9].y};
+      const int j = 2 * (kk + 2 * tq);
+      const float w[4] = {ws[j], ws[j + 2], ws[j + 16], ws[j + 18]};
       uint32_t z[NC][NU][4];
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
         uint32_t a[4];
-        frag_at<VP>(a, uv, kk, cl + 16 * n, lane);
+        ldsm_t(a, uv + kk * VP + (lbv ^ (n * 32)));
         weighted<NU>(z[n], a, w);
       }
 #pragma unroll
       for (int t = 0; t < KD / 16; ++t) {
         uint32_t b[1][4];
-        frag_bt<QP>(b[0], uk, kk, t * 16, lane);
+        ldsm_t(b[0], uk + kk * QP + (laq ^ (t * 32)));
+        if constexpr (NU > 2) {
 #pragma unroll
-        for (int n = 0; n < NC; ++n) mma_planes<NU, 1, (NU > 2)>(st[n][2 * t], st[n][2 * t + 1], z[n], b);
+          for (int n = 0; n < NC; ++n) mma_planes<NU, 1, true>(st[n][2 * t], st[n][2 * t + 1], z[n], b);
+        } else {
+#pragma unroll
+          for (int s = NU - 1; s >= 0; --s)
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+              mma16(st[n][2 * t], z[n][s], b[0][0], b[0][1]);
+              mma16(st[n][2 * t + 1], z[n][s], b[0][2], b[0][3]);
+            }
+        }
       }
     }
   }
@@ -376,7 +451,7 @@ __global__ void __launch_bounds__(128, 2) fast_walk_kernel(const Walk p) {
       __syncthreads();
       const int c0 = 64 * (chunks - 1);
       if (tid < len - c0)
-        p.rdot[(vt * (p.cu ? p.T : p.nseq * p.T) + run.base + run.lo + c0 + tid) * p.H + h] = (rd[tid] + rd[64 + tid]) + (rd[128 + tid] + rd[192 + tid]);
+        p.rdot[(vt * (p.cu ? p.T : p.nseq * p.T) + r0 + c0 + tid) * p.H + h] = (rd[tid] + rd[64 + tid]) + (rd[128 + tid] + rd[192 + tid]);
     }
     if ((p.fin || p.fin32) && run.last) {
 #pragma unroll
@@ -428,8 +503,8 @@ struct Back {
 template <int DK, int DV, int NS>
 struct BLay {
   static constexpr int TK = 128 * DK, TV = 128 * DV, STAGE = 2 * TK + 2 * TV;
-  static constexpr int S0 = 2 * STAGE, SP = DK * DV * 2, P0 = S0 + NS * SP, D0 = P0 + 8192, LAM = D0 + 8192, WT = LAM + 1024;
-  static constexpr int RS = WT + 1024, CS = RS + 2 * 2048, BD = CS + 2 * 1024, RED = BD + 2 * 512, END = RED + 64;
+  static constexpr int S0 = 2 * STAGE, SP = DK * DV * 2, P0 = S0 + NS * SP, D0 = P0 + 8192, G0 = D0 + 8192;
+  static constexpr int RS = G0 + 2 * (int)sizeof(Gates), CS = RS + 2 * 2048, BD = CS + 2 * 1024, RED = BD + 2 * 512, END = RED + 64;
 };
 template <int DK, int DV, bool GATE>
 __global__ void __launch_bounds__(256, 1) fast_back_kernel(const Back q) {
@@ -437,9 +512,8 @@ __global__ void __launch_bounds__(256, 1) fast_back_kernel(const Back q) {
   using Y = BLay<DK, DV, NS>;
   constexpr int KP = 2 * DK, VP = 2 * DV, MR = DK / 64, NV = DV / 16;   // update: MR x 16 rows and NV tiles of 8 columns per warp
   const Walk& p = q.w;
-  extern __shared__ __align__(128) uint8_t sm[];
-  float2* lam_ = reinterpret_cast<float2*>(sm + Y::LAM);
-  float2* wt_ = reinterpret_cast<float2*>(sm + Y::WT);
+  extern __shared__ __align__(256) uint8_t sm[];
+  Gates* gates_ = reinterpret_cast<Gates*>(sm + Y::G0);
   float* rs_ = reinterpret_cast<float*>(sm + Y::RS);           // [2][8 tiles of columns][64]: sums of a row of M over 8 columns
   float* cs_ = reinterpret_cast<float*>(sm + Y::CS);           // [2][4 tiles of rows][64]
   float* bd_ = reinterpret_cast<float*>(sm + Y::BD);           // [2][2 halves][64]
@@ -482,23 +556,23 @@ __global__ void __launch_bounds__(256, 1) fast_back_kernel(const Back q) {
   }
   const int Hq = p.H / p.gq, len = (int)(run.hi - run.lo), chunks = (len + 63) / 64;
   const uint32_t base = sm32(sm);
+  const int64_t r0_ = run.base + run.lo, sk = (int64_t)Hq * p.kd, sv = (int64_t)p.H * p.vd;
+  const int64_t ok = r0_ * sk + h / p.gq * p.kd, ov = r0_ * sv + (int64_t)h * p.vd;
   const auto fetch = [&](int i) {
     const int nv = len - 64 * i < 64 ? len - 64 * i : 64;
-    const int64_t t0 = run.base + run.lo + 64 * i;
     const uint32_t s = base + (i & 1) * Y::STAGE;
-    const int64_t rk = (t0 * Hq + h / p.gq) * p.kd, rv = (t0 * p.H + h) * p.vd;
-    fetch_tile<DK, 256>(s, p.q, rk, (int64_t)Hq * p.kd, nv, p.kd);
-    fetch_tile<DK, 256>(s + Y::TK, p.k, rk, (int64_t)Hq * p.kd, nv, p.kd);
-    fetch_tile<DV, 256>(s + 2 * Y::TK, p.v, rv, (int64_t)p.H * p.vd, nv, p.vd);
-    fetch_tile<DV, 256>(s + 2 * Y::TK + Y::TV, q.dout, rv, (int64_t)p.H * p.vd, nv, p.vd);
+    const int64_t rk = ok + 64 * i * sk, rv = ov + 64 * i * sv;
+    fetch_tile<DK, 256>(s, (const bf16*)p.q + rk, sk, nv, p.kd);
+    fetch_tile<DK, 256>(s + Y::TK, (const bf16*)p.k + rk, sk, nv, p.kd);
+    fetch_tile<DV, 256>(s + 2 * Y::TK, (const bf16*)p.v + rv, sv, nv, p.vd);
+    fetch_tile<DV, 256>(s + 2 * Y::TK + Y::TV, (const bf16*)q.dout + rv, sv, nv, p.vd);
   };
   if (chunks) {
     fetch(chunks - 1);
-    if (warp == 0)
-      scan_gates(gates_of(p, run.base + run.lo + 64 * (chunks - 1), len - 64 * (chunks - 1), h, lane), lam_ + 64 * ((chunks - 1) & 1),
-                 wt_ + 64 * ((chunks - 1) & 1), lane);
+    if (warp == 0) scan_gates(gates_of(p, r0_ + 64 * (chunks - 1), len - 64 * (chunks - 1), h, lane), gates_[(chunks - 1) & 1], lane);
   }
   cp_commit();
+  const uint32_t lak = lane_a<KP>(lane), lbk = lane_b<KP>(lane), lav = lane_a<VP>(lane), lbv = lane_b<VP>(lane), lbp = lane_b<128>(lane);
   // gradient of the gates of chunk i, by one warp, once its sums are there
   const auto gates = [&](int i) {
     const int nv = len - 64 * i < 64 ? len - 64 * i : 64;
@@ -530,7 +604,7 @@ __global__ void __launch_bounds__(256, 1) fast_back_kernel(const Back q) {
     const int nv = len - 64 * i < 64 ? len - 64 * i : 64;
     const int64_t t0 = run.base + run.lo + 64 * i;
     const uint32_t uq = base + (i & 1) * Y::STAGE, uk = uq + Y::TK, uv = uk + Y::TK, uo = uv + Y::TV, us = base + Y::S0, up = base + Y::P0, ud = base + Y::D0;
-    const float2 *lam = lam_ + 64 * (i & 1), *wt = wt_ + 64 * (i & 1);
+    const Gates& gs = gates_[i & 1];
     cp_wait<0>();
     __syncthreads();
     float2 gn = make_float2(0.f, 0.f);
@@ -556,53 +630,56 @@ __global__ void __launch_bounds__(256, 1) fast_back_kernel(const Back q) {
     // scores and their gradients, 16 x 8 of both at a time
 #pragma unroll 1
     for (int u = warp; u < 20; u += 8) {
-      const int mi = u < 2 ? 0 : u < 6 ? 1 : u < 12 ? 2 : 3, nt = u - mi * (mi + 1);
+      const int mi = u < 2 ? 0 : u < 6 ? 1 : u < 12 ? 2 : 3, nt = u - mi * (mi + 1), r = mi * 16 + gr, j = nt * 8 + 2 * tq;
       float c[4] = {}, d[4] = {};
+      // eight rows of K (V) x 32 features: four matrices side by side
+      const uint32_t l8 = (lane & 7) * KP + (((lane >> 3) ^ (lane & 7)) << 4), l8v = (lane & 7) * VP + (((lane >> 3) ^ (lane & 7)) << 4);
 #pragma unroll
       for (int kk = 0; kk < DK / 32; ++kk) {
         uint32_t a[4], a2[4], b[4];
-        ldsm(b, at16<KP>(uk, nt * 8 + (lane & 7), kk * 4 + (lane >> 3)));
-        frag_a<KP>(a, uq, mi * 16, kk * 32, lane);
-        frag_a<KP>(a2, uq, mi * 16, kk * 32 + 16, lane);
+        ldsm(b, uk + nt * 8 * KP + (l8 ^ (kk * 64)));
+        ldsm(a, uq + mi * 16 * KP + (lak ^ (kk * 64)));
+        ldsm(a2, uq + mi * 16 * KP + (lak ^ (kk * 64 + 32)));
         mma16(c, a, b[0], b[1]);
         mma16(c, a2, b[2], b[3]);
       }
 #pragma unroll
       for (int kk = 0; kk < DV / 32; ++kk) {
         uint32_t a[4], a2[4], b[4];
-        ldsm(b, at16<VP>(uv, nt * 8 + (lane & 7), kk * 4 + (lane >> 3)));
-        frag_a<VP>(a, uo, mi * 16, kk * 32, lane);
-        frag_a<VP>(a2, uo, mi * 16, kk * 32 + 16, lane);
+        ldsm(b, uv + nt * 8 * VP + (l8v ^ (kk * 64)));
+        ldsm(a, uo + mi * 16 * VP + (lav ^ (kk * 64)));
+        ldsm(a2, uo + mi * 16 * VP + (lav ^ (kk * 64 + 32)));
         mma16(d, a, b[0], b[1]);
         mma16(d, a2, b[2], b[3]);
       }
-      float cm[2] = {0.f, 0.f};
+      float w[4], x[4], m[4];
+      weights_of(w, gs, mi, nt / 2, r, j);
+      const bool diag = mi == nt / 2;
 #pragma unroll
-      for (int e = 0; e < 4; e += 2) {
-        const int r = mi * 16 + gr + 4 * e, j = nt * 8 + 2 * tq;
-        const float w0 = j <= r ? decay_of(lam[r], lam[j]) : 0.f, w1 = j + 1 <= r ? decay_of(lam[r], lam[j + 1]) : 0.f;
-        const float x0 = j <= r ? c[e] * w0 : 0.f, x1 = j + 1 <= r ? c[e + 1] * w1 : 0.f;
-        const uint32_t at = at16<128>(0, r, nt) + 4 * tq;
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(up + at), "r"(pack_bf16x2(x0, x1)) : "memory");
-        asm volatile("st.shared.b32 [%0], %1;" ::"r"(ud + at), "r"(pack_bf16x2(j <= r ? d[e] * w0 : 0.f, j + 1 <= r ? d[e + 1] * w1 : 0.f)) : "memory");
-        if constexpr (GATE) {
-          const float m0 = j <= r ? x0 * d[e] : 0.f, m1 = j + 1 <= r ? x1 * d[e + 1] : 0.f;
-          cm[0] += m0;
-          cm[1] += m1;
-          float x = m0 + m1;
-          x += __shfl_xor_sync(0xffffffffu, x, 1);
-          x += __shfl_xor_sync(0xffffffffu, x, 2);
-          if (tq == 0) rs_[(i & 1) * 512 + nt * 64 + r] = x;
-        }
+      for (int e = 0; e < 4; ++e) {
+        const bool off = diag && j + e % 2 > r + 8 * (e / 2);
+        x[e] = off ? 0.f : c[e] * w[e];
+        m[e] = off ? 0.f : x[e] * d[e];
+        d[e] = off ? 0.f : d[e] * w[e];
       }
+      const uint32_t at = at16<128>(0, r, nt) + 4 * tq;
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(up + at), "r"(pack_bf16x2(x[0], x[1])) : "memory");
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(up + at + 1024), "r"(pack_bf16x2(x[2], x[3])) : "memory");
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(ud + at), "r"(pack_bf16x2(d[0], d[1])) : "memory");
+      asm volatile("st.shared.b32 [%0], %1;" ::"r"(ud + at + 1024), "r"(pack_bf16x2(d[2], d[3])) : "memory");
       if constexpr (GATE) {
+        float a = m[0] + m[1], b = m[2] + m[3], y = m[0] + m[2], z = m[1] + m[3];
 #pragma unroll
-        for (int s = 4; s < 32; s <<= 1) { cm[0] += __shfl_xor_sync(0xffffffffu, cm[0], s); cm[1] += __shfl_xor_sync(0xffffffffu, cm[1], s); }
-        if (gr == 0) *reinterpret_cast<float2*>(cs_ + (i & 1) * 256 + mi * 64 + nt * 8 + 2 * tq) = make_float2(cm[0], cm[1]);
+        for (int s = 1; s < 4; s <<= 1) { a += __shfl_xor_sync(0xffffffffu, a, s); b += __shfl_xor_sync(0xffffffffu, b, s); }
+#pragma unroll
+        for (int s = 4; s < 32; s <<= 1) { y += __shfl_xor_sync(0xffffffffu, y, s); z += __shfl_xor_sync(0xffffffffu, z, s); }
+        float* rs = rs_ + (i & 1) * 512 + nt * 64 + r;
+        if (tq == 0) { rs[0] = a; rs[8] = b; }
+        if (gr == 0) *reinterpret_cast<float2*>(cs_ + (i & 1) * 256 + mi * 64 + j) = make_float2(y, z);
       }
     }
     if (warp == 7) {
-      if (i > 0) scan_gates(gn, lam_ + 64 * ((i - 1) & 1), wt_ + 64 * ((i - 1) & 1), lane);
+      if (i > 0) scan_gates(gn, gates_[(i - 1) & 1], lane);
       if (GATE && i + 1 < chunks) gates(i + 1);
     }
     __syncthreads();
@@ -615,123 +692,104 @@ __global__ void __launch_bounds__(256, 1) fast_back_kernel(const Back q) {
         constexpr int AP = DKO ? VP : KP, BP = DKO ? KP : VP, NT8 = ND / 16;
         const uint32_t ta = DKO ? uv : uk, tb = DKO ? uq : uo, ts = DKO ? ud : up;
         const int n0 = half * (ND / 2), nd = DKO ? p.kd : p.vd;
-        float o[2][NT8][4];
-        const auto inter = [&](float (&x)[2][NT8][4]) {
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int n = 0; n < NT8; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) x[r][n][e] = 0.f;
+          float o[2][NT8][4] = {};
 #pragma unroll 2
           for (int kk = 0; kk < KD / 16; ++kk) {
             uint32_t a[2][4];
-            frag_a<AP>(a[0], ta, r0, kk * 16, lane);
-            frag_a<AP>(a[1], ta, r1, kk * 16, lane);
+            ldsm(a[0], ta + r0 * AP + ((DKO ? lav : lak) ^ (kk * 32)));
+            ldsm(a[1], ta + r1 * AP + ((DKO ? lav : lak) ^ (kk * 32)));
 #pragma unroll
-            for (int n = 0; n < NT8 / 2; ++n)
+            for (int s = NS - 1; s >= 0; --s)
 #pragma unroll
-              for (int s = NS - 1; s >= 0; --s) {
+              for (int n = 0; n < NT8 / 2; ++n) {
                 uint32_t b[4];
-                if constexpr (DKO) frag_b<VP>(b, us + s * Y::SP, n0 + 16 * n, kk * 16, lane);
-                else frag_bt<VP>(b, us + s * Y::SP, kk * 16, n0 + 16 * n, lane);
+                if constexpr (DKO) ldsm(b, us + s * Y::SP + (n0 + 16 * n) * VP + (lbv ^ (kk * 32)));
+                else ldsm_t(b, us + s * Y::SP + kk * 16 * VP + (lav ^ (n0 * 2 + 32 * n)));
 #pragma unroll
-                for (int r = 0; r < 2; ++r) { mma16(x[r][2 * n], a[r], b[0], b[1]); mma16(x[r][2 * n + 1], a[r], b[2], b[3]); }
+                for (int r = 0; r < 2; ++r) { mma16(o[r][2 * n], a[r], b[0], b[1]); mma16(o[r][2 * n + 1], a[r], b[2], b[3]); }
               }
           }
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
             const int row = (r ? r1 : r0) + gr;
-            const float w0 = wt[row].y, w1 = wt[row + 8].y;
+            const float w0 = gs.wt[row].y, w1 = gs.wt[row + 8].y;
 #pragma unroll
-            for (int n = 0; n < NT8; ++n) { x[r][n][0] *= w0; x[r][n][1] *= w0; x[r][n][2] *= w1; x[r][n][3] *= w1; }
+            for (int n = 0; n < NT8; ++n) { o[r][n][0] *= w0; o[r][n][1] *= w0; o[r][n][2] *= w1; o[r][n][3] *= w1; }
           }
-        };
-        inter(o);
-        if constexpr (DKO && GATE) {
+          if constexpr (DKO && GATE) {
+#pragma unroll
+            for (int r = 0; r < 2; ++r)
+#pragma unroll
+              for (int hf = 0; hf < 2; ++hf) {
+                const int row = (r ? r1 : r0) + gr + 8 * hf;
+                float x = 0.f;
+#pragma unroll
+                for (int n = 0; n < NT8; ++n) {
+                  uint32_t kk;
+                  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(kk) : "r"(at16<KP>(uk, row, n0 / 8 + n) + 4 * tq));
+                  const float2 y = pair_of(kk);
+                  x = fmaf(o[r][n][2 * hf], y.x, fmaf(o[r][n][2 * hf + 1], y.y, x));
+                }
+                x += __shfl_xor_sync(0xffffffffu, x, 1);
+                x += __shfl_xor_sync(0xffffffffu, x, 2);
+                if (tq == 0) bd_[(i & 1) * 128 + half * 64 + row] = x;
+              }
+          }
+#pragma unroll 1
+          for (int ki = r0; ki < 64 && ki < nv; ki += 16) {
+            uint32_t a[2][4];
+            ldsm_t(a[0], ts + ki * 128 + (lbp ^ (r0 * 2)));
+            const bool both = ki >= r1;
+            if (both) ldsm_t(a[1], ts + ki * 128 + (lbp ^ (r1 * 2)));
+            uint32_t b[NT8 / 2][4];
+            bool odd = false;
+#pragma unroll
+            for (int n = 0; n < NT8 / 2; ++n) {
+              ldsm_t(b[n], tb + ki * BP + ((DKO ? lak : lav) ^ (n0 * 2 + 32 * n)));
+              odd = odd || not_finite(b[n]);
+            }
+            odd = __any_sync(0xffffffffu, odd);
+            if (odd && ki == r0) {
+              diagonal_by_sums<BP, NT8, true>(o[0], ts, tb, ki, n0, gr, tq);
+            } else {
+#pragma unroll
+              for (int n = 0; n < NT8 / 2; ++n) { mma16(o[0][2 * n], a[0], b[n][0], b[n][1]); mma16(o[0][2 * n + 1], a[0], b[n][2], b[n][3]); }
+            }
+            if (odd && ki == r1) {
+              diagonal_by_sums<BP, NT8, true>(o[1], ts, tb, ki, n0, gr, tq);
+            } else if (both) {
+#pragma unroll
+              for (int n = 0; n < NT8 / 2; ++n) { mma16(o[1][2 * n], a[1], b[n][0], b[n][1]); mma16(o[1][2 * n + 1], a[1], b[n][2], b[n][3]); }
+            }
+          }
 #pragma unroll
           for (int r = 0; r < 2; ++r)
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
               const int row = (r ? r1 : r0) + gr + 8 * hf;
-              float x = 0.f;
+              const int64_t at = ((t0 + row) * p.H + h) * nd + n0;
+              if (DKO && q.dk_f32) {
 #pragma unroll
-              for (int n = 0; n < NT8; ++n) {
-                uint32_t kk;
-                asm volatile("ld.shared.b32 %0, [%1];" : "=r"(kk) : "r"(at16<KP>(uk, row, n0 / 8 + n) + 4 * tq));
-                const float2 y = pair_of(kk);
-                x = fmaf(o[r][n][2 * hf], y.x, fmaf(o[r][n][2 * hf + 1], y.y, x));
+                for (int n = 0; n < NT8; ++n)
+                  if (row < nv && n0 + 8 * n < nd)
+                    *reinterpret_cast<float2*>((float*)q.dk + at + 8 * n + 2 * tq) = make_float2(o[r][n][2 * hf], o[r][n][2 * hf + 1]);
+              } else {
+#pragma unroll
+                for (int g = 0; g < NT8; g += 4) {
+                  uint32_t v[4];
+#pragma unroll
+                  for (int n = 0; n < 4; ++n) v[n] = pack_bf16x2(o[r][g + n][2 * hf], o[r][g + n][2 * hf + 1]);
+                  transpose4(v, tq);
+                  if (row < nv && n0 + 8 * (g + tq) < nd)
+                    *reinterpret_cast<uint4*>((bf16*)(DKO ? q.dk : q.dv) + at + 8 * (g + tq)) = make_uint4(v[0], v[1], v[2], v[3]);
+                }
               }
-              x += __shfl_xor_sync(0xffffffffu, x, 1);
-              x += __shfl_xor_sync(0xffffffffu, x, 2);
-              if (tq == 0) bd_[(i & 1) * 128 + half * 64 + row] = x;
             }
-        }
-        for (int ki = r0 / 16; ki < 4 && ki * 16 < nv; ++ki) {
-          uint32_t a[2][4];
-          frag_at<128>(a[0], ts, ki * 16, r0, lane);
-          if (ki * 16 >= r1) frag_at<128>(a[1], ts, ki * 16, r1, lane);
-#pragma unroll
-          for (int n = 0; n < NT8 / 2; ++n) {
-            uint32_t b[4];
-            frag_bt<BP>(b, tb, ki * 16, n0 + 16 * n, lane);
-            mma16(o[0][2 * n], a[0], b[0], b[1]);
-            mma16(o[0][2 * n + 1], a[0], b[2], b[3]);
-            if (ki * 16 >= r1) { mma16(o[1][2 * n], a[1], b[0], b[1]); mma16(o[1][2 * n + 1], a[1], b[2], b[3]); }
-          }
-        }
-        float bad = 0.f;
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int n = 0; n < NT8; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) bad = fmaf(o[r][n][e], 0.f, bad);
-        if (__any_sync(0xffffffffu, bad != 0.f)) {
-          // as in the forward: what is not finite is summed again, here over i >= j
-          float keep[2][NT8][4];
-          inter(keep);
-#pragma unroll
-          for (int r = 0; r < 2; ++r)
-#pragma unroll
-            for (int n = 0; n < NT8; ++n)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (!(fabsf(o[r][n][e]) <= 3.402823466e38f)) {
-                  const int j = (r ? r1 : r0) + gr + 8 * (e / 2), c = n0 + 8 * n + 2 * tq + e % 2;
-                  float x = keep[r][n][e];
-#pragma unroll 1
-                  for (int t = j; t < nv; ++t) {
-                    uint16_t s, v;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(s) : "r"(at16<128>(ts, t, j / 8) + (j % 8) * 2));
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(at16<BP>(tb, t, c / 8) + (c % 8) * 2));
-                    x = fmaf(__uint_as_float((uint32_t)s << 16), __uint_as_float((uint32_t)v << 16), x);
-                  }
-                  o[r][n][e] = x;
-                }
-        }
-        __syncwarp();
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {
-            const int row = (r ? r1 : r0) + gr + 8 * hf;
-            if (row < nv) {
-              const int64_t at = ((t0 + row) * p.H + h) * nd + n0 + 2 * tq;
-#pragma unroll
-              for (int n = 0; n < NT8; ++n)
-                if (n0 + 8 * n < nd) {
-                  const float x = o[r][n][2 * hf], y = o[r][n][2 * hf + 1];
-                  if (DKO && q.dk_f32) *reinterpret_cast<float2*>((float*)q.dk + at + 8 * n) = make_float2(x, y);
-                  else *reinterpret_cast<uint32_t*>((bf16*)(DKO ? q.dk : q.dv) + at + 8 * n) = pack_bf16x2(x, y);
-                }
-            }
-          }
       };
       if (warp >> 2) tile(std::true_type()); else tile(std::false_type());
     }
     // dS = exp(lam_L) dS + (exp(lam_i) Q)^T dO
-    const float all = wt[63].x;
+    const float all = gs.wt[63].x;
 #pragma unroll
     for (int m = 0; m < MR; ++m)
 #pragma unroll
@@ -741,20 +799,22 @@ __global__ void __launch_bounds__(256, 1) fast_back_kernel(const Back q) {
 #pragma unroll 1
     for (int kk = 0; kk < 64 && kk < nv; kk += 16) {
       const int j = kk + 2 * tq;
-      const float w[4] = {wt[j].x, wt[j + 1].x, wt[j + 8].x, wt[j + 9].x};
+      const float w[4] = {gs.wt[j].x, gs.wt[j + 1].x, gs.wt[j + 8].x, gs.wt[j + 9].x};
       uint32_t z[MR][2][4];
 #pragma unroll
       for (int m = 0; m < MR; ++m) {
         uint32_t a[4];
-        frag_at<KP>(a, uq, kk, ur + 16 * m, lane);
+        ldsm_t(a, uq + kk * KP + (lbk ^ (ur * 2 + 32 * m)));
         weighted<2>(z[m], a, w);
       }
 #pragma unroll
       for (int n = 0; n < NV / 2; ++n) {
-        uint32_t b[1][4];
-        frag_bt<VP>(b[0], uo, kk, uc + 16 * n, lane);
+        uint32_t b[4];
+        ldsm_t(b, uo + kk * VP + (lav ^ (uc * 2 + 32 * n)));
 #pragma unroll
-        for (int m = 0; m < MR; ++m) mma_planes<2, 1, false>(st[m][2 * n], st[m][2 * n + 1], z[m], b);
+        for (int s = 1; s >= 0; --s)
+#pragma unroll
+          for (int m = 0; m < MR; ++m) { mma16(st[m][2 * n], z[m][s], b[0], b[1]); mma16(st[m][2 * n + 1], z[m][s], b[2], b[3]); }
       }
     }
   }
