@@ -134,8 +134,8 @@ int64_t run_tokens(int64_t T, int64_t nseq, int64_t H, int64_t vd, bool packed) 
   int64_t n = packed ? want / (H * ((vd + 127) / 128)) : want / blocks;      // runs: of the packed axis, of each sequence
   if (blocks * 2 > want) n = 1;
   if (n > T / 256) n = T / 256;
-  if (n <= 1) return align_up(T, 64);
-  return align_up((T + n - 1) / n, 64);
+  if (n <= 1) return align_up(T, 128);
+  return align_up((T + n - 1) / n, 128);
 }
 
 }  // namespace
