@@ -130,7 +130,7 @@ int sm_count() {
 // Tokens of a run.  A walk has a block per run, head and tile of value columns; with fewer blocks than the device holds
 // (two per SM) sequences are cut into runs, at the price of reading k and v twice.  Runs shorter than 256 tokens do not pay.
 int64_t run_tokens(int64_t T, int64_t nseq, int64_t H, int64_t vd, bool packed) {
-  const int64_t blocks = H * ((vd + 127) / 128) * nseq, want = 2 * (int64_t)sm_count();
+  const int64_t blocks = H * ((vd + 127) / 128) * nseq, want = (int64_t)sm_count();
   int64_t n = packed ? want / (H * ((vd + 127) / 128)) : want / blocks;      // runs: of the packed axis, of each sequence
   if (blocks * 2 > want) n = 1;
   if (n > T / 256) n = T / 256;

@@ -63,7 +63,7 @@ __device__ __forceinline__ void fetch128(uint32_t tile, const bf16* src, int64_t
   const bf16* g = src + r0 * step + c * 8;
   const uint32_t dst = tile + (c >> 3) * 16384 + sw128_chunk(r0, c & 7);
   const int n = c * 8 < d ? nv - r0 : 0;
-#pragma unroll
+#pragma unroll 2
   for (int j = 0; j < 128 / RS; ++j) {
     cp16(dst + j * RS * 128, RS * j < n ? g : src, RS * j < n);
     g += RS * step;
@@ -121,13 +121,14 @@ __device__ __forceinline__ float decay_of(float2 i, float2 j) { return ex2((i.x 
 template <int D, int NU>
 __device__ __forceinline__ void weigh(uint32_t tile, uint32_t lo, uint32_t plane, const float2* wt, bool rev) {
   const int r0 = threadIdx.x / 8, c = threadIdx.x % 8;
+  const float* w_ = &wt[r0].x + (rev ? 0 : 1);
+  const uint32_t at0 = sw128_chunk(r0, c);
+#pragma unroll 1
+  for (int j = 0; j < 4; ++j) {
+    const float w = w_[64 * j];
 #pragma unroll
-  for (int b = 0; b < D / 64; ++b)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = r0 + 32 * j;
-      const uint32_t at = b * 16384 + sw128_chunk(r, c);
-      const float w = rev ? wt[r].x : wt[r].y;
+    for (int b = 0; b < D / 64; ++b) {
+      const uint32_t at = b * 16384 + j * 4096 + at0;
       const uint4 x = lds16(tile + at);
       const uint32_t u[4] = {x.x, x.y, x.z, x.w};
       uint32_t s[4][NU];
@@ -140,6 +141,7 @@ __device__ __forceinline__ void weigh(uint32_t tile, uint32_t lo, uint32_t plane
 #pragma unroll
       for (int k = 1; k < NU; ++k) sts16(lo + (k - 1) * plane + at, make_uint4(s[0][k], s[1][k], s[2][k], s[3][k]));
     }
+  }
 }
 // whether the pieces that the thread itself fetched of a tile hold something that is not finite
 template <int D>
@@ -147,7 +149,7 @@ __device__ __forceinline__ bool odd_values(uint32_t tile) {
   constexpr int C8 = D / 8, RS = 256 / C8;
   const int r0 = threadIdx.x / C8, c = threadIdx.x % C8;
   bool x = false;
-#pragma unroll
+#pragma unroll 2
   for (int j = 0; j < 128 / RS; ++j) {
     const uint4 v = lds16(tile + (c >> 3) * 16384 + sw128_chunk(r0, c & 7) + j * RS * 128);
     const uint32_t u[4] = {v.x, v.y, v.z, v.w};
@@ -270,13 +272,19 @@ __global__ void __launch_bounds__(256, 1) tc_walk_kernel(const Walk p) {
 
   // the state: row `row` (a key feature), columns HV half + [0, HV)
   float S[HV];
+  const int cols = row < p.kd ? p.vd - HV * half : 0;           // that there are of them
+  if (!OUT) {
 #pragma unroll
-  for (int j = 0; j < HV; ++j) {
-    const int c = HV * half + j;
-    float x = 0.f;
-    if (OUT && row < p.kd && c < p.vd)
-      x = p.seg_state ? p.seg_state[slot_h * dd + row * p.sk + c * p.sc] : ld_any(p.init, !p.init_f32, sh * dd + row * p.ik + c * p.ic);
-    S[j] = x;
+    for (int j = 0; j < HV; ++j) S[j] = 0.f;
+  } else if (p.seg_state || p.init_f32) {
+    const float* x = p.seg_state ? p.seg_state + slot_h * dd + row * p.sk + HV * half * p.sc : (const float*)p.init + sh * dd + row * p.ik + HV * half * p.ic;
+    const int64_t d = p.seg_state ? p.sc : p.ic;
+#pragma unroll
+    for (int j = 0; j < HV; ++j, x += d) S[j] = j < cols ? *x : 0.f;
+  } else {
+    const bf16* x = (const bf16*)p.init + sh * dd + row * p.ik + HV * half * p.ic;
+#pragma unroll
+    for (int j = 0; j < HV; ++j, x += p.ic) S[j] = j < cols ? __bfloat162float(*x) : 0.f;
   }
   // its image for Q S: [feature][column], 64 columns a tile
   const auto put_state = [&]() {
@@ -334,7 +342,7 @@ __global__ void __launch_bounds__(256, 1) tc_walk_kernel(const Walk p) {
     if constexpr (OUT) {
       if (ok) ok = mbar_wait(bar, ph);    // scores; K may be overwritten
       tc_fence_after();
-#pragma unroll
+#pragma unroll 1
       for (int g = 0; g < 2; ++g) {
         const int grp = 2 * half + g;     // columns 32 grp + [0, 32)
         uint32_t pk[16];
@@ -404,7 +412,7 @@ __global__ void __launch_bounds__(256, 1) tc_walk_kernel(const Walk p) {
       const int64_t at = ((t0 + row) * p.H + h) * p.vd + HV * half;
       const int64_t ra = p.r ? ((t0 + row) * (p.H / p.gr) + h / p.gr) * p.vd + HV * half : 0;
       float dot = 0.f;
-#pragma unroll
+#pragma unroll 1
       for (int c0 = 0; c0 < HV; c0 += 16) {
         uint32_t a[16], b[16];
         tmem_ld16(tOI + lane_base + HV * half + c0, a);
@@ -473,26 +481,32 @@ __global__ void __launch_bounds__(256, 1) tc_walk_kernel(const Walk p) {
   if (warp == 0) tmem_dealloc(tmem, 512);
 
   if constexpr (OUT) {
-    if ((p.fin || p.fin32) && run.last && row < p.kd) {
+    if (run.last) {
+      const int64_t at = sh * dd + row * p.ik + HV * half * p.ic;
+      float* f = p.fin_f32 ? (float*)p.fin + at : p.fin32 + at;
+      if (p.fin_f32 ? p.fin != nullptr : p.fin32 != nullptr)
 #pragma unroll
-      for (int j = 0; j < HV; ++j) {
-        const int c = HV * half + j;
-        if (c < p.vd) {
-          const int64_t at = sh * dd + row * p.ik + c * p.ic;
-          if (p.fin) st_any(p.fin, !p.fin_f32, at, S[j]);
-          if (p.fin32) p.fin32[at] = S[j];
-        }
+        for (int j = 0; j < HV; ++j, f += p.ic)
+          if (j < cols) *f = S[j];
+      if (p.fin_f32 && p.fin32) {
+        f = p.fin32 + at;
+#pragma unroll
+        for (int j = 0; j < HV; ++j, f += p.ic)
+          if (j < cols) *f = S[j];
+      }
+      if (!p.fin_f32 && p.fin) {
+        bf16* o = (bf16*)p.fin + at;
+#pragma unroll
+        for (int j = 0; j < HV; ++j, o += p.ic)
+          if (j < cols) *o = __float2bfloat16_rn(S[j]);
       }
     }
   } else {
     if (warp == 7 && lane == 0) p.seg_total[slot_h] = total;
-    if (row < p.kd) {
+    float* f = p.seg_state + slot_h * dd + (int64_t)HV * half * p.kd + row;
 #pragma unroll
-      for (int j = 0; j < HV; ++j) {
-        const int c = HV * half + j;
-        if (c < p.vd) p.seg_state[slot_h * dd + (int64_t)c * p.kd + row] = S[j];
-      }
-    }
+    for (int j = 0; j < HV; ++j, f += p.kd)
+      if (j < cols) *f = S[j];
   }
 }
 
