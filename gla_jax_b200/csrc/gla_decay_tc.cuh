@@ -1,19 +1,21 @@
 // The walks of gla_decay.cuh on the fifth-generation tensor cores: bf16, head sizes up to 128, 128 tokens at a time.
 //
-// Per chunk, one thread issues  SC = Q K^T,  OI = Q S,  OA = P V  and  U = (w K)^T V  (w = exp(lam_L - lam_j), in two or three
-// bf16 planes); 256 threads turn SC into P in tensor memory (a thread per row and half of the columns), weigh K in place, add
-// exp(lam_i) OI + OA into out, and keep the state in registers: S <- exp(lam_L) S + U, from where its bf16 image goes to
-// shared memory for the next chunk.
+// Per chunk:  SC = Q K^T,  OI = Q S,  OA = P V  and  U = (w K)^T V  (w = exp(lam_L - lam_j), in two or three bf16 planes).  Eight
+// warps turn SC into P in tensor memory (a thread per row and half of the columns), weigh K in place, write exp(lam_i) OI + OA,
+// and keep the state in registers: S <- exp(lam_L) S + U, from where its bf16 image goes to shared memory for the next chunk.
+// One warp issues the products, one the tensor copies, one prepares the gates of the chunk to come.
 //
 // Why.  The same walk in mma.sync spends 14,000 instructions per 64 tokens, of which 1900 multiply: operand fragments, their
 // conversion and the accumulators' addressing are the work.  Here operands go from shared memory to the tensor cores as the
-// copies left them, and a chunk of 128 takes about 1500 instructions in each of eight warps.
+// copies left them.  The work is the CUDA cores' still (scores, weights, output and state: about 5000 cycles a chunk at
+// 128 x 128, the products 2600), which is why everything else has a warp of its own.
 //
 // Tiles: 128 rows x 64 columns of bf16, 128-byte rows, 16-byte pieces at piece ^ (row % 8) (tc_ptx.cuh); D columns are D / 64
-// of them.  Copies are cp.async rather than tensor copies, because a sequence may start and end anywhere: rows past its end
-// are zeros.
+// of them.  A copy brings 128 rows whatever the sequence's length: rows past its end are another sequence's or beyond the
+// array (zeros), and are zeroed where a product would meet them (keys as they are weighed, values in place).
 #pragma once
 #include "gla_decay.cuh"
+#include "tma_maps.cuh"
 
 namespace gla {
 namespace decay {
@@ -55,19 +57,40 @@ static inline unsigned int read_wait_timeouts() {
   return v;
 }
 
-// 128 rows of D columns into D / 64 tiles; src: row 0.  Rows from nv on and columns from d on are zeros.
-template <int D>
-__device__ __forceinline__ void fetch128(uint32_t tile, const bf16* src, int64_t step, int nv, int d) {
-  constexpr int C8 = D / 8, RS = 256 / C8;
-  const int r0 = threadIdx.x / C8, c = threadIdx.x % C8;
-  const bf16* g = src + r0 * step + c * 8;
-  const uint32_t dst = tile + (c >> 3) * 16384 + sw128_chunk(r0, c & 7);
-  const int n = c * 8 < d ? nv - r0 : 0;
-#pragma unroll 2
-  for (int j = 0; j < 128 / RS; ++j) {
-    cp16(dst + j * RS * 128, RS * j < n ? g : src, RS * j < n);
-    g += RS * step;
+// (tokens, heads, D) seen as 3-d (d, head, token); box 64 x 1 x 128, columns past D zeros
+inline int make_map_tokens(CUtensorMap* m, const void* ptr, int64_t rows, int64_t heads, int64_t D) {
+  if (rows > 0x7fffffffLL) return GLA_ERR_TOO_LARGE;
+  const MapKey key{ptr, rows, heads, 17, (int)D, 0, 0};
+  if (const CUtensorMap* hit = map_cache().find(key)) { *m = *hit; return GLA_OK; }
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return GLA_ERR_NO_DEVICE;
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows}, strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)(heads * D) * 2};
+  cuuint32_t box[3] = {64, 1, 128}, estr[3] = {1, 1, 1};
+  const auto encode = [&]() {
+    return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void*)ptr, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // a host thread that has not launched yet (autograd's, in a process's first backward): selecting its device binds it
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return GLA_ERR_NO_DEVICE;
+    r = encode();
   }
+  if (r != CUDA_SUCCESS) return GLA_ERR_LAUNCH;
+  map_cache().put(key, *m);
+  return GLA_OK;
+}
+// A wait that looks before it sleeps; bounded like mbar_wait, and after one that ran out nothing waits any more.
+__device__ __forceinline__ void wait_for(bool& ok, uint32_t bar, uint32_t parity) {
+  if (!ok) return;
+  for (int it = 0; it < 64; ++it) {
+    uint32_t done;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+    if (done) return;
+  }
+  ok = mbar_wait(bar, parity);
 }
 
 // What a chunk of 128 needs of its gates, made by one warp, four rows a lane.  lam: running sums, base 2, as two floats;
@@ -83,54 +106,80 @@ __device__ __forceinline__ float4 gates_of(const Walk& p, int64_t t0, int nv, in
   for (int i = 0; i < 4; ++i) g[i] = 4 * lane + i < nv ? p.g[(t0 + 4 * lane + i) * p.gt + h] : 0.f;
   return make_float4(g[0], g[1], g[2], g[3]);
 }
-__device__ __forceinline__ double scan_gates(float4 g, Gates& s, int lane) {
+// Sums in 64-bit fixed point with 40 bits behind the point (|sum| <= 128 x 289 < 2^16): exact, and a fifth of the time that
+// shuffled doubles take.
+__device__ __forceinline__ float2 two_floats(long long v) {
+  const float hi = __ll2float_rn(v);                       // (a multiple of its own last place: the difference is exact)
+  return make_float2(hi * 0x1p-40f, __ll2float_rn(v - __float2ll_rn(hi)) * 0x1p-40f);
+}
+__device__ __forceinline__ float2 scan_gates(float4 g, Gates& s, int lane) {
   const float x[4] = {g.x, g.y, g.z, g.w};
-  double v[4], sum = 0.0;
+  long long v[4], sum = 0;
+  bool nan = false;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    // exp of less than -200 is 0 either way; -inf would leave inf - inf
-    sum += (double)(x[i] < -200.f ? -200.f : x[i]) * 1.4426950408889634;
+    // exp of less than -200 is 0 either way, of more than 200 inf; -inf would leave inf - inf
+    const float y = fminf(fmaxf(x[i], -200.f), 200.f), hi = y * 1.44269504f, lo = fmaf(y, 1.44269504f, -hi) + y * 1.92596299e-8f;
+    sum += __float2ll_rn(hi * 0x1p40f) + __float2ll_rn(lo * 0x1p40f);
+    nan = nan || x[i] != x[i];
     v[i] = sum;
   }
-  double inc = sum;
+  long long inc = sum;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const double y = __shfl_up_sync(0xffffffffu, inc, d);
+    const long long y = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += y;
   }
-  const double all = __shfl_sync(0xffffffffu, inc, 31), before = inc - sum;
-  const double at[3] = {__shfl_sync(0xffffffffu, inc, 7), __shfl_sync(0xffffffffu, inc, 15), __shfl_sync(0xffffffffu, inc, 23)};
-  const double own = lane < 8 ? 0.0 : lane < 16 ? at[0] : lane < 24 ? at[1] : at[2];
+  // a gate that is not a number makes every sum from it on one
+  const unsigned int odd = __ballot_sync(0xffffffffu, nan);
+  const float qnan = __int_as_float(0x7fffffff);
+  float2 all = two_floats(__shfl_sync(0xffffffffu, inc, 31));
+  if (odd) all.x = qnan;
+  float2 at[3];
+#pragma unroll
+  for (int m = 0; m < 3; ++m) {
+    at[m] = two_floats(__shfl_sync(0xffffffffu, inc, 8 * m + 7));
+    if (odd & ((1u << (8 * m + 8)) - 1)) at[m].x = qnan;
+  }
+  const float2 own = lane < 8 ? make_float2(0.f, 0.f) : lane < 16 ? at[0] : lane < 24 ? at[1] : at[2];
+  bool bad = (odd & ((1u << lane) - 1)) != 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const double y = before + v[i];
-    const float hi = (float)y;
+    float2 y = two_floats(inc - sum + v[i]);
+    bad = bad || x[i] != x[i];
+    if (bad) y.x = qnan;
     const int r = 4 * lane + i;
-    s.lam[r] = make_float2(hi, (float)(y - hi));
-    s.wt[r] = make_float2(ex2(hi), ex2((float)(all - y)));
-    s.rf[r] = ex2((float)(y - own));
+    s.lam[r] = y;
+    s.wt[r] = make_float2(ex2(y.x + y.y), ex2((all.x - y.x) + (all.y - y.y)));
+    s.rf[r] = ex2((y.x - own.x) + (y.y - own.y));
 #pragma unroll
     for (int m = 0; m < 3; ++m)
-      if (lane < 8 * (m + 1)) s.cf[m][r] = ex2((float)(at[m] - y));
+      if (lane < 8 * (m + 1)) s.cf[m][r] = ex2((at[m].x - y.x) + (at[m].y - y.y));
   }
   return all;
 }
 __device__ __forceinline__ float decay_of(float2 i, float2 j) { return ex2((i.x - j.x) + (i.y - j.y)); }
 
-// Rows of a tile times a weight per row, in NU planes: the first in place, the others at lo, lo + plane, ...
+// Rows of a tile times a weight per row, in NU planes: the first in place, the others at lo, lo + plane, ...  Rows from nv on are
+// zeros.
 template <int D, int NU>
-__device__ __forceinline__ void weigh(uint32_t tile, uint32_t lo, uint32_t plane, const float2* wt, bool rev) {
+__device__ __forceinline__ void weigh(uint32_t tile, uint32_t lo, uint32_t plane, const float2* wt, bool rev, int nv) {
   const int r0 = threadIdx.x / 8, c = threadIdx.x % 8;
   const float* w_ = &wt[r0].x + (rev ? 0 : 1);
   const uint32_t at0 = sw128_chunk(r0, c);
 #pragma unroll 1
   for (int j = 0; j < 4; ++j) {
     const float w = w_[64 * j];
+    uint4 x[D / 64];
+#pragma unroll
+    for (int b = 0; b < D / 64; ++b) x[b] = lds16(tile + b * 16384 + j * 4096 + at0);
+    if (r0 + 32 * j >= nv)
+#pragma unroll
+      for (int b = 0; b < D / 64; ++b) x[b] = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
     for (int b = 0; b < D / 64; ++b) {
       const uint32_t at = b * 16384 + j * 4096 + at0;
-      const uint4 x = lds16(tile + at);
-      const uint32_t u[4] = {x.x, x.y, x.z, x.w};
+      const uint32_t u[4] = {x[b].x, x[b].y, x[b].z, x[b].w};
       uint32_t s[4][NU];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -143,20 +192,25 @@ __device__ __forceinline__ void weigh(uint32_t tile, uint32_t lo, uint32_t plane
     }
   }
 }
-// whether the pieces that the thread itself fetched of a tile hold something that is not finite
+// Rows from nv on become zeros; returns whether what is left holds something that is not finite (of the thread's pieces).
 template <int D>
-__device__ __forceinline__ bool odd_values(uint32_t tile) {
-  constexpr int C8 = D / 8, RS = 256 / C8;
-  const int r0 = threadIdx.x / C8, c = threadIdx.x % C8;
-  bool x = false;
-#pragma unroll 2
-  for (int j = 0; j < 128 / RS; ++j) {
-    const uint4 v = lds16(tile + (c >> 3) * 16384 + sw128_chunk(r0, c & 7) + j * RS * 128);
-    const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ bool check_rows(uint32_t tile, int nv) {
+  const int r0 = threadIdx.x / 8, c = threadIdx.x % 8;
+  const uint32_t at0 = tile + sw128_chunk(r0, c);
+  uint32_t m = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x = x || (u[e] & 0x7f80u) == 0x7f80u || (u[e] & 0x7f800000u) == 0x7f800000u;
-  }
-  return x;
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int b = 0; b < D / 64; ++b) {
+      const uint32_t at = at0 + b * 16384 + j * 4096;
+      if (r0 + 32 * j < nv) {
+        const uint4 v = lds16(at);
+        m = __vmaxu2(__vmaxu2(m, v.x & 0x7fff7fffu), __vmaxu2(v.y & 0x7fff7fffu, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+      } else {
+        sts16(at, make_uint4(0u, 0u, 0u, 0u));
+      }
+    }
+  return (m & 0xffffu) >= 0x7f80u || (m >> 16) >= 0x7f80u;
 }
 // What is not finite in OA = P V, by sums over the tokens up to the row's own (UP = false) or from it on (UP): in the product,
 // zeros of P meet what is not finite in V, and 0 x inf is not a number, where the recurrence has it at its own token and after
@@ -206,28 +260,38 @@ __device__ __noinline__ void masked_sums(uint32_t tp, uint32_t to, uint32_t tv, 
 
 template <int DK, int DV, int NU, int NS, bool OUT>
 struct TLay {
-  static constexpr int NK = OUT && NU + NS <= 3 ? 2 : 1;                  // stages of K
+  static constexpr int NK = !OUT || NU + NS <= 3 ? 2 : 1, NV = OUT ? 1 : 2, NL = OUT || NU > 2 ? 1 : 2;   // stages of K, V, the lower planes
   static constexpr int TK = DK * 256, TV = DV * 256, SP = DK * DV * 2;
-  static constexpr int Q0 = 0, K0 = Q0 + (OUT ? TK : 0), V0 = K0 + NK * TK, L0 = V0 + TV, S0 = L0 + (NU - 1) * TK;
-  static constexpr int G0 = S0 + (OUT ? NS * SP : 0), BAR = G0 + 2 * (int)sizeof(Gates), USED = BAR + 64;
+  static constexpr int Q0 = 0, K0 = Q0 + (OUT ? TK : 0), V0 = K0 + NK * TK, L0 = V0 + NV * TV, S0 = L0 + NL * (NU - 1) * TK;
+  static constexpr int G0 = S0 + (OUT ? NS * SP : 0), BAR = G0 + 2 * (int)sizeof(Gates);
+  // (64 features make rows 0 to 63 of a product of 128: the others are made of the 16 KB behind the keys' tile, whatever is there)
+  static constexpr int USED = BAR + 192 + (DK == 64 ? 16384 : 0);
   // one block per SM, whatever the sizes: each takes all of the tensor memory
   static constexpr int END = USED < 120 * 1024 ? 120 * 1024 : USED;
   static_assert(END <= 232448, "shared memory");
 };
+// barriers, 8 bytes each from BAR on
+enum TcBar { B_Q = 0, B_K = 1, B_V = 3, B_QK = 5, B_QS = 6, B_PV = 7, B_U = 8, B_P = 10, B_S = 12, B_G = 13, B_GFREE = 15, B_COUNT = 17, B_TMEM = 17, B_ODD = 18 };
+
+struct TcWalk {
+  CUtensorMap q, k, v;
+  Walk w;
+};
 
 // NU: planes of the weighted keys; NS: planes of the state as an operand
 template <int DK, int DV, int NU, int NS, bool OUT>
-__global__ void __launch_bounds__(256, 1) tc_walk_kernel(const Walk p) {
+__global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__ TcWalk a) {
   using Y = TLay<DK, DV, NU, NS, OUT>;
-  constexpr int HV = DV / 2;                                   // value columns of a thread
+  constexpr int HV = DV / 2;                                   // value columns of a worker
+  const Walk& p = a.w;
   extern __shared__ __align__(1024) uint8_t sm[];
   Gates* gates = reinterpret_cast<Gates*>(sm + Y::G0);
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, q4 = warp & 3, half = warp >> 2, row = 32 * q4 + lane;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int h = blockIdx.y;
   const Run run = find_run(p, blockIdx.x);
   if constexpr (OUT) {
     if (run.zlo < run.zhi)
-      for (int64_t i = tid; i < (run.zhi - run.zlo) * p.vd; i += 256)
+      for (int64_t i = tid; i < (run.zhi - run.zlo) * p.vd; i += 352)
         st_any(p.out, !p.out_f32, ((run.zlo + i / p.vd) * p.H + h) * p.vd + i % p.vd, 0.f);
     if (p.count_bad && run.any && run.first && blockIdx.y == 0 && tid == 0) {
       const int64_t a = p.cu ? p.cu[run.s] : 0, b = p.cu ? p.cu[run.s + 1] : 0;
@@ -238,276 +302,350 @@ __global__ void __launch_bounds__(256, 1) tc_walk_kernel(const Walk p) {
   // the run that the sequence is left through has nobody to pass its sum to
   if (!OUT && (p.rev ? run.first : run.last)) return;
 
-  const uint32_t base = smem_u32(sm), bar = base + Y::BAR;      // Q K^T, Q S, P V, U; tensor memory address
+  const uint32_t base = smem_u32(sm), bars = base + Y::BAR;
+  const auto bar = [&](int b) { return bars + 8 * b; };
   if (tid == 0) {
-    for (int i = 0; i < 4; ++i) mbar_init(bar + 8 * i, 1);
+    for (int i = 0; i < B_COUNT; ++i) mbar_init(bar(i), i == B_P || i == B_P + 1 || i == B_S || i == B_GFREE || i == B_GFREE + 1 ? 8 : 1);
+    asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(bar(B_ODD)), "r"(0) : "memory");
     mbar_fence_init();
   }
   if (warp == 0) {
-    tmem_alloc(bar + 32, 512);
+    tmem_alloc(bar(B_TMEM), 512);
     tmem_relinquish();
   }
   const int64_t sh = run.s * p.H + h, dd = (int64_t)p.kd * p.vd, slot_h = (int64_t)blockIdx.x * p.H + h;
-  const int Hq = p.H / p.gq, Hk = p.H / p.gk, Hv = p.H / p.gv;
   const int len = (int)(run.hi - run.lo), chunks = (len + 127) / 128;
   const int64_t r0 = run.base + run.lo;                         // the run's first token
-  const int64_t sk = (int64_t)Hk * p.kd, sv = (int64_t)Hv * p.vd, sq = (int64_t)Hq * p.kd;
-  const bf16* gk = (const bf16*)p.k + r0 * sk + h / p.gk * p.kd;
-  const bf16* gv = (const bf16*)p.v + r0 * sv + h / p.gv * p.vd;
-  const bf16* gq = OUT ? (const bf16*)p.q + r0 * sq + h / p.gq * p.kd : nullptr;
   // chunk i of the walk; backwards in time (sums only) from the last one
   const auto first_of = [&](int i) { return 128 * (p.rev ? chunks - 1 - i : i); };
   const auto rows_of = [&](int i) { const int c0 = first_of(i); return len - c0 < 128 ? len - c0 : 128; };
-  const auto kbuf = [&](int i) { return base + Y::K0 + (Y::NK == 2 ? (i & 1) * Y::TK : 0); };
-  const auto load_q = [&](int i) { if (i < chunks) fetch128<DK>(base + Y::Q0, gq + first_of(i) * sq, sq, rows_of(i), p.kd); };
-  const auto load_k = [&](int i) { if (i < chunks) fetch128<DK>(kbuf(i), gk + first_of(i) * sk, sk, rows_of(i), p.kd); };
-  const auto load_v = [&](int i) { if (i < chunks) fetch128<DV>(base + Y::V0, gv + first_of(i) * sv, sv, rows_of(i), p.vd); };
-  if constexpr (OUT) load_q(0);
-  load_k(0);
-  cp_commit();
-  load_v(0);
-  cp_commit();
-  double total = 0.0;
-  if (warp == 7 && chunks) total += scan_gates(gates_of(p, r0 + first_of(0), rows_of(0), h, lane), gates[0], lane);
-
-  // the state: row `row` (a key feature), columns HV half + [0, HV)
-  float S[HV];
-  const int cols = row < p.kd ? p.vd - HV * half : 0;           // that there are of them
-  if (!OUT) {
-#pragma unroll
-    for (int j = 0; j < HV; ++j) S[j] = 0.f;
-  } else if (p.seg_state || p.init_f32) {
-    const float* x = p.seg_state ? p.seg_state + slot_h * dd + row * p.sk + HV * half * p.sc : (const float*)p.init + sh * dd + row * p.ik + HV * half * p.ic;
-    const int64_t d = p.seg_state ? p.sc : p.ic;
-#pragma unroll
-    for (int j = 0; j < HV; ++j, x += d) S[j] = j < cols ? *x : 0.f;
-  } else {
-    const bf16* x = (const bf16*)p.init + sh * dd + row * p.ik + HV * half * p.ic;
-#pragma unroll
-    for (int j = 0; j < HV; ++j, x += p.ic) S[j] = j < cols ? __bfloat162float(*x) : 0.f;
-  }
-  // its image for Q S: [feature][column], 64 columns a tile
-  const auto put_state = [&]() {
-    if (row < DK) {
-#pragma unroll
-      for (int j = 0; j < HV; j += 8) {
-        uint32_t s[4][NS];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) planes<NS>(S[j + 2 * e], S[j + 2 * e + 1], s[e]);
-        const int c8 = (HV * half + j) / 8;
-#pragma unroll
-        for (int k = 0; k < NS; ++k)
-          sts16(base + Y::S0 + k * Y::SP + (c8 >> 3) * DK * 128 + sw128_chunk(row, c8 & 7), make_uint4(s[0][k], s[1][k], s[2][k], s[3][k]));
-      }
-    }
-  };
-  if constexpr (OUT) put_state();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   uint32_t tmem;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(bar + 32));
-  const uint32_t tSC = tmem, tOI = tmem + 128, tOA = tmem + 256, tU = tmem + 384, lane_base = (uint32_t)(32 * q4) << 16;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(tmem) : "r"(bar(B_TMEM)));
+  const uint32_t tSC = tmem, tOI = tmem + 128, tOA = tmem + 256, tU = tmem + 384;      // (sums only: U in two stages, 0 and 384)
+  const auto ubuf = [&](int i) { return OUT || (i & 1) ? tU : tmem; };
   bool ok = true;
-  const bool wide = p.vd % 16 == 0 && ((uintptr_t)p.out & 31) == 0;
+  // whether the workers found values that are not finite in chunk i, whose P and V they then read behind the product
+  const auto was_odd = [&](int i) {
+    uint32_t x;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x) : "r"(bar(B_ODD) + 4 * (i & 1)) : "memory");
+    return x == (uint32_t)(i + 1);
+  };
 
-  for (int i = 0; i < chunks; ++i) {
-    const int nv = rows_of(i);
-    const int64_t t0 = r0 + first_of(i);
-    const uint32_t ph = i & 1, uk = kbuf(i), uv = base + Y::V0;
-    const Gates& gs = gates[i & 1];
-    if constexpr (OUT) {
-      cp_wait<1>();                       // Q and K
-      fence_async_smem();                 // (the state's image too)
-      tc_fence_before();
-      __syncthreads();
-      if (tid == 0) {
+  if (warp == 8) {
+    // ================= products =================
+    if (lane == 0) {
+      const uint64_t dQ = desc_kmajor(base + Y::Q0, 16384, 0), dK = desc_kmajor(base + Y::K0, 16384, 0);
+      const uint64_t dKm = desc_mnmajor(base + Y::K0, 16384, 0), dV = desc_mnmajor(base + Y::V0, 16384, 0);
+      const uint64_t dL = desc_mnmajor(base + Y::L0, 16384, 0), dS = desc_mnmajor(base + Y::S0, DK * 128, 0);
+      constexpr uint32_t i_qk = idesc_bf16(128, 128, 0, 0), i_qs = idesc_bf16(128, DV, 0, 1), i_pv = idesc_bf16(128, DV, 0, 1),
+                         i_u = idesc_bf16(128, DV, 1, 1);
+      const auto kcol = [](int s) { return (uint32_t)((s >> 2) * 16384 + (s & 3) * 32); };     // 16 columns of a K-major operand
+      for (int i = 0; i < chunks; ++i) {
+        const uint32_t ph = i & 1, kst = Y::NK == 2 ? (i & 1) * Y::TK : 0, kph = Y::NK == 2 ? (i >> 1) & 1 : ph;
+        const int kb = Y::NK == 2 ? i & 1 : 0, vb = Y::NV == 2 ? i & 1 : 0;
+        if constexpr (OUT) {
+          wait_for(ok, bar(B_Q), ph);
+          wait_for(ok, bar(B_K + kb), kph);
+          if (i >= 1 && was_odd(i - 1)) wait_for(ok, bar(B_S), ph);      // (P is read until the chunk before is done with)
+          tc_fence_after();
+#pragma unroll
+          for (int s = 0; s < DK / 16; ++s) umma_bf16(tSC, desc_advance(dQ, kcol(s)), desc_advance(dK, kst + kcol(s)), i_qk, s > 0);
+          umma_commit(bar(B_QK));
+          wait_for(ok, bar(B_S), ph);              // the state's image; OI, OA and U of the chunk before are read
+          tc_fence_after();
+#pragma unroll
+          for (int n = NS - 1; n >= 0; --n)
+#pragma unroll
+            for (int s = 0; s < DK / 16; ++s)
+              umma_bf16(tOI, desc_advance(dQ, kcol(s)), desc_advance(dS, n * Y::SP + s * 2048), i_qs, n < NS - 1 || s > 0);
+          umma_commit(bar(B_QS));
+        }
+        wait_for(ok, bar(B_P + (i & 1)), (i >> 1) & 1);      // P, the weighted keys, the values checked
+        if constexpr (!OUT) wait_for(ok, bar(B_V + vb), (i >> 1) & 1);
         tc_fence_after();
-        constexpr uint32_t d_qk = idesc_bf16(128, 128, 0, 0), d_qs = idesc_bf16(128, DV, 0, 1);
+        const uint32_t vst = vb * Y::TV;
+        if constexpr (OUT) {
 #pragma unroll
-        for (int s = 0; s < DK / 16; ++s) umma_bf16(tSC, desc_kmajor(base + Y::Q0, 16384, s), desc_kmajor(uk, 16384, s), d_qk, s > 0);
-        umma_commit(bar);
+          for (int s = 0; s < 8; ++s) umma_ts(tOA, tSC + 64 * (s >> 2) + 8 * (s & 3), desc_advance(dV, s * 2048), i_pv, s > 0);
+          umma_commit(bar(B_PV));
+        }
+        const uint32_t lst = Y::NL == 2 ? (i & 1) * (NU - 1) * Y::TK : 0;
 #pragma unroll
-        for (int n = NS - 1; n >= 0; --n)
+        for (int n = NU - 1; n >= 0; --n)
 #pragma unroll
-          for (int s = 0; s < DK / 16; ++s)
-            umma_bf16(tOI, desc_kmajor(base + Y::Q0, 16384, s), desc_mnmajor(base + Y::S0 + n * Y::SP, DK * 128, s), d_qs, n < NS - 1 || s > 0);
-        umma_commit(bar + 8);
+          for (int s = 0; s < 8; ++s)
+            umma_bf16(ubuf(i), n ? desc_advance(dL, lst + (n - 1) * Y::TK + s * 2048) : desc_advance(dKm, kst + s * 2048),
+                      desc_advance(dV, vst + s * 2048), i_u, n < NU - 1 || s > 0);
+        umma_commit(bar(B_U + (OUT ? 0 : i & 1)));
       }
     }
-    float4 gn = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (warp == 7 && i + 1 < chunks) gn = gates_of(p, r0 + first_of(i + 1), rows_of(i + 1), h, lane);
-    cp_wait<0>();                         // V (and, without Q, K)
-    if constexpr (!OUT) __syncthreads();
-    if constexpr (OUT) {
-      if (ok) ok = mbar_wait(bar, ph);    // scores; K may be overwritten
-      tc_fence_after();
-#pragma unroll 1
-      for (int g = 0; g < 2; ++g) {
-        const int grp = 2 * half + g;     // columns 32 grp + [0, 32)
-        uint32_t pk[16];
-        if (grp > q4) {
-#pragma unroll
-          for (int e = 0; e < 16; ++e) pk[e] = 0u;
+    __syncwarp();
+  } else if (warp == 9) {
+    // ================= tensor copies =================
+    if (lane == 0) {
+      const int hq = h / p.gq, hk = h / p.gk, hv = h / p.gv;
+      for (int i = 0; i < chunks; ++i) {
+        const int z = (int)(r0 + first_of(i)), kb = Y::NK == 2 ? i & 1 : 0, vb = Y::NV == 2 ? i & 1 : 0;
+        if constexpr (OUT) {
+          if (i >= 1) wait_for(ok, bar(B_QS), (i - 1) & 1);
+          mbar_arrive_expect_tx(bar(B_Q), Y::TK);
+          for (int b = 0; b < DK / 64; ++b) tma_load_3d(base + Y::Q0 + b * 16384, &a.q, 64 * b, hq, z, bar(B_Q));
+        }
+        if constexpr (OUT) {
+          // (with two stages of K: the values of the chunk before waited for the product that used this one)
+          if (i >= 1 && Y::NK == 1) wait_for(ok, bar(B_U), (i - 1) & 1);
         } else {
-          uint32_t x[32];
-          tmem_ld32(tSC + lane_base + 32 * grp, x);
-          tmem_ld_wait();
-          if (grp < q4) {
-            const float rf = gs.rf[row];
-            const float4* cf = reinterpret_cast<const float4*>(&gs.cf[q4 - 1][32 * grp]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float4 c = cf[e];
-              pk[2 * e] = pack_bf16x2(__uint_as_float(x[4 * e]) * (rf * c.x), __uint_as_float(x[4 * e + 1]) * (rf * c.y));
-              pk[2 * e + 1] = pack_bf16x2(__uint_as_float(x[4 * e + 2]) * (rf * c.z), __uint_as_float(x[4 * e + 3]) * (rf * c.w));
-            }
-          } else {
-            const float2 li = gs.lam[row];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float4 l = *reinterpret_cast<const float4*>(&gs.lam[32 * grp + 2 * e]);
-              const float a = 2 * e <= lane ? __uint_as_float(x[2 * e]) * decay_of(li, make_float2(l.x, l.y)) : 0.f;
-              const float b = 2 * e + 1 <= lane ? __uint_as_float(x[2 * e + 1]) * decay_of(li, make_float2(l.z, l.w)) : 0.f;
-              pk[e] = pack_bf16x2(a, b);
-            }
-          }
+          if (i >= 2) wait_for(ok, bar(B_U + (i & 1)), ((i - 2) >> 1) & 1);
         }
-        // P over its own half of SC: 64 half + [0, 32)
-        tmem_st16(tSC + lane_base + 64 * half + 16 * g, pk);
+        mbar_arrive_expect_tx(bar(B_K + kb), Y::TK);
+        for (int b = 0; b < DK / 64; ++b) tma_load_3d(base + Y::K0 + kb * Y::TK + b * 16384, &a.k, 64 * b, hk, z, bar(B_K + kb));
+        if constexpr (OUT)
+          if (i >= 1) {
+            if (Y::NK == 2) wait_for(ok, bar(B_U), (i - 1) & 1);
+            if (was_odd(i - 1)) wait_for(ok, bar(B_S), i & 1);
+          }
+        mbar_arrive_expect_tx(bar(B_V + vb), Y::TV);
+        for (int b = 0; b < DV / 64; ++b) tma_load_3d(base + Y::V0 + vb * Y::TV + b * 16384, &a.v, 64 * b, hv, z, bar(B_V + vb));
       }
-      tmem_st_wait();
     }
-    weigh<DK, NU>(uk, base + Y::L0, Y::TK, gs.wt, p.rev);
-    bool odd = false;
-    if constexpr (OUT) odd = odd_values<DV>(uv);
-    fence_async_smem();
-    tc_fence_before();
-    odd = __syncthreads_or(odd) != 0;
-    if (tid == 0) {
-      tc_fence_after();
-      constexpr uint32_t d_pv = idesc_bf16(128, DV, 0, 1), d_u = idesc_bf16(128, DV, 1, 1);
-      if constexpr (OUT) {
+    __syncwarp();
+  } else if (warp == 10) {
+    // ================= gates =================
+    double total = 0.0;
+    float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (chunks) g = gates_of(p, r0 + first_of(0), rows_of(0), h, lane);
+    for (int i = 0; i < chunks; ++i) {
+      if (i >= 2) wait_for(ok, bar(B_GFREE + (i & 1)), ((i - 2) >> 1) & 1);
+      const float2 all = scan_gates(g, gates[i & 1], lane);
+      total += (double)all.x + (double)all.y;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_G + (i & 1)));
+      if (i + 1 < chunks) g = gates_of(p, r0 + first_of(i + 1), rows_of(i + 1), h, lane);
+    }
+    if (!OUT && lane == 0) p.seg_total[slot_h] = total;
+  } else {
+    // ================= workers =================
+    const int q4 = warp & 3, half = warp >> 2, row = 32 * q4 + lane;
+    const uint32_t lane_base = (uint32_t)(32 * q4) << 16;
+    // the state: row `row` (a key feature), columns HV half + [0, HV)
+    float S[HV];
+    const int cols = row < p.kd ? p.vd - HV * half : 0;           // that there are of them
+    if (!OUT) {
 #pragma unroll
-        for (int s = 0; s < 8; ++s) umma_ts(tOA, tSC + 64 * (s >> 2) + 8 * (s & 3), desc_mnmajor(uv, 16384, s), d_pv, s > 0);
-        umma_commit(bar + 16);
+      for (int j = 0; j < HV; ++j) S[j] = 0.f;
+    } else if (p.seg_state || p.init_f32) {
+      const float* x = p.seg_state ? p.seg_state + slot_h * dd + row * p.sk + HV * half * p.sc : (const float*)p.init + sh * dd + row * p.ik + HV * half * p.ic;
+      const int64_t d = p.seg_state ? p.sc : p.ic;
+#pragma unroll
+      for (int j = 0; j < HV; ++j, x += d) S[j] = j < cols ? *x : 0.f;
+    } else {
+      const bf16* x = (const bf16*)p.init + sh * dd + row * p.ik + HV * half * p.ic;
+#pragma unroll
+      for (int j = 0; j < HV; ++j, x += p.ic) S[j] = j < cols ? __bfloat162float(*x) : 0.f;
+    }
+    // its image for Q S: [feature][column], 64 columns a tile
+    const auto put_state = [&]() {
+      if (row < DK) {
+#pragma unroll
+        for (int j = 0; j < HV; j += 8) {
+          uint32_t s[4][NS];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) planes<NS>(S[j + 2 * e], S[j + 2 * e + 1], s[e]);
+          const int c8 = (HV * half + j) / 8;
+#pragma unroll
+          for (int k = 0; k < NS; ++k)
+            sts16(base + Y::S0 + k * Y::SP + (c8 >> 3) * DK * 128 + sw128_chunk(row, c8 & 7), make_uint4(s[0][k], s[1][k], s[2][k], s[3][k]));
+        }
       }
+      fence_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_S));
+    };
+    const auto take_u = [&](int i) {
+      const float all = gates[i & 1].wt[127].x;
 #pragma unroll
-      for (int n = NU - 1; n >= 0; --n)
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-          umma_bf16(tU, desc_mnmajor(n ? base + Y::L0 + (n - 1) * Y::TK : uk, 16384, s), desc_mnmajor(uv, 16384, s), d_u, n < NU - 1 || s > 0);
-      umma_commit(bar + 24);
-    }
-    if (warp == 7 && i + 1 < chunks) total += scan_gates(gn, gates[(i + 1) & 1], lane);
-    if constexpr (OUT) {
-      if (ok) ok = mbar_wait(bar + 8, ph);          // Q S: Q may be overwritten
-      load_q(i + 1);
-      if constexpr (Y::NK == 2) load_k(i + 1);
-      cp_commit();
-      if (ok) ok = mbar_wait(bar + 16, ph);
-      tc_fence_after();
-      if (odd) masked_sums<DV, false>(tSC + lane_base, tOA + lane_base, uv, row, half);
-      const float wi = gs.wt[row].x;
-      const int64_t at = ((t0 + row) * p.H + h) * p.vd + HV * half;
-      const int64_t ra = p.r ? ((t0 + row) * (p.H / p.gr) + h / p.gr) * p.vd + HV * half : 0;
-      float dot = 0.f;
-#pragma unroll 1
-      for (int c0 = 0; c0 < HV; c0 += 16) {
-        uint32_t a[16], b[16];
-        tmem_ld16(tOI + lane_base + HV * half + c0, a);
-        tmem_ld16(tOA + lane_base + HV * half + c0, b);
+      for (int c0 = 0; c0 < HV; c0 += 32) {
+        uint32_t u[32];
+        tmem_ld32(ubuf(i) + lane_base + HV * half + c0, u);
         tmem_ld_wait();
-        if (row < nv) {
-          if (p.r) {
-            // the row's product with what comes from before the chunk
 #pragma unroll
-            for (int e = 0; e < 16; e += 8)
-              if (HV * half + c0 + e < p.vd) {
-                const uint4 u = __ldg((const uint4*)((const bf16*)p.r + ra + c0 + e));
-                const uint32_t y[4] = {u.x, u.y, u.z, u.w};
+        for (int e = 0; e < 32; ++e) S[c0 + e] = fmaf(all, S[c0 + e], __uint_as_float(u[e]));
+      }
+    };
+    if constexpr (OUT) put_state();
+    const bool wide = p.vd % 16 == 0 && ((uintptr_t)p.out & 31) == 0;
+
+    for (int i = 0; i < chunks; ++i) {
+      const int nv = rows_of(i), kb = Y::NK == 2 ? i & 1 : 0, vb = Y::NV == 2 ? i & 1 : 0;
+      const uint32_t ph = i & 1, kph = Y::NK == 2 ? (i >> 1) & 1 : ph;
+      const uint32_t uk = base + Y::K0 + kb * Y::TK, uv = base + Y::V0 + vb * Y::TV;
+      const Gates& gs = gates[i & 1];
+      wait_for(ok, bar(B_G + (i & 1)), (i >> 1) & 1);
+      if constexpr (OUT) {
+        wait_for(ok, bar(B_QK), ph);
+        tc_fence_after();
+#pragma unroll 1
+        for (int g = 0; g < 2; ++g) {
+          const int grp = 2 * half + g;     // columns 32 grp + [0, 32)
+          uint32_t pk[16];
+          if (grp > q4) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const float2 z = pair_of(y[k]);
-                  dot = fmaf(__uint_as_float(a[e + 2 * k]), z.x, fmaf(__uint_as_float(a[e + 2 * k + 1]), z.y, dot));
-                }
-              }
-          }
-          float o[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = fmaf(wi, __uint_as_float(a[e]), __uint_as_float(b[e]));
-          const int left = p.vd - (HV * half + c0);
-          if (p.out_f32) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 4)
-              if (e < left) *reinterpret_cast<float4*>((float*)p.out + at + c0 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            for (int e = 0; e < 16; ++e) pk[e] = 0u;
           } else {
-            uint32_t w[8];
+            uint32_t x[32];
+            tmem_ld32(tSC + lane_base + 32 * grp, x);
+            tmem_ld_wait();
+            if (grp < q4) {
+              const float rf = gs.rf[row];
+              const float4* cf = reinterpret_cast<const float4*>(&gs.cf[q4 - 1][32 * grp]);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(o[2 * e], o[2 * e + 1]);
-            bf16* d = (bf16*)p.out + at + c0;
-            if (wide) {
-              if (left > 0) st_global_v8(d, w);
+              for (int e = 0; e < 8; ++e) {
+                const float4 c = cf[e];
+                pk[2 * e] = pack_bf16x2(__uint_as_float(x[4 * e]) * (rf * c.x), __uint_as_float(x[4 * e + 1]) * (rf * c.y));
+                pk[2 * e + 1] = pack_bf16x2(__uint_as_float(x[4 * e + 2]) * (rf * c.z), __uint_as_float(x[4 * e + 3]) * (rf * c.w));
+              }
             } else {
-              if (left > 0) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-              if (left > 8) *reinterpret_cast<uint4*>(d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+              const float2 li = gs.lam[row];
+#pragma unroll
+              for (int e = 0; e < 16; ++e) {
+                const float4 l = *reinterpret_cast<const float4*>(&gs.lam[32 * grp + 2 * e]);
+                const float x0 = 2 * e <= lane ? __uint_as_float(x[2 * e]) * decay_of(li, make_float2(l.x, l.y)) : 0.f;
+                const float x1 = 2 * e + 1 <= lane ? __uint_as_float(x[2 * e + 1]) * decay_of(li, make_float2(l.z, l.w)) : 0.f;
+                pk[e] = pack_bf16x2(x0, x1);
+              }
+            }
+          }
+          // P over this thread's own part of SC: columns 64 half + [0, 32)
+          tmem_st16(tSC + lane_base + 64 * half + 16 * g, pk);
+        }
+        tmem_st_wait();
+      }
+      wait_for(ok, bar(B_K + kb), kph);
+      if constexpr (!OUT)
+        if (i >= Y::NL) wait_for(ok, bar(B_U + ((i - Y::NL) & 1)), ((i - Y::NL) >> 1) & 1);      // (the lower planes' stage)
+      weigh<DK, NU>(uk, base + Y::L0 + (Y::NL == 2 ? (i & 1) * (NU - 1) * Y::TK : 0), Y::TK, gs.wt, p.rev, nv);
+      if (OUT || nv < 128) {
+        wait_for(ok, bar(B_V + vb), Y::NV == 2 ? (i >> 1) & 1 : ph);
+        const bool odd = check_rows<DV>(uv, nv);
+        if (OUT && odd) asm volatile("st.shared.u32 [%0], %1;" ::"r"(bar(B_ODD) + 4 * (i & 1)), "r"(i + 1) : "memory");
+      }
+      fence_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(B_P + (i & 1)));
+      if constexpr (OUT) {
+        const int64_t t0 = r0 + first_of(i);
+        wait_for(ok, bar(B_QS), ph);
+        wait_for(ok, bar(B_PV), ph);
+        tc_fence_after();
+        if (was_odd(i)) masked_sums<DV, false>(tSC + lane_base, tOA + lane_base, uv, row, half);
+        const float wi = gs.wt[row].x;
+        const int64_t at = ((t0 + row) * p.H + h) * p.vd + HV * half;
+        const int64_t ra = p.r ? ((t0 + row) * (p.H / p.gr) + h / p.gr) * p.vd + HV * half : 0;
+        float dot = 0.f;
+#pragma unroll 1
+        for (int c0 = 0; c0 < HV; c0 += 16) {
+          uint32_t x[16], y[16];
+          tmem_ld16(tOI + lane_base + HV * half + c0, x);
+          tmem_ld16(tOA + lane_base + HV * half + c0, y);
+          tmem_ld_wait();
+          if (row < nv) {
+            if (p.r) {
+              // the row's product with what comes from before the chunk
+#pragma unroll
+              for (int e = 0; e < 16; e += 8)
+                if (HV * half + c0 + e < p.vd) {
+                  const uint4 u = __ldg((const uint4*)((const bf16*)p.r + ra + c0 + e));
+                  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    const float2 z = pair_of(w[k]);
+                    dot = fmaf(__uint_as_float(x[e + 2 * k]), z.x, fmaf(__uint_as_float(x[e + 2 * k + 1]), z.y, dot));
+                  }
+                }
+            }
+            float o[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = fmaf(wi, __uint_as_float(x[e]), __uint_as_float(y[e]));
+            const int left = p.vd - (HV * half + c0);
+            if (p.out_f32) {
+#pragma unroll
+              for (int e = 0; e < 16; e += 4)
+                if (e < left) *reinterpret_cast<float4*>((float*)p.out + at + c0 + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            } else {
+              uint32_t w[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(o[2 * e], o[2 * e + 1]);
+              bf16* d = (bf16*)p.out + at + c0;
+              if (wide) {
+                if (left > 0) st_global_v8(d, w);
+              } else {
+                if (left > 0) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+                if (left > 8) *reinterpret_cast<uint4*>(d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+              }
             }
           }
         }
+        if (p.r && row < nv) p.rdot[(half * (p.cu ? p.T : p.nseq * p.T) + t0 + row) * p.H + h] = wi * dot;
+        wait_for(ok, bar(B_U), ph);
+        tc_fence_after();
+        take_u(i);
+        if (i + 1 < chunks) put_state();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(B_GFREE + (i & 1)));
+      } else {
+        // the product of this chunk runs while the sums of the one before are taken
+        if (i >= 1) {
+          wait_for(ok, bar(B_U + ((i - 1) & 1)), ((i - 1) >> 1) & 1);
+          tc_fence_after();
+          take_u(i - 1);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar(B_GFREE + ((i - 1) & 1)));
+        }
       }
-      if (p.r && row < nv) p.rdot[(half * (p.cu ? p.T : p.nseq * p.T) + t0 + row) * p.H + h] = wi * dot;
     }
-    if (ok) ok = mbar_wait(bar + 24, ph);           // U: K and V may be overwritten
-    tc_fence_after();
-    if constexpr (Y::NK == 1) load_k(i + 1);
-    if constexpr (Y::NK == 1 && OUT) cp_commit();
-    load_v(i + 1);
-    cp_commit();
-    const float all = gs.wt[127].x;
-#pragma unroll
-    for (int c0 = 0; c0 < HV; c0 += 16) {
-      uint32_t u[16];
-      tmem_ld16(tU + lane_base + HV * half + c0, u);
-      tmem_ld_wait();
-#pragma unroll
-      for (int e = 0; e < 16; ++e) S[c0 + e] = fmaf(all, S[c0 + e], __uint_as_float(u[e]));
+    if (!OUT && chunks) {
+      wait_for(ok, bar(B_U + ((chunks - 1) & 1)), ((chunks - 1) >> 1) & 1);
+      tc_fence_after();
+      take_u(chunks - 1);
     }
-    if constexpr (OUT) put_state();
+    if constexpr (OUT) {
+      if (run.last) {
+        const int64_t at = sh * dd + row * p.ik + HV * half * p.ic;
+        float* f = p.fin_f32 ? (float*)p.fin + at : p.fin32 + at;
+        if (p.fin_f32 ? p.fin != nullptr : p.fin32 != nullptr)
+#pragma unroll
+          for (int j = 0; j < HV; ++j, f += p.ic)
+            if (j < cols) *f = S[j];
+        if (p.fin_f32 && p.fin32) {
+          f = p.fin32 + at;
+#pragma unroll
+          for (int j = 0; j < HV; ++j, f += p.ic)
+            if (j < cols) *f = S[j];
+        }
+        if (!p.fin_f32 && p.fin) {
+          bf16* o = (bf16*)p.fin + at;
+#pragma unroll
+          for (int j = 0; j < HV; ++j, o += p.ic)
+            if (j < cols) *o = __float2bfloat16_rn(S[j]);
+        }
+      }
+    } else {
+      float* f = p.seg_state + slot_h * dd + (int64_t)HV * half * p.kd + row;
+#pragma unroll
+      for (int j = 0; j < HV; ++j, f += p.kd)
+        if (j < cols) *f = S[j];
+    }
   }
   if (!ok && lane == 0) atomicAdd(&g_wait_timeouts, 1u);
-  cp_wait<0>();
   tc_fence_before();
   __syncthreads();
   if (warp == 0) tmem_dealloc(tmem, 512);
-
-  if constexpr (OUT) {
-    if (run.last) {
-      const int64_t at = sh * dd + row * p.ik + HV * half * p.ic;
-      float* f = p.fin_f32 ? (float*)p.fin + at : p.fin32 + at;
-      if (p.fin_f32 ? p.fin != nullptr : p.fin32 != nullptr)
-#pragma unroll
-        for (int j = 0; j < HV; ++j, f += p.ic)
-          if (j < cols) *f = S[j];
-      if (p.fin_f32 && p.fin32) {
-        f = p.fin32 + at;
-#pragma unroll
-        for (int j = 0; j < HV; ++j, f += p.ic)
-          if (j < cols) *f = S[j];
-      }
-      if (!p.fin_f32 && p.fin) {
-        bf16* o = (bf16*)p.fin + at;
-#pragma unroll
-        for (int j = 0; j < HV; ++j, o += p.ic)
-          if (j < cols) *o = __float2bfloat16_rn(S[j]);
-      }
-    }
-  } else {
-    if (warp == 7 && lane == 0) p.seg_total[slot_h] = total;
-    float* f = p.seg_state + slot_h * dd + (int64_t)HV * half * p.kd + row;
-#pragma unroll
-    for (int j = 0; j < HV; ++j, f += p.kd)
-      if (j < cols) *f = S[j];
-  }
 }
 
 template <int DK, int DV, int NU, int NS, bool OUT>
@@ -515,8 +653,15 @@ int launch_tc(cudaStream_t stream, const Walk& p, const char* name) {
   using Y = TLay<DK, DV, NU, NS, OUT>;
   static SmemAttrOnce attr;
   GLA_TRY(attr.ensure(tc_walk_kernel<DK, DV, NU, NS, OUT>, Y::END));
+  TcWalk a;
+  a.w = p;
+  const int64_t rows = p.cu ? p.T : p.nseq * p.T;
+  GLA_TRY(make_map_tokens(&a.k, p.k, rows, p.H / p.gk, p.kd));
+  GLA_TRY(make_map_tokens(&a.v, p.v, rows, p.H / p.gv, p.vd));
+  if (OUT) GLA_TRY(make_map_tokens(&a.q, p.q, rows, p.H / p.gq, p.kd));
+  else a.q = a.k;
   ProfScope ps(name, stream);
-  tc_walk_kernel<DK, DV, NU, NS, OUT><<<dim3((unsigned)p.nslots, (unsigned)p.H), 256, Y::END, stream>>>(p);
+  tc_walk_kernel<DK, DV, NU, NS, OUT><<<dim3((unsigned)p.nslots, (unsigned)p.H), 352, Y::END, stream>>>(a);
   GLA_CHECK_LAUNCH();
   return GLA_OK;
 }
