@@ -57,6 +57,15 @@ static inline unsigned int read_wait_timeouts() {
   return v;
 }
 
+// Looks at three barriers at once (a look takes some 200 cycles, done or not).
+__device__ __forceinline__ bool all_done(uint32_t a, uint32_t pa, uint32_t b, uint32_t pb, uint32_t c, uint32_t pc) {
+  uint32_t x, y, z;
+  asm volatile("{\n\t.reg .pred p, q, r;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%3], %4;\n\t"
+               "mbarrier.test_wait.parity.shared::cta.b64 q, [%5], %6;\n\tmbarrier.test_wait.parity.shared::cta.b64 r, [%7], %8;\n\t"
+               "selp.u32 %0, 1, 0, p;\n\tselp.u32 %1, 1, 0, q;\n\tselp.u32 %2, 1, 0, r;\n\t}\n"
+               : "=r"(x), "=r"(y), "=r"(z) : "r"(a), "r"(pa), "r"(b), "r"(pb), "r"(c), "r"(pc) : "memory");
+  return x && y && z;
+}
 // (tokens, heads, D) seen as 3-d (d, head, token); box 64 x 1 x 128, columns past D zeros
 inline int make_map_tokens(CUtensorMap* m, const void* ptr, int64_t rows, int64_t heads, int64_t D) {
   if (rows > 0x7fffffffLL) return GLA_ERR_TOO_LARGE;
@@ -94,11 +103,13 @@ __device__ __forceinline__ void wait_for(bool& ok, uint32_t bar, uint32_t parity
 }
 
 // What a chunk of 128 needs of its gates, made by one warp, four rows a lane.  lam: running sums, base 2, as two floats;
-// wt: exp(lam_i), exp(lam_L - lam_i).  The weight exp(lam_i - lam_j) of a pair in different groups of 32 rows is rf_i cf_j over
-// the last token before i's group (384 exponentials for 12288 pairs), inside a group it is formed as it stands.
+// wt: exp(lam_i), exp(lam_L - lam_i).  With a the last token before i's group of 32 rows, the weight exp(lam_i - lam_j) of a pair
+// is rf_i cf_j, cf[g - 1]: exp(lam_a - lam_j) for the tokens before group g, cd: for those of the group itself, as long as
+// the sums move by at most `span` <= 80 inside it; where a gate is sharper, the weights inside a group are formed pair by pair.
 struct Gates {
   float2 lam[128], wt[128];
-  float rf[128], cf[3][128];           // cf[g - 1]: to the last token before row group g
+  float rf[128], cd[128], cf[3][128];
+  float span[4];
 };
 __device__ __forceinline__ float4 gates_of(const Walk& p, int64_t t0, int nv, int h, int lane) {
   float g[4];
@@ -106,56 +117,52 @@ __device__ __forceinline__ float4 gates_of(const Walk& p, int64_t t0, int nv, in
   for (int i = 0; i < 4; ++i) g[i] = 4 * lane + i < nv ? p.g[(t0 + 4 * lane + i) * p.gt + h] : 0.f;
   return make_float4(g[0], g[1], g[2], g[3]);
 }
-// Sums in 64-bit fixed point with 40 bits behind the point (|sum| <= 128 x 289 < 2^16): exact, and a fifth of the time that
-// shuffled doubles take.
-__device__ __forceinline__ float2 two_floats(long long v) {
-  const float hi = __ll2float_rn(v);                       // (a multiple of its own last place: the difference is exact)
-  return make_float2(hi * 0x1p-40f, __ll2float_rn(v - __float2ll_rn(hi)) * 0x1p-40f);
+// Sums of two floats each (46 bits and more): a gate of -200 must not cost the weights behind it their last places, and doubles
+// take five times as long.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  const float s = a.x + b.x, t = s - a.x, e = ((a.x - (s - t)) + (b.x - t)) + (a.y + b.y), h = s + e;
+  return make_float2(h, e - (h - s));
 }
 __device__ __forceinline__ float2 scan_gates(float4 g, Gates& s, int lane) {
   const float x[4] = {g.x, g.y, g.z, g.w};
-  long long v[4], sum = 0;
-  bool nan = false;
+  float2 v[4], sum = make_float2(0.f, 0.f);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    // exp of less than -200 is 0 either way, of more than 200 inf; -inf would leave inf - inf
-    const float y = fminf(fmaxf(x[i], -200.f), 200.f), hi = y * 1.44269504f, lo = fmaf(y, 1.44269504f, -hi) + y * 1.92596299e-8f;
-    sum += __float2ll_rn(hi * 0x1p40f) + __float2ll_rn(lo * 0x1p40f);
-    nan = nan || x[i] != x[i];
+    // exp of less than -200 is 0 either way; -inf would leave inf - inf
+    const float y = x[i] < -200.f ? -200.f : x[i], hi = y * 1.44269504f, lo = fmaf(y, 1.44269504f, -hi) + y * 1.92596299e-8f;
+    sum = add2(sum, make_float2(hi, lo));
     v[i] = sum;
   }
-  long long inc = sum;
+  float2 inc = sum;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, inc, d);
-    if (lane >= d) inc += y;
+    const float2 y = make_float2(__shfl_up_sync(0xffffffffu, inc.x, d), __shfl_up_sync(0xffffffffu, inc.y, d));
+    if (lane >= d) inc = add2(inc, y);
   }
-  // a gate that is not a number makes every sum from it on one
-  const unsigned int odd = __ballot_sync(0xffffffffu, nan);
-  const float qnan = __int_as_float(0x7fffffff);
-  float2 all = two_floats(__shfl_sync(0xffffffffu, inc, 31));
-  if (odd) all.x = qnan;
-  float2 at[3];
-#pragma unroll
-  for (int m = 0; m < 3; ++m) {
-    at[m] = two_floats(__shfl_sync(0xffffffffu, inc, 8 * m + 7));
-    if (odd & ((1u << (8 * m + 8)) - 1)) at[m].x = qnan;
-  }
-  const float2 own = lane < 8 ? make_float2(0.f, 0.f) : lane < 16 ? at[0] : lane < 24 ? at[1] : at[2];
-  bool bad = (odd & ((1u << lane) - 1)) != 0;
+  const auto of = [&](int l) { return make_float2(__shfl_sync(0xffffffffu, inc.x, l), __shfl_sync(0xffffffffu, inc.y, l)); };
+  const float2 all = of(31), at[3] = {of(7), of(15), of(23)}, left = make_float2(__shfl_up_sync(0xffffffffu, inc.x, 1), __shfl_up_sync(0xffffffffu, inc.y, 1));
+  const float2 before = lane ? left : make_float2(0.f, 0.f), own = lane < 8 ? make_float2(0.f, 0.f) : lane < 16 ? at[0] : lane < 24 ? at[1] : at[2];
+  float span = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float2 y = two_floats(inc - sum + v[i]);
-    bad = bad || x[i] != x[i];
-    if (bad) y.x = qnan;
+    const float2 y = add2(before, v[i]);
+    const float d = (y.x - own.x) + (y.y - own.y);
     const int r = 4 * lane + i;
+    span = !(fabsf(d) <= span) ? fabsf(d) : span;           // (what is not a number stays)
     s.lam[r] = y;
     s.wt[r] = make_float2(ex2(y.x + y.y), ex2((all.x - y.x) + (all.y - y.y)));
-    s.rf[r] = ex2((y.x - own.x) + (y.y - own.y));
+    s.rf[r] = ex2(d);
+    s.cd[r] = ex2(-d);
 #pragma unroll
     for (int m = 0; m < 3; ++m)
       if (lane < 8 * (m + 1)) s.cf[m][r] = ex2((at[m].x - y.x) + (at[m].y - y.y));
   }
+#pragma unroll
+  for (int d = 1; d < 8; d <<= 1) {
+    const float y = __shfl_xor_sync(0xffffffffu, span, d);
+    span = !(y <= span) ? y : span;
+  }
+  if (lane % 8 == 0) s.span[lane / 8] = span;
   return all;
 }
 __device__ __forceinline__ float decay_of(float2 i, float2 j) { return ex2((i.x - j.x) + (i.y - j.y)); }
@@ -167,7 +174,7 @@ __device__ __forceinline__ void weigh(uint32_t tile, uint32_t lo, uint32_t plane
   const int r0 = threadIdx.x / 8, c = threadIdx.x % 8;
   const float* w_ = &wt[r0].x + (rev ? 0 : 1);
   const uint32_t at0 = sw128_chunk(r0, c);
-#pragma unroll 1
+#pragma unroll 2
   for (int j = 0; j < 4; ++j) {
     const float w = w_[64 * j];
     uint4 x[D / 64];
@@ -263,8 +270,11 @@ struct TLay {
   static constexpr int NK = !OUT || NU + NS <= 3 ? 2 : 1, NV = OUT ? 1 : 2, NL = OUT || NU > 2 ? 1 : 2;   // stages of K, V, the lower planes
   static constexpr int TK = DK * 256, TV = DV * 256, SP = DK * DV * 2;
   static constexpr int Q0 = 0, K0 = Q0 + (OUT ? TK : 0), V0 = K0 + NK * TK, L0 = V0 + NV * TV, S0 = L0 + NL * (NU - 1) * TK;
-  static constexpr int G0 = S0 + (OUT ? NS * SP : 0), BAR = G0 + 2 * (int)sizeof(Gates);
+  static constexpr int STG = S0 + (OUT ? NS * SP : 0), G0 = STG + (OUT && DK == 64 ? 128 * DV * 2 : 0), BAR = G0 + 2 * (int)sizeof(Gates);
   // (64 features make rows 0 to 63 of a product of 128: the others are made of the 16 KB behind the keys' tile, whatever is there)
+  // outputs are put together in the state's image once it has been used (64 features: its rows are too few, they have a tile of
+  // their own)
+  static constexpr int O0 = DK == 64 ? STG : S0;
   static constexpr int USED = BAR + 192 + (DK == 64 ? 16384 : 0);
   // one block per SM, whatever the sizes: each takes all of the tensor memory
   static constexpr int END = USED < 120 * 1024 ? 120 * 1024 : USED;
@@ -477,16 +487,18 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
       }
     };
     if constexpr (OUT) put_state();
-    const bool wide = p.vd % 16 == 0 && ((uintptr_t)p.out & 31) == 0;
 
     for (int i = 0; i < chunks; ++i) {
       const int nv = rows_of(i), kb = Y::NK == 2 ? i & 1 : 0, vb = Y::NV == 2 ? i & 1 : 0;
       const uint32_t ph = i & 1, kph = Y::NK == 2 ? (i >> 1) & 1 : ph;
       const uint32_t uk = base + Y::K0 + kb * Y::TK, uv = base + Y::V0 + vb * Y::TV;
       const Gates& gs = gates[i & 1];
-      wait_for(ok, bar(B_G + (i & 1)), (i >> 1) & 1);
       if constexpr (OUT) {
-        wait_for(ok, bar(B_QK), ph);
+        if (!all_done(bar(B_G + (i & 1)), (i >> 1) & 1, bar(B_QK), ph, bar(B_K + kb), kph)) {
+          wait_for(ok, bar(B_G + (i & 1)), (i >> 1) & 1);
+          wait_for(ok, bar(B_K + kb), kph);
+          wait_for(ok, bar(B_QK), ph);
+        }
         tc_fence_after();
 #pragma unroll 1
         for (int g = 0; g < 2; ++g) {
@@ -499,14 +511,20 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
             uint32_t x[32];
             tmem_ld32(tSC + lane_base + 32 * grp, x);
             tmem_ld_wait();
-            if (grp < q4) {
+            const bool own = grp == q4;
+            if (!own || gs.span[q4] <= 80.f) {
               const float rf = gs.rf[row];
-              const float4* cf = reinterpret_cast<const float4*>(&gs.cf[q4 - 1][32 * grp]);
+              const float4* cf = reinterpret_cast<const float4*>(own ? &gs.cd[32 * grp] : &gs.cf[q4 - 1][32 * grp]);
+              const int last = own ? lane : 31;            // the row's last column
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 const float4 c = cf[e];
-                pk[2 * e] = pack_bf16x2(__uint_as_float(x[4 * e]) * (rf * c.x), __uint_as_float(x[4 * e + 1]) * (rf * c.y));
-                pk[2 * e + 1] = pack_bf16x2(__uint_as_float(x[4 * e + 2]) * (rf * c.z), __uint_as_float(x[4 * e + 3]) * (rf * c.w));
+                const float y0 = 4 * e <= last ? __uint_as_float(x[4 * e]) * (rf * c.x) : 0.f;
+                const float y1 = 4 * e + 1 <= last ? __uint_as_float(x[4 * e + 1]) * (rf * c.y) : 0.f;
+                const float y2 = 4 * e + 2 <= last ? __uint_as_float(x[4 * e + 2]) * (rf * c.z) : 0.f;
+                const float y3 = 4 * e + 3 <= last ? __uint_as_float(x[4 * e + 3]) * (rf * c.w) : 0.f;
+                pk[2 * e] = pack_bf16x2(y0, y1);
+                pk[2 * e + 1] = pack_bf16x2(y2, y3);
               }
             } else {
               const float2 li = gs.lam[row];
@@ -524,7 +542,13 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
         }
         tmem_st_wait();
       }
-      wait_for(ok, bar(B_K + kb), kph);
+      if constexpr (!OUT) {
+        const uint32_t bu = i >= Y::NL ? bar(B_U + ((i - Y::NL) & 1)) : bar(B_K + kb), pu = i >= Y::NL ? ((i - Y::NL) >> 1) & 1 : kph;
+        if (!all_done(bar(B_G + (i & 1)), (i >> 1) & 1, bar(B_K + kb), kph, bu, pu)) {
+          wait_for(ok, bar(B_G + (i & 1)), (i >> 1) & 1);
+          wait_for(ok, bar(B_K + kb), kph);
+        }
+      }
       if constexpr (!OUT)
         if (i >= Y::NL) wait_for(ok, bar(B_U + ((i - Y::NL) & 1)), ((i - Y::NL) >> 1) & 1);      // (the lower planes' stage)
       weigh<DK, NU>(uk, base + Y::L0 + (Y::NL == 2 ? (i & 1) * (NU - 1) * Y::TK : 0), Y::TK, gs.wt, p.rev, nv);
@@ -539,15 +563,14 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
       if (lane == 0) mbar_arrive(bar(B_P + (i & 1)));
       if constexpr (OUT) {
         const int64_t t0 = r0 + first_of(i);
-        wait_for(ok, bar(B_QS), ph);
-        wait_for(ok, bar(B_PV), ph);
+        wait_for(ok, bar(B_PV), ph);             // (and Q S, which was issued before)
         tc_fence_after();
         if (was_odd(i)) masked_sums<DV, false>(tSC + lane_base, tOA + lane_base, uv, row, half);
         const float wi = gs.wt[row].x;
-        const int64_t at = ((t0 + row) * p.H + h) * p.vd + HV * half;
+        const int64_t at = ((t0 + row) * p.H + h) * p.vd + HV * half;      // (float32 outputs)
         const int64_t ra = p.r ? ((t0 + row) * (p.H / p.gr) + h / p.gr) * p.vd + HV * half : 0;
         float dot = 0.f;
-#pragma unroll 1
+#pragma unroll 2
         for (int c0 = 0; c0 < HV; c0 += 16) {
           uint32_t x[16], y[16];
           tmem_ld16(tOI + lane_base + HV * half + c0, x);
@@ -580,15 +603,27 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
               uint32_t w[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(o[2 * e], o[2 * e + 1]);
-              bf16* d = (bf16*)p.out + at + c0;
-              if (wide) {
-                if (left > 0) st_global_v8(d, w);
-              } else {
-                if (left > 0) *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-                if (left > 8) *reinterpret_cast<uint4*>(d + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-              }
+              const int c8 = (HV * half + c0) / 8;
+              const uint32_t d = base + Y::O0 + (c8 >> 3) * 16384;
+              sts16(d + sw128_chunk(row, c8 & 7), make_uint4(w[0], w[1], w[2], w[3]));
+              sts16(d + sw128_chunk(row, (c8 & 7) + 1), make_uint4(w[4], w[5], w[6], w[7]));
             }
           }
+        }
+        if (!p.out_f32) {
+          // the warp's 32 rows of HV columns, whole rows of them side by side
+          constexpr int LR = HV / 8, RI = 32 / LR;             // lanes a row, rows at once
+          __syncwarp();
+          const int c8 = HV / 8 * half + lane % LR;
+          const uint32_t d = base + Y::O0 + (c8 >> 3) * 16384;
+          bf16* o = (bf16*)p.out + ((t0 + 32 * q4 + lane / LR) * p.H + h) * p.vd + 8 * c8;
+#pragma unroll
+          for (int j = 0; j < 32; j += RI) {
+            const int r = 32 * q4 + j + lane / LR;
+            if (r < nv && 8 * c8 < p.vd) *reinterpret_cast<uint4*>(o) = lds16(d + sw128_chunk(r, c8 & 7));
+            o += (int64_t)RI * p.H * p.vd;
+          }
+          __syncwarp();
         }
         if (p.r && row < nv) p.rdot[(half * (p.cu ? p.T : p.nseq * p.T) + t0 + row) * p.H + h] = wi * dot;
         wait_for(ok, bar(B_U), ph);
