@@ -17,7 +17,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libgla_b200.so"
 SOURCES = ["gla_api.cu", "gla_scan.cu", "gla_simt.cu", "gla_split.cu", "gla_recurrent.cu", "gla_chunk_sm100.cu", "gla_state_sm100.cu", "gla_static.cu", "gla_decode.cu", "gla_layer.cu",
-           "gla_decay.cu", "gla_decay_one.cu", "gla_decay_state.cu", "gla_decay_fine.cu", "gla_decay_full.cu", "gla_decay_fast.cu", "gla_decay_back.cu", "gla_decay_tc.cu", "gla_beam.cu"]
+           "gla_decay.cu", "gla_decay_one.cu", "gla_decay_state.cu", "gla_decay_fine.cu", "gla_decay_full.cu", "gla_decay_back.cu", "gla_decay_tc.cu", "gla_beam.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",

@@ -1,6 +1,6 @@
 // Linear attention with one decay per head: what runs around the walks of gla_decay.cuh (runs of a sequence and their
 // states, sums over shared heads, the gradient of the decays), forward and backward.
-#include "gla_decay_bf16.cuh"
+#include "gla_decay_fast.cuh"
 
 namespace gla {
 namespace decay {
@@ -180,7 +180,7 @@ static int run_walk(cudaStream_t st, const Dims& d, int mode, Walk p, void* ws, 
   return walk(st, mode, p, true, name);
 }
 
-// ---- bf16, head sizes up to 128: the walks of gla_decay_bf16.cuh ---------------------------------------------------------
+// ---- bf16, head sizes up to 128: the walks of gla_decay_tc.cuh and gla_decay_tcb.cuh ---------------------------------------------------------
 static bool fast(const Dims& d) { return d.bf && d.Dk <= 128 && d.Dv <= 128; }
 static size_t state_bytes(const Dims& d, int64_t n) { return align_up((size_t)(n * d.H * d.Dk * d.Dv) * 4, 256); }
 // saved: final states in float32 | states that enter the runs (where sequences are cut)
@@ -225,7 +225,7 @@ static size_t fast_bwd_parts(const Dims& d, bool gate, size_t (&at)[4]) {
   const int64_t s = d.seg(128);
   at[0] = d.cut(s) ? fast_totals(d) : 0;
   at[1] = at[0] + (d.cut(s) ? state_bytes(d, d.slots(s)) : 0);
-  at[2] = at[1] + (gate ? align_up((size_t)(d.rows() * d.H) * 4, 256) : 0);
+  at[2] = at[1] + (gate ? align_up((size_t)(2 * d.rows() * d.H) * 4, 256) : 0);
   at[3] = at[2] + (d.H > d.Hk ? align_up((size_t)(d.rows() * d.H * d.Dk) * 4, 256) : 0);
   return at[3];
 }

@@ -57,7 +57,7 @@ struct Walk {
   int64_t ik, ic;
   int init_f32, fin_f32;
   float* seg_state;                 // [slot][H][vd][kd]: what a run adds (first pass), then the state that enters it
-  int64_t sk, sc;                   // strides in it that the walks of gla_decay_bf16.cuh read the entering state with
+  int64_t sk, sc;                   // strides in it that the walks of gla_decay_tc.cuh read the entering state with
   double* seg_total;                // [slot][H]: log2 of a run's decay
   void* out;                        // [token][H][vd]
   int out_f32;

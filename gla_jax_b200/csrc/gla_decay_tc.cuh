@@ -700,7 +700,6 @@ int launch_tc(cudaStream_t stream, const Walk& p, const char* name) {
   GLA_CHECK_LAUNCH();
   return GLA_OK;
 }
-unsigned int tc_walk_timeouts();
 
 }  // namespace decay
 }  // namespace gla
