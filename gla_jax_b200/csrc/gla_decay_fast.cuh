@@ -9,7 +9,7 @@ namespace decay {
 struct Back {
   Walk w;                                  // k, q, v; H, sizes, gates, runs; seg_state: gradients that enter each run backwards
   const void* dout;
-  const float* a;                          // [2][token][H], with gates: what the walk for dq leaves in rdot
+  const float* a;                          // [4][token][H], with gates: what the walk for dq leaves in rdot
   const float *S_runs, *S_end;             // entering states of the runs [slot][H][vd][kd] (NULL: one run each), final states
   void *dk, *dv;
   int dk_f32;

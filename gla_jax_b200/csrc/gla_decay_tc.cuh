@@ -1,7 +1,7 @@
 // The walks of gla_decay.cuh on the fifth-generation tensor cores: bf16, head sizes up to 128, 128 tokens at a time.
 //
-// Per chunk:  SC = Q K^T,  OI = Q S,  OA = P V  and  U = (w K)^T V  (w = exp(lam_L - lam_j), in two or three bf16 planes).  Eight
-// warps turn SC into P in tensor memory (a thread per row and half of the columns), weigh K in place, write exp(lam_i) OI + OA,
+// Per chunk:  SC = Q K^T,  OI = Q S,  OA = P V  and  U = (w K)^T V  (w = exp(lam_L - lam_j), in two or three bf16 planes).  Sixteen
+// warps turn SC into P in tensor memory (a thread per row and quarter of the columns), weigh K in place, write exp(lam_i) OI + OA,
 // and keep the state in registers: S <- exp(lam_L) S + U, from where its bf16 image goes to shared memory for the next chunk.
 // One warp issues the products, one the tensor copies, one prepares the gates of the chunk to come.
 //
@@ -174,18 +174,18 @@ __device__ __forceinline__ void weigh(uint32_t tile, uint32_t lo, uint32_t plane
   const int r0 = threadIdx.x / 8, c = threadIdx.x % 8;
   const float* w_ = &wt[r0].x + (rev ? 0 : 1);
   const uint32_t at0 = sw128_chunk(r0, c);
-#pragma unroll 2
-  for (int j = 0; j < 4; ++j) {
-    const float w = w_[64 * j];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float w = w_[128 * j];
     uint4 x[D / 64];
 #pragma unroll
-    for (int b = 0; b < D / 64; ++b) x[b] = lds16(tile + b * 16384 + j * 4096 + at0);
-    if (r0 + 32 * j >= nv)
+    for (int b = 0; b < D / 64; ++b) x[b] = lds16(tile + b * 16384 + j * 8192 + at0);
+    if (r0 + 64 * j >= nv)
 #pragma unroll
       for (int b = 0; b < D / 64; ++b) x[b] = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
     for (int b = 0; b < D / 64; ++b) {
-      const uint32_t at = b * 16384 + j * 4096 + at0;
+      const uint32_t at = b * 16384 + j * 8192 + at0;
       const uint32_t u[4] = {x[b].x, x[b].y, x[b].z, x[b].w};
       uint32_t s[4][NU];
 #pragma unroll
@@ -206,11 +206,11 @@ __device__ __forceinline__ bool check_rows(uint32_t tile, int nv) {
   const uint32_t at0 = tile + sw128_chunk(r0, c);
   uint32_t m = 0;
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
+  for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int b = 0; b < D / 64; ++b) {
-      const uint32_t at = at0 + b * 16384 + j * 4096;
-      if (r0 + 32 * j < nv) {
+      const uint32_t at = at0 + b * 16384 + j * 8192;
+      if (r0 + 64 * j < nv) {
         const uint4 v = lds16(at);
         m = __vmaxu2(__vmaxu2(m, v.x & 0x7fff7fffu), __vmaxu2(v.y & 0x7fff7fffu, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
       } else {
@@ -222,11 +222,11 @@ __device__ __forceinline__ bool check_rows(uint32_t tile, int nv) {
 // What is not finite in OA = P V, by sums over the tokens up to the row's own (UP = false) or from it on (UP): in the product,
 // zeros of P meet what is not finite in V, and 0 x inf is not a number, where the recurrence has it at its own token and after
 // (before) only.
-// P: this lane's row in tensor memory; 16 columns at a time.
+// P: this lane's row in tensor memory, 32 tokens in 16 columns at multiples of 32; 16 columns of V at a time.
 template <int DV, bool UP>
-__device__ __noinline__ void masked_sums(uint32_t tp, uint32_t to, uint32_t tv, int row, int half) {
+__device__ __noinline__ void masked_sums(uint32_t tp, uint32_t to, uint32_t tv, int row, int qt) {
 #pragma unroll 1
-  for (int c0 = half * (DV / 2); c0 < (half + 1) * (DV / 2); c0 += 16) {
+  for (int c0 = qt * (DV / 4); c0 < (qt + 1) * (DV / 4); c0 += 16) {
     float o[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[e] = 0.f;
@@ -234,7 +234,7 @@ __device__ __noinline__ void masked_sums(uint32_t tp, uint32_t to, uint32_t tv, 
     for (int k = 0; k < 8; ++k) {
       uint32_t pk[8];
       __syncwarp();
-      tmem_ld8(tp + 64 * (k >> 2) + 8 * (k & 3), pk);
+      tmem_ld8(tp + 32 * (k >> 1) + 8 * (k & 1), pk);
       tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -265,6 +265,8 @@ __device__ __noinline__ void masked_sums(uint32_t tp, uint32_t to, uint32_t tv, 
   tmem_st_wait();
 }
 
+constexpr int TC_WORK = 16, TC_THREADS = (TC_WORK + 3) * 32;             // worker warps; and products, copies, gates
+
 template <int DK, int DV, int NU, int NS, bool OUT>
 struct TLay {
   static constexpr int NK = !OUT || NU + NS <= 3 ? 2 : 1, NV = OUT ? 1 : 2, NL = OUT || NU > 2 ? 1 : 2;   // stages of K, V, the lower planes
@@ -290,9 +292,9 @@ struct TcWalk {
 
 // NU: planes of the weighted keys; NS: planes of the state as an operand
 template <int DK, int DV, int NU, int NS, bool OUT>
-__global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__ TcWalk a) {
+__global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_constant__ TcWalk a) {
   using Y = TLay<DK, DV, NU, NS, OUT>;
-  constexpr int HV = DV / 2;                                   // value columns of a worker
+  constexpr int HV = DV / 4;                                   // value columns of a worker
   const Walk& p = a.w;
   extern __shared__ __align__(1024) uint8_t sm[];
   Gates* gates = reinterpret_cast<Gates*>(sm + Y::G0);
@@ -301,7 +303,7 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
   const Run run = find_run(p, blockIdx.x);
   if constexpr (OUT) {
     if (run.zlo < run.zhi)
-      for (int64_t i = tid; i < (run.zhi - run.zlo) * p.vd; i += 352)
+      for (int64_t i = tid; i < (run.zhi - run.zlo) * p.vd; i += TC_THREADS)
         st_any(p.out, !p.out_f32, ((run.zlo + i / p.vd) * p.H + h) * p.vd + i % p.vd, 0.f);
     if (p.count_bad && run.any && run.first && blockIdx.y == 0 && tid == 0) {
       const int64_t a = p.cu ? p.cu[run.s] : 0, b = p.cu ? p.cu[run.s + 1] : 0;
@@ -315,7 +317,7 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
   const uint32_t base = smem_u32(sm), bars = base + Y::BAR;
   const auto bar = [&](int b) { return bars + 8 * b; };
   if (tid == 0) {
-    for (int i = 0; i < B_COUNT; ++i) mbar_init(bar(i), i == B_P || i == B_P + 1 || i == B_S || i == B_GFREE || i == B_GFREE + 1 ? 8 : 1);
+    for (int i = 0; i < B_COUNT; ++i) mbar_init(bar(i), i == B_P || i == B_P + 1 || i == B_S || i == B_GFREE || i == B_GFREE + 1 ? TC_WORK : 1);
     asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(bar(B_ODD)), "r"(0) : "memory");
     mbar_fence_init();
   }
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
     return x == (uint32_t)(i + 1);
   };
 
-  if (warp == 8) {
+  if (warp == TC_WORK) {
     // ================= products =================
     if (lane == 0) {
       const uint64_t dQ = desc_kmajor(base + Y::Q0, 16384, 0), dK = desc_kmajor(base + Y::K0, 16384, 0);
@@ -379,7 +381,7 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
         const uint32_t vst = vb * Y::TV;
         if constexpr (OUT) {
 #pragma unroll
-          for (int s = 0; s < 8; ++s) umma_ts(tOA, tSC + 64 * (s >> 2) + 8 * (s & 3), desc_advance(dV, s * 2048), i_pv, s > 0);
+          for (int s = 0; s < 8; ++s) umma_ts(tOA, tSC + 32 * (s >> 1) + 8 * (s & 1), desc_advance(dV, s * 2048), i_pv, s > 0);
           umma_commit(bar(B_PV));
         }
         const uint32_t lst = Y::NL == 2 ? (i & 1) * (NU - 1) * Y::TK : 0;
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == TC_WORK + 1) {
     // ================= tensor copies =================
     if (lane == 0) {
       const int hq = h / p.gq, hk = h / p.gk, hv = h / p.gv;
@@ -422,7 +424,7 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
       }
     }
     __syncwarp();
-  } else if (warp == 10) {
+  } else if (warp == TC_WORK + 2) {
     // ================= gates =================
     double total = 0.0;
     float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -438,21 +440,28 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
     if (!OUT && lane == 0) p.seg_total[slot_h] = total;
   } else {
     // ================= workers =================
-    const int q4 = warp & 3, half = warp >> 2, row = 32 * q4 + lane;
+    const int q4 = warp & 3, qt = warp >> 2, row = 32 * q4 + lane;
     const uint32_t lane_base = (uint32_t)(32 * q4) << 16;
-    // the state: row `row` (a key feature), columns HV half + [0, HV)
+    // the state: row `row` (a key feature), columns HV qt + [0, HV)
     float S[HV];
-    const int cols = row < p.kd ? p.vd - HV * half : 0;           // that there are of them
+    const int cols = row < p.kd ? p.vd - HV * qt : 0;           // that there are of them
     if (!OUT) {
 #pragma unroll
       for (int j = 0; j < HV; ++j) S[j] = 0.f;
-    } else if (p.seg_state || p.init_f32) {
-      const float* x = p.seg_state ? p.seg_state + slot_h * dd + row * p.sk + HV * half * p.sc : (const float*)p.init + sh * dd + row * p.ik + HV * half * p.ic;
+    } else if (p.seg_state && p.sc == 1) {
+    const float* x = p.seg_state + slot_h * dd + row * p.sk + HV * qt;
+#pragma unroll
+    for (int j = 0; j < HV; j += 4) {
+      const float4 y = j < cols ? *reinterpret_cast<const float4*>(x + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+      S[j] = y.x; S[j + 1] = y.y; S[j + 2] = y.z; S[j + 3] = y.w;
+    }
+  } else if (p.seg_state || p.init_f32) {
+      const float* x = p.seg_state ? p.seg_state + slot_h * dd + row * p.sk + HV * qt * p.sc : (const float*)p.init + sh * dd + row * p.ik + HV * qt * p.ic;
       const int64_t d = p.seg_state ? p.sc : p.ic;
 #pragma unroll
       for (int j = 0; j < HV; ++j, x += d) S[j] = j < cols ? *x : 0.f;
     } else {
-      const bf16* x = (const bf16*)p.init + sh * dd + row * p.ik + HV * half * p.ic;
+      const bf16* x = (const bf16*)p.init + sh * dd + row * p.ik + HV * qt * p.ic;
 #pragma unroll
       for (int j = 0; j < HV; ++j, x += p.ic) S[j] = j < cols ? __bfloat162float(*x) : 0.f;
     }
@@ -464,7 +473,7 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
           uint32_t s[4][NS];
 #pragma unroll
           for (int e = 0; e < 4; ++e) planes<NS>(S[j + 2 * e], S[j + 2 * e + 1], s[e]);
-          const int c8 = (HV * half + j) / 8;
+          const int c8 = (HV * qt + j) / 8;
 #pragma unroll
           for (int k = 0; k < NS; ++k)
             sts16(base + Y::S0 + k * Y::SP + (c8 >> 3) * DK * 128 + sw128_chunk(row, c8 & 7), make_uint4(s[0][k], s[1][k], s[2][k], s[3][k]));
@@ -478,16 +487,14 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
     const auto take_u = [&](int i) {
       const float all = gates[i & 1].wt[127].x;
 #pragma unroll
-      for (int c0 = 0; c0 < HV; c0 += 32) {
-        uint32_t u[32];
-        tmem_ld32(ubuf(i) + lane_base + HV * half + c0, u);
+      for (int c0 = 0; c0 < HV; c0 += 16) {
+        uint32_t u[16];
+        tmem_ld16(ubuf(i) + lane_base + HV * qt + c0, u);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) S[c0 + e] = fmaf(all, S[c0 + e], __uint_as_float(u[e]));
+        for (int e = 0; e < 16; ++e) S[c0 + e] = fmaf(all, S[c0 + e], __uint_as_float(u[e]));
       }
     };
-    if constexpr (OUT) put_state();
-
     for (int i = 0; i < chunks; ++i) {
       const int nv = rows_of(i), kb = Y::NK == 2 ? i & 1 : 0, vb = Y::NV == 2 ? i & 1 : 0;
       const uint32_t ph = i & 1, kph = Y::NK == 2 ? (i >> 1) & 1 : ph;
@@ -500,9 +507,8 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
           wait_for(ok, bar(B_QK), ph);
         }
         tc_fence_after();
-#pragma unroll 1
-        for (int g = 0; g < 2; ++g) {
-          const int grp = 2 * half + g;     // columns 32 grp + [0, 32)
+        {
+          const int grp = qt;               // columns 32 grp + [0, 32)
           uint32_t pk[16];
           if (grp > q4) {
 #pragma unroll
@@ -537,8 +543,8 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
               }
             }
           }
-          // P over this thread's own part of SC: columns 64 half + [0, 32)
-          tmem_st16(tSC + lane_base + 64 * half + 16 * g, pk);
+          // P over this thread's own part of SC
+          tmem_st16(tSC + lane_base + 32 * grp, pk);
         }
         tmem_st_wait();
       }
@@ -552,6 +558,8 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
       if constexpr (!OUT)
         if (i >= Y::NL) wait_for(ok, bar(B_U + ((i - Y::NL) & 1)), ((i - Y::NL) >> 1) & 1);      // (the lower planes' stage)
       weigh<DK, NU>(uk, base + Y::L0 + (Y::NL == 2 ? (i & 1) * (NU - 1) * Y::TK : 0), Y::TK, gs.wt, p.rev, nv);
+      if constexpr (OUT)
+        if (i == 0) put_state();            // (here, so that the state is on its way during the first scores)
       if (OUT || nv < 128) {
         wait_for(ok, bar(B_V + vb), Y::NV == 2 ? (i >> 1) & 1 : ph);
         const bool odd = check_rows<DV>(uv, nv);
@@ -565,23 +573,23 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
         const int64_t t0 = r0 + first_of(i);
         wait_for(ok, bar(B_PV), ph);             // (and Q S, which was issued before)
         tc_fence_after();
-        if (was_odd(i)) masked_sums<DV, false>(tSC + lane_base, tOA + lane_base, uv, row, half);
+        if (was_odd(i)) masked_sums<DV, false>(tSC + lane_base, tOA + lane_base, uv, row, qt);
         const float wi = gs.wt[row].x;
-        const int64_t at = ((t0 + row) * p.H + h) * p.vd + HV * half;      // (float32 outputs)
-        const int64_t ra = p.r ? ((t0 + row) * (p.H / p.gr) + h / p.gr) * p.vd + HV * half : 0;
+        const int64_t at = ((t0 + row) * p.H + h) * p.vd + HV * qt;      // (float32 outputs)
+        const int64_t ra = p.r ? ((t0 + row) * (p.H / p.gr) + h / p.gr) * p.vd + HV * qt : 0;
         float dot = 0.f;
 #pragma unroll 2
         for (int c0 = 0; c0 < HV; c0 += 16) {
           uint32_t x[16], y[16];
-          tmem_ld16(tOI + lane_base + HV * half + c0, x);
-          tmem_ld16(tOA + lane_base + HV * half + c0, y);
+          tmem_ld16(tOI + lane_base + HV * qt + c0, x);
+          tmem_ld16(tOA + lane_base + HV * qt + c0, y);
           tmem_ld_wait();
           if (row < nv) {
             if (p.r) {
               // the row's product with what comes from before the chunk
 #pragma unroll
               for (int e = 0; e < 16; e += 8)
-                if (HV * half + c0 + e < p.vd) {
+                if (HV * qt + c0 + e < p.vd) {
                   const uint4 u = __ldg((const uint4*)((const bf16*)p.r + ra + c0 + e));
                   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -594,7 +602,7 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
             float o[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = fmaf(wi, __uint_as_float(x[e]), __uint_as_float(y[e]));
-            const int left = p.vd - (HV * half + c0);
+            const int left = p.vd - (HV * qt + c0);
             if (p.out_f32) {
 #pragma unroll
               for (int e = 0; e < 16; e += 4)
@@ -603,7 +611,7 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
               uint32_t w[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(o[2 * e], o[2 * e + 1]);
-              const int c8 = (HV * half + c0) / 8;
+              const int c8 = (HV * qt + c0) / 8;
               const uint32_t d = base + Y::O0 + (c8 >> 3) * 16384;
               sts16(d + sw128_chunk(row, c8 & 7), make_uint4(w[0], w[1], w[2], w[3]));
               sts16(d + sw128_chunk(row, (c8 & 7) + 1), make_uint4(w[4], w[5], w[6], w[7]));
@@ -614,7 +622,7 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
           // the warp's 32 rows of HV columns, whole rows of them side by side
           constexpr int LR = HV / 8, RI = 32 / LR;             // lanes a row, rows at once
           __syncwarp();
-          const int c8 = HV / 8 * half + lane % LR;
+          const int c8 = HV / 8 * qt + lane % LR;
           const uint32_t d = base + Y::O0 + (c8 >> 3) * 16384;
           bf16* o = (bf16*)p.out + ((t0 + 32 * q4 + lane / LR) * p.H + h) * p.vd + 8 * c8;
 #pragma unroll
@@ -625,7 +633,7 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
           }
           __syncwarp();
         }
-        if (p.r && row < nv) p.rdot[(half * (p.cu ? p.T : p.nseq * p.T) + t0 + row) * p.H + h] = wi * dot;
+        if (p.r && row < nv) p.rdot[(qt * (p.cu ? p.T : p.nseq * p.T) + t0 + row) * p.H + h] = wi * dot;
         wait_for(ok, bar(B_U), ph);
         tc_fence_after();
         take_u(i);
@@ -651,7 +659,7 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
     }
     if constexpr (OUT) {
       if (run.last) {
-        const int64_t at = sh * dd + row * p.ik + HV * half * p.ic;
+        const int64_t at = sh * dd + row * p.ik + HV * qt * p.ic;
         float* f = p.fin_f32 ? (float*)p.fin + at : p.fin32 + at;
         if (p.fin_f32 ? p.fin != nullptr : p.fin32 != nullptr)
 #pragma unroll
@@ -671,7 +679,7 @@ __global__ void __launch_bounds__(352, 1) tc_walk_kernel(const __grid_constant__
         }
       }
     } else {
-      float* f = p.seg_state + slot_h * dd + (int64_t)HV * half * p.kd + row;
+      float* f = p.seg_state + slot_h * dd + (int64_t)HV * qt * p.kd + row;
 #pragma unroll
       for (int j = 0; j < HV; ++j, f += p.kd)
         if (j < cols) *f = S[j];
@@ -696,7 +704,7 @@ int launch_tc(cudaStream_t stream, const Walk& p, const char* name) {
   if (OUT) GLA_TRY(make_map_tokens(&a.q, p.q, rows, p.H / p.gq, p.kd));
   else a.q = a.k;
   ProfScope ps(name, stream);
-  tc_walk_kernel<DK, DV, NU, NS, OUT><<<dim3((unsigned)p.nslots, (unsigned)p.H), 352, Y::END, stream>>>(a);
+  tc_walk_kernel<DK, DV, NU, NS, OUT><<<dim3((unsigned)p.nslots, (unsigned)p.H), TC_THREADS, Y::END, stream>>>(a);
   GLA_CHECK_LAUNCH();
   return GLA_OK;
 }

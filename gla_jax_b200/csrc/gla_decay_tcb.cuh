@@ -19,7 +19,7 @@ namespace decay {
 struct TcBack {
   CUtensorMap q, k, v, o;
   Walk w;                                  // k, q, v; H, sizes, gates, runs; seg_state: gradients that enter each run backwards
-  const float* a;                          // [2][token][H], with gates
+  const float* a;                          // [4][token][H], with gates
   const float *S_runs, *S_end;             // entering states of the runs [slot][H][vd][kd], final states
   void *dk, *dv;
   int dk_f32;
@@ -34,7 +34,7 @@ struct BTLay {
   static constexpr int S0 = H0 + (DV < DK ? TK : 0), STG = S0 + NS * SP;
   static constexpr bool OWN = DK != 128 || DV != 128;                                   // outputs are put together in a place of their own
   static constexpr int G0 = STG + (OWN ? 256 * (DK > DV ? DK : DV) : 0), SUM = G0 + 2 * (int)sizeof(Gates);
-  static constexpr int RED = SUM + (GATE ? 2 * 4096 : 0), BAR = RED + 64, USED = BAR + 192 + (DK == 64 ? 16384 : 0);
+  static constexpr int RED = SUM + (GATE ? 2 * 6144 : 0), BAR = RED + 128, USED = BAR + 192 + (DK == 64 ? 16384 : 0);
   static constexpr int END = USED < 120 * 1024 ? 120 * 1024 : USED;
   static constexpr int HI = DV < DK ? H0 : V0, OUT0 = OWN ? STG : S0;
   static_assert(END <= 232448, "shared memory");
@@ -42,12 +42,12 @@ struct BTLay {
 };
 enum TbBar { C_LOAD = 0, C_ST = 1, C_I = 2, C_DV = 3, C_U = 4, C_P = 5, C_W = 6, C_S = 7, C_G = 8, C_GFREE = 10, C_E = 12, C_COUNT = 14, C_TMEM = 14, C_ODD = 15 };
 
-// o (a row of tensor memory, D / 2 columns from the half's first) += sum over i >= row of P_i V_i, for a chunk in which V holds
+// o (a row of tensor memory, D / 4 columns from the quarter's first) += sum over i >= row of P_i V_i, for a chunk in which V holds
 // something that is not finite (see masked_sums)
 template <int D>
-__device__ __noinline__ void masked_add(uint32_t tp, uint32_t to, uint32_t tv, int row, int half) {
+__device__ __noinline__ void masked_add(uint32_t tp, uint32_t to, uint32_t tv, int row, int qt) {
 #pragma unroll 1
-  for (int c0 = half * (D / 2); c0 < (half + 1) * (D / 2); c0 += 16) {
+  for (int c0 = qt * (D / 4); c0 < (qt + 1) * (D / 4); c0 += 16) {
     uint32_t r[16];
     __syncwarp();
     tmem_ld16(to + c0, r);
@@ -56,7 +56,7 @@ __device__ __noinline__ void masked_add(uint32_t tp, uint32_t to, uint32_t tv, i
     for (int k = 0; k < 8; ++k) {
       uint32_t pk[8];
       __syncwarp();
-      tmem_ld8(tp + 64 * (k >> 2) + 8 * (k & 3), pk);
+      tmem_ld8(tp + 32 * (k >> 1) + 8 * (k & 1), pk);
       tmem_ld_wait();
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
@@ -85,12 +85,12 @@ template <int D>
 __device__ __forceinline__ void weigh_to(uint32_t tile, uint32_t hi, uint32_t lo, const float2* wt) {
   const int r0 = threadIdx.x / 8, c = threadIdx.x % 8;
   const uint32_t at0 = sw128_chunk(r0, c);
-#pragma unroll 2
-  for (int j = 0; j < 4; ++j) {
-    const float w = wt[r0 + 32 * j].x;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float w = wt[r0 + 64 * j].x;
 #pragma unroll
     for (int b = 0; b < D / 64; ++b) {
-      const uint32_t at = b * 16384 + j * 4096 + at0;
+      const uint32_t at = b * 16384 + j * 8192 + at0;
       const uint4 x = lds16(tile + at);
       const uint32_t u[4] = {x.x, x.y, x.z, x.w};
       uint32_t s[4][2];
@@ -104,9 +104,9 @@ __device__ __forceinline__ void weigh_to(uint32_t tile, uint32_t hi, uint32_t lo
     }
   }
 }
-__device__ __forceinline__ bool workers_or(bool x) {          // barrier of the 256 workers, and whether any has x
+__device__ __forceinline__ bool workers_or(bool x) {          // barrier of the workers, and whether any has x
   uint32_t r;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 512, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
                : "=r"(r) : "r"((uint32_t)x) : "memory");
   return r != 0;
 }
@@ -123,28 +123,29 @@ __device__ __forceinline__ float lane_sums(float (&v)[32], int lane) {
 }
 
 template <int DK, int DV, bool GATE>
-__global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__ TcBack a) {
+__global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_constant__ TcBack a) {
   using Y = BTLay<DK, DV, GATE>;
-  constexpr int NS = Y::NS, HV = DV / 2, HK = DK / 2;
+  constexpr int NS = Y::NS, HV = DV / 4, HK = DK / 4;
+  static_assert(TC_WORK == 16, "workers_or");
   const Walk& p = a.w;
   extern __shared__ __align__(1024) uint8_t sm[];
   Gates* gates = reinterpret_cast<Gates*>(sm + Y::G0);
-  float* sums = reinterpret_cast<float*>(sm + Y::SUM);          // [2][8][128]: r by row group, c and b by half
+  float* sums = reinterpret_cast<float*>(sm + Y::SUM);          // [2][12][128]: r by row group, c and b by quarter
   double* red = reinterpret_cast<double*>(sm + Y::RED);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int h = blockIdx.y;
   const Run run = find_run(p, blockIdx.x);
   if (run.zlo < run.zhi) {
-    for (int64_t i = tid; i < (run.zhi - run.zlo) * p.kd; i += 352) st_any(a.dk, !a.dk_f32, ((run.zlo + i / p.kd) * p.H + h) * p.kd + i % p.kd, 0.f);
-    for (int64_t i = tid; i < (run.zhi - run.zlo) * p.vd; i += 352) st_any(a.dv, 1, ((run.zlo + i / p.vd) * p.H + h) * p.vd + i % p.vd, 0.f);
+    for (int64_t i = tid; i < (run.zhi - run.zlo) * p.kd; i += TC_THREADS) st_any(a.dk, !a.dk_f32, ((run.zlo + i / p.kd) * p.H + h) * p.kd + i % p.kd, 0.f);
+    for (int64_t i = tid; i < (run.zhi - run.zlo) * p.vd; i += TC_THREADS) st_any(a.dv, 1, ((run.zlo + i / p.vd) * p.H + h) * p.vd + i % p.vd, 0.f);
     if (GATE)
-      for (int64_t i = tid; i < run.zhi - run.zlo; i += 352) a.dg[(run.zlo + i) * p.H + h] = 0.f;
+      for (int64_t i = tid; i < run.zhi - run.zlo; i += TC_THREADS) a.dg[(run.zlo + i) * p.H + h] = 0.f;
   }
   if (!run.any) return;
   const uint32_t base = smem_u32(sm), bars = base + Y::BAR;
   const auto bar = [&](int b) { return bars + 8 * b; };
   if (tid == 0) {
-    for (int i = 0; i < C_COUNT; ++i) mbar_init(bar(i), i == C_P || i == C_W || i == C_S || i >= C_GFREE ? 8 : 1);
+    for (int i = 0; i < C_COUNT; ++i) mbar_init(bar(i), i == C_P || i == C_W || i == C_S || i >= C_GFREE ? TC_WORK : 1);
     asm volatile("st.shared.v2.u32 [%0], {%1, %1};" ::"r"(bar(C_ODD)), "r"(0) : "memory");
     mbar_fence_init();
   }
@@ -158,15 +159,15 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
   const auto rows_of = [&](int i) { const int c0 = 128 * (chunks - 1 - i); return len - c0 < 128 ? len - c0 : 128; };   // step i: from the end
   const auto token = [&](int i) { return r0 + 128 * (chunks - 1 - i); };
 
-  const int q4 = warp & 3, half = (warp >> 2) & 1, row = 32 * q4 + lane;      // (workers)
+  const int q4 = warp & 3, qt = (warp >> 2) & 3, row = 32 * q4 + lane;      // (workers)
   const uint32_t lane_base = (uint32_t)(32 * q4) << 16;
-  float S[HV];                                                               // dS: row `row`, columns HV half + [0, HV)
-  const int cols = row < p.kd ? p.vd - HV * half : 0;
-  if (warp < 8) {
+  float S[HV];                                                               // dS: row `row`, columns HV qt + [0, HV)
+  const int cols = row < p.kd ? p.vd - HV * qt : 0;
+  if (warp < TC_WORK) {
     double dot = 0.0;
-    const float* xs = p.seg_state ? p.seg_state + slot_h * dd + row + (int64_t)HV * half * p.kd : nullptr;
-    const float* leave = !GATE ? nullptr : run.last ? a.S_end + sh * dd + (int64_t)row * p.vd + HV * half : a.S_runs + (slot_h + p.H) * dd + row + (int64_t)HV * half * p.kd;
-    const int64_t ld = run.last ? 1 : p.kd, at = sh * dd + (int64_t)row * p.vd + HV * half;
+    const float* xs = p.seg_state ? p.seg_state + slot_h * dd + row + (int64_t)HV * qt * p.kd : nullptr;
+    const float* leave = !GATE ? nullptr : run.last ? a.S_end + sh * dd + (int64_t)row * p.vd + HV * qt : a.S_runs + (slot_h + p.H) * dd + row + (int64_t)HV * qt * p.kd;
+    const int64_t ld = run.last ? 1 : p.kd, at = sh * dd + (int64_t)row * p.vd + HV * qt;
 #pragma unroll
     for (int j = 0; j < HV; ++j) {
       float x = 0.f;
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
   const uint32_t tST = tmem, tDT = tmem + 128, tIV = tmem + 256, tIK = tmem + 384;
   bool ok = true;
 
-  if (warp == 8) {
+  if (warp == TC_WORK) {
     // ================= products =================
     if (lane == 0) {
       const auto kcol = [](int s) { return (uint32_t)((s >> 2) * 16384 + (s & 3) * 32); };
@@ -226,9 +227,9 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(odd) : "r"(bar(C_ODD) + 4 * (i & 1)) : "memory");
         if (odd != (uint32_t)(i + 1)) {
 #pragma unroll
-          for (int s = 0; s < 8; ++s) umma_ts(tIV, tST + 64 * (s >> 2) + 8 * (s & 3), desc_advance(mO, s * 2048), idesc_bf16(128, DV, 0, 1), 1);
+          for (int s = 0; s < 8; ++s) umma_ts(tIV, tST + 32 * (s >> 1) + 8 * (s & 1), desc_advance(mO, s * 2048), idesc_bf16(128, DV, 0, 1), 1);
 #pragma unroll
-          for (int s = 0; s < 8; ++s) umma_ts(tIK, tDT + 64 * (s >> 2) + 8 * (s & 3), desc_advance(mQ, s * 2048), idesc_bf16(128, DK, 0, 1), 1);
+          for (int s = 0; s < 8; ++s) umma_ts(tIK, tDT + 32 * (s >> 1) + 8 * (s & 1), desc_advance(mQ, s * 2048), idesc_bf16(128, DK, 0, 1), 1);
         }
         umma_commit(bar(C_DV));
         wait_for(ok, bar(C_W), ph);
@@ -242,7 +243,7 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
       }
     }
     __syncwarp();
-  } else if (warp == 9) {
+  } else if (warp == TC_WORK + 1) {
     // ================= tensor copies =================
     if (lane == 0) {
       const int hk = h / p.gq;
@@ -266,15 +267,15 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
       }
     }
     __syncwarp();
-  } else if (warp == 10) {
+  } else if (warp == TC_WORK + 2) {
     // ================= gates, and their gradient a step behind =================
     double carry = 0.0;
     if (GATE)
-      for (int w = 0; w < 8; ++w) carry += red[w];
+      for (int w = 0; w < TC_WORK; ++w) carry += red[w];
     const auto gradient = [&](int i) {
       const int nv = rows_of(i);
       const int64_t t0 = token(i);
-      const float* s = sums + (i & 1) * 1024;
+      const float* s = sums + (i & 1) * 1536;
       wait_for(ok, bar(C_E + (i & 1)), (i >> 1) & 1);
       double e[4], sum = 0.0;
 #pragma unroll
@@ -283,8 +284,9 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
         double x = 0.0;
         if (t < nv) {
           const float* y = s + t;
-          x = ((double)y[0] + y[128]) + ((double)y[256] + y[384]) - ((double)y[512] + y[640]) - ((double)y[768] + y[896]);
-          x += (double)a.a[(t0 + t) * p.H + h] + a.a[(rows + t0 + t) * p.H + h];
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+            x += (double)y[128 * m] - (double)y[512 + 128 * m] - (double)y[1024 + 128 * m] + (double)a.a[(m * rows + t0 + t) * p.H + h];
         }
         sum += x;
         e[u] = sum;
@@ -322,7 +324,7 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
           uint32_t s[4][NS];
 #pragma unroll
           for (int e = 0; e < 4; ++e) planes<NS>(S[j + 2 * e], S[j + 2 * e + 1], s[e]);
-          const int c8 = (HV * half + j) / 8;
+          const int c8 = (HV * qt + j) / 8;
 #pragma unroll
           for (int k = 0; k < NS; ++k)
             sts16(base + Y::S0 + k * Y::SP + (c8 >> 3) * DK * 128 + sw128_chunk(row, c8 & 7), make_uint4(s[0][k], s[1][k], s[2][k], s[3][k]));
@@ -339,7 +341,7 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
       const int64_t t0 = token(i);
       const uint32_t ph = i & 1;
       const Gates& gs = gates[i & 1];
-      float* sum = sums + (i & 1) * 1024;
+      float* sum = sums + (i & 1) * 1536;
       if (!all_done(bar(C_G + (i & 1)), (i >> 1) & 1, bar(C_LOAD), ph, bar(C_ST), ph)) {
         wait_for(ok, bar(C_G + (i & 1)), (i >> 1) & 1);
         wait_for(ok, bar(C_LOAD), ph);
@@ -347,9 +349,8 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
       }
       tc_fence_after();
       float rowsum = 0.f;
-#pragma unroll 1
-      for (int g = 0; g < 2; ++g) {
-        const int grp = 2 * half + g;     // columns (tokens i) 32 grp + [0, 32)
+      {
+        const int grp = qt;               // columns (tokens i) 32 grp + [0, 32)
         uint32_t pk[16], ek[16];
         if (grp < q4) {
 #pragma unroll
@@ -385,10 +386,10 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
           }
           if constexpr (GATE) sum[128 * q4 + 32 * grp + lane] = lane_sums(m, lane);
         }
-        tmem_st16(tST + lane_base + 64 * half + 16 * g, pk);
-        tmem_st16(tDT + lane_base + 64 * half + 16 * g, ek);
+        tmem_st16(tST + lane_base + 32 * grp, pk);
+        tmem_st16(tDT + lane_base + 32 * grp, ek);
       }
-      if (GATE) sum[512 + 128 * half + row] = rowsum;
+      if (GATE) sum[512 + 128 * qt + row] = rowsum;
       bool odd = check_rows<DV>(base + Y::O0, nv);
       odd = check_rows<DK>(base + Y::Q0, nv) || odd;
       wait_for(ok, bar(C_I), ph);
@@ -398,22 +399,22 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
 #pragma unroll 1
       for (int c0 = 0; c0 < HV; c0 += 16) {
         uint32_t x[16];
-        tmem_ld16(tIV + lane_base + HV * half + c0, x);
+        tmem_ld16(tIV + lane_base + HV * qt + c0, x);
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(wj * __uint_as_float(x[e]));
-        tmem_st16(tIV + lane_base + HV * half + c0, x);
+        tmem_st16(tIV + lane_base + HV * qt + c0, x);
       }
 #pragma unroll 1
       for (int c0 = 0; c0 < HK; c0 += 16) {
         uint32_t x[16];
-        tmem_ld16(tIK + lane_base + HK * half + c0, x);
+        tmem_ld16(tIK + lane_base + HK * qt + c0, x);
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(wj * __uint_as_float(x[e]));
-        tmem_st16(tIK + lane_base + HK * half + c0, x);
+        tmem_st16(tIK + lane_base + HK * qt + c0, x);
         if constexpr (GATE) {
-          const int c8 = (HK * half + c0) / 8;
+          const int c8 = (HK * qt + c0) / 8;
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             const uint4 k = lds16(base + Y::K0 + (c8 >> 3) * 16384 + sw128_chunk(row, (c8 & 7) + b));
@@ -426,15 +427,15 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
           }
         }
       }
-      if (GATE) sum[768 + 128 * half + row] = dot;
+      if (GATE) sum[1024 + 128 * qt + row] = dot;
       tmem_st_wait();
       fence_async_smem();
       tc_fence_before();
       odd = workers_or(odd);              // (and K and V are done with)
       if (odd) {
         tc_fence_after();
-        masked_add<DV>(tST + lane_base, tIV + lane_base, base + Y::O0, row, half);
-        masked_add<DK>(tDT + lane_base, tIK + lane_base, base + Y::Q0, row, half);
+        masked_add<DV>(tST + lane_base, tIV + lane_base, base + Y::O0, row, qt);
+        masked_add<DK>(tDT + lane_base, tIK + lane_base, base + Y::Q0, row, qt);
         tc_fence_before();
         if (tid == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(bar(C_ODD) + 4 * (i & 1)), "r"(i + 1) : "memory");
       }
@@ -454,9 +455,9 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
         constexpr bool DKO = decltype(is_dk)::value;
         constexpr int HD = DKO ? HK : HV;
         const int nd = DKO ? p.kd : p.vd;
-        const uint32_t t = (DKO ? tIK : tIV) + lane_base + HD * half;
+        const uint32_t t = (DKO ? tIK : tIV) + lane_base + HD * qt;
         if (DKO && a.dk_f32) {
-          float* o = (float*)a.dk + ((t0 + row) * p.H + h) * nd + HD * half;
+          float* o = (float*)a.dk + ((t0 + row) * p.H + h) * nd + HD * qt;
 #pragma unroll 1
           for (int c0 = 0; c0 < HD; c0 += 16) {
             uint32_t x[16];
@@ -464,7 +465,7 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
-              if (row < nv && HD * half + c0 + e < nd)
+              if (row < nv && HD * qt + c0 + e < nd)
                 *reinterpret_cast<float4*>(o + c0 + e) = make_float4(__uint_as_float(x[e]), __uint_as_float(x[e + 1]), __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
           }
           return;
@@ -476,14 +477,14 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
           tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
-          const int c8 = (HD * half + c0) / 8;
+          const int c8 = (HD * qt + c0) / 8;
           const uint32_t d = base + Y::OUT0 + (c8 >> 3) * 16384;
           sts16(d + sw128_chunk(row, c8 & 7), make_uint4(w[0], w[1], w[2], w[3]));
           sts16(d + sw128_chunk(row, (c8 & 7) + 1), make_uint4(w[4], w[5], w[6], w[7]));
         }
         constexpr int LR = HD / 8, RI = 32 / LR;
         __syncwarp();
-        const int c8 = HD / 8 * half + lane % LR;
+        const int c8 = HD / 8 * qt + lane % LR;
         const uint32_t d = base + Y::OUT0 + (c8 >> 3) * 16384;
         bf16* o = (bf16*)(DKO ? a.dk : a.dv) + ((t0 + 32 * q4 + lane / LR) * p.H + h) * nd + 8 * c8;
 #pragma unroll
@@ -500,19 +501,19 @@ __global__ void __launch_bounds__(352, 1) tc_back_kernel(const __grid_constant__
       tc_fence_after();
       const float all = gs.wt[127].x;
 #pragma unroll
-      for (int c0 = 0; c0 < HV; c0 += 32) {
-        uint32_t u[32];
-        tmem_ld32(tST + lane_base + HV * half + c0, u);
+      for (int c0 = 0; c0 < HV; c0 += 16) {
+        uint32_t u[16];
+        tmem_ld16(tST + lane_base + HV * qt + c0, u);
         tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 32; ++e) S[c0 + e] = fmaf(all, S[c0 + e], __uint_as_float(u[e]));
+        for (int e = 0; e < 16; ++e) S[c0 + e] = fmaf(all, S[c0 + e], __uint_as_float(u[e]));
       }
       if (i + 1 < chunks) put_state();
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(C_GFREE + (i & 1)));
     }
     if (p.fin && run.first) {
-      const int64_t at = sh * dd + (int64_t)row * p.vd + HV * half;
+      const int64_t at = sh * dd + (int64_t)row * p.vd + HV * qt;
 #pragma unroll
       for (int j = 0; j < HV; ++j)
         if (j < cols) st_any(p.fin, !p.fin_f32, at + j, S[j]);
@@ -536,7 +537,7 @@ int launch_tc_back(cudaStream_t stream, TcBack& b, const void* dout) {
   GLA_TRY(make_map_tokens(&b.v, p.v, rows, p.H, p.vd));
   GLA_TRY(make_map_tokens(&b.o, dout, rows, p.H, p.vd));
   ProfScope ps("decay_back_kernel", stream);
-  tc_back_kernel<DK, DV, GATE><<<dim3((unsigned)p.nslots, (unsigned)p.H), 352, Y::END, stream>>>(b);
+  tc_back_kernel<DK, DV, GATE><<<dim3((unsigned)p.nslots, (unsigned)p.H), TC_THREADS, Y::END, stream>>>(b);
   GLA_CHECK_LAUNCH();
   return GLA_OK;
 }
