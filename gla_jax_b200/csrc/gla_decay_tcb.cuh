@@ -259,11 +259,6 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
           tma_load_3d(base + Y::V0 + b * 16384, &a.v, 64 * b, h, z, bar(C_LOAD));
           tma_load_3d(base + Y::O0 + b * 16384, &a.o, 64 * b, h, z, bar(C_LOAD));
         }
-        if (i + 1 < chunks) {
-          // the next chunk's rows on their way into L2
-          for (int b = 0; b < DK / 64; ++b) { tma_prefetch_l2_3d(&a.k, 64 * b, hk, z - 128); tma_prefetch_l2_3d(&a.q, 64 * b, hk, z - 128); }
-          for (int b = 0; b < DV / 64; ++b) { tma_prefetch_l2_3d(&a.v, 64 * b, h, z - 128); tma_prefetch_l2_3d(&a.o, 64 * b, h, z - 128); }
-        }
       }
     }
     __syncwarp();
