@@ -38,14 +38,16 @@ struct Step {
 };
 constexpr int SNT = 128;
 
-// One row per block, its loads all in flight before the first is used.
+// One row per block, its loads all in flight before the first is used.  Measured, 32 requests x 16 heads, 128 x 128, bf16: 13.5 us
+// with k and q read by every thread for itself -> 12.3 us through shared memory (the bytes at the copy rate: 10.3).
 template <int W, int RPT>
 __global__ void __launch_bounds__(SNT) step_kernel(const Step p) {
   constexpr int CL = W / 4, RL = SNT / CL;
   __shared__ float red[4][W];
+  __shared__ float kq[2][RPT * RL];
   const int cl = threadIdx.x % CL, rl = threadIdx.x / CL;
   const int64_t row = blockIdx.y;                                 // (request, head)
-  const int64_t b = row / p.H, h = row % p.H, kv = b * (p.H / p.share) + h / p.share;
+  const int64_t b = row / p.H, h = row % p.H, kv = (b * (p.H / p.share) + h / p.share) * p.Dk;
   const int c0 = blockIdx.x * W + 4 * cl;
   const bool on = c0 < p.Dv;
   float* Sp = p.S + (row * p.Dk + rl) * (int64_t)p.Dv + c0;
@@ -55,17 +57,22 @@ __global__ void __launch_bounds__(SNT) step_kernel(const Step p) {
 #pragma unroll
   for (int i = 0; i < RPT; ++i)
     if (on && rl + i * RL < p.Dk) s[i] = *reinterpret_cast<const float4*>(Sp + (int64_t)i * RL * p.Dv);
+  for (int i = threadIdx.x; i < p.Dk; i += SNT) {
+    kq[0][i] = ld_any(p.k, p.bf, kv + i);
+    kq[1][i] = ld_any(p.q, p.bf, kv + i);
+  }
   const float f = expf(p.g[row]);
   float4 vv = make_float4(0.f, 0.f, 0.f, 0.f), acc = vv;
   if (on) {
     const int64_t at = row * p.Dv + c0;
     vv = make_float4(ld_any(p.v, p.bf, at), ld_any(p.v, p.bf, at + 1), ld_any(p.v, p.bf, at + 2), ld_any(p.v, p.bf, at + 3));
   }
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < RPT; ++i) {
     const int r = rl + i * RL;
     if (!on || r >= p.Dk) continue;
-    const float kr = ld_any(p.k, p.bf, kv * p.Dk + r), qr = ld_any(p.q, p.bf, kv * p.Dk + r);
+    const float kr = kq[0][r], qr = kq[1][r];
     float4 n;
     n.x = fmaf(f, s[i].x, kr * vv.x); n.y = fmaf(f, s[i].y, kr * vv.y);
     n.z = fmaf(f, s[i].z, kr * vv.z); n.w = fmaf(f, s[i].w, kr * vv.w);
@@ -95,14 +102,18 @@ __global__ void __launch_bounds__(SNT) step_beams_kernel(const Step p) {
   const int rpt = (p.Dk + RL - 1) / RL;
   float4* old = reinterpret_cast<float4*>(sm);                                        // [K][rpt][SNT]
   float* red = reinterpret_cast<float*>(sm + (size_t)p.K * rpt * SNT * 16);           // [K][4][W]
+  float* kq = red + p.K * 4 * W;                                                      // [K][k, q][Dk]
+  float* vf = kq + 2 * p.K * p.Dk;                                                    // [K][v (W), exp(g), parent, 2 spare]
   const int cl = threadIdx.x % CL, rl = threadIdx.x / CL, warp = threadIdx.x / 32;
   const int64_t n = blockIdx.y / p.H, h = blockIdx.y % p.H;
   const int c0 = blockIdx.x * W + 4 * cl;
   const bool on = c0 < p.Dv;
   grid_dep_wait();
   grid_dep_launch();
-  unsigned int used = 0;                                                              // beams that are somebody's parent
-  for (int j = 0; j < p.K; ++j) used |= 1u << parent_of(p.parents, n, p.K, j, blockIdx.x == 0 && h == 0 && threadIdx.x == 0);
+  // beams that are somebody's parent: a lane looks at one
+  const int lane = threadIdx.x % 32;
+  const int par = lane < p.K ? parent_of(p.parents, n, p.K, lane, blockIdx.x == 0 && h == 0 && warp == 0) : 0;
+  const unsigned int used = __reduce_or_sync(0xffffffffu, lane < p.K ? 1u << par : 0u);
   for (int j = 0; j < p.K; ++j) {
     if (!((used >> j) & 1u)) continue;
     const float* Sp = p.S + (((n * p.K + j) * p.H + h) * p.Dk + rl) * (int64_t)p.Dv + c0;
@@ -110,22 +121,37 @@ __global__ void __launch_bounds__(SNT) step_beams_kernel(const Step p) {
       if (on && rl + i * RL < p.Dk) cp16(sm32(old + (j * rpt + i) * SNT + threadIdx.x), Sp + (int64_t)i * RL * p.Dv, true);
   }
   cp_commit();
+  for (int i = threadIdx.x; i < p.K * p.Dk; i += SNT) {
+    const int j = i / p.Dk, r = i % p.Dk;
+    const int64_t b = n * p.K + j, kv = (b * (p.H / p.share) + h / p.share) * p.Dk + r;
+    kq[2 * j * p.Dk + r] = ld_any(p.k, p.bf, kv);
+    kq[(2 * j + 1) * p.Dk + r] = ld_any(p.q, p.bf, kv);
+  }
+  for (int i = threadIdx.x; i < p.K * W; i += SNT) {
+    const int j = i / W, c = blockIdx.x * W + i % W;
+    vf[j * (W + 4) + i % W] = c < p.Dv ? ld_any(p.v, p.bf, ((n * p.K + j) * p.H + h) * p.Dv + c) : 0.f;
+  }
+  if (warp == 0 && lane < p.K) {
+    vf[lane * (W + 4) + W] = KEYED ? 0.f : expf(p.g[(n * p.K + lane) * p.H + h]);
+    vf[lane * (W + 4) + W + 1] = __int_as_float(par);
+  }
   cp_wait<0>();
+  __syncthreads();
   for (int j = 0; j < p.K; ++j) {
-    const int from = parent_of(p.parents, n, p.K, j, false);
-    const int64_t b = n * p.K + j, row = b * p.H + h, kv = b * (p.H / p.share) + h / p.share;
+    const float* vj = vf + j * (W + 4);
+    const int from = __float_as_int(vj[W + 1]);
+    const int64_t row = (n * p.K + j) * p.H + h;
     float* Sp = p.S + (row * p.Dk + rl) * (int64_t)p.Dv + c0;
-    const float f1 = KEYED ? 0.f : expf(p.g[row]);
-    float4 vv = make_float4(0.f, 0.f, 0.f, 0.f), acc = vv;
-    if (on) {
-      const int64_t at = row * p.Dv + c0;
-      vv = make_float4(ld_any(p.v, p.bf, at), ld_any(p.v, p.bf, at + 1), ld_any(p.v, p.bf, at + 2), ld_any(p.v, p.bf, at + 3));
-    }
+    const float f1 = vj[W];
+    const float* kj = kq + 2 * j * p.Dk;
+    const float4 vv = *reinterpret_cast<const float4*>(vj + 4 * cl);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int i = 0; i < rpt; ++i) {
       const int r = rl + i * RL;
       if (!on || r >= p.Dk) continue;
       const float f = KEYED ? expf(p.g[row * p.Dk + r]) : f1;
-      const float kr = ld_any(p.k, p.bf, kv * p.Dk + r), qr = ld_any(p.q, p.bf, kv * p.Dk + r);
+      const float kr = kj[r], qr = kj[p.Dk + r];
       const float4 s = old[(from * rpt + i) * SNT + threadIdx.x];
       float4 x;
       x.x = fmaf(f, s.x, kr * vv.x); x.y = fmaf(f, s.y, kr * vv.y);
@@ -158,19 +184,20 @@ static int launch_step(cudaStream_t st, const Step& p, int64_t rows) {
 template <int W, bool KEYED>
 static int launch_beams(cudaStream_t st, const Step& p, int64_t groups) {
   constexpr int RL = SNT / (W / 4);
-  const size_t smem = (size_t)p.K * ((p.Dk + RL - 1) / RL) * SNT * 16 + (size_t)p.K * 4 * W * 4;
+  const size_t smem = (size_t)p.K * ((p.Dk + RL - 1) / RL) * SNT * 16 + (size_t)p.K * (4 * W + 2 * p.Dk + W + 4) * 4;
   static SmemAttrOnce attr;
-  GLA_TRY(attr.ensure(step_beams_kernel<W, KEYED>, 200 << 10));
+  GLA_TRY(attr.ensure(step_beams_kernel<W, KEYED>, 200 << 10));      // (32 beams of 256 features: 194 KB)
   ProfScope ps("step_beams_kernel", st);
   GLA_LAUNCHED(launch_overlapped(step_beams_kernel<W, KEYED>, dim3((unsigned)((p.Dv + W - 1) / W), (unsigned)groups), dim3(SNT), smem, st, p));
   return GLA_OK;
 }
-// Columns per block: the widest whose K beams fit 64 KB (three blocks per SM), narrower with more beams and features; below
-// 16 the rows of a block no longer fill 64 bytes.
+// Columns per block: as many as leave room for six blocks on an SM, so that one block's copies run beside another's steps
+// (16 requests of 4 beams, 16 heads of 128 x 64: 25.2 us with 32 columns and three blocks); below 16 the rows of a block no
+// longer fill 64 bytes.
 template <bool KEYED>
 static int step_beams(cudaStream_t st, const Step& p, int64_t groups) {
   const int64_t col = (int64_t)p.K * (p.Dk + 31) / 32 * 32 * 4;      // bytes of a column
-  if (col * 32 <= 64 << 10) return launch_beams<32, KEYED>(st, p, groups);
+  if (col * 32 <= 32 << 10) return launch_beams<32, KEYED>(st, p, groups);
   if (col * 16 <= 96 << 10) return launch_beams<16, KEYED>(st, p, groups);
   return launch_beams<4, KEYED>(st, p, groups);
 }
@@ -233,14 +260,15 @@ static int launch_reorder(cudaStream_t st, const Tensors& t) {
 // For each request the M best of its K V continuations by score[k] + log_softmax(logits[k])[v], the largest first, the
 // lowest (beam, token) first among equal ones.
 //
-// One pass over the logits: a block streams a part of a row, keeps the running maximum and sum of exponentials of the
-// softmax per thread, and the part's M largest logits.  Within a row the order of the totals is that of the logits, so that
-// nothing but M candidates per part and its (maximum, sum) leaves the pass; a second kernel forms the totals of the
-// candidates in 64 bits and orders them.
-// The candidates of a part: a threshold below which nothing can be among the M any more (M larger ones have been seen).
-// Values above it go to a list in shared memory, which is cut to its M largest when it has grown (each counts how many are
-// larger) and raises the threshold.  Where many threads have one, as in the first tile, the M-th largest of a warp's 32
-// largest raises it first, so that a tile never adds more than a few of each warp.
+// One pass over the logits: a block streams a part of a row, its threads keep the running maximum and sum of exponentials of
+// the softmax and their two largest logits.  Within a row the order of the totals is that of the logits, so that nothing but
+// M candidates per part and its (maximum, sum) leaves the pass; a second kernel forms the totals of the candidates in 64 bits
+// and orders them.
+// The M-th largest of the threads' largest is a bound: M logits reach it.  Threads whose second reaches it too may have
+// more, which is one in a part on average and is looked up again; where few threads hold most of the large logits (nothing
+// that a model leaves, but a sorted row may), the M largest are found one after the other.
+// Measured, 64 x 8 rows of 128000 bf16 logits, M = 16: lists in shared memory that are cut as they grow 136 us, a sorted list
+// per warp 312 us, this 37 us (the bytes at the copy rate: 17.5).
 // A key is (order of the value, lowest index first), 0: none.
 typedef unsigned long long u64;
 __device__ __forceinline__ unsigned int order_of(float x) {
@@ -249,8 +277,9 @@ __device__ __forceinline__ unsigned int order_of(float x) {
 }
 __device__ __forceinline__ float value_of(unsigned int o) { return __uint_as_float((o >> 31) ? o & 0x7fffffffu : ~o); }
 __device__ __forceinline__ u64 key_of(float x, unsigned int i) { return ((u64)order_of(x) << 32) | (unsigned int)~i; }
+constexpr float FMOST = 3.402823466e38f;
 // what a logit counts as: not-a-number as one that is masked, +inf as the largest finite number
-__device__ __forceinline__ float clean(float x) { return x != x ? -CUDART_INF_F : fminf(x, 3.402823466e38f); }
+__device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -CUDART_INF_F), FMOST); }
 
 __device__ __forceinline__ u64 warp_sorted(u64 x, int lane) {           // descending over the lanes
 #pragma unroll
@@ -265,7 +294,7 @@ __device__ __forceinline__ u64 warp_sorted(u64 x, int lane) {           // desce
 }
 
 constexpr int QNT = 256, QV = 16, TILE = QNT * QV;                      // threads, logits per thread and tile
-constexpr int QCAP = 32 * 8 * QV + 512;                                 // list: what a tile adds at most, and what may be left over
+constexpr int CAP = 1024;                                               // candidates of a part before the last cut
 struct Select {
   const void* logits;
   const float* scores;
@@ -281,33 +310,24 @@ struct Select {
   int* parents;
 };
 
-// the list's M largest, in order, to its front (0 behind them); cnt becomes their number, returns the M-th (0: fewer)
-__device__ __forceinline__ u64 cut_list(u64* list, u64* best, int* cnt, int M) {
-  __syncthreads();
-  const int n = *cnt;
-  for (int i = threadIdx.x; i < M; i += QNT) best[i] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += QNT) {
-    const u64 x = list[i];
-    int rank = 0;
-    for (int j = 0; j < n; ++j) rank += list[j] > x;
-    if (rank < M) best[rank] = x;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < M; i += QNT) list[i] = best[i];
-  if (threadIdx.x == 0) *cnt = n < M ? n : M;
-  __syncthreads();
-  return list[M - 1];
+// exp(x - m) with x <= m: the difference first, which is exact where it counts
+__device__ __forceinline__ float exp_of(float d) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(d * 1.4426950408889634f));
+  return y;
 }
 
 template <bool BF>
 __global__ void __launch_bounds__(QNT) select_parts_kernel(const Select p) {
-  __shared__ u64 list[QCAP], best[32], wtau[8];
+  __shared__ u64 list[CAP], tau_;
+  __shared__ int cnt, more, who[QNT];
+  __shared__ u64 below[QNT];
   __shared__ float wm[8];
   __shared__ double ws[8];
-  __shared__ int cnt;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   const int64_t row = blockIdx.y, V = p.V;
+  grid_dep_wait();
+  grid_dep_launch();
   u64* cand = p.cand + (row * p.parts + blockIdx.x) * p.M;
   const float score = p.scores[row];
   const bool dead = !(score > -CUDART_INF_F), done = p.finished && p.finished[row];
@@ -329,22 +349,35 @@ __global__ void __launch_bounds__(QNT) select_parts_kernel(const Select p) {
   // totals tie.  Rows that do not start on 16 bytes are put together from two aligned accesses.
   constexpr int E = BF ? 8 : 4, NV = QV / E, ES = BF ? 2 : 4;         // logits per 16 bytes, accesses per tile
   const char* base = (const char*)p.logits + row * V * ES;
+  const auto w_of = [](int i) { return i / E; };                      // the access that logit i of a thread's tile came by
   const int shift = (int)((uintptr_t)base & 15) / ES;
   const int64_t lo = blockIdx.x * p.part, hi = lo + p.part < V ? lo + p.part : V;
-  if (tid == 0) cnt = 0;
   float m = -CUDART_INF_F, s = 0.f;
-  u64 tau = 0;
-  __syncthreads();
+  float v1 = 0.f, v2 = 0.f;           // the two largest, and where (-1: none)
+  int i1 = -1, i2 = -1;
+  uint4 raw[2 * NV];                  // the next tile's 16 bytes, and the 16 behind them where a row starts anywhere
+  const auto whole = [&](int64_t e) { return shift ? e >= shift && e - shift + 2 * E <= V : e + E <= V; };
+  const auto request = [&](int64_t t0) {
+#pragma unroll
+    for (int w = 0; w < NV; ++w) {
+      const int64_t e = t0 + (int64_t)(w * QNT + tid) * E;
+      if (t0 < hi && whole(e)) {
+        raw[w] = __ldg((const uint4*)(base + (e - shift) * ES));
+        if (shift) raw[NV + w] = __ldg((const uint4*)(base + (e - shift + E) * ES));
+      }
+    }
+  };
+  request(lo);
   for (int64_t t0 = lo; t0 < hi; t0 += TILE) {
     float x[QV];
     unsigned int has = 0;
 #pragma unroll
     for (int w = 0; w < NV; ++w) {
       const int64_t e = t0 + (int64_t)(w * QNT + tid) * E;
-      if (shift ? e >= shift && e - shift + 2 * E <= V : e + E <= V) {
-        uint4 u = __ldg((const uint4*)(base + (e - shift) * ES));
+      if (whole(e)) {
+        uint4 u = raw[w];
         if (shift) {
-          const uint4 n = __ldg((const uint4*)(base + (e - shift + E) * ES));
+          const uint4 n = raw[NV + w];
           const unsigned int z[8] = {u.x, u.y, u.z, u.w, n.x, n.y, n.z, n.w};
           unsigned int y[4];
 #pragma unroll
@@ -353,7 +386,7 @@ __global__ void __launch_bounds__(QNT) select_parts_kernel(const Select p) {
             unsigned int a = z[i], b = z[i + 1];
 #pragma unroll
             for (int j = 1; j < 4; ++j)
-              if (shift * ES / 4 == j) { a = z[i + j]; b = i + j + 1 < 8 ? z[i + j + 1 < 8 ? i + j + 1 : 7] : 0; }
+              if (shift * ES / 4 == j) { a = z[i + j]; b = z[i + j + 1 < 8 ? i + j + 1 : 7]; }
             y[i] = __funnelshift_r(a, b, shift * ES % 4 * 8);
           }
           u = make_uint4(y[0], y[1], y[2], y[3]);
@@ -369,60 +402,114 @@ __global__ void __launch_bounds__(QNT) select_parts_kernel(const Select p) {
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           x[w * E + i] = -CUDART_INF_F;
-          if (e + i < V) {
+          if (e + i < hi) {
             x[w * E + i] = BF ? __bfloat162float(((const bf16*)base)[e + i]) : ((const float*)base)[e + i];
             has |= 1u << (w * E + i);
           }
         }
       }
     }
+    request(t0 + TILE);
     float top = -CUDART_INF_F;
 #pragma unroll
-    for (int i = 0; i < QV; ++i) { x[i] = clean(x[i]); top = fmaxf(top, x[i]); }
-    if (top > m) { s *= exp2f((m - top) * 1.4426950408889634f); m = top; }
+    for (int i = 0; i < QV; ++i) top = fmaxf(top, x[i]);      // (passes over what is not a number)
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < QV; ++i) odd = odd || x[i] != x[i];
+    if (odd || top > FMOST) {
+      top = clean(top);
+#pragma unroll
+      for (int i = 0; i < QV; ++i) x[i] = clean(x[i]);
+    }
+    if (top > m) { s *= exp_of(m - top); m = top; }
     if (m > -CUDART_INF_F) {
 #pragma unroll
-      for (int i = 0; i < QV; ++i) s += expf(x[i] - m);
+      for (int i = 0; i < QV; ++i) s += exp_of(x[i] - m);
     }
-    // the thread's largest key
-    u64 first = 0;
-    if (order_of(top) >= (unsigned int)(tau >> 32)) {
-#pragma unroll
-      for (int i = QV - 1; i >= 0; --i) {
-        const int64_t e = t0 + (int64_t)(i / E * QNT + tid) * E + i % E;
-        if (((has >> i) & 1u) && x[i] == top) first = key_of(x[i], (unsigned int)e);
-      }
-    }
-    const int many = __syncthreads_count(first > tau);
-    if (many > 64) {
-      const u64 o = warp_sorted(first, lane);
-      const u64 mth = __shfl_sync(0xffffffffu, o, p.M - 1);
-      if (lane == 0) wtau[warp] = mth;
-      __syncthreads();
-      u64 y = tau;
-#pragma unroll
-      for (int w = 0; w < 8; ++w) y = wtau[w] > y ? wtau[w] : y;
-      tau = y > 0 ? y - 1 : 0;                                // (the M-th itself stays in)
-    }
-    if (first > tau) {
+    if (has && (i2 < 0 || top > v2)) {
 #pragma unroll
       for (int i = 0; i < QV; ++i) {
-        const int64_t e = t0 + (int64_t)(i / E * QNT + tid) * E + i % E;
-        const u64 y = ((has >> i) & 1u) ? key_of(x[i], (unsigned int)e) : 0;
-        if (y > tau) list[atomicAdd(&cnt, 1)] = y;
+        const int e = (int)(t0 + (w_of(i) * QNT + tid) * E + i % E);
+        if ((has >> i) & 1u) {
+          if (i1 < 0 || x[i] > v1) { v2 = v1; i2 = i1; v1 = x[i]; i1 = e; }
+          else if (i2 < 0 || x[i] > v2) { v2 = x[i]; i2 = e; }
+        }
       }
     }
-    if (many) {
-      __syncthreads();
-      if (cnt > 256 || many > 64) {
-        const u64 y = cut_list(list, best, &cnt, p.M);
-        tau = y > tau ? y : tau;
-      }
-    }
-    __syncthreads();
   }
-  cut_list(list, best, &cnt, p.M);
-  if (tid < p.M) cand[tid] = list[tid];
+  // the bound: sorted by warp, a key's place among all is its place in its warp and what is larger in the others
+  const u64 first = i1 < 0 ? 0 : key_of(v1, (unsigned int)i1), second = i2 < 0 ? 0 : key_of(v2, (unsigned int)i2);
+  const u64 own = warp_sorted(first, lane);
+  below[tid] = own;
+  if (tid == 0) { tau_ = 1; cnt = 0; more = 0; }
+  __syncthreads();
+  {
+    int place = lane;
+    for (int w = 0; w < 8; ++w) {
+      if (w == warp) continue;
+      const u64* l = below + 32 * w;
+      int n = 0;                       // of the 32, in descending order, those above
+#pragma unroll
+      for (int d = 16; d; d >>= 1)
+        if (l[n + d - 1] > own) n += d;
+      place += n + (n == 31 && l[31] > own);
+    }
+    if (own && place == p.M - 1) tau_ = own;
+  }
+  __syncthreads();
+  const u64 tau = tau_;
+  // (the table is read by now)
+  if (first >= tau) list[atomicAdd(&cnt, 1)] = first;
+  if (second >= tau) {
+    list[atomicAdd(&cnt, 1)] = second;
+    const int i = atomicAdd(&more, 1);
+    who[i] = tid;
+    below[i] = second;
+  }
+  __syncthreads();
+  const auto logit = [&](int64_t e) { return clean(BF ? __bfloat162float(((const bf16*)base)[e]) : ((const float*)base)[e]); };
+  const int tiles = hi > lo ? (int)((hi - lo + TILE - 1) / TILE) : 0;
+  for (int k = 0; k < more; ++k) {
+    // the logits that thread who[k] met, below its second
+    for (int j = tid; j < tiles * QV; j += QNT) {
+      const int64_t e = lo + (int64_t)(j / QV) * TILE + (w_of(j % QV) * QNT + who[k]) * E + j % QV % E;
+      if (e < V) {
+        const u64 y = key_of(logit(e), (unsigned int)e);
+        if (y >= tau && y < below[k]) {
+          const int at = atomicAdd(&cnt, 1);
+          if (at < CAP) list[at] = y;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int n = cnt;
+  if (n <= CAP) {
+    for (int i = tid; i < n; i += QNT) {
+      const u64 y = list[i];
+      int rank = 0;
+      for (int j = 0; j < n; ++j) rank += list[j] > y;
+      if (rank < p.M) cand[rank] = y;
+    }
+    if (tid >= n && tid < p.M) cand[tid] = 0;
+  } else {
+    u64 prev = ~0ull;
+    for (int k = 0; k < p.M; ++k) {
+      u64 y = 0;
+      for (int64_t e = lo + tid; e < hi; e += QNT) {
+        const u64 z = key_of(logit(e), (unsigned int)e);
+        if (z < prev && z > y) y = z;
+      }
+      y = warp_sorted(y, lane);
+      if (lane == 0) below[warp] = y;
+      __syncthreads();
+      y = below[0];
+      for (int w = 1; w < 8; ++w) y = below[w] > y ? below[w] : y;
+      prev = y;
+      if (tid == 0) cand[k] = y;
+      __syncthreads();
+    }
+  }
   // (maximum, sum) of the part
   float top = m;
 #pragma unroll
@@ -431,7 +518,7 @@ __global__ void __launch_bounds__(QNT) select_parts_kernel(const Select p) {
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 8; ++w) top = fmaxf(top, wm[w]);
-  double sum = m > -CUDART_INF_F ? (double)s * expf(m - top) : 0.0;
+  double sum = m > -CUDART_INF_F ? (double)s * exp_of(m - top) : 0.0;
 #pragma unroll
   for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   if (lane == 0) ws[warp] = sum;
@@ -448,49 +535,55 @@ __device__ __forceinline__ u64 order_of(double x) {
   const long long u = __double_as_longlong(x + 0.0);
   return u < 0 ? ~(u64)u : (u64)u | 0x8000000000000000ull;
 }
-constexpr int SCAP = 1024;              // candidates of a request: K parts M, at most
-__global__ void __launch_bounds__(QNT) select_beams_kernel(const Select p) {
-  __shared__ u64 key[SCAP];
-  __shared__ u64 where[SCAP];           // (beam, token)
-  __shared__ double base[64][2];        // per beam: maximum, log of the sum
-  __shared__ double tot[SCAP];
+constexpr int SCAP = 1024, BNT = 512;   // candidates of a request: K parts M, at most; threads
+__global__ void __launch_bounds__(BNT) select_beams_kernel(const Select p) {
+  __shared__ u64 key[SCAP], where[SCAP];  // total's order; (beam, token)
+  __shared__ double base[32][2];          // per beam: maximum, log of the sum
   const int tid = threadIdx.x, K = p.K, M = p.M, per = p.parts * M, n = K * per;
   const int64_t req = blockIdx.x;
-  for (int k = tid; k < K; k += QNT) {
+  grid_dep_wait();
+  for (int k = tid / 32; k < K; k += BNT / 32) {
     const double2* sm = p.sums + (req * K + k) * p.parts;
     double top = -CUDART_INF, s = 0.0;
-    for (int i = 0; i < p.parts; ++i) top = fmax(top, sm[i].x);
-    for (int i = 0; i < p.parts; ++i)
+    for (int i = tid % 32; i < p.parts; i += 32) top = fmax(top, sm[i].x);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, d));
+    for (int i = tid % 32; i < p.parts; i += 32)
       if (sm[i].x > -CUDART_INF) s += sm[i].y * exp(sm[i].x - top);
-    base[k][0] = top;
-    base[k][1] = log(s);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if (tid % 32 == 0) { base[k][0] = top; base[k][1] = log(s); }
   }
   __syncthreads();
   const u64* cand = p.cand + req * n;
-  for (int i = tid; i < n; i += QNT) {
+  for (int i = tid; i < n; i += BNT) {
     const u64 c = cand[i];
     const int k = i / per;
-    double t = -CUDART_INF;
     u64 o = 0;
     if (c) {
+      double t = -CUDART_INF;
       const float x = value_of((unsigned int)(c >> 32));
       if (x > -CUDART_INF_F && base[k][0] > -CUDART_INF) t = (double)p.scores[req * K + k] + (((double)x - base[k][0]) - base[k][1]);
       if (!(t > -CUDART_INF)) t = -CUDART_INF;
       o = order_of(t);
     }
     key[i] = o;
-    tot[i] = t;
     where[i] = ((u64)k << 32) | (unsigned int)~(unsigned int)c;
   }
   __syncthreads();
-  for (int i = tid; i < n; i += QNT) {
-    const u64 x = key[i];
-    if (!x) continue;
-    const u64 at = where[i];
+  // a candidate's place is the number of larger ones, counted by eight lanes
+  const int part = tid % 8;
+  for (int i0 = 0; i0 < n; i0 += BNT / 8) {
+    const int i = i0 + tid / 8;
+    const u64 x = i < n ? key[i] : 0, at = i < n ? where[i] : 0;
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += key[j] > x || (key[j] == x && where[j] < at);
-    if (rank < M) {
-      p.out_scores[req * M + rank] = (float)tot[i];
+    if (x)
+      for (int j = part; j < n; j += 8) rank += key[j] > x || (key[j] == x && where[j] < at);
+#pragma unroll
+    for (int d = 1; d < 8; d <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, d);
+    if (x && part == 0 && rank < M) {
+      const long long u = (x >> 63) ? (long long)(x & 0x7fffffffffffffffull) : (long long)~x;
+      p.out_scores[req * M + rank] = (float)__longlong_as_double(u);
       p.tokens[req * M + rank] = (long long)(at & 0xffffffffu);
       p.parents[req * M + rank] = (int)(at >> 32);
     }
@@ -630,13 +723,10 @@ int gla_beam_select(void* stream, int64_t N, int64_t K, int64_t V, int64_t M, in
   {
     ProfScope ps("select_parts_kernel", st);
     const dim3 grid((unsigned)p.parts, (unsigned)(N * K));
-    if (p.bf) beam::select_parts_kernel<true><<<grid, beam::QNT, 0, st>>>(p);
-    else beam::select_parts_kernel<false><<<grid, beam::QNT, 0, st>>>(p);
-    GLA_CHECK_LAUNCH();
+    GLA_LAUNCHED(launch_overlapped(p.bf ? beam::select_parts_kernel<true> : beam::select_parts_kernel<false>, grid, dim3(beam::QNT), 0, st, p));
   }
   ProfScope ps("select_beams_kernel", st);
-  beam::select_beams_kernel<<<(unsigned)N, beam::QNT, 0, st>>>(p);
-  GLA_CHECK_LAUNCH();
+  GLA_LAUNCHED(launch_overlapped(beam::select_beams_kernel, dim3((unsigned)N), dim3(beam::BNT), 0, st, p));
   return GLA_OK;
 }
 

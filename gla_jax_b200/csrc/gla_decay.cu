@@ -11,6 +11,8 @@ namespace {
 __global__ void __launch_bounds__(128) entering_kernel(const Walk p) {
   const int64_t s = blockIdx.z, h = blockIdx.y, dd = (int64_t)p.kd * p.vd;
   const int e = (blockIdx.x * 128 + threadIdx.x) * 4;
+  grid_dep_wait();
+  grid_dep_launch();
   if (e >= dd) return;
   const int c = e / p.kd, k = e % p.kd;
   int64_t n = 1;
@@ -154,30 +156,43 @@ struct Dims {
   }
 };
 
-static int walk(cudaStream_t st, int mode, const Walk& p, bool out, const char* name) {
+static int walk(cudaStream_t st, int mode, const Walks& p, int n, bool out, const char* name) {
   switch (mode) {
-    case M_ONE: return walk_one(st, p, out, name);
-    case M_STATE: return walk_state(st, p, out, name);
-    case M_FINE: return walk_fine(st, p, out, name);
-    default: return walk_full(st, p, out, name);
+    case M_ONE: return walk_one(st, p, n, out, name);
+    case M_STATE: return walk_state(st, p, n, out, name);
+    case M_FINE: return walk_fine(st, p, n, out, name);
+    default: return walk_full(st, p, n, out, name);
   }
 }
-// A whole walk: the runs' sums and their entering states first where sequences are cut.
-static int run_walk(cudaStream_t st, const Dims& d, int mode, Walk p, void* ws, const char* first, const char* name) {
-  p.H = (int)d.H; p.T = d.T; p.nseq = d.seqs();
-  p.seg = d.seg(p.vd);
-  p.nslots = d.slots(p.seg);
-  if (p.nslots > 2147483647LL || d.H * ((p.vd + 63) / 64) > 65535 || p.nseq > 65535 * 32767LL) return GLA_ERR_TOO_LARGE;
-  if (d.cut(p.seg)) {
-    if (p.nseq > 65535) return GLA_ERR_TOO_LARGE;
-    p.seg_state = (float*)ws;
-    p.seg_total = (double*)((char*)ws + align_up((size_t)(p.nslots * d.H * d.Dk * d.Dv) * 4, 256));
-    GLA_TRY(walk(st, mode, p, false, first));
-    ProfScope ps("decay_entering_kernel", st);
-    entering_kernel<<<dim3((unsigned)((d.Dk * d.Dv + 511) / 512), (unsigned)d.H, (unsigned)p.nseq), 128, 0, st>>>(p);
-    GLA_CHECK_LAUNCH();
+static int entering(cudaStream_t st, const Walk& p) {
+  ProfScope ps("decay_entering_kernel", st);
+  GLA_LAUNCHED(launch_overlapped(entering_kernel, dim3((unsigned)(((int64_t)p.kd * p.vd + 511) / 512), (unsigned)p.H, (unsigned)p.nseq), dim3(128), 0, st, p));
+  return GLA_OK;
+}
+// Whole walks of one kind of sizes: the runs' sums and their entering states first where sequences are cut (ws: seg_bytes for
+// each).
+static int run_walks(cudaStream_t st, const Dims& d, int mode, Walks p, int n, void* ws, const char* first, const char* name) {
+  for (int i = 0; i < n; ++i) {
+    Walk& w = p.w[i];
+    w.H = (int)d.H; w.T = d.T; w.nseq = d.seqs();
+    w.seg = d.seg(w.vd);
+    w.nslots = d.slots(w.seg);
+    if (w.nslots > 2147483647LL) return GLA_ERR_TOO_LARGE;
+    if (d.cut(w.seg)) {
+      w.seg_state = (float*)((char*)ws + i * d.seg_bytes(w.vd));
+      w.seg_total = (double*)((char*)w.seg_state + align_up((size_t)(w.nslots * d.H * d.Dk * d.Dv) * 4, 256));
+    }
   }
-  return walk(st, mode, p, true, name);
+  if (d.cut(p.w[0].seg)) {
+    GLA_TRY(walk(st, mode, p, n, false, first));
+    for (int i = 0; i < n; ++i) GLA_TRY(entering(st, p.w[i]));
+  }
+  return walk(st, mode, p, n, true, name);
+}
+static int run_walk(cudaStream_t st, const Dims& d, int mode, const Walk& p, void* ws, const char* first, const char* name) {
+  Walks all{};
+  all.w[0] = p;
+  return run_walks(st, d, mode, all, 1, ws, first, name);
 }
 
 // ---- bf16, head sizes up to 128: the walks of gla_decay_tc.cuh and gla_decay_tcb.cuh ---------------------------------------------------------
@@ -194,12 +209,6 @@ static Walk fast_base(const Dims& d, const int* cu, const float* g, int64_t gt) 
   p.g = g; p.gt = gt; p.cu = cu;
   p.init_f32 = p.fin_f32 = d.hid_f32;
   return p;
-}
-static int entering(cudaStream_t st, const Walk& p) {
-  ProfScope ps("decay_entering_kernel", st);
-  entering_kernel<<<dim3((unsigned)(((int64_t)p.kd * p.vd + 511) / 512), (unsigned)p.H, (unsigned)p.nseq), 128, 0, st>>>(p);
-  GLA_CHECK_LAUNCH();
-  return GLA_OK;
 }
 static int fast_fwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const float* g, int64_t gt, const void* v, const void* k,
                     const void* q, void* hf, void* out, void* saved, void* ws) {
@@ -287,9 +296,14 @@ int fwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const flo
   return run_walk(st, d, !d.bf ? M_FULL : d.hid_f32 ? M_STATE : M_ONE, p, ws, "decay_runs_kernel", "decay_walk_kernel");
 }
 
+// whether the three walks of a backward run the same kernel on the same runs, and few blocks each: then they run side by side
+static bool alike(const Dims& d) {
+  const auto kind = [](int64_t x) { return x <= 64 ? 0 : x <= 128 ? 1 : 2; };
+  return d.H == d.Hk && kind(d.Dk) == kind(d.Dv) && column_tiles((int)d.Dk) == column_tiles((int)d.Dv) && d.seg(d.Dk) == d.seg(d.Dv);
+}
 static size_t bwd_parts(const Dims& d, bool gate, size_t (&at)[5]) {
   const int64_t share = d.H / d.Hk, tiles = (d.Dk + 127) / 128;
-  const size_t seg = d.seg_bytes(d.Dv) > d.seg_bytes(d.Dk) ? d.seg_bytes(d.Dv) : d.seg_bytes(d.Dk);
+  const size_t seg = alike(d) ? 3 * d.seg_bytes(d.Dv) : d.seg_bytes(d.Dv) > d.seg_bytes(d.Dk) ? d.seg_bytes(d.Dv) : d.seg_bytes(d.Dk);
   const size_t dots = gate ? align_up((size_t)(tiles * d.rows() * d.H) * 4, 256) : 0;
   at[0] = seg;
   at[1] = at[0] + dots;
@@ -317,29 +331,36 @@ int bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const flo
   bwd_parts(d, dg != nullptr, at);
   float *rq = (float*)((char*)ws + at[0]), *rk = (float*)((char*)ws + at[1]), *wide = (float*)((char*)ws + at[2]);
   const int share = (int)(d.H / d.Hk), mode = d.bf ? M_FINE : M_FULL;
-  Walk p{};
+  Walks all{};
+  Walk &p = all.w[0], &r = all.w[1], &t = all.w[2];
   p.g = g; p.gt = gt; p.cu = cu;
   p.init_f32 = p.fin_f32 = d.hid_f32;
+  r = t = p;
   // dq, forwards over the states of the forward, transposed
   p.q = dout; p.k = v; p.v = k; p.gq = p.gk = 1; p.gv = share; p.kd = (int)d.Dv; p.vd = (int)d.Dk;
   p.init = h0; p.ik = 1; p.ic = d.Dv;
   p.out = share > 1 ? (void*)wide : dq; p.out_f32 = share > 1 || !d.bf;
   p.r = dg ? q : nullptr; p.gr = share; p.rdot = rq;
-  GLA_TRY(run_walk(st, d, mode, p, ws, "decay_runs_kernel", "decay_dq_kernel"));
-  if (share > 1) GLA_TRY(share_sum(st, d, wide, dq));
   // dk, backwards
-  p.rev = 1;
-  p.q = v; p.k = dout; p.v = q;
-  p.init = dhf;
-  p.out = share > 1 ? (void*)wide : dk;
-  p.r = dg ? k : nullptr; p.rdot = rk;
-  GLA_TRY(run_walk(st, d, mode, p, ws, "decay_runs_kernel", "decay_dk_kernel"));
-  if (share > 1) GLA_TRY(share_sum(st, d, wide, dk));
+  r.rev = 1;
+  r.q = v; r.k = dout; r.v = q; r.gq = r.gk = 1; r.gv = share; r.kd = (int)d.Dv; r.vd = (int)d.Dk;
+  r.init = dhf; r.ik = 1; r.ic = d.Dv;
+  r.out = share > 1 ? (void*)wide : dk; r.out_f32 = share > 1 || !d.bf;
+  r.r = dg ? k : nullptr; r.gr = share; r.rdot = rk;
   // dv and the gradient of the first state, backwards
-  p.q = k; p.k = q; p.v = dout; p.gq = p.gk = share; p.gv = 1; p.kd = (int)d.Dk; p.vd = (int)d.Dv;
-  p.ik = d.Dv; p.ic = 1; p.fin = dh;
-  p.out = dv; p.out_f32 = !d.bf; p.r = nullptr; p.rdot = nullptr;
-  GLA_TRY(run_walk(st, d, mode, p, ws, "decay_runs_kernel", "decay_dv_kernel"));
+  t.rev = 1;
+  t.q = k; t.k = q; t.v = dout; t.gq = t.gk = share; t.gv = 1; t.kd = (int)d.Dk; t.vd = (int)d.Dv;
+  t.init = dhf; t.ik = d.Dv; t.ic = 1; t.fin = dh;
+  t.out = dv; t.out_f32 = !d.bf;
+  if (alike(d)) {
+    GLA_TRY(run_walks(st, d, mode, all, 3, ws, "decay_runs_kernel", "decay_grads_kernel"));
+  } else {
+    GLA_TRY(run_walk(st, d, mode, p, ws, "decay_runs_kernel", "decay_dq_kernel"));
+    if (share > 1) GLA_TRY(share_sum(st, d, wide, dq));
+    GLA_TRY(run_walk(st, d, mode, r, ws, "decay_runs_kernel", "decay_dk_kernel"));
+    if (share > 1) GLA_TRY(share_sum(st, d, wide, dk));
+    GLA_TRY(run_walk(st, d, mode, t, ws, "decay_runs_kernel", "decay_dv_kernel"));
+  }
   if (dg) {
     Gate w{};
     w.rq = rq; w.rk = rk; w.nq = w.nk = (int)((d.Dk + 127) / 128);

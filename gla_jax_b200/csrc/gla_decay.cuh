@@ -218,8 +218,11 @@ static inline unsigned int read_bad_offsets() {
   return v;
 }
 
+// Up to three walks side by side (blockIdx.z): those of a backward do not wait for one another.
+struct Walks { Walk w[3]; };
 template <int MODE, int KD, int NW, bool OUT>
-__global__ void __launch_bounds__(NW * 32, KD <= 128 && MODE <= M_STATE ? 16 / NW : 1) walk_kernel(const Walk p) {
+__global__ void __launch_bounds__(NW * 32, KD <= 128 && MODE <= M_STATE ? 16 / NW : 1) walk_kernel(const __grid_constant__ Walks all) {
+  const Walk& p = all.w[blockIdx.z];
   using M = Mode<MODE>;
   using Y = Lay<MODE, KD, NW, OUT>;
   constexpr int L = Y::L, NT = Y::NT, KT = KD / 8;
@@ -516,35 +519,42 @@ __global__ void __launch_bounds__(NW * 32, KD <= 128 && MODE <= M_STATE ? 16 / N
   }
 }
 
-// One launch for the modes of a file: see gla_decay_*.cu.
 template <int MODE, int KD, int NW, bool OUT>
-int launch_walk(cudaStream_t stream, const Walk& p, const char* name) {
+int launch_walk(cudaStream_t stream, const Walks& p, int n, const char* name) {
   using Y = Lay<MODE, KD, NW, OUT>;
   static SmemAttrOnce attr;
   GLA_TRY(attr.ensure(walk_kernel<MODE, KD, NW, OUT>, Y::END));
   ProfScope ps(name, stream);
-  walk_kernel<MODE, KD, NW, OUT><<<dim3((unsigned)p.nslots, (unsigned)(p.H * p.vt)), Y::NT, Y::END, stream>>>(p);
+  walk_kernel<MODE, KD, NW, OUT><<<dim3((unsigned)p.w[0].nslots, (unsigned)(p.w[0].H * p.w[0].vt), (unsigned)n), Y::NT, Y::END, stream>>>(p);
   GLA_CHECK_LAUNCH();
   return GLA_OK;
 }
 template <int MODE, int NW, bool OUT>
-int walk_kd(cudaStream_t stream, const Walk& p, const char* name) {
-  if (p.kd <= 64) return launch_walk<MODE, 64, NW, OUT>(stream, p, name);
-  if (p.kd <= 128) return launch_walk<MODE, 128, NW, OUT>(stream, p, name);
-  return launch_walk<MODE, 256, NW, OUT>(stream, p, name);
+int walk_kd(cudaStream_t stream, const Walks& p, int n, const char* name) {
+  const int kd = p.w[0].kd;
+  if (kd <= 64) return launch_walk<MODE, 64, NW, OUT>(stream, p, n, name);
+  if (kd <= 128) return launch_walk<MODE, 128, NW, OUT>(stream, p, n, name);
+  return launch_walk<MODE, 256, NW, OUT>(stream, p, n, name);
 }
-// blocks of 64 columns where there are no more, of 128 otherwise
+// Blocks of 64 columns where there are no more, of 128 otherwise.  (bf16 heads of up to 128 have walks of their own, so that in the
+// bf16 modes columns or features go beyond that.)
+static inline int column_tiles(int vd) { return vd <= 64 ? 1 : (vd + 127) / 128; }
+template <int MODE, bool OUT>
+int walk_nw(cudaStream_t stream, const Walks& p, int n, const char* name) {
+  if (p.w[0].vd > 64) return walk_kd<MODE, 8, OUT>(stream, p, n, name);
+  if constexpr (MODE == M_FULL) return walk_kd<MODE, 4, OUT>(stream, p, n, name);
+  else return launch_walk<MODE, 256, 4, OUT>(stream, p, n, name);
+}
+// n walks of one kind: the same sizes, runs and column tiles
 template <int MODE>
-int walk_mode(cudaStream_t stream, Walk p, bool out, const char* name) {
-  const bool narrow = p.vd <= 64;
-  p.vt = narrow ? 1 : (p.vd + 127) / 128;
-  if (out) return narrow ? walk_kd<MODE, 4, true>(stream, p, name) : walk_kd<MODE, 8, true>(stream, p, name);
-  return narrow ? walk_kd<MODE, 4, false>(stream, p, name) : walk_kd<MODE, 8, false>(stream, p, name);
+int walk_mode(cudaStream_t stream, Walks p, int n, bool out, const char* name) {
+  for (int i = 0; i < n; ++i) p.w[i].vt = column_tiles(p.w[i].vd);
+  return out ? walk_nw<MODE, true>(stream, p, n, name) : walk_nw<MODE, false>(stream, p, n, name);
 }
-int walk_one(cudaStream_t, const Walk&, bool out, const char* name);
-int walk_state(cudaStream_t, const Walk&, bool out, const char* name);
-int walk_fine(cudaStream_t, const Walk&, bool out, const char* name);
-int walk_full(cudaStream_t, const Walk&, bool out, const char* name);
+int walk_one(cudaStream_t, const Walks&, int n, bool out, const char* name);
+int walk_state(cudaStream_t, const Walks&, int n, bool out, const char* name);
+int walk_fine(cudaStream_t, const Walks&, int n, bool out, const char* name);
+int walk_full(cudaStream_t, const Walks&, int n, bool out, const char* name);
 unsigned int bad_offsets_one();
 unsigned int bad_offsets_state();
 unsigned int bad_offsets_fine();

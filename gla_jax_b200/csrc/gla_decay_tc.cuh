@@ -300,6 +300,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
   Gates* gates = reinterpret_cast<Gates*>(sm + Y::G0);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int h = blockIdx.y;
+  grid_dep_wait();
+  grid_dep_launch();
   const Run run = find_run(p, blockIdx.x);
   if constexpr (OUT) {
     if (run.zlo < run.zhi)
@@ -704,8 +706,7 @@ int launch_tc(cudaStream_t stream, const Walk& p, const char* name) {
   if (OUT) GLA_TRY(make_map_tokens(&a.q, p.q, rows, p.H / p.gq, p.kd));
   else a.q = a.k;
   ProfScope ps(name, stream);
-  tc_walk_kernel<DK, DV, NU, NS, OUT><<<dim3((unsigned)p.nslots, (unsigned)p.H), TC_THREADS, Y::END, stream>>>(a);
-  GLA_CHECK_LAUNCH();
+  GLA_LAUNCHED(launch_overlapped(tc_walk_kernel<DK, DV, NU, NS, OUT>, dim3((unsigned)p.nslots, (unsigned)p.H), dim3(TC_THREADS), Y::END, stream, a));
   return GLA_OK;
 }
 

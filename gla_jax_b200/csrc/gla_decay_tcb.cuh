@@ -134,6 +134,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
   double* red = reinterpret_cast<double*>(sm + Y::RED);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int h = blockIdx.y;
+  grid_dep_wait();
+  grid_dep_launch();
   const Run run = find_run(p, blockIdx.x);
   if (run.zlo < run.zhi) {
     for (int64_t i = tid; i < (run.zhi - run.zlo) * p.kd; i += TC_THREADS) st_any(a.dk, !a.dk_f32, ((run.zlo + i / p.kd) * p.H + h) * p.kd + i % p.kd, 0.f);
@@ -532,8 +534,7 @@ int launch_tc_back(cudaStream_t stream, TcBack& b, const void* dout) {
   GLA_TRY(make_map_tokens(&b.v, p.v, rows, p.H, p.vd));
   GLA_TRY(make_map_tokens(&b.o, dout, rows, p.H, p.vd));
   ProfScope ps("decay_back_kernel", stream);
-  tc_back_kernel<DK, DV, GATE><<<dim3((unsigned)p.nslots, (unsigned)p.H), TC_THREADS, Y::END, stream>>>(b);
-  GLA_CHECK_LAUNCH();
+  GLA_LAUNCHED(launch_overlapped(tc_back_kernel<DK, DV, GATE>, dim3((unsigned)p.nslots, (unsigned)p.H), dim3(TC_THREADS), Y::END, stream, b));
   return GLA_OK;
 }
 
