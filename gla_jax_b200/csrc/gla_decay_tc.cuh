@@ -50,6 +50,49 @@ __device__ __forceinline__ void sts16(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+// `cols` (a multiple of 8, at most N) elements side by side, from or to an address that may be anything its type allows
+template <int N>
+__device__ __forceinline__ void load_side(float (&S)[N], const void* p, int f32, int cols) {
+  const bool vec = ((uintptr_t)p & 15) == 0;
+#pragma unroll
+  for (int j = 0; j < N; j += 8) {
+    float* s = S + j;
+    if (j >= cols) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = 0.f;
+    } else if (!vec) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] = ld_any(p, !f32, j + e);
+    } else if (f32) {
+      const float4 a = *reinterpret_cast<const float4*>((const float*)p + j), b = *reinterpret_cast<const float4*>((const float*)p + j + 4);
+      s[0] = a.x; s[1] = a.y; s[2] = a.z; s[3] = a.w; s[4] = b.x; s[5] = b.y; s[6] = b.z; s[7] = b.w;
+    } else {
+      const uint4 a = *reinterpret_cast<const uint4*>((const bf16*)p + j);
+      const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) { const float2 y = pair_of(u[e]); s[2 * e] = y.x; s[2 * e + 1] = y.y; }
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void store_side(const float (&S)[N], void* p, int f32, int cols) {
+  const bool vec = ((uintptr_t)p & 15) == 0;
+#pragma unroll
+  for (int j = 0; j < N; j += 8) {
+    const float* s = S + j;
+    if (j >= cols) continue;
+    if (!vec) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) st_any(p, !f32, j + e, s[e]);
+    } else if (f32) {
+      *reinterpret_cast<float4*>((float*)p + j) = make_float4(s[0], s[1], s[2], s[3]);
+      *reinterpret_cast<float4*>((float*)p + j + 4) = make_float4(s[4], s[5], s[6], s[7]);
+    } else {
+      *reinterpret_cast<uint4*>((bf16*)p + j) = make_uint4(pack_bf16x2(s[0], s[1]), pack_bf16x2(s[2], s[3]), pack_bf16x2(s[4], s[5]), pack_bf16x2(s[6], s[7]));
+    }
+  }
+}
+
 static __device__ unsigned int g_wait_timeouts = 0;
 static inline unsigned int read_wait_timeouts() {
   unsigned int v = 0;
@@ -450,22 +493,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
     if (!OUT) {
 #pragma unroll
       for (int j = 0; j < HV; ++j) S[j] = 0.f;
-    } else if (p.seg_state && p.sc == 1) {
-    const float* x = p.seg_state + slot_h * dd + row * p.sk + HV * qt;
-#pragma unroll
-    for (int j = 0; j < HV; j += 4) {
-      const float4 y = j < cols ? *reinterpret_cast<const float4*>(x + j) : make_float4(0.f, 0.f, 0.f, 0.f);
-      S[j] = y.x; S[j + 1] = y.y; S[j + 2] = y.z; S[j + 3] = y.w;
-    }
-  } else if (p.seg_state || p.init_f32) {
-      const float* x = p.seg_state ? p.seg_state + slot_h * dd + row * p.sk + HV * qt * p.sc : (const float*)p.init + sh * dd + row * p.ik + HV * qt * p.ic;
-      const int64_t d = p.seg_state ? p.sc : p.ic;
-#pragma unroll
-      for (int j = 0; j < HV; ++j, x += d) S[j] = j < cols ? *x : 0.f;
     } else {
-      const bf16* x = (const bf16*)p.init + sh * dd + row * p.ik + HV * qt * p.ic;
+      const int64_t sk = p.seg_state ? p.sk : p.ik, sc = p.seg_state ? p.sc : p.ic, at = (p.seg_state ? slot_h : sh) * dd + row * sk + HV * qt * sc;
+      const int f32 = p.seg_state != nullptr || p.init_f32;
+      const char* x = (const char*)(p.seg_state ? (const void*)p.seg_state : p.init) + at * (f32 ? 4 : 2);
+      if (sc == 1) {
+        load_side<HV>(S, x, f32, cols);
+      } else {
 #pragma unroll
-      for (int j = 0; j < HV; ++j, x += p.ic) S[j] = j < cols ? __bfloat162float(*x) : 0.f;
+        for (int j = 0; j < HV; ++j) S[j] = j < cols ? ld_any(x, !f32, j * sc) : 0.f;
+      }
     }
     // its image for Q S: [feature][column], 64 columns a tile
     const auto put_state = [&]() {
@@ -661,24 +698,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
     }
     if constexpr (OUT) {
       if (run.last) {
-        const int64_t at = sh * dd + row * p.ik + HV * qt * p.ic;
-        float* f = p.fin_f32 ? (float*)p.fin + at : p.fin32 + at;
-        if (p.fin_f32 ? p.fin != nullptr : p.fin32 != nullptr)
-#pragma unroll
-          for (int j = 0; j < HV; ++j, f += p.ic)
-            if (j < cols) *f = S[j];
-        if (p.fin_f32 && p.fin32) {
-          f = p.fin32 + at;
-#pragma unroll
-          for (int j = 0; j < HV; ++j, f += p.ic)
-            if (j < cols) *f = S[j];
-        }
-        if (!p.fin_f32 && p.fin) {
-          bf16* o = (bf16*)p.fin + at;
-#pragma unroll
-          for (int j = 0; j < HV; ++j, o += p.ic)
-            if (j < cols) *o = __float2bfloat16_rn(S[j]);
-        }
+        // (only the forward's own walk leaves its state: columns side by side)
+        const int64_t at = sh * dd + row * p.ik + HV * qt;
+        if (p.fin) store_side<HV>(S, p.fin_f32 ? (void*)((float*)p.fin + at) : (void*)((bf16*)p.fin + at), p.fin_f32, cols);
+        if (p.fin32) store_side<HV>(S, p.fin32 + at, 1, cols);
       }
     } else {
       float* f = p.seg_state + slot_h * dd + (int64_t)HV * qt * p.kd + row;

@@ -167,17 +167,26 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
   const int cols = row < p.kd ? p.vd - HV * qt : 0;
   if (warp < TC_WORK) {
     double dot = 0.0;
-    const float* xs = p.seg_state ? p.seg_state + slot_h * dd + row + (int64_t)HV * qt * p.kd : nullptr;
-    const float* leave = !GATE ? nullptr : run.last ? a.S_end + sh * dd + (int64_t)row * p.vd + HV * qt : a.S_runs + (slot_h + p.H) * dd + row + (int64_t)HV * qt * p.kd;
-    const int64_t ld = run.last ? 1 : p.kd, at = sh * dd + (int64_t)row * p.vd + HV * qt;
+    const int64_t at = sh * dd + (int64_t)row * p.vd + HV * qt, across = row + (int64_t)HV * qt * p.kd;      // [feature][column], [column][feature]
+    if (p.seg_state) {
+      const float* x = p.seg_state + slot_h * dd + across;
 #pragma unroll
-    for (int j = 0; j < HV; ++j) {
-      float x = 0.f;
-      if (j < cols) {
-        x = xs ? xs[(int64_t)j * p.kd] : ld_any(p.init, !p.init_f32, at + j);
-        if (GATE) dot += (double)x * leave[j * ld];
+      for (int j = 0; j < HV; ++j) S[j] = j < cols ? x[(int64_t)j * p.kd] : 0.f;
+    } else {
+      load_side<HV>(S, p.init_f32 ? (const void*)((const float*)p.init + at) : (const void*)((const bf16*)p.init + at), p.init_f32, cols);
+    }
+    if (GATE) {
+      // with the state that leaves the run
+      float x[HV];
+      if (run.last) {
+        load_side<HV>(x, a.S_end + at, 1, cols);
+      } else {
+        const float* y = a.S_runs + (slot_h + p.H) * dd + across;
+#pragma unroll
+        for (int j = 0; j < HV; ++j) x[j] = j < cols ? y[(int64_t)j * p.kd] : 0.f;
       }
-      S[j] = x;
+#pragma unroll
+      for (int j = 0; j < HV; ++j) dot += (double)S[j] * x[j];
     }
     if (GATE) {
 #pragma unroll
@@ -511,9 +520,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
     }
     if (p.fin && run.first) {
       const int64_t at = sh * dd + (int64_t)row * p.vd + HV * qt;
-#pragma unroll
-      for (int j = 0; j < HV; ++j)
-        if (j < cols) st_any(p.fin, !p.fin_f32, at + j, S[j]);
+      store_side<HV>(S, p.fin_f32 ? (void*)((float*)p.fin + at) : (void*)((bf16*)p.fin + at), p.fin_f32, cols);
     }
   }
   if (!ok && lane == 0) atomicAdd(&g_wait_timeouts, 1u);
