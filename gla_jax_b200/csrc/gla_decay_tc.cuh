@@ -149,11 +149,17 @@ __device__ __forceinline__ void wait_for(bool& ok, uint32_t bar, uint32_t parity
 // wt: exp(lam_i), exp(lam_L - lam_i).  With a the last token before i's group of 32 rows, the weight exp(lam_i - lam_j) of a pair
 // is rf_i cf_j, cf[g - 1]: exp(lam_a - lam_j) for the tokens before group g, cd: for those of the group itself, as long as
 // the sums move by at most `span` <= 80 inside it; where a gate is sharper, the weights inside a group are formed pair by pair.
-struct Gates {
+struct alignas(16) Gates {
   float2 lam[128], wt[128];
   float rf[128], cd[128], cf[3][128];
   float span[4];
+  // exp(-lam_j) and exp(lam_i - lam_L), and the largest |lam|, |lam_L - lam| (base 2).  As long as these are below MILD a product
+  // of scores needs one weight a column, and what is left of the weights multiplies a row of the result, which what comes from
+  // the state shares: both add up in one accumulator.
+  float dn[128], up[128];
+  float low, reach;
 };
+constexpr float MILD = 100.f;          // of the 127 that float32 and bf16 exponents reach
 __device__ __forceinline__ float4 gates_of(const Walk& p, int64_t t0, int nv, int h, int lane) {
   float g[4];
 #pragma unroll
@@ -185,15 +191,21 @@ __device__ __forceinline__ float2 scan_gates(float4 g, Gates& s, int lane) {
   const auto of = [&](int l) { return make_float2(__shfl_sync(0xffffffffu, inc.x, l), __shfl_sync(0xffffffffu, inc.y, l)); };
   const float2 all = of(31), at[3] = {of(7), of(15), of(23)}, left = make_float2(__shfl_up_sync(0xffffffffu, inc.x, 1), __shfl_up_sync(0xffffffffu, inc.y, 1));
   const float2 before = lane ? left : make_float2(0.f, 0.f), own = lane < 8 ? make_float2(0.f, 0.f) : lane < 16 ? at[0] : lane < 24 ? at[1] : at[2];
-  float span = 0.f;
+  float span = 0.f, low = 0.f, reach = 0.f;
+  const auto most = [](float a, float b) { return !(b <= a) ? b : a; };          // (what is not a number stays)
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 y = add2(before, v[i]);
     const float d = (y.x - own.x) + (y.y - own.y);
     const int r = 4 * lane + i;
-    span = !(fabsf(d) <= span) ? fabsf(d) : span;           // (what is not a number stays)
+    const float l = y.x + y.y, u = (all.x - y.x) + (all.y - y.y);
+    span = most(span, fabsf(d));
+    low = most(low, fabsf(l));
+    reach = most(reach, fabsf(u));
+    s.dn[r] = ex2(-l);
+    s.up[r] = ex2(-u);
     s.lam[r] = y;
-    s.wt[r] = make_float2(ex2(y.x + y.y), ex2((all.x - y.x) + (all.y - y.y)));
+    s.wt[r] = make_float2(ex2(l), ex2(u));
     s.rf[r] = ex2(d);
     s.cd[r] = ex2(-d);
 #pragma unroll
@@ -201,10 +213,12 @@ __device__ __forceinline__ float2 scan_gates(float4 g, Gates& s, int lane) {
       if (lane < 8 * (m + 1)) s.cf[m][r] = ex2((at[m].x - y.x) + (at[m].y - y.y));
   }
 #pragma unroll
-  for (int d = 1; d < 8; d <<= 1) {
-    const float y = __shfl_xor_sync(0xffffffffu, span, d);
-    span = !(y <= span) ? y : span;
+  for (int d = 1; d < 32; d <<= 1) {
+    if (d < 8) span = most(span, __shfl_xor_sync(0xffffffffu, span, d));
+    low = most(low, __shfl_xor_sync(0xffffffffu, low, d));
+    reach = most(reach, __shfl_xor_sync(0xffffffffu, reach, d));
   }
+  if (lane == 0) { s.low = low; s.reach = reach; }
   if (lane % 8 == 0) s.span[lane / 8] = span;
   return all;
 }
@@ -425,8 +439,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
         tc_fence_after();
         const uint32_t vst = vb * Y::TV;
         if constexpr (OUT) {
+          const bool one = gates[i & 1].low <= MILD && !p.r && !was_odd(i);         // (on top of Q S)
+          const uint32_t to = one ? tOI : tOA;
 #pragma unroll
-          for (int s = 0; s < 8; ++s) umma_ts(tOA, tSC + 32 * (s >> 1) + 8 * (s & 1), desc_advance(dV, s * 2048), i_pv, s > 0);
+          for (int s = 0; s < 8; ++s) umma_ts(to, tSC + 32 * (s >> 1) + 8 * (s & 1), desc_advance(dV, s * 2048), i_pv, one || s > 0);
           umma_commit(bar(B_PV));
         }
         const uint32_t lst = Y::NL == 2 ? (i & 1) * (NU - 1) * Y::TK : 0;
@@ -539,6 +555,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
       const uint32_t ph = i & 1, kph = Y::NK == 2 ? (i >> 1) & 1 : ph;
       const uint32_t uk = base + Y::K0 + kb * Y::TK, uv = base + Y::V0 + vb * Y::TV;
       const Gates& gs = gates[i & 1];
+      bool mild = false;
       if constexpr (OUT) {
         if (!all_done(bar(B_G + (i & 1)), (i >> 1) & 1, bar(B_QK), ph, bar(B_K + kb), kph)) {
           wait_for(ok, bar(B_G + (i & 1)), (i >> 1) & 1);
@@ -546,6 +563,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
           wait_for(ok, bar(B_QK), ph);
         }
         tc_fence_after();
+        mild = gs.low <= MILD && !p.r;
         {
           const int grp = qt;               // columns 32 grp + [0, 32)
           uint32_t pk[16];
@@ -557,9 +575,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
             tmem_ld32(tSC + lane_base + 32 * grp, x);
             tmem_ld_wait();
             const bool own = grp == q4;
-            if (!own || gs.span[q4] <= 80.f) {
-              const float rf = gs.rf[row];
-              const float4* cf = reinterpret_cast<const float4*>(own ? &gs.cd[32 * grp] : &gs.cf[q4 - 1][32 * grp]);
+            if (mild || !own || gs.span[q4] <= 80.f) {
+              const float rf = mild ? 1.f : gs.rf[row];
+              const float4* cf = reinterpret_cast<const float4*>(mild ? &gs.dn[32 * grp] : own ? &gs.cd[32 * grp] : &gs.cf[q4 - 1][32 * grp]);
               const int last = own ? lane : 31;            // the row's last column
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
@@ -612,8 +630,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
         const int64_t t0 = r0 + first_of(i);
         wait_for(ok, bar(B_PV), ph);             // (and Q S, which was issued before)
         tc_fence_after();
-        if (was_odd(i)) masked_sums<DV, false>(tSC + lane_base, tOA + lane_base, uv, row, qt);
-        const float wi = gs.wt[row].x;
+        const bool odd = was_odd(i), one = mild && !odd;
+        if (odd) masked_sums<DV, false>(tSC + lane_base, tOA + lane_base, uv, row, qt);
+        const float wi = gs.wt[row].x, wp = mild ? wi : 1.f;
         const int64_t at = ((t0 + row) * p.H + h) * p.vd + HV * qt;      // (float32 outputs)
         const int64_t ra = p.r ? ((t0 + row) * (p.H / p.gr) + h / p.gr) * p.vd + HV * qt : 0;
         float dot = 0.f;
@@ -621,7 +640,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
         for (int c0 = 0; c0 < HV; c0 += 16) {
           uint32_t x[16], y[16];
           tmem_ld16(tOI + lane_base + HV * qt + c0, x);
-          tmem_ld16(tOA + lane_base + HV * qt + c0, y);
+          if (one) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] = 0u;
+          } else {
+            tmem_ld16(tOA + lane_base + HV * qt + c0, y);
+          }
           tmem_ld_wait();
           if (row < nv) {
             if (p.r) {
@@ -640,7 +664,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
             }
             float o[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = fmaf(wi, __uint_as_float(x[e]), __uint_as_float(y[e]));
+            for (int e = 0; e < 16; ++e) o[e] = fmaf(wi, __uint_as_float(x[e]), wp * __uint_as_float(y[e]));
             const int left = p.vd - (HV * qt + c0);
             if (p.out_f32) {
 #pragma unroll

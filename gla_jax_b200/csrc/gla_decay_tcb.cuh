@@ -1,8 +1,10 @@
 // The backward walk of decay attention on the fifth-generation tensor cores: dk, dv, the gates' and the first state's gradient,
 // 128 tokens at a time, from the sequence's (run's) end.  With dS the gradient of the state that leaves the chunk:
 //   ST = K Q^T    DT = V dO^T    IV = K dS    IK = V dS^T                                     (rows j, columns i)
-//   P_ji = w_ij ST_ji,  E_ji = w_ij DT_ji  for i >= j        IV <- exp(lam_L - lam_j) IV,  IK <- the same
-//   dV = IV + P dO      dK = IK + E Q      dS <- exp(lam_L) dS + (exp(lam_i) Q)^T dO
+//   P_ji = w_ij ST_ji,  E_ji = w_ij DT_ji  for i >= j        f_j = exp(lam_L - lam_j)
+//   dV = f IV + P dO      dK = f IK + E Q      dS <- exp(lam_L) dS + (exp(lam_i) Q)^T dO
+// In a chunk of mild gates P and E carry exp(lam_i - lam_L) and the outputs f as they leave; in others IV and IK are multiplied
+// in place before P and E, with their whole weights, add to them.
 // The scores are formed transposed, so that P and E are where a product takes its left operand from tensor memory, and both
 // outputs add up in place.  Tensor memory is full (4 x 128 columns); the sum for dS takes ST's place once P is used.  Shared
 // memory holds the four tiles, dS and nothing else: the weighted queries' two planes take the places of V and K, whose
@@ -354,6 +356,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
         wait_for(ok, bar(C_ST), ph);
       }
       tc_fence_after();
+      const bool mild = gs.reach <= MILD;
+      const float wj = gs.wt[row].y;
       float rowsum = 0.f;
       {
         const int grp = qt;               // columns (tokens i) 32 grp + [0, 32)
@@ -378,12 +382,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               const int c = 2 * e + u;
-              const float w = sharp ? decay_of(gs.lam[32 * grp + c], lj) : gs.rf[32 * grp + c] * cf;
+              const float w = mild ? gs.up[32 * grp + c] : sharp ? decay_of(gs.lam[32 * grp + c], lj) : gs.rf[32 * grp + c] * cf;
               const bool in = c >= first && c < end;
               s[u] = in ? __uint_as_float(x[c]) * w : 0.f;
               d[u] = in ? __uint_as_float(y[c]) * w : 0.f;
               if constexpr (GATE) {
-                m[c] = in ? s[u] * __uint_as_float(y[c]) : 0.f;
+                m[c] = in ? s[u] * __uint_as_float(y[c]) * (mild ? wj : 1.f) : 0.f;
                 rowsum += m[c];
               }
             }
@@ -400,17 +404,19 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
       odd = check_rows<DK>(base + Y::Q0, nv) || odd;
       wait_for(ok, bar(C_I), ph);
       tc_fence_after();
-      const float wj = gs.wt[row].y;
       float dot = 0.f;
+      if (!mild) {
 #pragma unroll 1
-      for (int c0 = 0; c0 < HV; c0 += 16) {
-        uint32_t x[16];
-        tmem_ld16(tIV + lane_base + HV * qt + c0, x);
-        tmem_ld_wait();
+        for (int c0 = 0; c0 < HV; c0 += 16) {
+          uint32_t x[16];
+          tmem_ld16(tIV + lane_base + HV * qt + c0, x);
+          tmem_ld_wait();
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(wj * __uint_as_float(x[e]));
-        tmem_st16(tIV + lane_base + HV * qt + c0, x);
+          for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(wj * __uint_as_float(x[e]));
+          tmem_st16(tIV + lane_base + HV * qt + c0, x);
+        }
       }
+      if (!mild || GATE)
 #pragma unroll 1
       for (int c0 = 0; c0 < HK; c0 += 16) {
         uint32_t x[16];
@@ -418,7 +424,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
         tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < 16; ++e) x[e] = __float_as_uint(wj * __uint_as_float(x[e]));
-        tmem_st16(tIK + lane_base + HK * qt + c0, x);
+        if (!mild) tmem_st16(tIK + lane_base + HK * qt + c0, x);
         if constexpr (GATE) {
           const int c8 = (HK * qt + c0) / 8;
 #pragma unroll
@@ -462,6 +468,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
         constexpr int HD = DKO ? HK : HV;
         const int nd = DKO ? p.kd : p.vd;
         const uint32_t t = (DKO ? tIK : tIV) + lane_base + HD * qt;
+        const float f = mild ? wj : 1.f;
         if (DKO && a.dk_f32) {
           float* o = (float*)a.dk + ((t0 + row) * p.H + h) * nd + HD * qt;
 #pragma unroll 1
@@ -472,7 +479,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
               if (row < nv && HD * qt + c0 + e < nd)
-                *reinterpret_cast<float4*>(o + c0 + e) = make_float4(__uint_as_float(x[e]), __uint_as_float(x[e + 1]), __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+                *reinterpret_cast<float4*>(o + c0 + e) = make_float4(f * __uint_as_float(x[e]), f * __uint_as_float(x[e + 1]), f * __uint_as_float(x[e + 2]), f * __uint_as_float(x[e + 3]));
           }
           return;
         }
@@ -482,7 +489,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
           tmem_ld16(t + c0, x);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+          for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(f * __uint_as_float(x[2 * e]), f * __uint_as_float(x[2 * e + 1]));
           const int c8 = (HD * qt + c0) / 8;
           const uint32_t d = base + Y::OUT0 + (c8 >> 3) * 16384;
           sts16(d + sw128_chunk(row, c8 & 7), make_uint4(w[0], w[1], w[2], w[3]));
