@@ -235,7 +235,7 @@ static size_t fast_bwd_parts(const Dims& d, bool gate, size_t (&at)[4]) {
   const int64_t s = d.seg(128);
   at[0] = d.cut(s) ? fast_totals(d) : 0;
   at[1] = at[0] + (d.cut(s) ? state_bytes(d, d.slots(s)) : 0);
-  at[2] = at[1] + (gate ? align_up((size_t)(4 * d.rows() * d.H) * 4, 256) : 0);
+  at[2] = at[1] + (gate ? align_up((size_t)(WALK_COLS * d.rows() * d.H) * 4, 256) : 0);
   at[3] = at[2] + (d.H > d.Hk ? align_up((size_t)(d.rows() * d.H * d.Dk) * 4, 256) : 0);
   return at[3];
 }

@@ -5,11 +5,13 @@
 namespace gla {
 namespace decay {
 
+constexpr int WALK_COLS = 2;               // partial sums that a walk leaves in rdot
+
 // A backward walk: dk, dv, the gates (dg, with `gate`) and the first state's gradient (w.fin).
 struct Back {
   Walk w;                                  // k, q, v; H, sizes, gates, runs; seg_state: gradients that enter each run backwards
   const void* dout;
-  const float* a;                          // [4][token][H], with gates: what the walk for dq leaves in rdot
+  const float* a;                          // [WALK_COLS][token][H], with gates: what the walk for dq leaves in rdot
   const float *S_runs, *S_end;             // entering states of the runs [slot][H][vd][kd] (NULL: one run each), final states
   void *dk, *dv;
   int dk_f32;

@@ -5,6 +5,8 @@
 namespace gla {
 namespace decay {
 
+static_assert(WALK_COLS == TC_COLS, "partial sums of rdot");
+
 template <int NU, int NS, bool OUT>
 static int sizes(cudaStream_t stream, const Walk& p, const char* name) {
   if (p.kd <= 64) return p.vd <= 64 ? launch_tc<64, 64, NU, NS, OUT>(stream, p, name) : launch_tc<64, 128, NU, NS, OUT>(stream, p, name);

@@ -1,7 +1,7 @@
 // The walks of gla_decay.cuh on the fifth-generation tensor cores: bf16, head sizes up to 128, 128 tokens at a time.
 //
-// Per chunk:  SC = Q K^T,  OI = Q S,  OA = P V  and  U = (w K)^T V  (w = exp(lam_L - lam_j), in two or three bf16 planes).  Sixteen
-// warps turn SC into P in tensor memory (a thread per row and quarter of the columns), weigh K in place, write exp(lam_i) OI + OA,
+// Per chunk:  SC = Q K^T,  OI = Q S,  OA = P V  and  U = (w K)^T V  (w = exp(lam_L - lam_j), in two or three bf16 planes).  Eight
+// warps turn SC into P in tensor memory (a thread per row and half of the columns), weigh K in place, write exp(lam_i) OI + OA,
 // and keep the state in registers: S <- exp(lam_L) S + U, from where its bf16 image goes to shared memory for the next chunk.
 // One warp issues the products, one the tensor copies, one prepares the gates of the chunk to come.
 //
@@ -27,6 +27,10 @@ __device__ __forceinline__ void tmem_st16(uint32_t a, const uint32_t (&r)[16]) {
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
       :: "r"(a), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
          "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t a, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
+               :: "r"(a), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // D (+)= A[tensor memory] B[shared memory]
@@ -145,6 +149,11 @@ __device__ __forceinline__ void wait_for(bool& ok, uint32_t bar, uint32_t parity
   ok = mbar_wait(bar, parity);
 }
 
+// Worker warps (eight: with sixteen, whose threads have half the registers, what does not fit them goes through an L1 that shared
+// memory leaves next to nothing of); warps for products, copies, gates.  The workers stand side by side in TC_COLS groups of 128
+// threads, a thread per row, and TC_ROWS of 8 threads a row.
+constexpr int TC_WORK = 8, TC_THREADS = (TC_WORK + 3) * 32, TC_COLS = TC_WORK / 4, TC_ROWS = TC_WORK * 4;
+
 // What a chunk of 128 needs of its gates, made by one warp, four rows a lane.  lam: running sums, base 2, as two floats;
 // wt: exp(lam_i), exp(lam_L - lam_i).  With a the last token before i's group of 32 rows, the weight exp(lam_i - lam_j) of a pair
 // is rf_i cf_j, cf[g - 1]: exp(lam_a - lam_j) for the tokens before group g, cd: for those of the group itself, as long as
@@ -231,18 +240,18 @@ __device__ __forceinline__ void weigh(uint32_t tile, uint32_t lo, uint32_t plane
   const int r0 = threadIdx.x / 8, c = threadIdx.x % 8;
   const float* w_ = &wt[r0].x + (rev ? 0 : 1);
   const uint32_t at0 = sw128_chunk(r0, c);
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const float w = w_[128 * j];
+#pragma unroll 2
+  for (int j = 0; j < 128 / TC_ROWS; ++j) {
+    const float w = w_[2 * TC_ROWS * j];
     uint4 x[D / 64];
 #pragma unroll
-    for (int b = 0; b < D / 64; ++b) x[b] = lds16(tile + b * 16384 + j * 8192 + at0);
-    if (r0 + 64 * j >= nv)
+    for (int b = 0; b < D / 64; ++b) x[b] = lds16(tile + b * 16384 + j * TC_ROWS * 128 + at0);
+    if (r0 + TC_ROWS * j >= nv)
 #pragma unroll
       for (int b = 0; b < D / 64; ++b) x[b] = make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
     for (int b = 0; b < D / 64; ++b) {
-      const uint32_t at = b * 16384 + j * 8192 + at0;
+      const uint32_t at = b * 16384 + j * TC_ROWS * 128 + at0;
       const uint32_t u[4] = {x[b].x, x[b].y, x[b].z, x[b].w};
       uint32_t s[4][NU];
 #pragma unroll
@@ -263,11 +272,11 @@ __device__ __forceinline__ bool check_rows(uint32_t tile, int nv) {
   const uint32_t at0 = tile + sw128_chunk(r0, c);
   uint32_t m = 0;
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < 128 / TC_ROWS; ++j)
 #pragma unroll
     for (int b = 0; b < D / 64; ++b) {
-      const uint32_t at = at0 + b * 16384 + j * 8192;
-      if (r0 + 64 * j < nv) {
+      const uint32_t at = at0 + b * 16384 + j * TC_ROWS * 128;
+      if (r0 + TC_ROWS * j < nv) {
         const uint4 v = lds16(at);
         m = __vmaxu2(__vmaxu2(m, v.x & 0x7fff7fffu), __vmaxu2(v.y & 0x7fff7fffu, __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
       } else {
@@ -283,7 +292,7 @@ __device__ __forceinline__ bool check_rows(uint32_t tile, int nv) {
 template <int DV, bool UP>
 __device__ __noinline__ void masked_sums(uint32_t tp, uint32_t to, uint32_t tv, int row, int qt) {
 #pragma unroll 1
-  for (int c0 = qt * (DV / 4); c0 < (qt + 1) * (DV / 4); c0 += 16) {
+  for (int c0 = qt * (DV / TC_COLS); c0 < (qt + 1) * (DV / TC_COLS); c0 += 16) {
     float o[16];
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[e] = 0.f;
@@ -322,8 +331,6 @@ __device__ __noinline__ void masked_sums(uint32_t tp, uint32_t to, uint32_t tv, 
   tmem_st_wait();
 }
 
-constexpr int TC_WORK = 16, TC_THREADS = (TC_WORK + 3) * 32;             // worker warps; and products, copies, gates
-
 template <int DK, int DV, int NU, int NS, bool OUT>
 struct TLay {
   static constexpr int NK = !OUT || NU + NS <= 3 ? 2 : 1, NV = OUT ? 1 : 2, NL = OUT || NU > 2 ? 1 : 2;   // stages of K, V, the lower planes
@@ -351,7 +358,7 @@ struct TcWalk {
 template <int DK, int DV, int NU, int NS, bool OUT>
 __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_constant__ TcWalk a) {
   using Y = TLay<DK, DV, NU, NS, OUT>;
-  constexpr int HV = DV / 4;                                   // value columns of a worker
+  constexpr int HV = DV / TC_COLS;                             // value columns of a worker
   const Walk& p = a.w;
   extern __shared__ __align__(1024) uint8_t sm[];
   Gates* gates = reinterpret_cast<Gates*>(sm + Y::G0);
@@ -487,13 +494,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
     __syncwarp();
   } else if (warp == TC_WORK + 2) {
     // ================= gates =================
-    double total = 0.0;
+    double total = 0.0, all[2] = {0.0, 0.0};
     float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
     if (chunks) g = gates_of(p, r0 + first_of(0), rows_of(0), h, lane);
     for (int i = 0; i < chunks; ++i) {
       if (i >= 2) wait_for(ok, bar(B_GFREE + (i & 1)), ((i - 2) >> 1) & 1);
-      const float2 all = scan_gates(g, gates[i & 1], lane);
-      total += (double)all.x + (double)all.y;
+      // (a decay that no token changes makes the same of every whole chunk)
+      if (p.gt != 0 || i < 2 || rows_of(i) != rows_of(i - 2)) {
+        const float2 x = scan_gates(g, gates[i & 1], lane);
+        all[i & 1] = (double)x.x + (double)x.y;
+      }
+      total += all[i & 1];
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(B_G + (i & 1)));
       if (i + 1 < chunks) g = gates_of(p, r0 + first_of(i + 1), rows_of(i + 1), h, lane);
@@ -564,23 +575,24 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
         }
         tc_fence_after();
         mild = gs.low <= MILD && !p.r;
-        {
-          const int grp = qt;               // columns 32 grp + [0, 32)
-          uint32_t pk[16];
+#pragma unroll 1
+        for (int sb = qt * (8 / TC_COLS); sb < (qt + 1) * (8 / TC_COLS); ++sb) {
+          const int grp = sb >> 1;          // columns 16 sb + [0, 16), of the group of 32
+          uint32_t pk[8];
           if (grp > q4) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) pk[e] = 0u;
+            for (int e = 0; e < 8; ++e) pk[e] = 0u;
           } else {
-            uint32_t x[32];
-            tmem_ld32(tSC + lane_base + 32 * grp, x);
+            uint32_t x[16];
+            tmem_ld16(tSC + lane_base + 16 * sb, x);
             tmem_ld_wait();
             const bool own = grp == q4;
+            const int last = own ? lane - 16 * (sb & 1) : 15;          // the row's last column
             if (mild || !own || gs.span[q4] <= 80.f) {
               const float rf = mild ? 1.f : gs.rf[row];
-              const float4* cf = reinterpret_cast<const float4*>(mild ? &gs.dn[32 * grp] : own ? &gs.cd[32 * grp] : &gs.cf[q4 - 1][32 * grp]);
-              const int last = own ? lane : 31;            // the row's last column
+              const float4* cf = reinterpret_cast<const float4*>(mild ? &gs.dn[16 * sb] : own ? &gs.cd[16 * sb] : &gs.cf[q4 - 1][16 * sb]);
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
+              for (int e = 0; e < 4; ++e) {
                 const float4 c = cf[e];
                 const float y0 = 4 * e <= last ? __uint_as_float(x[4 * e]) * (rf * c.x) : 0.f;
                 const float y1 = 4 * e + 1 <= last ? __uint_as_float(x[4 * e + 1]) * (rf * c.y) : 0.f;
@@ -592,16 +604,16 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
             } else {
               const float2 li = gs.lam[row];
 #pragma unroll
-              for (int e = 0; e < 16; ++e) {
-                const float4 l = *reinterpret_cast<const float4*>(&gs.lam[32 * grp + 2 * e]);
-                const float x0 = 2 * e <= lane ? __uint_as_float(x[2 * e]) * decay_of(li, make_float2(l.x, l.y)) : 0.f;
-                const float x1 = 2 * e + 1 <= lane ? __uint_as_float(x[2 * e + 1]) * decay_of(li, make_float2(l.z, l.w)) : 0.f;
+              for (int e = 0; e < 8; ++e) {
+                const float4 l = *reinterpret_cast<const float4*>(&gs.lam[16 * sb + 2 * e]);
+                const float x0 = 2 * e <= last ? __uint_as_float(x[2 * e]) * decay_of(li, make_float2(l.x, l.y)) : 0.f;
+                const float x1 = 2 * e + 1 <= last ? __uint_as_float(x[2 * e + 1]) * decay_of(li, make_float2(l.z, l.w)) : 0.f;
                 pk[e] = pack_bf16x2(x0, x1);
               }
             }
           }
-          // P over this thread's own part of SC
-          tmem_st16(tSC + lane_base + 32 * grp, pk);
+          // P over this thread's own part of SC, which it has read up to here
+          tmem_st8(tSC + lane_base + 32 * grp + 8 * (sb & 1), pk);
         }
         tmem_st_wait();
       }

@@ -21,7 +21,7 @@ namespace decay {
 struct TcBack {
   CUtensorMap q, k, v, o;
   Walk w;                                  // k, q, v; H, sizes, gates, runs; seg_state: gradients that enter each run backwards
-  const float* a;                          // [4][token][H], with gates
+  const float* a;                          // [TC_COLS][token][H], with gates
   const float *S_runs, *S_end;             // entering states of the runs [slot][H][vd][kd], final states
   void *dk, *dv;
   int dk_f32;
@@ -44,12 +44,12 @@ struct BTLay {
 };
 enum TbBar { C_LOAD = 0, C_ST = 1, C_I = 2, C_DV = 3, C_U = 4, C_P = 5, C_W = 6, C_S = 7, C_G = 8, C_GFREE = 10, C_E = 12, C_COUNT = 14, C_TMEM = 14, C_ODD = 15 };
 
-// o (a row of tensor memory, D / 4 columns from the quarter's first) += sum over i >= row of P_i V_i, for a chunk in which V holds
+// o (a row of tensor memory, D / TC_COLS columns from the worker's first) += sum over i >= row of P_i V_i, for a chunk in which V holds
 // something that is not finite (see masked_sums)
 template <int D>
 __device__ __noinline__ void masked_add(uint32_t tp, uint32_t to, uint32_t tv, int row, int qt) {
 #pragma unroll 1
-  for (int c0 = qt * (D / 4); c0 < (qt + 1) * (D / 4); c0 += 16) {
+  for (int c0 = qt * (D / TC_COLS); c0 < (qt + 1) * (D / TC_COLS); c0 += 16) {
     uint32_t r[16];
     __syncwarp();
     tmem_ld16(to + c0, r);
@@ -87,12 +87,12 @@ template <int D>
 __device__ __forceinline__ void weigh_to(uint32_t tile, uint32_t hi, uint32_t lo, const float2* wt) {
   const int r0 = threadIdx.x / 8, c = threadIdx.x % 8;
   const uint32_t at0 = sw128_chunk(r0, c);
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const float w = wt[r0 + 64 * j].x;
+#pragma unroll 2
+  for (int j = 0; j < 128 / TC_ROWS; ++j) {
+    const float w = wt[r0 + TC_ROWS * j].x;
 #pragma unroll
     for (int b = 0; b < D / 64; ++b) {
-      const uint32_t at = b * 16384 + j * 8192 + at0;
+      const uint32_t at = b * 16384 + j * TC_ROWS * 128 + at0;
       const uint4 x = lds16(tile + at);
       const uint32_t u[4] = {x.x, x.y, x.z, x.w};
       uint32_t s[4][2];
@@ -108,14 +108,16 @@ __device__ __forceinline__ void weigh_to(uint32_t tile, uint32_t hi, uint32_t lo
 }
 __device__ __forceinline__ bool workers_or(bool x) {          // barrier of the workers, and whether any has x
   uint32_t r;
-  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, 512, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
-               : "=r"(r) : "r"((uint32_t)x) : "memory");
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}\n"
+               : "=r"(r) : "r"((uint32_t)x), "n"(TC_WORK * 32) : "memory");
   return r != 0;
 }
-// 32 values of each of 32 lanes summed over the lanes: lane l is left with the sum of value l
-__device__ __forceinline__ float lane_sums(float (&v)[32], int lane) {
+// 16 values of each of 32 lanes summed over the lanes: lane l is left with the sum of value l % 16
+__device__ __forceinline__ float lane_sums(float (&v)[16], int lane) {
 #pragma unroll
-  for (int s = 16; s; s >>= 1)
+  for (int j = 0; j < 16; ++j) v[j] += __shfl_xor_sync(0xffffffffu, v[j], 16);
+#pragma unroll
+  for (int s = 8; s; s >>= 1)
 #pragma unroll
     for (int j = 0; j < s; ++j) {
       const float give = (lane & s) ? v[j] : v[j + s], keep = (lane & s) ? v[j + s] : v[j];
@@ -127,12 +129,11 @@ __device__ __forceinline__ float lane_sums(float (&v)[32], int lane) {
 template <int DK, int DV, bool GATE>
 __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_constant__ TcBack a) {
   using Y = BTLay<DK, DV, GATE>;
-  constexpr int NS = Y::NS, HV = DV / 4, HK = DK / 4;
-  static_assert(TC_WORK == 16, "workers_or");
+  constexpr int NS = Y::NS, HV = DV / TC_COLS, HK = DK / TC_COLS;
   const Walk& p = a.w;
   extern __shared__ __align__(1024) uint8_t sm[];
   Gates* gates = reinterpret_cast<Gates*>(sm + Y::G0);
-  float* sums = reinterpret_cast<float*>(sm + Y::SUM);          // [2][12][128]: r by row group, c and b by quarter
+  float* sums = reinterpret_cast<float*>(sm + Y::SUM);          // [2][12][128]: r by row group, c and b by half
   double* red = reinterpret_cast<double*>(sm + Y::RED);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   const int h = blockIdx.y;
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
   const auto rows_of = [&](int i) { const int c0 = 128 * (chunks - 1 - i); return len - c0 < 128 ? len - c0 : 128; };   // step i: from the end
   const auto token = [&](int i) { return r0 + 128 * (chunks - 1 - i); };
 
-  const int q4 = warp & 3, qt = (warp >> 2) & 3, row = 32 * q4 + lane;      // (workers)
+  const int q4 = warp & 3, qt = (warp >> 2) % TC_COLS, row = 32 * q4 + lane;      // (workers)
   const uint32_t lane_base = (uint32_t)(32 * q4) << 16;
   float S[HV];                                                               // dS: row `row`, columns HV qt + [0, HV)
   const int cols = row < p.kd ? p.vd - HV * qt : 0;
@@ -293,8 +294,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
         if (t < nv) {
           const float* y = s + t;
 #pragma unroll
-          for (int m = 0; m < 4; ++m)
-            x += (double)y[128 * m] - (double)y[512 + 128 * m] - (double)y[1024 + 128 * m] + (double)a.a[(m * rows + t0 + t) * p.H + h];
+          for (int m = 0; m < 4; ++m) x += (double)y[128 * m];
+#pragma unroll
+          for (int m = 0; m < TC_COLS; ++m) x += (double)a.a[(m * rows + t0 + t) * p.H + h] - (double)y[512 + 128 * m] - (double)y[1024 + 128 * m];
         }
         sum += x;
         e[u] = sum;
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
     for (int i = 0; i < chunks; ++i) {
       if (GATE && i >= 2) gradient(i - 2);
       if (i >= 2) wait_for(ok, bar(C_GFREE + (i & 1)), ((i - 2) >> 1) & 1);
-      scan_gates(g, gates[i & 1], lane);
+      if (p.gt != 0 || i < 2 || rows_of(i) != rows_of(i - 2)) scan_gates(g, gates[i & 1], lane);      // (as in the forward)
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(C_G + (i & 1)));
       if (i + 1 < chunks) g = gates_of(p, token(i + 1), rows_of(i + 1), h, lane);
@@ -359,45 +361,51 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
       const bool mild = gs.reach <= MILD;
       const float wj = gs.wt[row].y;
       float rowsum = 0.f;
-      {
-        const int grp = qt;               // columns (tokens i) 32 grp + [0, 32)
-        uint32_t pk[16], ek[16];
+#pragma unroll 1
+      for (int sb = qt * (8 / TC_COLS); sb < (qt + 1) * (8 / TC_COLS); ++sb) {
+        const int grp = sb >> 1;             // columns (tokens i) 16 sb + [0, 16), of the group of 32
+        uint32_t pk[8], ek[8];
         if (grp < q4) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) pk[e] = ek[e] = 0u;
-          if (GATE) sum[128 * q4 + 32 * grp + lane] = 0.f;
+          for (int e = 0; e < 8; ++e) pk[e] = ek[e] = 0u;
+          if (GATE && lane < 16) sum[128 * q4 + 16 * sb + lane] = 0.f;
         } else {
-          uint32_t x[32], y[32];
-          float m[GATE ? 32 : 1];
-          tmem_ld32(tST + lane_base + 32 * grp, x);
-          tmem_ld32(tDT + lane_base + 32 * grp, y);
+          uint32_t x[16], y[16];
+          float m[GATE ? 16 : 1];
+          tmem_ld16(tST + lane_base + 16 * sb, x);
+          tmem_ld16(tDT + lane_base + 16 * sb, y);
           tmem_ld_wait();
-          const bool own = grp == q4, sharp = own && !(gs.span[q4] <= 80.f);
-          const float cf = own ? gs.cd[row] : gs.cf[grp - 1][row];
+          const bool own = grp == q4, sharp = !mild && own && !(gs.span[q4] <= 80.f);
+          const float cf = mild ? 1.f : own ? gs.cd[row] : gs.cf[grp - 1][row];
+          const float* rf = mild ? gs.up : gs.rf;
           const float2 lj = gs.lam[row];
-          const int first = own ? lane : 0, end = nv - 32 * grp;           // columns that count
+          const int first = own ? lane - 16 * (sb & 1) : 0, end = nv - 16 * sb;           // columns that count
+          const float wm = mild ? wj : 1.f;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
+          for (int e = 0; e < 8; ++e) {
             float s[2], d[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
               const int c = 2 * e + u;
-              const float w = mild ? gs.up[32 * grp + c] : sharp ? decay_of(gs.lam[32 * grp + c], lj) : gs.rf[32 * grp + c] * cf;
+              const float w = sharp ? decay_of(gs.lam[16 * sb + c], lj) : rf[16 * sb + c] * cf;
               const bool in = c >= first && c < end;
               s[u] = in ? __uint_as_float(x[c]) * w : 0.f;
               d[u] = in ? __uint_as_float(y[c]) * w : 0.f;
               if constexpr (GATE) {
-                m[c] = in ? s[u] * __uint_as_float(y[c]) * (mild ? wj : 1.f) : 0.f;
+                m[c] = in ? s[u] * __uint_as_float(y[c]) * wm : 0.f;
                 rowsum += m[c];
               }
             }
             pk[e] = pack_bf16x2(s[0], s[1]);
             ek[e] = pack_bf16x2(d[0], d[1]);
           }
-          if constexpr (GATE) sum[128 * q4 + 32 * grp + lane] = lane_sums(m, lane);
+          if constexpr (GATE) {
+            const float t = lane_sums(m, lane);
+            if (lane < 16) sum[128 * q4 + 16 * sb + lane] = t;
+          }
         }
-        tmem_st16(tST + lane_base + 32 * grp, pk);
-        tmem_st16(tDT + lane_base + 32 * grp, ek);
+        tmem_st8(tST + lane_base + 32 * grp + 8 * (sb & 1), pk);
+        tmem_st8(tDT + lane_base + 32 * grp + 8 * (sb & 1), ek);
       }
       if (GATE) sum[512 + 128 * qt + row] = rowsum;
       bool odd = check_rows<DV>(base + Y::O0, nv);
