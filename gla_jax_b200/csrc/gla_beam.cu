@@ -352,9 +352,9 @@ __global__ void __launch_bounds__(QNT) select_parts_kernel(const Select p) {
   const auto w_of = [](int i) { return i / E; };                      // the access that logit i of a thread's tile came by
   const int shift = (int)((uintptr_t)base & 15) / ES;
   const int64_t lo = blockIdx.x * p.part, hi = lo + p.part < V ? lo + p.part : V;
-  float m = -CUDART_INF_F, s = 0.f;
-  float v1 = 0.f, v2 = 0.f;           // the two largest, and where (-1: none)
-  int i1 = -1, i2 = -1;
+  float s = 0.f;
+  float v1 = -CUDART_INF_F, v2 = -CUDART_INF_F;      // the two largest (v1 is the running maximum), and the tiles that they came in
+  int64_t t1 = lo, t2 = lo;
   uint4 raw[2 * NV];                  // the next tile's 16 bytes, and the 16 behind them where a row starts anywhere
   const auto whole = [&](int64_t e) { return shift ? e >= shift && e - shift + 2 * E <= V : e + E <= V; };
   const auto request = [&](int64_t t0) {
@@ -369,8 +369,7 @@ __global__ void __launch_bounds__(QNT) select_parts_kernel(const Select p) {
   };
   request(lo);
   for (int64_t t0 = lo; t0 < hi; t0 += TILE) {
-    float x[QV];
-    unsigned int has = 0;
+    float x[QV];                      // (-inf where there is none)
 #pragma unroll
     for (int w = 0; w < NV; ++w) {
       const int64_t e = t0 + (int64_t)(w * QNT + tid) * E;
@@ -397,46 +396,60 @@ __global__ void __launch_bounds__(QNT) select_parts_kernel(const Select p) {
           if constexpr (BF) { x[w * E + 2 * i] = __uint_as_float(y[i] << 16); x[w * E + 2 * i + 1] = __uint_as_float(y[i] & 0xffff0000u); }
           else x[w * E + i] = __uint_as_float(y[i]);
         }
-        has |= ((1u << E) - 1) << (w * E);
       } else {
 #pragma unroll
         for (int i = 0; i < E; ++i) {
           x[w * E + i] = -CUDART_INF_F;
-          if (e + i < hi) {
-            x[w * E + i] = BF ? __bfloat162float(((const bf16*)base)[e + i]) : ((const float*)base)[e + i];
-            has |= 1u << (w * E + i);
-          }
+          if (e + i < hi) x[w * E + i] = BF ? __bfloat162float(((const bf16*)base)[e + i]) : ((const float*)base)[e + i];
         }
       }
     }
     request(t0 + TILE);
-    float top = -CUDART_INF_F;
-#pragma unroll
-    for (int i = 0; i < QV; ++i) top = fmaxf(top, x[i]);      // (passes over what is not a number)
-    bool odd = false;
-#pragma unroll
-    for (int i = 0; i < QV; ++i) odd = odd || x[i] != x[i];
-    if (odd || top > FMOST) {
-      top = clean(top);
-#pragma unroll
-      for (int i = 0; i < QV; ++i) x[i] = clean(x[i]);
-    }
-    if (top > m) { s *= exp_of(m - top); m = top; }
-    if (m > -CUDART_INF_F) {
-#pragma unroll
-      for (int i = 0; i < QV; ++i) s += exp_of(x[i] - m);
-    }
-    if (has && (i2 < 0 || top > v2)) {
+    const float o1 = v1, o2 = v2;
+    float t;
+    const auto take = [&]() {
 #pragma unroll
       for (int i = 0; i < QV; ++i) {
-        const int e = (int)(t0 + (w_of(i) * QNT + tid) * E + i % E);
-        if ((has >> i) & 1u) {
-          if (i1 < 0 || x[i] > v1) { v2 = v1; i2 = i1; v1 = x[i]; i1 = e; }
-          else if (i2 < 0 || x[i] > v2) { v2 = x[i]; i2 = e; }
-        }
+        v2 = fmaxf(v2, fminf(v1, x[i]));
+        v1 = fmaxf(v1, x[i]);
       }
+      t = 0.f;
+      if (v1 > -CUDART_INF_F) {
+#pragma unroll
+        for (int i = 0; i < QV; ++i) t += exp_of(x[i] - v1);
+      }
+    };
+    take();
+    if (t != t) {                      // +inf or what is not a number is among them
+#pragma unroll
+      for (int i = 0; i < QV; ++i) x[i] = clean(x[i]);
+      v1 = o1;
+      v2 = o2;
+      take();
     }
+    if (v1 > o1) {
+      s *= exp_of(o1 - v1);
+      if (v2 == o1) t2 = t1;           // (the first before is the second now, also among equal ones)
+      else t2 = t0;
+      t1 = t0;
+    } else if (v2 > o2) {
+      t2 = t0;
+    }
+    s += t;
   }
+  const auto logit = [&](int64_t e) { return clean(BF ? __bfloat162float(((const bf16*)base)[e]) : ((const float*)base)[e]); };
+  // the first of a tile's logits that is v, other than `but` (-1: none)
+  const auto find = [&](int64_t t0, float v, int but) {
+    int at = -1;
+#pragma unroll
+    for (int i = QV - 1; i >= 0; --i) {
+      const int64_t e = t0 + (w_of(i) * QNT + tid) * E + i % E;
+      if (e < hi && e != but && logit(e) == v) at = (int)e;
+    }
+    return at;
+  };
+  const int i1 = find(t1, v1, -1), i2 = find(t2, v2, i1);
+  const float m = v1;
   // the bound: sorted by warp, a key's place among all is its place in its warp and what is larger in the others
   const u64 first = i1 < 0 ? 0 : key_of(v1, (unsigned int)i1), second = i2 < 0 ? 0 : key_of(v2, (unsigned int)i2);
   const u64 own = warp_sorted(first, lane);
@@ -467,7 +480,6 @@ __global__ void __launch_bounds__(QNT) select_parts_kernel(const Select p) {
     below[i] = second;
   }
   __syncthreads();
-  const auto logit = [&](int64_t e) { return clean(BF ? __bfloat162float(((const bf16*)base)[e]) : ((const float*)base)[e]); };
   const int tiles = hi > lo ? (int)((hi - lo + TILE - 1) / TILE) : 0;
   for (int k = 0; k < more; ++k) {
     // the logits that thread who[k] met, below its second
