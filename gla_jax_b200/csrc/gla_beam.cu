@@ -590,6 +590,7 @@ __global__ void __launch_bounds__(BNT) select_beams_kernel(const Select p) {
     const u64 x = i < n ? key[i] : 0, at = i < n ? where[i] : 0;
     int rank = 0;
     if (x)
+#pragma unroll 4
       for (int j = part; j < n; j += 8) rank += key[j] > x || (key[j] == x && where[j] < at);
 #pragma unroll
     for (int d = 1; d < 8; d <<= 1) rank += __shfl_xor_sync(0xffffffffu, rank, d);

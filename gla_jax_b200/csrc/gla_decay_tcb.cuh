@@ -40,6 +40,7 @@ struct BTLay {
   static constexpr int END = USED < 120 * 1024 ? 120 * 1024 : USED;
   static constexpr int HI = DV < DK ? H0 : V0, OUT0 = OWN ? STG : S0;
   static_assert(END <= 232448, "shared memory");
+  static_assert(DK == DV || 256 * (DK > DV ? DK : DV) >= 4096 * TC_WORK, "a place per warp");
   static_assert(S0 % 1024 == 0 && STG % 1024 == 0, "tiles");
 };
 enum TbBar { C_LOAD = 0, C_ST = 1, C_I = 2, C_DV = 3, C_U = 4, C_P = 5, C_W = 6, C_S = 7, C_G = 8, C_GFREE = 10, C_E = 12, C_COUNT = 14, C_TMEM = 14, C_ODD = 15 };
@@ -307,7 +308,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
         const double y = __shfl_down_sync(0xffffffffu, inc, d);
         if (lane + d < 32) inc += y;
       }
-      const double behind = carry + inc - sum;
+      // (what is behind this lane's tokens; not inc - sum, which is lost where sum is not finite)
+      const double next = __shfl_down_sync(0xffffffffu, inc, 1), behind = carry + (lane < 31 ? next : 0.0);
 #pragma unroll
       for (int u = 0; u < 4; ++u)
         if (4 * lane + u < nv) a.dg[(t0 + 4 * lane + u) * p.H + h] = (float)(behind + e[u]);
@@ -476,6 +478,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
         constexpr int HD = DKO ? HK : HV;
         const int nd = DKO ? p.kd : p.vd;
         const uint32_t t = (DKO ? tIK : tIV) + lane_base + HD * qt;
+        // a warp's place must be its own for dv and dk both: with equal sizes that is its part of the rows, else 4 KB of their own
+        const auto place = [&](int r, int c) {             // of piece c of row r of the warp
+          const int c8 = HD / 8 * qt + c;
+          return base + Y::OUT0 + (DK == DV ? (c8 >> 3) * 16384 + sw128_chunk(32 * q4 + r, c8 & 7) : 4096 * warp + sw128_chunk(r, c));
+        };
         const float f = mild ? wj : 1.f;
         if (DKO && a.dk_f32) {
           float* o = (float*)a.dk + ((t0 + row) * p.H + h) * nd + HD * qt;
@@ -498,20 +505,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
           tmem_ld_wait();
 #pragma unroll
           for (int e = 0; e < 8; ++e) w[e] = pack_bf16x2(f * __uint_as_float(x[2 * e]), f * __uint_as_float(x[2 * e + 1]));
-          const int c8 = (HD * qt + c0) / 8;
-          const uint32_t d = base + Y::OUT0 + (c8 >> 3) * 16384;
-          sts16(d + sw128_chunk(row, c8 & 7), make_uint4(w[0], w[1], w[2], w[3]));
-          sts16(d + sw128_chunk(row, (c8 & 7) + 1), make_uint4(w[4], w[5], w[6], w[7]));
+          sts16(place(lane, c0 / 8), make_uint4(w[0], w[1], w[2], w[3]));
+          sts16(place(lane, c0 / 8 + 1), make_uint4(w[4], w[5], w[6], w[7]));
         }
         constexpr int LR = HD / 8, RI = 32 / LR;
         __syncwarp();
         const int c8 = HD / 8 * qt + lane % LR;
-        const uint32_t d = base + Y::OUT0 + (c8 >> 3) * 16384;
         bf16* o = (bf16*)(DKO ? a.dk : a.dv) + ((t0 + 32 * q4 + lane / LR) * p.H + h) * nd + 8 * c8;
 #pragma unroll
         for (int j = 0; j < 32; j += RI) {
-          const int r = 32 * q4 + j + lane / LR;
-          if (r < nv && 8 * c8 < nd) *reinterpret_cast<uint4*>(o) = lds16(d + sw128_chunk(r, c8 & 7));
+          const int r = j + lane / LR;
+          if (32 * q4 + r < nv && 8 * c8 < nd) *reinterpret_cast<uint4*>(o) = lds16(place(r, lane % LR));
           o += (int64_t)RI * p.H * nd;
         }
         __syncwarp();

@@ -248,3 +248,41 @@ def test_refusals(cuda_device):
         reorder_states([y], p.float())
     with pytest.raises(RuntimeError, match="not differentiable"):
         reorder_states([y.clone().requires_grad_(True)], p)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_selection_where_a_few_threads_hold_all_that_is_large(cuda_device, dtype):
+    """Columns laid out as the kernel's threads meet them: the first thirty of 256 hold what is large, so that the bound is low
+    and the M largest are found one after the other; and rows of four distinct values."""
+    from gla_jax_b200 import beam_select
+    N, K, V, M = 1, 2, 60000, 32
+    gen = torch.Generator(device=cuda_device).manual_seed(11)
+    x = torch.randn(N, K, V, generator=gen, device=cuda_device)
+    width = 8 if dtype == torch.bfloat16 else 4
+    few = (torch.arange(V, device=cuda_device) // width) % 256 < 30
+    logits = torch.where(few, x + 20, x).to(dtype)
+    scores = torch.tensor([[-1.0, -1.5]], device=cuda_device)
+    same(beam_select(logits, scores, M), selected(logits, scores, M))
+    coarse = torch.randint(0, 4, (3, 4, 20000), generator=gen, device=cuda_device).to(dtype)
+    flat = torch.tensor([[0.0, 0.0, -1.0, 0.0]], device=cuda_device).expand(3, 4).contiguous()
+    # (sums of exponentials of equal counts are not equal to the last bit: the beams are told apart by a whole unit)
+    flat = flat - torch.arange(4, device=cuda_device)
+    same(beam_select(coarse, flat, M), selected(coarse, flat, M))
+    # rising and falling runs: the second largest before, at and behind the largest
+    saw = ((torch.arange(20000, device=cuda_device) * 7919) % 251).float().expand(3, 4, 20000).contiguous().to(dtype)
+    same(beam_select(saw, flat, M), selected(saw, flat, M))
+
+
+@pytest.mark.parametrize("D", [32, 256])
+def test_decode_steps_of_thirty_two_beams(cuda_device, D):
+    from gla_jax_b200 import decode_step
+    gen = torch.Generator(device=cuda_device).manual_seed(D)
+    n = lambda *s: torch.randn(*s, generator=gen, device=cuda_device)  # noqa: E731
+    parents = torch.randint(0, 32, (2, 32), generator=gen, device=cuda_device, dtype=torch.int32)
+    row = (torch.arange(2, device=cuda_device)[:, None] * 32 + parents).flatten()
+    state, f = n(64, 2, D, D), -n(64, 2, D).abs()
+    v, k, q = (n(64, 2, D) for _ in range(3))
+    a, b = state.clone(), state[row].contiguous()
+    o1, o2 = decode_step(a, f, v, k, q, parents=parents), decode_step(b, f, v, k, q)
+    # (the order of up to 256 additions)
+    assert torch.equal(a, b) and ((o1 - o2).abs() <= 2.0 ** -16 * (q.abs()[..., None] * b.abs()).sum(-2)).all()

@@ -319,3 +319,64 @@ def test_refusals(cuda_device):
     with fwd.dual_level():
         with pytest.raises(NotImplementedError):
             f(h, g, fwd.make_dual(v, v), k, q)
+
+
+@pytest.mark.parametrize("hdtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("H,Hk,Dk,Dv", [(4, 2, 128, 64), (2, 2, 64, 128), (1, 1, 128, 128), (2, 1, 40, 200)])
+def test_gates_of_every_sharpness(cuda_device, H, Hk, Dk, Dv, hdtype):
+    """Stretches of 128 tokens whose gates sum up to 2, 100, 200 and 800: weights of whole chunks, of groups, of pairs."""
+    from gla_jax_b200 import chunk_decay_attention
+    T = 5 * 128 + 37
+    xs = make(cuda_device, 1, T, H, Hk, Dk, Dv, torch.bfloat16, hdtype, seed=Dk)
+    rate = torch.tensor([0.015, 0.8, 1.6, 6.0, 0.3, 0.02], device=cuda_device)
+    xs[1] = -rate.repeat_interleave(128)[:T, None] * (0.5 + torch.rand(1, T, H, device=cuda_device))
+    cots = [torch.randn_like(xs[0]), torch.randn_like(xs[2])]
+    got, grads = with_grads(chunk_decay_attention, xs, cots)
+    check(xs, cots, got, grads, torch.bfloat16, hdtype, (Dk, Dv))
+
+
+@pytest.mark.parametrize("shift", [5.0, -3.0])
+@pytest.mark.parametrize("D", [64, 128])
+def test_gradients_that_are_not_finite_stay_with_earlier_tokens(cuda_device, D, shift):
+    """A cotangent or a query that is not finite at token t reaches the gradients of tokens up to t of its own head."""
+    from gla_jax_b200 import chunk_decay_attention
+    xs = make(cuda_device, 1, 300, 2, 2, D, D, torch.bfloat16, torch.float32, shift=shift)
+    cots = [torch.randn_like(xs[0]), torch.randn_like(xs[2])]
+    _, want = with_grads(chunk_decay_attention, xs, cots)
+    mags = [xs[0].double().abs(), xs[1].double(), *(x.double().abs() for x in xs[2:])]
+    _, mag = with_grads(recurrence, mags, [c.double().abs() for c in cots])
+    for t in (37, 127, 128, 201):
+        for bad in (math.nan, math.inf):
+            for what in ("cotangent", "query"):
+                ys, cs = [x.clone() for x in xs], [c.clone() for c in cots]
+                (cs[1] if what == "cotangent" else ys[4])[0, t, 0, 5] = bad
+                _, got = with_grads(chunk_decay_attention, ys, cs)
+                for i in (1, 2, 3, 4):
+                    assert torch.equal(got[i][:, :, 1], want[i][:, :, 1]), (t, bad, what, i)
+                for i in (2, 3, 4):
+                    # terms summed in another order, each sum within F4 of them, and a rounding that may fall the other way
+                    a, b = got[i][:, t + 1:, 0].double(), want[i][:, t + 1:, 0].double()
+                    assert ((a - b).abs() <= 2 * F4 * mag[i][:, t + 1:, 0] + 2 * BF * b.abs()).all(), (t, bad, what, i)
+                assert torch.isfinite(got[1][:, t + 1:]).all()
+                if what == "query":
+                    assert torch.equal(got[4][:, :t], want[4][:, :t])            # (its own gradient does not read it)
+                    assert not torch.isfinite(got[3][0, t, 0]).all()
+                else:
+                    assert not torch.isfinite(got[2][0, t, 0]).all()
+
+
+def test_two_streams_at_once(cuda_device):
+    from gla_jax_b200 import chunk_decay_attention
+    xs = [make(cuda_device, 2, 1500, 3, 3, 128, 128, torch.bfloat16, torch.bfloat16, seed=s) for s in (1, 2)]
+    cots = [torch.randn_like(xs[0][0]), torch.randn_like(xs[0][2])]
+    want = [with_grads(chunk_decay_attention, x, cots) for x in xs]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None, None]
+    for _ in range(3):
+        for i in (0, 1):
+            streams[i].wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(streams[i]):
+                got[i] = with_grads(chunk_decay_attention, xs[i], cots)
+    torch.cuda.synchronize()
+    for (a, ga), (b, gb) in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip([*a, *ga], [*b, *gb]))
