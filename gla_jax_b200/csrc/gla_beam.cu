@@ -39,7 +39,7 @@ struct Step {
 constexpr int SNT = 128;
 
 // One row per block, its loads all in flight before the first is used.  Measured, 32 requests x 16 heads, 128 x 128, bf16: 13.5 us
-// with k and q read by every thread for itself -> 12.3 us through shared memory (the bytes at the copy rate: 10.3).
+// with k and q read by every thread for itself -> 12.8 us through shared memory (the bytes at the copy rate: 10.3).
 template <int W, int RPT>
 __global__ void __launch_bounds__(SNT) step_kernel(const Step p) {
   constexpr int CL = W / 4, RL = SNT / CL;
@@ -261,14 +261,16 @@ static int launch_reorder(cudaStream_t st, const Tensors& t) {
 // lowest (beam, token) first among equal ones.
 //
 // One pass over the logits: a block streams a part of a row, its threads keep the running maximum and sum of exponentials of
-// the softmax and their two largest logits.  Within a row the order of the totals is that of the logits, so that nothing but
+// the softmax and their two largest logits, as values: a minimum and two maxima a logit, of which the larger is the running
+// maximum as well; the tile that they came in is kept, and looked through at the end for where.  Within a row the order of the totals is that of the logits, so that nothing but
 // M candidates per part and its (maximum, sum) leaves the pass; a second kernel forms the totals of the candidates in 64 bits
 // and orders them.
 // The M-th largest of the threads' largest is a bound: M logits reach it.  Threads whose second reaches it too may have
 // more, which is one in a part on average and is looked up again; where few threads hold most of the large logits (nothing
 // that a model leaves, but a sorted row may), the M largest are found one after the other.
-// Measured, 64 x 8 rows of 128000 bf16 logits, M = 16: lists in shared memory that are cut as they grow 136 us, a sorted list
-// per warp 312 us, this 37 us (the bytes at the copy rate: 17.5).
+// Measured, 64 x 8 rows of 128000 bf16 logits, M = 16, the pass alone: lists in shared memory that are cut as they grow 136 us,
+// a sorted list per warp 312 us, the two largest with their places 79 us, this 57 us (the bytes at the copy rate: 17.5); both
+// kernels 73 us.  What bounds it: instructions, some ten a logit and an exponential, and the search at the end of each part.
 // A key is (order of the value, lowest index first), 0: none.
 typedef unsigned long long u64;
 __device__ __forceinline__ unsigned int order_of(float x) {

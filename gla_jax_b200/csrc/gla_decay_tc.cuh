@@ -7,8 +7,14 @@
 //
 // Why.  The same walk in mma.sync spends 14,000 instructions per 64 tokens, of which 1900 multiply: operand fragments, their
 // conversion and the accumulators' addressing are the work.  Here operands go from shared memory to the tensor cores as the
-// copies left them.  The work is the CUDA cores' still (scores, weights, output and state: about 5000 cycles a chunk at
-// 128 x 128, the products 2600), which is why everything else has a warp of its own.
+// copies left them.
+//
+// What bounds it (4 x 4096 tokens of 6 heads, 128 x 128, runs of 768 tokens: 48 us a walk with outputs, 22 us one of sums).  A
+// chunk takes 8700 cycles: the products 2600, during which their operands (128 x 16 and 16 x 128 in 64 cycles) take all that
+// shared memory gives, so that the workers' accesses wait; scores 1900, weights 1100, the check of the values 600, outputs and
+// their stores 3000, the state 600, in a row, since each needs the one before.  All bytes through shared memory are 4750
+// cycles, those from and to HBM 5500 with all SMs at work.  Measured besides: sixteen workers the same; eight for the scores
+// and eight for outputs and state side by side 49 to 57 us.
 //
 // Tiles: 128 rows x 64 columns of bf16, 128-byte rows, 16-byte pieces at piece ^ (row % 8) (tc_ptx.cuh); D columns are D / 64
 // of them.  A copy brings 128 rows whatever the sequence's length: rows past its end are another sequence's or beyond the
@@ -168,7 +174,7 @@ struct alignas(16) Gates {
   float dn[128], up[128];
   float low, reach;
 };
-constexpr float MILD = 100.f;          // of the 127 that float32 and bf16 exponents reach
+constexpr float MILD = 64.f;           // of the 127 that float32 and bf16 exponents reach: scores and sums below 2^63 stay finite
 __device__ __forceinline__ float4 gates_of(const Walk& p, int64_t t0, int nv, int h, int lane) {
   float g[4];
 #pragma unroll

@@ -380,3 +380,36 @@ def test_two_streams_at_once(cuda_device):
     torch.cuda.synchronize()
     for (a, ga), (b, gb) in zip(got, want):
         assert all(torch.equal(x, y) for x, y in zip([*a, *ga], [*b, *gb]))
+
+
+@pytest.mark.parametrize("rate", [0.02, 0.45, 2.0])
+def test_large_scores_under_decay(cuda_device, rate):
+    """Queries and keys of 2^14 each, so that scores reach 2^35: nothing between the inputs and the results may overflow."""
+    from gla_jax_b200 import chunk_decay_attention
+    xs = make(cuda_device, 1, 260, 2, 2, 128, 128, torch.bfloat16, torch.float32)
+    xs[1] = torch.full_like(xs[1], -rate)
+    xs[3], xs[4] = xs[3] * 2.0 ** 17, xs[4] * 2.0 ** 14
+    cots = [torch.randn_like(xs[0]), torch.randn_like(xs[2])]
+    got, grads = with_grads(chunk_decay_attention, xs, cots)
+    check(xs, cots, got, grads, torch.bfloat16, torch.float32, rate)
+
+
+def test_gradients_of_a_part_of_the_results(cuda_device):
+    """Either result alone, and any subset of the arguments, against all of them."""
+    from gla_jax_b200 import chunk_decay_attention
+    for dtype in (torch.bfloat16, torch.float32):
+        xs = make(cuda_device, 2, 150, 4, 2, 64, 64, dtype, dtype)
+        cots = [torch.randn_like(xs[0]), torch.randn_like(xs[2])]
+        zero = [torch.zeros_like(c) for c in cots]
+        for keep in (0, 1):
+            _, want = with_grads(chunk_decay_attention, xs, [c if i == keep else zero[i] for i, c in enumerate(cots)])
+            leaves = [x.clone().requires_grad_(True) for x in xs]
+            got = torch.autograd.grad(chunk_decay_attention(*leaves)[keep], leaves, cots[keep])
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+        _, want = with_grads(chunk_decay_attention, xs, cots)
+        for which in ((0,), (1,), (2,), (3,), (4,), (1, 4), (0, 2, 3)):
+            leaves = [x.clone().requires_grad_(i in which) for i, x in enumerate(xs)]
+            got = torch.autograd.grad(chunk_decay_attention(*leaves), [leaves[i] for i in which], cots)
+            # (without the gates' gradient the others need one plane of the state less)
+            for i, a in zip(which, got):
+                assert (a.double() - want[i].double()).norm() <= (2 * BF if dtype == torch.bfloat16 else 1e-5) * want[i].double().norm(), (which, i)
