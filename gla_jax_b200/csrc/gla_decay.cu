@@ -59,7 +59,10 @@ __global__ void __launch_bounds__(256) share_sum_kernel(const float* x, T* out, 
 }
 
 // dg_t = sum over i >= t of (q dq - k dk) + <S_T, dS_T>: a block per sequence and head, from the end, the running sum in
-// 64 bits
+// 64 bits.
+// The terms cancel over the sequence, while their errors (float32 products, some 2^-23 of each, cut off to one side) add up.
+// At the first token the sum has to be <S_0, dS_0>.  Where these states are float32, what it is off by is taken back, in
+// proportion to the magnitudes of the terms summed so far (2 x 250 tokens, 2 heads of 64: error 2.1e-6 of the norm without).
 struct Gate {
   const float *rq, *rk;             // [tiles][token][H]
   int nq, nk;
@@ -69,6 +72,7 @@ struct Gate {
   const float* S;                   // [s][h] final state, float32
   const void* dS;
   int dS_f32;
+  const float *S0, *dS0;            // [s][h], or NULL
   int64_t dd;
   float* dg;
 };
@@ -85,24 +89,48 @@ __global__ void __launch_bounds__(512) gate_grad_kernel(const Gate p) {
     if (s == p.nseq - 1)
       for (int64_t t = b + tid; t < p.T; t += 512) p.dg[t * p.H + h] = 0.f;
   }
-  double dot = 0.0;
-  for (int64_t e = tid; e < p.dd; e += 512) dot += (double)p.S[(s * p.H + h) * p.dd + e] * ld_any(p.dS, !p.dS_f32, (s * p.H + h) * p.dd + e);
+  const auto term = [&](int64_t t, double& size) {
+    double x = 0.0, y = 0.0;
+    for (int i = 0; i < p.nq; ++i) x += p.rq[(i * p.rows + t) * p.H + h];
+    for (int i = 0; i < p.nk; ++i) y += p.rk[(i * p.rows + t) * p.H + h];
+    size = fabs(x) + fabs(y);
+    return x - y;
+  };
+  const auto total = [&](double x) {
 #pragma unroll
-  for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-  if (lane == 0) part[warp] = dot;
-  __syncthreads();
-  if (tid == 0) {
-    double x = 0.0;
+    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    __syncthreads();
+    if (lane == 0) part[warp] = x;
+    __syncthreads();
+    x = 0.0;
     for (int w = 0; w < 16; ++w) x += part[w];
-    carry = x;
+    return x;
+  };
+  const int64_t at0 = (s * p.H + h) * p.dd;
+  double dot = 0.0, off = 0.0, all = 0.0;
+  for (int64_t e = tid; e < p.dd; e += 512) dot += (double)p.S[at0 + e] * ld_any(p.dS, !p.dS_f32, at0 + e);
+  dot = total(dot);
+  if (p.S0) {
+    for (int64_t e = tid; e < p.dd; e += 512) off -= (double)p.S0[at0 + e] * p.dS0[at0 + e];
+    for (int64_t t = a + tid; t < b; t += 512) {
+      double m;
+      off += term(t, m);
+      all += m;
+    }
+    off = total(off) + dot;
+    all = total(all);
   }
+  // per magnitude; none where something is not finite, which has to stay with its tokens
+  const double rate = p.S0 && all > 0.0 && isfinite(off / all) ? off / all : 0.0;
+  if (tid == 0) carry = dot;
   __syncthreads();
   for (int64_t end = b; end > a; end -= 512) {
     const int64_t t = end - 1 - tid;
     double x = 0.0;
     if (t >= a) {
-      for (int i = 0; i < p.nq; ++i) x += p.rq[(i * p.rows + t) * p.H + h];
-      for (int i = 0; i < p.nk; ++i) x -= p.rk[(i * p.rows + t) * p.H + h];
+      double m;
+      x = term(t, m);
+      if (rate != 0.0) x -= rate * m;
     }
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -367,6 +395,7 @@ int bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const flo
     w.rq = rq; w.rk = rk; w.nq = w.nk = (int)((d.Dk + 127) / 128);
     w.cu = cu; w.T = d.T; w.nseq = d.seqs(); w.rows = d.rows(); w.H = (int)d.H;
     w.S = (const float*)saved; w.dS = dhf; w.dS_f32 = d.hid_f32; w.dd = d.Dk * d.Dv; w.dg = dg;
+    if (d.hid_f32) { w.S0 = (const float*)h0; w.dS0 = (const float*)dh; }
     ProfScope ps("decay_gate_grad_kernel", st);
     gate_grad_kernel<<<dim3((unsigned)w.nseq, (unsigned)d.H), 512, 0, st>>>(w);
     GLA_CHECK_LAUNCH();
