@@ -53,6 +53,11 @@ Tensor bytes_or(const Tensor& like, size_t n, size_t least) {
   }
 }
 size_t size_of(const Tensor& t) { return t.defined() ? (size_t)t.numel() : 0; }
+// contiguous, and from a multiple of 16 bytes on, as tensor copies want it (a slice of a flat buffer may start anywhere)
+Tensor flat16(const Tensor& x) {
+  const Tensor y = x.contiguous();
+  return (uintptr_t)y.data_ptr() % 16 ? y.clone() : y;
+}
 Tensor f32(const Tensor& g) { return (g.scalar_type() == torch::kFloat32 ? g : g.to(torch::kFloat32)).contiguous(); }
 bool wants_any(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts) if (t->requires_grad()) return true;
@@ -346,7 +351,7 @@ struct DecayFn : torch::autograd::Function<DecayFn> {
                                const Tensor& cu0, std::vector<int64_t> dims) {
     const DecayDims d = DecayDims::of(dims);
     const Tensor cu = d.nseq ? cu0 : Tensor();
-    Tensor h = h0.contiguous(), g = f32(g0), v = v0.contiguous(), k = k0.contiguous(), q = q0.contiguous();
+    Tensor h = h0.contiguous(), g = f32(g0), v = flat16(v0), k = flat16(k0), q = flat16(q0);
     const bool gate = g0.requires_grad();
     variable_list r = run(d, h, g, v, k, q, cu, true);
     ctx->save_for_backward({h, g, v, k, q, r[2], cu});
@@ -362,7 +367,7 @@ struct DecayFn : torch::autograd::Function<DecayFn> {
     const variable_list s = ctx->get_saved_variables();
     const Tensor &h = s[0], &g = s[1], &v = s[2], &k = s[3], &q = s[4], &cu = s[6];
     const bool gate = a[10];
-    Tensor dhf = grad_or_zeros(grads[0], h), dout = grad_or_zeros(grads[1], v);
+    Tensor dhf = grad_or_zeros(grads[0], h), dout = flat16(grad_or_zeros(grads[1], v));
     Tensor dh = torch::empty_like(h), dg = gate ? torch::empty_like(g) : Tensor(), dv = torch::empty_like(v), dk = torch::empty_like(k),
            dq = torch::empty_like(q);
     const size_t n = gla_decay_workspace_bytes(d.B, d.T, d.H, d.Hk, d.Dk, d.Dv, d.dt, d.hdt, d.nseq, gate ? 3 : 2);
@@ -391,7 +396,7 @@ std::optional<std::tuple<Tensor, Tensor>> chunk_decay(const Tensor& h, const Ten
   }
   // (a node takes no undefined tensor)
   variable_list r = grad ? DecayFn::apply(h, g, v, k, q, d.nseq ? cu : v.detach(), d.list())
-                         : DecayFn::run(d, h.contiguous(), f32(g), v.contiguous(), k.contiguous(), q.contiguous(), cu, false);
+                         : DecayFn::run(d, h.contiguous(), f32(g), flat16(v), flat16(k), flat16(q), cu, false);
   return std::make_tuple(r[0], r[1]);
 }
 

@@ -413,3 +413,28 @@ def test_gradients_of_a_part_of_the_results(cuda_device):
             # (without the gates' gradient the others need one plane of the state less)
             for i, a in zip(which, got):
                 assert (a.double() - want[i].double()).norm() <= (2 * BF if dtype == torch.bfloat16 else 1e-5) * want[i].double().norm(), (which, i)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_arrays_that_start_anywhere(cuda_device, dtype):
+    """Contiguous arrays off 16 bytes, as slices of a flat buffer are, cotangents among them."""
+    from gla_jax_b200 import chunk_decay_attention, decay_attention_step
+
+    def moved(x):
+        flat = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)[1:]
+        return flat.copy_(x.flatten()).view(x.shape)
+
+    xs = make(cuda_device, 1, 300, 2, 1, 64, 64, dtype, dtype)
+    cots = [torch.randn_like(xs[0]), torch.randn_like(xs[2])]
+    got, want = [], []
+    for res, f in ((want, lambda x: x), (got, moved)):
+        leaves = [f(x).requires_grad_(True) for x in xs]
+        outs = chunk_decay_attention(*leaves)
+        res += [*outs, *torch.autograd.grad(outs, leaves, [f(c) for c in cots])]
+    for i, (a, b) in enumerate(zip(got, want)):
+        assert torch.equal(a, b), i
+    state = xs[0].float()
+    a, b = state.clone(), state.clone()
+    o1 = decay_attention_step(a, xs[1][:, 0], *(x[:, 0] for x in xs[2:]))
+    o2 = decay_attention_step(b, moved(xs[1][:, 0].contiguous()), *(moved(x[:, 0].contiguous()) for x in xs[2:]))
+    assert torch.equal(a, b) and torch.equal(o1, o2)
