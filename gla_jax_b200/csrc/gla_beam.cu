@@ -270,7 +270,7 @@ static int launch_reorder(cudaStream_t st, const Tensors& t) {
 // that a model leaves, but a sorted row may), the M largest are found one after the other.
 // Measured, 64 x 8 rows of 128000 bf16 logits, M = 16, the pass alone: lists in shared memory that are cut as they grow 136 us,
 // a sorted list per warp 312 us, the two largest with their places 79 us, this 57 us (the bytes at the copy rate: 17.5); both
-// kernels 73 us.  What bounds it: instructions, some ten a logit and an exponential, and the search at the end of each part.
+// kernels 70 us.  What bounds it: instructions, some ten a logit and an exponential, and the search at the end of each part.
 // A key is (order of the value, lowest index first), 0: none.
 typedef unsigned long long u64;
 __device__ __forceinline__ unsigned int order_of(float x) {

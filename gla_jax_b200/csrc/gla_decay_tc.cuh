@@ -146,13 +146,10 @@ inline int make_map_tokens(CUtensorMap* m, const void* ptr, int64_t rows, int64_
 // A wait that looks before it sleeps; bounded like mbar_wait, and after one that ran out nothing waits any more.
 __device__ __forceinline__ void wait_for(bool& ok, uint32_t bar, uint32_t parity) {
   if (!ok) return;
-  for (int it = 0; it < 1; ++it) {
-    uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
-                 : "=r"(done) : "r"(bar), "r"(parity) : "memory");
-    if (done) return;
-  }
-  ok = mbar_wait(bar, parity);
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+               : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  if (!done) ok = mbar_wait(bar, parity);
 }
 
 // Worker warps (eight: with sixteen, whose threads have half the registers, what does not fit them goes through an L1 that shared
