@@ -172,7 +172,7 @@ int ragged_tables(cudaStream_t st, int64_t nseq, const int* cu_host, void* mem, 
 unsigned int tc_state_read_wait_timeouts();
 unsigned int scan_read_wait_timeouts();
 unsigned int tc_state_read_bad_offsets();
-namespace decay { unsigned int read_all_bad_offsets(); unsigned int tc_walk_timeouts(); unsigned int tc_back_timeouts(); }
+namespace decay { unsigned int read_bad_offsets(); unsigned int tc_walk_timeouts(); unsigned int tc_back_timeouts(); }
 int tc_chunk_bwd(cudaStream_t st, int64_t B, int64_t T, int64_t H, int64_t D, int64_t C,
                  const float* g, const void* v, const void* k, const void* q, const void* saved,
                  const void* dhidden_final, const void* dout, void* dhidden_init, float* dg,

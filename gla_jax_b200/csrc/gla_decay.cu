@@ -6,6 +6,43 @@ namespace gla {
 namespace decay {
 namespace {
 
+// The offsets that the walks go by: the first is 0, none falls or leaves [0, T].  Runs are found by a search over them, which
+// only offsets that rise lead to every run once, and every row is some sequence's or behind the last.  One block, since the running
+// maximum needs all before it; 3 us of a packed call.
+__device__ unsigned int g_bad_offsets = 0;      // sequences whose offsets had to be changed
+__global__ void __launch_bounds__(256) offsets_kernel(const int* cu, int64_t nseq, int T, int* clean) {
+  __shared__ int part[8];
+  const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
+  int carry = 0;
+  grid_dep_wait();
+  grid_dep_launch();
+  for (int64_t i0 = 0; i0 <= nseq; i0 += 256) {
+    const int64_t i = i0 + tid;
+    int x = 0;
+    if (i > 0 && i <= nseq) {
+      const int a = cu[i - 1], b = cu[i];
+      if (a < 0 || b < a || b > T || (i == 1 && a != 0)) atomicAdd(&g_bad_offsets, 1u);
+      x = b < 0 ? 0 : b > T ? T : b;
+    }
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d && y > x) x = y;
+    }
+    if (lane == 31) part[warp] = x;
+    __syncthreads();
+    int all = carry;
+    for (int w = 0; w < 8; ++w) {
+      if (w < warp && part[w] > x) x = part[w];
+      if (part[w] > all) all = part[w];
+    }
+    if (carry > x) x = carry;
+    if (i <= nseq) clean[i] = x;
+    carry = all;
+    __syncthreads();
+  }
+}
+
 // The state that enters each run of a sequence, from what each run adds: four elements a thread, in place.  Four runs' sums
 // are requested before the first is used.
 __global__ void __launch_bounds__(128) entering_kernel(const Walk p) {
@@ -83,9 +120,7 @@ __global__ void __launch_bounds__(512) gate_grad_kernel(const Gate p) {
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   int64_t a = s * p.T, b = a + p.T;
   if (p.cu) {
-    const auto at = [&](int64_t i) { const int64_t x = p.cu[i]; return x < 0 ? (int64_t)0 : x > p.T ? p.T : x; };
-    a = at(s); b = at(s + 1);
-    if (b < a) b = a;
+    a = p.cu[s]; b = p.cu[s + 1];
     if (s == p.nseq - 1)
       for (int64_t t = b + tid; t < p.T; t += 512) p.dg[t * p.H + h] = 0.f;
   }
@@ -227,10 +262,12 @@ static int run_walk(cudaStream_t st, const Dims& d, int mode, const Walk& p, voi
 // ---- bf16, head sizes up to 128: the walks of gla_decay_tc.cuh and gla_decay_tcb.cuh ---------------------------------------------------------
 static bool fast(const Dims& d) { return d.bf && d.Dk <= 128 && d.Dv <= 128; }
 static size_t state_bytes(const Dims& d, int64_t n) { return align_up((size_t)(n * d.H * d.Dk * d.Dv) * 4, 256); }
-// saved: final states in float32 | states that enter the runs (where sequences are cut)
-size_t saved_bytes(const Dims& d) {
+// saved: final states in float32 | states that enter the runs (where sequences are cut) | offsets (where packed)
+static size_t saved_states(const Dims& d) {
   return state_bytes(d, d.seqs()) + (fast(d) && d.cut(d.seg(128)) ? state_bytes(d, d.slots(d.seg(128))) : 0);
 }
+static size_t offset_bytes(const Dims& d) { return d.nseq ? align_up((size_t)(d.nseq + 1) * 4, 256) : 0; }
+size_t saved_bytes(const Dims& d) { return saved_states(d) + offset_bytes(d); }
 static size_t fast_totals(const Dims& d) { return align_up((size_t)(d.slots(d.seg(128)) * d.H) * 8, 256); }
 static Walk fast_base(const Dims& d, const int* cu, const float* g, int64_t gt) {
   Walk p{};
@@ -246,7 +283,6 @@ static int fast_fwd(cudaStream_t st, const Dims& d, const int* cu, const void* h
   p.gq = p.gk = (int)(d.H / d.Hk); p.gv = 1;
   p.kd = (int)d.Dk; p.vd = (int)d.Dv;
   p.init = h0; p.ik = d.Dv; p.ic = 1;
-  p.count_bad = cu != nullptr;
   if (d.cut(p.seg)) {
     p.seg_total = (double*)ws;
     p.seg_state = (float*)(saved ? (char*)saved + state_bytes(d, d.seqs()) : (char*)ws + fast_totals(d));
@@ -307,19 +343,26 @@ static int fast_bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h
   return share > 1 ? share_sum(st, d, wide, dk) : GLA_OK;
 }
 
-size_t fwd_ws_bytes(const Dims& d, bool saved) {
+static size_t run_bytes(const Dims& d, bool saved) {
   if (!fast(d)) return d.seg_bytes(d.Dv);
   const int64_t s = d.seg(128);
   return d.cut(s) ? fast_totals(d) + (saved ? 0 : state_bytes(d, d.slots(s))) : 0;
 }
+size_t fwd_ws_bytes(const Dims& d, bool saved) { return run_bytes(d, saved) + (saved ? 0 : offset_bytes(d)); }
 int fwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const float* g, int64_t gt, const void* v, const void* k,
         const void* q, void* hf, void* out, void* saved, void* ws) {
+  if (cu) {
+    int* clean = (int*)(saved ? (char*)saved + saved_states(d) : (char*)ws + run_bytes(d, false));
+    ProfScope ps("decay_offsets_kernel", st);
+    GLA_LAUNCHED(launch_overlapped(offsets_kernel, dim3(1), dim3(256), 0, st, cu, d.nseq, (int)d.T, clean));
+    cu = clean;
+  }
   if (fast(d)) return fast_fwd(st, d, cu, h0, g, gt, v, k, q, hf, out, saved, ws);
   Walk p{};
   p.q = q; p.k = k; p.v = v;
   p.gq = p.gk = (int)(d.H / d.Hk); p.gv = 1;
   p.kd = (int)d.Dk; p.vd = (int)d.Dv;
-  p.g = g; p.gt = gt; p.cu = cu; p.count_bad = cu != nullptr;
+  p.g = g; p.gt = gt; p.cu = cu;
   p.init = h0; p.fin = hf; p.fin32 = (float*)saved; p.ik = d.Dv; p.ic = 1; p.init_f32 = p.fin_f32 = d.hid_f32;
   p.out = out; p.out_f32 = !d.bf;
   return run_walk(st, d, !d.bf ? M_FULL : d.hid_f32 ? M_STATE : M_ONE, p, ws, "decay_runs_kernel", "decay_walk_kernel");
@@ -355,6 +398,7 @@ static int share_sum(cudaStream_t st, const Dims& d, const float* x, void* out) 
 }
 int bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const float* g, int64_t gt, const void* v, const void* k,
         const void* q, const void* saved, const void* dhf, const void* dout, void* dh, float* dg, void* dv, void* dk, void* dq, void* ws) {
+  if (cu) cu = (const int*)((const char*)saved + saved_states(d));
   if (fast(d)) return fast_bwd(st, d, cu, h0, g, gt, v, k, q, saved, dhf, dout, dh, dg, dv, dk, dq, ws);
   size_t at[5];
   bwd_parts(d, dg != nullptr, at);
@@ -402,7 +446,11 @@ int bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const flo
   }
   return GLA_OK;
 }
-unsigned int read_all_bad_offsets() { return bad_offsets_one() + bad_offsets_state() + bad_offsets_fine() + bad_offsets_full() + bad_offsets_fast(); }
+unsigned int read_bad_offsets() {
+  unsigned int v = 0;
+  cudaMemcpyFromSymbol(&v, g_bad_offsets, sizeof(v));
+  return v;
+}
 
 // What the entry points share: sizes, types, alignment, workspace.
 static int check(const Dims& d, int dtype, int hidden_dtype, const int* cu) {

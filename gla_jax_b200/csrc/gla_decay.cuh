@@ -48,9 +48,9 @@ struct Walk {
   int H, kd, vd, vt;                // value heads, actual sizes, tiles of value columns
   const float* g;                   // [token][H] (gt = H), or [H] (gt = 0)
   int64_t gt;
-  const int* cu;                    // packed offsets, or NULL: sequence s holds tokens [s T, (s + 1) T)
+  const int* cu;                    // packed offsets (rising from 0 to at most T), or NULL: sequence s holds tokens [s T, (s + 1) T)
   int64_t T, nseq, seg, nslots;     // tokens of a sequence (of all, packed), sequences, tokens of a run, runs
-  int rev, count_bad;
+  int rev;
   const void* init;                 // entering state, element (k, c) of [s][h] at k ik + c ic
   void* fin;                        // leaving state, the same strides; may be NULL
   float* fin32;                     // the same in float32; may be NULL
@@ -73,10 +73,6 @@ struct Run {
   bool any, first, last;            // whether there is one; whether the sequence starts / ends with it
   int64_t zlo, zhi;                 // rows behind the last sequence, to be zeroed
 };
-__device__ __forceinline__ int64_t cu_at(const Walk& p, int64_t s) {
-  const int64_t x = p.cu[s];
-  return x < 0 ? 0 : x > p.T ? p.T : x;
-}
 __device__ __forceinline__ Run find_run(const Walk& p, int64_t slot) {
   Run r{};
   if (!p.cu) {
@@ -92,12 +88,11 @@ __device__ __forceinline__ Run find_run(const Walk& p, int64_t slot) {
   int64_t l = 0, u = p.nseq - 1;                 // the last s with s + cu[s] / seg <= slot
   while (l < u) {
     const int64_t m = (l + u + 1) / 2;
-    if (m + cu_at(p, m) / p.seg <= slot) l = m; else u = m - 1;
+    if (m + p.cu[m] / p.seg <= slot) l = m; else u = m - 1;
   }
   r.s = l;
-  r.a = cu_at(p, l);
-  r.b = cu_at(p, l + 1);
-  if (r.b < r.a) r.b = r.a;
+  r.a = p.cu[l];
+  r.b = p.cu[l + 1];
   const int64_t cell = slot - l;
   r.lo = cell * p.seg > r.a ? cell * p.seg : r.a;
   r.hi = (cell + 1) * p.seg < r.b ? (cell + 1) * p.seg : r.b;
@@ -116,7 +111,7 @@ __device__ __forceinline__ int64_t slot_of(const Walk& p, int64_t s, int64_t i, 
     n = (p.T + p.seg - 1) / p.seg;
     return s * n + i;
   }
-  const int64_t a = cu_at(p, s), b = cu_at(p, s + 1), c = a / p.seg;
+  const int64_t a = p.cu[s], b = p.cu[s + 1], c = a / p.seg;
   n = b > a ? (b - 1) / p.seg - c + 1 : 1;
   return s + c + i;
 }
@@ -210,14 +205,6 @@ template <int N> __device__ __forceinline__ float sum_planes(const uint8_t* at, 
   return x;
 }
 
-// Packed sequences whose offsets had to be clamped, counted by the forward (one counter per translation unit).
-static __device__ unsigned int g_bad_offsets = 0;
-static inline unsigned int read_bad_offsets() {
-  unsigned int v = 0;
-  cudaMemcpyFromSymbol(&v, g_bad_offsets, sizeof(v));
-  return v;
-}
-
 // Up to three walks side by side (blockIdx.z): those of a backward do not wait for one another.
 struct Walks { Walk w[3]; };
 template <int MODE, int KD, int NW, bool OUT>
@@ -239,10 +226,6 @@ __global__ void __launch_bounds__(NW * 32, KD <= 128 && MODE <= M_STATE ? 16 / N
       const int w = p.vd - cbase < Y::VT ? p.vd - cbase : Y::VT;
       for (int64_t i = tid; i < (run.zhi - run.zlo) * w; i += NT)
         st_any(p.out, !p.out_f32, ((run.zlo + i / w) * p.H + h) * p.vd + cbase + i % w, 0.f);
-    }
-    if (p.count_bad && run.any && run.first && blockIdx.y == 0 && tid == 0) {
-      const int64_t a = p.cu ? p.cu[run.s] : 0, b = p.cu ? p.cu[run.s + 1] : 0;
-      if (p.cu && (a < 0 || b < a || b > p.T || (run.s == 0 && a != 0))) atomicAdd(&g_bad_offsets, 1u);
     }
   }
   if (!run.any) return;
@@ -555,10 +538,6 @@ int walk_one(cudaStream_t, const Walks&, int n, bool out, const char* name);
 int walk_state(cudaStream_t, const Walks&, int n, bool out, const char* name);
 int walk_fine(cudaStream_t, const Walks&, int n, bool out, const char* name);
 int walk_full(cudaStream_t, const Walks&, int n, bool out, const char* name);
-unsigned int bad_offsets_one();
-unsigned int bad_offsets_state();
-unsigned int bad_offsets_fine();
-unsigned int bad_offsets_full();
 
 }  // namespace decay
 }  // namespace gla

@@ -22,7 +22,6 @@ struct Back {
 enum FastKind { F_ONE = 0, F_STATE = 1, F_FINE = 2, F_SUMS = 3, F_SUMS_STATE = 4 };
 int fast_walk(cudaStream_t, const Walk&, int kind, const char* name);
 int fast_back(cudaStream_t, const Back&, bool gate);
-unsigned int bad_offsets_fast();
 unsigned int tc_walk_timeouts();
 unsigned int tc_back_timeouts();
 

@@ -4,6 +4,5 @@
 namespace gla {
 namespace decay {
 int walk_state(cudaStream_t stream, const Walks& p, int n, bool out, const char* name) { return walk_mode<M_STATE>(stream, p, n, out, name); }
-unsigned int bad_offsets_state() { return read_bad_offsets(); }
 }  // namespace decay
 }  // namespace gla

@@ -21,7 +21,6 @@ int fast_walk(cudaStream_t stream, const Walk& p, int kind, const char* name) {
     default: return sizes<3, 1, false>(stream, p, name);
   }
 }
-unsigned int bad_offsets_fast() { return read_bad_offsets(); }
 unsigned int tc_walk_timeouts() { return read_wait_timeouts(); }
 
 }  // namespace decay

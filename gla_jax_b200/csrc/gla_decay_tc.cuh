@@ -370,15 +370,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
   grid_dep_wait();
   grid_dep_launch();
   const Run run = find_run(p, blockIdx.x);
-  if constexpr (OUT) {
+  if constexpr (OUT)
     if (run.zlo < run.zhi)
       for (int64_t i = tid; i < (run.zhi - run.zlo) * p.vd; i += TC_THREADS)
         st_any(p.out, !p.out_f32, ((run.zlo + i / p.vd) * p.H + h) * p.vd + i % p.vd, 0.f);
-    if (p.count_bad && run.any && run.first && blockIdx.y == 0 && tid == 0) {
-      const int64_t a = p.cu ? p.cu[run.s] : 0, b = p.cu ? p.cu[run.s + 1] : 0;
-      if (p.cu && (a < 0 || b < a || b > p.T || (run.s == 0 && a != 0))) atomicAdd(&g_bad_offsets, 1u);
-    }
-  }
   if (!run.any) return;
   // the run that the sequence is left through has nobody to pass its sum to
   if (!OUT && (p.rev ? run.first : run.last)) return;

@@ -513,12 +513,14 @@ GLA_API int gla_sp_combine2(void* stream, int64_t R, int64_t rank, int64_t BH, i
  *   log_decay (B, T, H) float32 with per_token != 0, else (H) float32.  -inf resets the state.
  *   nseq > 0: packed.  B = 1; the axis of T tokens holds nseq sequences, sequence s the tokens [cu_seqlens[s],
  *   cu_seqlens[s + 1]) (DEVICE, int32, rising from 0, any length, 0 included); hidden is (nseq, H, Dk, Dv).  Tokens behind the last
- *   sequence give zeros.  Offsets that fall or leave [0, T] are held inside and counted (gla_device_bad_offsets).
+ *   sequence give zeros.  Offsets that fall or leave [0, T] are held inside (the first is 0, each of the others at least the one
+ *   before it and at most T) and counted (gla_device_bad_offsets).
  * Dk and Dv multiples of 8 up to 256; any T > 0; H a multiple of Hk.  `dtype` is that of value, key, query, out and their
  * gradients; hidden_dtype that of hidden_init, hidden_final and their gradients: dtype or GLA_F32.  value, key, query, out and
  * gradients 16-byte aligned.
  * A forward that will be differentiated gets `saved` (gla_decay_saved_bytes), which the backward reads: final states in
- * float32 and, where few heads make the library cut sequences into runs, the states that enter the runs.  NULL otherwise.
+ * float32, where few heads make the library cut sequences into runs the states that enter the runs, and the offsets as they
+ * were used.  NULL otherwise.
  * bf16, head sizes up to 128: scores and the state as an operand are rounded to bf16 once, decayed values to two bf16
  * planes (three where hidden is float32; the state in two where dlog_decay is asked for); sums, states and decays in float32
  * and more.  bf16 beyond: one plane of each in the forward, two in the backward.  float32: three planes everywhere.

@@ -1,0 +1,70 @@
+"""Decay attention at the edges of what its documentation allows: offsets that fall, inputs that are not finite, many sequences."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_decay import ALL_FINE, BF, F4, make, recurrence, with_grads
+
+pytestmark = pytest.mark.gpu
+
+
+def packed(dev, nseq, T, H, Hk, Dk, Dv, dtype, seed=0):
+    xs = make(dev, 1, T, H, Hk, Dk, Dv, dtype, dtype, seed)
+    gen = torch.Generator(device=dev).manual_seed(seed + 1)
+    n = lambda *s: torch.randn(*s, generator=gen, device=dev).to(dtype)  # noqa: E731
+    xs = [n(nseq, H, Dk, Dv), *(x[0] for x in xs[1:])]
+    return xs, [n(nseq, H, Dk, Dv), n(T, H, Dv)]
+
+
+def held_inside(offsets, T):
+    """What offsets are taken as: rising from 0, none beyond T."""
+    out = [0]
+    for x in offsets[1:]:
+        out.append(max(out[-1], min(max(x, 0), T)))
+    return out
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float32, 64), (torch.bfloat16, 136)])
+@pytest.mark.parametrize("offsets", [[0, 1000, 10, 1200], [0, 600, 300, 1200], [0, 1100, 100, 300, 1200], [7, 9, 1200], [-3, 500, -1, 900],
+                                     [0, 5000, 3, 1100], [900, 800, 700], [0, 0, 2 ** 31 - 1, -2 ** 31, 1200]])
+def test_offsets_that_fall_or_leave_the_axis(cuda_device, offsets, dtype, D):
+    """1200 tokens of 2 heads are cut into runs: every row, state and gradient is what rising offsets give, and the call is reported."""
+    from gla_jax_b200 import check_device, chunk_decay_attention_packed
+    from gla_jax_b200._lib import GlaError
+    T, nseq = 1200, len(offsets) - 1
+    xs, cots = packed(cuda_device, nseq, T, 2, 1, D, D, dtype)
+    bad, good = (torch.tensor(c, dtype=torch.int32, device=cuda_device) for c in (offsets, held_inside(offsets, T)))
+    check_device()
+    want, gw = with_grads(lambda *a: chunk_decay_attention_packed(*a, good), xs, cots)
+    check_device()
+    got, gg = with_grads(lambda *a: chunk_decay_attention_packed(*a, bad), xs, cots)
+    with pytest.raises(GlaError, match="sequence"):
+        check_device()
+    for i, (a, b) in enumerate(zip([*got, *gg], [*want, *gw])):
+        assert torch.equal(a, b), i
+    end = int(good[-1])
+    assert (got[1][end:] == 0).all() and all((gg[i][end:] == 0).all() for i in (1, 2, 3, 4))
+    with torch.no_grad():
+        hf, out = chunk_decay_attention_packed(*xs, bad)
+    assert torch.equal(hf, want[0]) and torch.equal(out, want[1])
+    with pytest.raises(GlaError):
+        check_device()
+
+
+def test_offsets_of_many_sequences(cuda_device):
+    """More offsets than a pass over them takes at once, one in three falling."""
+    from gla_jax_b200 import check_device, chunk_decay_attention_packed
+    from gla_jax_b200._lib import GlaError
+    T, nseq = 3000, 700
+    gen = torch.Generator().manual_seed(2)
+    cu = torch.randint(0, T + 1, (nseq - 1,), generator=gen).sort().values.tolist()
+    offsets = [0, *(x - 40 * (i % 3 == 0) for i, x in enumerate(cu)), T]
+    xs, cots = packed(cuda_device, nseq, T, 1, 1, 32, 32, torch.bfloat16)
+    bad, good = (torch.tensor(c, dtype=torch.int32, device=cuda_device) for c in (offsets, held_inside(offsets, T)))
+    want, gw = with_grads(lambda *a: chunk_decay_attention_packed(*a, good), xs, cots)
+    check_device()
+    got, gg = with_grads(lambda *a: chunk_decay_attention_packed(*a, bad), xs, cots)
+    with pytest.raises(GlaError):
+        check_device()
+    assert all(torch.equal(a, b) for a, b in zip([*got, *gg], [*want, *gw]))
