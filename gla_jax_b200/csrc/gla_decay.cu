@@ -100,6 +100,8 @@ __global__ void __launch_bounds__(256) share_sum_kernel(const float* x, T* out, 
 // The terms cancel over the sequence, while their errors (float32 products, some 2^-23 of each, cut off to one side) add up.
 // At the first token the sum has to be <S_0, dS_0>.  Where these states are float32, what it is off by is taken back, in
 // proportion to the magnitudes of the terms summed so far (2 x 250 tokens, 2 heads of 64: error 2.1e-6 of the norm without).
+// A value or key that is not finite makes the sum not finite from there back, where dg reads neither: those tokens are summed
+// from the other end, dg_t = <S_0, dS_0> - sum over i < t.
 struct Gate {
   const float *rq, *rk;             // [tiles][token][H]
   int nq, nk;
@@ -107,9 +109,8 @@ struct Gate {
   int64_t T, nseq, rows;
   int H;
   const float* S;                   // [s][h] final state, float32
-  const void* dS;
-  int dS_f32;
-  const float *S0, *dS0;            // [s][h], or NULL
+  const void *dS, *S0, *dS0;        // [s][h]: gradient of it, first state, gradient of that
+  int state_f32;                    // their type
   int64_t dd;
   float* dg;
 };
@@ -143,10 +144,15 @@ __global__ void __launch_bounds__(512) gate_grad_kernel(const Gate p) {
   };
   const int64_t at0 = (s * p.H + h) * p.dd;
   double dot = 0.0, off = 0.0, all = 0.0;
-  for (int64_t e = tid; e < p.dd; e += 512) dot += (double)p.S[at0 + e] * ld_any(p.dS, !p.dS_f32, at0 + e);
+  for (int64_t e = tid; e < p.dd; e += 512) dot += (double)p.S[at0 + e] * ld_any(p.dS, !p.state_f32, at0 + e);
   dot = total(dot);
-  if (p.S0) {
-    for (int64_t e = tid; e < p.dd; e += 512) off -= (double)p.S0[at0 + e] * p.dS0[at0 + e];
+  const auto first = [&]() {
+    double x = 0.0;
+    for (int64_t e = tid; e < p.dd; e += 512) x += (double)ld_any(p.S0, !p.state_f32, at0 + e) * ld_any(p.dS0, !p.state_f32, at0 + e);
+    return x;
+  };
+  if (p.state_f32) {
+    off = -first();
     for (int64_t t = a + tid; t < b; t += 512) {
       double m;
       off += term(t, m);
@@ -156,7 +162,7 @@ __global__ void __launch_bounds__(512) gate_grad_kernel(const Gate p) {
     all = total(all);
   }
   // per magnitude; none where something is not finite, which has to stay with its tokens
-  const double rate = p.S0 && all > 0.0 && isfinite(off / all) ? off / all : 0.0;
+  const double rate = p.state_f32 && all > 0.0 && isfinite(off / all) ? off / all : 0.0;
   if (tid == 0) carry = dot;
   __syncthreads();
   for (int64_t end = b; end > a; end -= 512) {
@@ -180,6 +186,27 @@ __global__ void __launch_bounds__(512) gate_grad_kernel(const Gate p) {
     if (t >= a) p.dg[t * p.H + h] = (float)x;
     __syncthreads();
     if (tid == 511) carry = x;
+    __syncthreads();
+  }
+  if (isfinite(carry)) return;
+  double before = total(first());
+  for (int64_t t0 = a; t0 < b; t0 += 512) {
+    const int64_t t = t0 + tid;
+    double m, x = t < b ? term(t, m) : 0.0;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const double y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    const double prev = __shfl_up_sync(0xffffffffu, x, 1);
+    if (lane == 31) part[warp] = x;
+    __syncthreads();
+    double y = before - (lane ? prev : 0.0);
+    for (int w = 0; w < 16; ++w) {
+      if (w < warp) y -= part[w];
+      before -= part[w];
+    }
+    if (t < b && !isfinite(p.dg[t * p.H + h])) p.dg[t * p.H + h] = (float)y;
     __syncthreads();
   }
 }
@@ -337,7 +364,7 @@ static int fast_bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h
   }
   b.w.q = q; b.w.k = k; b.w.v = v; b.w.gq = b.w.gk = share; b.w.gv = 1;
   b.w.fin = dh;
-  b.dout = dout; b.a = a; b.S_runs = runs; b.S_end = (const float*)saved;
+  b.dout = dout; b.a = a; b.S_runs = runs; b.S_end = (const float*)saved; b.S_init = h0;
   b.dk = share > 1 ? (void*)wide : dk; b.dk_f32 = share > 1; b.dv = dv; b.dg = dg;
   GLA_TRY(fast_back(st, b, dg != nullptr));
   return share > 1 ? share_sum(st, d, wide, dk) : GLA_OK;
@@ -438,8 +465,7 @@ int bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const flo
     Gate w{};
     w.rq = rq; w.rk = rk; w.nq = w.nk = (int)((d.Dk + 127) / 128);
     w.cu = cu; w.T = d.T; w.nseq = d.seqs(); w.rows = d.rows(); w.H = (int)d.H;
-    w.S = (const float*)saved; w.dS = dhf; w.dS_f32 = d.hid_f32; w.dd = d.Dk * d.Dv; w.dg = dg;
-    if (d.hid_f32) { w.S0 = (const float*)h0; w.dS0 = (const float*)dh; }
+    w.S = (const float*)saved; w.dS = dhf; w.S0 = h0; w.dS0 = dh; w.state_f32 = d.hid_f32; w.dd = d.Dk * d.Dv; w.dg = dg;
     ProfScope ps("decay_gate_grad_kernel", st);
     gate_grad_kernel<<<dim3((unsigned)w.nseq, (unsigned)d.H), 512, 0, st>>>(w);
     GLA_CHECK_LAUNCH();

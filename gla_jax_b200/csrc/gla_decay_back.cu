@@ -13,7 +13,7 @@ static int back_gate(cudaStream_t stream, TcBack& b, const void* dout, bool gate
 int fast_back(cudaStream_t stream, const Back& x, bool gate) {
   TcBack b;
   b.w = x.w;
-  b.a = x.a; b.S_runs = x.S_runs; b.S_end = x.S_end; b.dk = x.dk; b.dv = x.dv; b.dk_f32 = x.dk_f32; b.dg = x.dg;
+  b.a = x.a; b.S_runs = x.S_runs; b.S_end = x.S_end; b.S_init = x.S_init; b.dk = x.dk; b.dv = x.dv; b.dk_f32 = x.dk_f32; b.dg = x.dg;
   if (b.w.kd <= 64) return b.w.vd <= 64 ? back_gate<64, 64>(stream, b, x.dout, gate) : back_gate<64, 128>(stream, b, x.dout, gate);
   return b.w.vd <= 64 ? back_gate<128, 64>(stream, b, x.dout, gate) : back_gate<128, 128>(stream, b, x.dout, gate);
 }

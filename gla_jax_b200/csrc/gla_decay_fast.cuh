@@ -13,6 +13,7 @@ struct Back {
   const void* dout;
   const float* a;                          // [WALK_COLS][token][H], with gates: what the walk for dq leaves in rdot
   const float *S_runs, *S_end;             // entering states of the runs [slot][H][vd][kd] (NULL: one run each), final states
+  const void* S_init;                      // the sequences' first states, in the type of w.init
   void *dk, *dv;
   int dk_f32;
   float* dg;

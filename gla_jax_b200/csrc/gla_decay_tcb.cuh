@@ -11,7 +11,9 @@
 // products are done by then.
 //   dg_t = sum over i >= t of (r_i + a_i - c_i - b_i) + <the state that leaves the run, its gradient>
 //   M_ji = P_ji DT_ji in float32, r its column and c its row sums;  a = q . (dq from before the chunk), b = k . (dk from behind it)
-// with the products of dS in two planes where this is asked for: the sum is over the whole run and its terms cancel.
+// with the products of dS in two planes where this is asked for: the sum is over the whole run and its terms cancel.  A value or key
+// that is not finite makes it not finite from there back, where dg reads neither: those tokens are summed from the other end,
+//   dg_t = <the state that enters the run, its gradient> - sum over i < t of (r_i + a_i - c_i - b_i)
 // Bounded as the forward is: 4 x 4096 tokens of 6 heads, 128 x 128: 78 us; 8191 packed tokens, 16 heads of 128 x 64 with the
 // gates' gradient: 180 us.
 #pragma once
@@ -25,6 +27,7 @@ struct TcBack {
   Walk w;                                  // k, q, v; H, sizes, gates, runs; seg_state: gradients that enter each run backwards
   const float* a;                          // [TC_COLS][token][H], with gates
   const float *S_runs, *S_end;             // entering states of the runs [slot][H][vd][kd], final states
+  const void* S_init;                      // the sequences' first states
   void *dk, *dv;
   int dk_f32;
   float* dg;
@@ -45,7 +48,7 @@ struct BTLay {
   static_assert(DK == DV || 256 * (DK > DV ? DK : DV) >= 4096 * TC_WORK, "a place per warp");
   static_assert(S0 % 1024 == 0 && STG % 1024 == 0, "tiles");
 };
-enum TbBar { C_LOAD = 0, C_ST = 1, C_I = 2, C_DV = 3, C_U = 4, C_P = 5, C_W = 6, C_S = 7, C_G = 8, C_GFREE = 10, C_E = 12, C_COUNT = 14, C_TMEM = 14, C_ODD = 15 };
+enum TbBar { C_LOAD = 0, C_ST = 1, C_I = 2, C_DV = 3, C_U = 4, C_P = 5, C_W = 6, C_S = 7, C_G = 8, C_GFREE = 10, C_E = 12, C_COUNT = 14, C_TMEM = 14, C_ODD = 15, C_BACK = 16 };
 
 // o (a row of tensor memory, D / TC_COLS columns from the worker's first) += sum over i >= row of P_i V_i, for a chunk in which V holds
 // something that is not finite (see masked_sums)
@@ -282,6 +285,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
   } else if (warp == TC_WORK + 2) {
     // ================= gates, and their gradient a step behind =================
     double carry = 0.0;
+    int back = 0;                                // tokens from the run's first on whose sum is not finite; their dg holds the term
     if (GATE)
       for (int w = 0; w < TC_WORK; ++w) carry += red[w];
     const auto gradient = [&](int i) {
@@ -290,6 +294,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
       const float* s = sums + (i & 1) * 1536;
       wait_for(ok, bar(C_E + (i & 1)), (i >> 1) & 1);
       double e[4], sum = 0.0;
+      float own[4];
 #pragma unroll
       for (int u = 3; u >= 0; --u) {
         const int t = 4 * lane + u;
@@ -303,6 +308,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
         }
         sum += x;
         e[u] = sum;
+        own[u] = (float)x;
       }
       double inc = sum;
 #pragma unroll
@@ -314,7 +320,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
       const double next = __shfl_down_sync(0xffffffffu, inc, 1), behind = carry + (lane < 31 ? next : 0.0);
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (4 * lane + u < nv) a.dg[(t0 + 4 * lane + u) * p.H + h] = (float)(behind + e[u]);
+        if (4 * lane + u < nv) {
+          const double y = behind + e[u];
+          a.dg[(t0 + 4 * lane + u) * p.H + h] = isfinite(y) ? (float)y : own[u];
+          if (!isfinite(y)) back = max(back, (int)(t0 - r0) + 4 * lane + u + 1);
+        }
       carry += __shfl_sync(0xffffffffu, inc, 0);
     };
     float4 g = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -329,6 +339,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
     }
     if (GATE)
       for (int i = chunks >= 2 ? chunks - 2 : 0; i < chunks; ++i) gradient(i);
+    if (GATE) {
+      back = __reduce_max_sync(0xffffffffu, back);
+      if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(bar(C_BACK)), "r"(back) : "memory");
+    }
   } else {
     // ================= workers =================
     const auto put_state = [&]() {
@@ -547,6 +561,43 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
   if (!ok && lane == 0) atomicAdd(&g_wait_timeouts, 1u);
   tc_fence_before();
   __syncthreads();
+  if constexpr (GATE) {
+    int back;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(back) : "r"(bar(C_BACK)) : "memory");
+    if (back) {
+      // from the run's first token on, with the state that enters the run (S is its gradient)
+      if (warp < TC_WORK) {
+        double dot = 0.0;
+        const int64_t at = sh * dd + (int64_t)row * p.vd + HV * qt;
+        const float* y = a.S_runs + slot_h * dd + row + (int64_t)HV * qt * p.kd;
+#pragma unroll
+        for (int j = 0; j < HV; ++j)
+          if (j < cols) dot += (double)S[j] * (run.first ? ld_any(a.S_init, !p.init_f32, at + j) : y[(int64_t)j * p.kd]);
+#pragma unroll
+        for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+        if (lane == 0) red[warp] = dot;
+      }
+      __syncthreads();
+      if (warp == TC_WORK + 2) {
+        double dot = 0.0;
+        for (int w = 0; w < TC_WORK; ++w) dot += red[w];
+        for (int t0 = 0; t0 < back; t0 += 32) {
+          float* at = a.dg + (r0 + t0 + lane) * p.H + h;
+          const double x = t0 + lane < back ? (double)*at : 0.0;
+          double inc = x;
+#pragma unroll
+          for (int d = 1; d < 32; d <<= 1) {
+            const double y = __shfl_up_sync(0xffffffffu, inc, d);
+            if (lane >= d) inc += y;
+          }
+          // (what is before this lane's token; not inc - x, which is lost where x is not finite)
+          const double prev = __shfl_up_sync(0xffffffffu, inc, 1);
+          if (t0 + lane < back) *at = (float)(dot - (lane ? prev : 0.0));
+          dot -= __shfl_sync(0xffffffffu, inc, 31);
+        }
+      }
+    }
+  }
   if (warp == 0) tmem_dealloc(tmem, 512);
 }
 

@@ -68,3 +68,37 @@ def test_offsets_of_many_sequences(cuda_device):
     with pytest.raises(GlaError):
         check_device()
     assert all(torch.equal(a, b) for a, b in zip([*got, *gg], [*want, *gw]))
+
+
+@pytest.mark.parametrize("dtype,hdtype,D", [(torch.bfloat16, torch.float32, 64), (torch.bfloat16, torch.bfloat16, 128), (torch.bfloat16, torch.bfloat16, 136),
+                                            (torch.float32, torch.float32, 64)])
+@pytest.mark.parametrize("T", [300, 900])
+def test_gates_gradient_before_a_value_or_key_that_is_not_finite(cuda_device, T, dtype, hdtype, D):
+    """dg_s = <exp(g_s) S_{s-1}, dS_s> reads values and keys before s only.  900 tokens of 2 heads are cut into runs.
+
+    The gradient may be summed from either end, so the unit is everything that either sum adds up: the terms of all tokens, and
+    the products of states and their gradients at both ends (which the states' own type rounds)."""
+    from gla_jax_b200 import chunk_decay_attention
+    xs = make(cuda_device, 1, T, 2, 1, D, D, dtype, hdtype, shift=4.0)
+    gen = torch.Generator(device=cuda_device).manual_seed(4)
+    cots = [torch.randn(x.shape, generator=gen, device=cuda_device).to(x.dtype) for x in (xs[0], xs[2])]
+    _, want = with_grads(recurrence, [x.double() for x in xs], [c.double() for c in cots])
+    mags = [xs[0].double().abs(), xs[1].double(), *(x.double().abs() for x in xs[2:])]
+    (mh, _), mag = with_grads(recurrence, mags, [c.double().abs() for c in cots])
+    per_head = lambda x, d: (x * d).sum(-1).repeat_interleave(2, 2)  # noqa: E731
+    terms = (per_head(mags[4], mag[4]) + per_head(mags[3], mag[3])).sum(1)
+    ends = (mh * cots[0].double().abs()).sum((-1, -2)) + (mags[0] * mag[0]).sum((-1, -2))
+    fine = F4 if dtype == torch.float32 else ALL_FINE + F4
+    lim = 2 * (fine * (terms + ends) + (F4 if hdtype == torch.float32 else BF) * ends)          # (1, H)
+    for t in (0, 5, 130, T - 1):
+        for what in (2, 3):
+            for bad in (math.nan, math.inf):
+                ys = [x.clone() for x in xs]
+                ys[what][0, t, 0, 3] = bad
+                _, got = with_grads(chunk_decay_attention, ys, cots)
+                heads = 1 if what == 2 else 2                    # (the key is shared by both value heads)
+                near = (got[1][:, : t + 1].double() - want[1][:, : t + 1]).abs()
+                assert (near <= lim).all(), (t, what, bad, near.max().item(), lim.min().item())
+                assert not torch.isfinite(got[1][:, t + 1:, :heads]).any(), (t, what, bad)
+                if what == 2:
+                    assert ((got[1][:, :, 1].double() - want[1][:, :, 1]).abs() <= lim[:, 1]).all()
