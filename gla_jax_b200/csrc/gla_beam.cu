@@ -260,11 +260,14 @@ static int launch_reorder(cudaStream_t st, const Tensors& t) {
 // For each request the M best of its K V continuations by score[k] + log_softmax(logits[k])[v], the largest first, the
 // lowest (beam, token) first among equal ones.
 //
-// One pass over the logits: a block streams a part of a row, its threads keep the running maximum and sum of exponentials of
+// Within a row the totals never fall as the logits rise, so that nothing but M candidates per part and its (maximum, sum) leaves the
+// pass; a second kernel forms the totals of the candidates in 64 bits and orders them.  Totals of unequal logits can be equal (a
+// score like -1e18 leaves none of a logit's digits), and among those it is the lowest place that counts, not the larger logit:
+// where the last candidate of a part meets the M-th total, and a logit next to its own would too, that row is read again.
+//
+// A block streams a part of a row, its threads keep the running maximum and sum of exponentials of
 // the softmax and their two largest logits, as values: a minimum and two maxima a logit, of which the larger is the running
-// maximum as well; the tile that they came in is kept, and looked through at the end for where.  Within a row the order of the totals is that of the logits, so that nothing but
-// M candidates per part and its (maximum, sum) leaves the pass; a second kernel forms the totals of the candidates in 64 bits
-// and orders them.
+// maximum as well; the tile that they came in is kept, and looked through at the end for where.
 // The M-th largest of the threads' largest is a bound: M logits reach it.  Threads whose second reaches it too may have
 // more, which is one in a part on average and is looked up again; where few threads hold most of the large logits (nothing
 // that a model leaves, but a sorted row may), the M largest are found one after the other.
@@ -553,9 +556,13 @@ constexpr int SCAP = 1024, BNT = 512;   // candidates of a request: K parts M, a
 __global__ void __launch_bounds__(BNT) select_beams_kernel(const Select p) {
   __shared__ u64 key[SCAP], where[SCAP];  // total's order; (beam, token)
   __shared__ double base[32][2];          // per beam: maximum, log of the sum
+  __shared__ u64 cut_;                    // the M-th total
+  __shared__ unsigned int doubt_;         // beams to be read again
+  __shared__ int above, hits[BNT / 32];
   const int tid = threadIdx.x, K = p.K, M = p.M, per = p.parts * M, n = K * per;
   const int64_t req = blockIdx.x;
   grid_dep_wait();
+  if (tid == 0) { doubt_ = 0; above = 0; }
   for (int k = tid / 32; k < K; k += BNT / 32) {
     const double2* sm = p.sums + (req * K + k) * p.parts;
     double top = -CUDART_INF, s = 0.0;
@@ -570,18 +577,16 @@ __global__ void __launch_bounds__(BNT) select_beams_kernel(const Select p) {
   }
   __syncthreads();
   const u64* cand = p.cand + req * n;
+  const auto total = [&](int k, float x) {
+    double t = -CUDART_INF;
+    if (x > -CUDART_INF_F && base[k][0] > -CUDART_INF) t = (double)p.scores[req * K + k] + (((double)x - base[k][0]) - base[k][1]);
+    if (!(t > -CUDART_INF)) t = -CUDART_INF;
+    return order_of(t);
+  };
   for (int i = tid; i < n; i += BNT) {
     const u64 c = cand[i];
     const int k = i / per;
-    u64 o = 0;
-    if (c) {
-      double t = -CUDART_INF;
-      const float x = value_of((unsigned int)(c >> 32));
-      if (x > -CUDART_INF_F && base[k][0] > -CUDART_INF) t = (double)p.scores[req * K + k] + (((double)x - base[k][0]) - base[k][1]);
-      if (!(t > -CUDART_INF)) t = -CUDART_INF;
-      o = order_of(t);
-    }
-    key[i] = o;
+    key[i] = c ? total(k, value_of((unsigned int)(c >> 32))) : 0;
     where[i] = ((u64)k << 32) | (unsigned int)~(unsigned int)c;
   }
   __syncthreads();
@@ -601,6 +606,50 @@ __global__ void __launch_bounds__(BNT) select_beams_kernel(const Select p) {
       p.out_scores[req * M + rank] = (float)__longlong_as_double(u);
       p.tokens[req * M + rank] = (long long)(at & 0xffffffffu);
       p.parents[req * M + rank] = (int)(at >> 32);
+      if (rank == M - 1) cut_ = x;
+    }
+  }
+  __syncthreads();
+  const u64 cut = cut_;
+  for (int i = tid; i < K * p.parts; i += BNT) {
+    const int k = i / p.parts, last = i * M + M - 1;
+    // (a beam that has ended or has no score left its tokens in order)
+    if (key[last] != cut || !(p.scores[req * K + k] > -CUDART_INF_F) || (p.finished && p.finished[req * K + k]) || !(base[k][0] > -CUDART_INF)) continue;
+    const unsigned int o = (unsigned int)(cand[last] >> 32), step = p.bf ? 0x10000u : 1u;
+    const float x = value_of(o), up = clean(value_of(o + step));
+    float down = value_of(o - step);
+    if (down == x) down = value_of(o - 2 * step);                       // (-0)
+    if (x > -CUDART_INF_F && ((up != x && total(k, up) == cut) || total(k, down) == cut)) atomicOr(&doubt_, 1u << k);
+  }
+  __syncthreads();
+  const unsigned int doubt = doubt_;
+  if (!doubt) return;
+  for (int i = tid; i < n; i += BNT) if (key[i] > cut) atomicAdd(&above, 1);
+  __syncthreads();
+  // the first of those that are equal to the M-th, by beam and token: from the logits where in doubt, else from the candidates
+  const int warp = tid / 32;
+  int at = above;
+  for (int k = 0; k < K && at < M; ++k) {
+    const bool again = (doubt >> k) & 1u;
+    const int64_t row = (req * K + k) * p.V, len = again ? p.V : per;
+    for (int64_t e0 = 0; e0 < len && at < M; e0 += BNT) {
+      const int64_t e = e0 + tid;
+      bool hit = false;
+      if (e < len)
+        hit = (again ? total(k, clean(p.bf ? __bfloat162float(((const bf16*)p.logits)[row + e]) : ((const float*)p.logits)[row + e])) : key[k * per + e]) == cut;
+      const unsigned int mask = __ballot_sync(0xffffffffu, hit);
+      if (tid % 32 == 0) hits[warp] = __popc(mask);
+      __syncthreads();
+      int place = at + __popc(mask & ((1u << tid % 32) - 1u));
+      for (int w = 0; w < BNT / 32; ++w) {
+        if (w < warp) place += hits[w];
+        at += hits[w];
+      }
+      if (hit && place < M) {
+        p.tokens[req * M + place] = again ? (long long)e : (long long)(where[k * per + e] & 0xffffffffu);
+        p.parents[req * M + place] = k;
+      }
+      __syncthreads();
     }
   }
 }

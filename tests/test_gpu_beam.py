@@ -286,3 +286,31 @@ def test_decode_steps_of_thirty_two_beams(cuda_device, D):
     o1, o2 = decode_step(a, f, v, k, q, parents=parents), decode_step(b, f, v, k, q)
     # (the order of up to 256 additions)
     assert torch.equal(a, b) and ((o1 - o2).abs() <= 2.0 ** -16 * (q.abs()[..., None] * b.abs()).sum(-2)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,K,V,M", [(2, 3, 700, 12), (1, 4, 40000, 16), (1, 32, 9000, 32), (3, 1, 5, 4)])
+def test_equal_totals_of_unequal_logits(cuda_device, N, K, V, M, dtype):
+    """The lowest (beam, token) comes first whatever the logits: where scores leave none of a logit's digits (-1e18 and the type's
+    lowest, the usual masks of a score), and where logits differ by less than a total resolves."""
+    from gla_jax_b200 import beam_select
+    gen = torch.Generator(device=cuda_device).manual_seed(V)
+    x = (3 * torch.randn(N, K, V, generator=gen, device=cuda_device)).to(dtype)
+    x[..., V // 3] = -math.inf
+    for low in (-1e18, torch.finfo(torch.float32).min):
+        s = torch.full((N, K), low, device=cuda_device)
+        same(beam_select(x, s, M), selected(x, s, M))
+        s[:, 0] = 0.0
+        few = x.clone()
+        few[:, 0, 3:] = -math.inf                           # three tokens of the one beam that counts, the rest from the others
+        same(beam_select(few, s, M), selected(few, s, M))
+        fin = torch.zeros(N, K, dtype=torch.bool, device=cuda_device)
+        fin[:, -1] = True
+        same(beam_select(few, s, M, finished=fin, pad_token=2), selected(few, s, M, fin, 2))
+    tiny = (torch.arange(V, device=cuda_device) * 1e-25).expand(N, K, V).contiguous().to(dtype)
+    s = -torch.arange(K, device=cuda_device).float().expand(N, K).contiguous()
+    same(beam_select(tiny, s, M), selected(tiny, s, M))
+    # zeros among larger and smaller ones
+    some = torch.where(torch.rand(N, K, V, generator=gen, device=cuda_device) < 0.001, x.float().abs(), -x.float().abs().nan_to_num(posinf=1.0)).to(dtype)
+    some[torch.rand(N, K, V, generator=gen, device=cuda_device) < 0.5] = 0.0
+    same(beam_select(some, s, M), selected(some, s, M))
