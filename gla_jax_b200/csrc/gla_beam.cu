@@ -714,7 +714,7 @@ int gla_decode_step_beams(void* stream, int64_t B, int64_t H, int64_t D, int dty
 
 int gla_reorder_states(void* stream, int64_t count, void* const* tensors, const int64_t* row_bytes, int64_t requests, int64_t beams,
                        const int32_t* parents) {
-  if (!tensors || !row_bytes || !parents) return GLA_ERR_NULL_POINTER;
+  if (!parents || (count > 0 && (!tensors || !row_bytes))) return GLA_ERR_NULL_POINTER;
   if (count < 0 || requests <= 0 || beams <= 0) return GLA_ERR_BAD_DIMS;
   if (beams > 32) return GLA_ERR_UNSUPPORTED;
   for (int64_t i = 0; i < count; ++i) {

@@ -59,3 +59,11 @@ def test_validation_without_gpu(lib):
     assert lib.gla_reorder_states(None, 0, p, p, 1, 2, p) == 0
     assert lib.gla_reorder_states(None, 1, None, p, 1, 2, p) == 1
     assert lib.gla_reorder_states(None, 0, p, p, 1, 33, p) == 3
+
+
+def test_no_states_to_move(lib):
+    """An empty list has no arrays behind it: there is nothing to do, which is no error."""
+    p = ctypes.c_void_p(4096)
+    assert lib.gla_reorder_states(None, 0, None, None, 2, 4, p) == 0
+    assert lib.gla_reorder_states(None, 0, None, None, 2, 4, None) == 1
+    assert lib.gla_reorder_states(None, 1, p, None, 2, 4, p) == 1

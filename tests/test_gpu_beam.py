@@ -314,3 +314,11 @@ def test_equal_totals_of_unequal_logits(cuda_device, N, K, V, M, dtype):
     some = torch.where(torch.rand(N, K, V, generator=gen, device=cuda_device) < 0.001, x.float().abs(), -x.float().abs().nan_to_num(posinf=1.0)).to(dtype)
     some[torch.rand(N, K, V, generator=gen, device=cuda_device) < 0.5] = 0.0
     same(beam_select(some, s, M), selected(some, s, M))
+
+
+def test_no_states_to_move(cuda_device):
+    from gla_jax_b200 import reorder_states
+    parents = torch.tensor([[1, 0]], dtype=torch.int32, device=cuda_device)
+    reorder_states([], parents)
+    reorder_states((), parents)
+    reorder_states([torch.empty(2, 0, device=cuda_device), torch.empty(2, 3, 0, 5, device=cuda_device)], parents)
