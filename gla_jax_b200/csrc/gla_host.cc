@@ -485,6 +485,7 @@ std::optional<Tensor> decode_step(Tensor state, const Tensor& g, const Tensor& v
   if (!par.has_value()) return std::nullopt;
   Tensor g32 = f32(g), vc = v.contiguous(), kc = k.contiguous(), qc = q.contiguous(), out = torch::empty({B, H, D}, v.options().dtype(od));
   if (par->defined()) {
+    if (B == 0) return out;
     check(gla_decode_step_beams(stream_of(v), B, H, D, dt_of(v), (float*)ptr(state), (const float*)ptr(g32), ptr(vc), ptr(kc), ptr(qc), ptr(out),
                                 dt_of(out), (const int32_t*)ptr(*par), par->size(1)), "gla_decode_step_beams");
     return out;

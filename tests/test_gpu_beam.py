@@ -322,3 +322,13 @@ def test_no_states_to_move(cuda_device):
     reorder_states([], parents)
     reorder_states((), parents)
     reorder_states([torch.empty(2, 0, device=cuda_device), torch.empty(2, 3, 0, 5, device=cuda_device)], parents)
+
+
+def test_steps_of_no_requests(cuda_device):
+    """The last request of a batch has ended."""
+    from gla_jax_b200 import decay_attention_step, decode_step
+    state, x = torch.empty(0, 2, 64, 64, device=cuda_device), torch.empty(0, 2, 64, device=cuda_device)
+    parents = torch.empty(0, 4, dtype=torch.int32, device=cuda_device)
+    assert decode_step(state, x, x, x, x, parents=parents).shape == (0, 2, 64)
+    assert decay_attention_step(state, x[..., 0], x, x, x, parents=parents).shape == (0, 2, 64)
+    assert decay_attention_step(state, x[..., 0], x, x, x).shape == (0, 2, 64)
