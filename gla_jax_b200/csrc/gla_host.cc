@@ -58,6 +58,14 @@ Tensor flat16(const Tensor& x) {
   const Tensor y = x.contiguous();
   return (uintptr_t)y.data_ptr() % 16 ? y.clone() : y;
 }
+// A state that a call updates in place, as the kernels of 16-byte accesses take it: itself, or where it starts between multiples of
+// 16 bytes a copy, which `back` brings home.
+struct State16 {
+  const Tensor& home;
+  Tensor at;
+  explicit State16(const Tensor& state) : home(state), at((uintptr_t)state.data_ptr() % 16 ? state.clone() : state) {}
+  void back() { if (!at.is_same(home)) home.copy_(at); }
+};
 Tensor f32(const Tensor& g) { return (g.scalar_type() == torch::kFloat32 ? g : g.to(torch::kFloat32)).contiguous(); }
 bool wants_any(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts) if (t->requires_grad()) return true;
@@ -424,8 +432,10 @@ std::optional<Tensor> decay_step(Tensor state, const Tensor& g, const Tensor& v,
   if (!par.has_value()) return std::nullopt;
   Tensor g32 = f32(g), vc = v.contiguous(), kc = k.contiguous(), qc = q.contiguous(), out = torch::empty({B, H, Dv}, v.options().dtype(od));
   if (B == 0) return out;
-  check(gla_decay_step(stream_of(v), B, H, k.size(1), Dk, Dv, dt_of(v), (float*)ptr(state), (const float*)ptr(g32), ptr(vc), ptr(kc), ptr(qc),
+  State16 s(state);
+  check(gla_decay_step(stream_of(v), B, H, k.size(1), Dk, Dv, dt_of(v), (float*)ptr(s.at), (const float*)ptr(g32), ptr(vc), ptr(kc), ptr(qc),
                        ptr(out), dt_of(out), (const int32_t*)ptr(*par), par->defined() ? par->size(1) : 1), "gla_decay_step");
+  s.back();
   return out;
 }
 bool reorder_states(const std::vector<Tensor>& states, const Tensor& parents) {
@@ -486,8 +496,10 @@ std::optional<Tensor> decode_step(Tensor state, const Tensor& g, const Tensor& v
   Tensor g32 = f32(g), vc = v.contiguous(), kc = k.contiguous(), qc = q.contiguous(), out = torch::empty({B, H, D}, v.options().dtype(od));
   if (par->defined()) {
     if (B == 0) return out;
-    check(gla_decode_step_beams(stream_of(v), B, H, D, dt_of(v), (float*)ptr(state), (const float*)ptr(g32), ptr(vc), ptr(kc), ptr(qc), ptr(out),
+    State16 s(state);
+    check(gla_decode_step_beams(stream_of(v), B, H, D, dt_of(v), (float*)ptr(s.at), (const float*)ptr(g32), ptr(vc), ptr(kc), ptr(qc), ptr(out),
                                 dt_of(out), (const int32_t*)ptr(*par), par->size(1)), "gla_decode_step_beams");
+    s.back();
     return out;
   }
   check(gla_decode_step(stream_of(v), B, H, D, dt_of(v), (float*)ptr(state), (const float*)ptr(g32), ptr(vc), ptr(kc), ptr(qc), ptr(out),

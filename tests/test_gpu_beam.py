@@ -332,3 +332,21 @@ def test_steps_of_no_requests(cuda_device):
     assert decode_step(state, x, x, x, x, parents=parents).shape == (0, 2, 64)
     assert decay_attention_step(state, x[..., 0], x, x, x, parents=parents).shape == (0, 2, 64)
     assert decay_attention_step(state, x[..., 0], x, x, x).shape == (0, 2, 64)
+
+
+def test_states_that_start_anywhere(cuda_device):
+    """A contiguous state between multiples of 16 bytes, as a slice of a flat buffer is, is stepped in place like any other."""
+    from gla_jax_b200 import decay_attention_step, decode_step
+    gen = torch.Generator(device=cuda_device).manual_seed(8)
+    n = lambda *s: torch.randn(*s, generator=gen, device=cuda_device)  # noqa: E731
+    B, H, D = 6, 2, 64
+    parents = torch.tensor([[1, 1, 0], [2, 0, 2]], dtype=torch.int32, device=cuda_device)
+    state, v, k, q = n(B, H, D, D), n(B, H, D), n(B, H, D), n(B, H, D)
+    for step, g in ((decay_attention_step, -n(B, H).abs()), (decode_step, -n(B, H, D).abs())):
+        for par in (None, parents):
+            a = state.clone()
+            flat = torch.zeros(state.numel() + 2, device=cuda_device)
+            b = flat[1:-1].view_as(state).copy_(state)
+            assert b.data_ptr() % 16 and b.is_contiguous()
+            assert torch.equal(step(a, g, v, k, q, parents=par), step(b, g, v, k, q, parents=par))
+            assert torch.equal(a, b) and flat[0] == 0 and flat[-1] == 0
