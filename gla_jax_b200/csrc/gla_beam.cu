@@ -46,9 +46,10 @@ __global__ void __launch_bounds__(SNT) step_kernel(const Step p) {
   __shared__ float red[4][W];
   __shared__ float kq[2][RPT * RL];
   const int cl = threadIdx.x % CL, rl = threadIdx.x / CL;
-  const int64_t row = blockIdx.y;                                 // (request, head)
+  const int tiles = (p.Dv + W - 1) / W, col = blockIdx.x % tiles * W;      // of the block's columns, the first
+  const int64_t row = blockIdx.x / tiles;                         // (request, head)
   const int64_t b = row / p.H, h = row % p.H, kv = (b * (p.H / p.share) + h / p.share) * p.Dk;
-  const int c0 = blockIdx.x * W + 4 * cl;
+  const int c0 = col + 4 * cl;
   const bool on = c0 < p.Dv;
   float* Sp = p.S + (row * p.Dk + rl) * (int64_t)p.Dv + c0;
   grid_dep_wait();
@@ -86,7 +87,7 @@ __global__ void __launch_bounds__(SNT) step_kernel(const Step p) {
   }
   if (threadIdx.x % 32 < CL) *reinterpret_cast<float4*>(&red[threadIdx.x / 32][4 * cl]) = acc;
   __syncthreads();
-  const int c = blockIdx.x * W + threadIdx.x;
+  const int c = col + threadIdx.x;
   if (threadIdx.x < W && c < p.Dv)
     st_any(p.out, p.out_bf, row * p.Dv + c, (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]));
 }
@@ -105,14 +106,15 @@ __global__ void __launch_bounds__(SNT) step_beams_kernel(const Step p) {
   float* kq = red + p.K * 4 * W;                                                      // [K][k, q][Dk]
   float* vf = kq + 2 * p.K * p.Dk;                                                    // [K][v (W), exp(g), parent, 2 spare]
   const int cl = threadIdx.x % CL, rl = threadIdx.x / CL, warp = threadIdx.x / 32;
-  const int64_t n = blockIdx.y / p.H, h = blockIdx.y % p.H;
-  const int c0 = blockIdx.x * W + 4 * cl;
+  const int tiles = (p.Dv + W - 1) / W, col = blockIdx.x % tiles * W;
+  const int64_t group = blockIdx.x / tiles, n = group / p.H, h = group % p.H;
+  const int c0 = col + 4 * cl;
   const bool on = c0 < p.Dv;
   grid_dep_wait();
   grid_dep_launch();
   // beams that are somebody's parent: a lane looks at one
   const int lane = threadIdx.x % 32;
-  const int par = lane < p.K ? parent_of(p.parents, n, p.K, lane, blockIdx.x == 0 && h == 0 && warp == 0) : 0;
+  const int par = lane < p.K ? parent_of(p.parents, n, p.K, lane, col == 0 && h == 0 && warp == 0) : 0;
   const unsigned int used = __reduce_or_sync(0xffffffffu, lane < p.K ? 1u << par : 0u);
   for (int j = 0; j < p.K; ++j) {
     if (!((used >> j) & 1u)) continue;
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(SNT) step_beams_kernel(const Step p) {
     kq[(2 * j + 1) * p.Dk + r] = ld_any(p.q, p.bf, kv);
   }
   for (int i = threadIdx.x; i < p.K * W; i += SNT) {
-    const int j = i / W, c = blockIdx.x * W + i % W;
+    const int j = i / W, c = col + i % W;
     vf[j * (W + 4) + i % W] = c < p.Dv ? ld_any(p.v, p.bf, ((n * p.K + j) * p.H + h) * p.Dv + c) : 0.f;
   }
   if (warp == 0 && lane < p.K) {
@@ -169,16 +171,16 @@ __global__ void __launch_bounds__(SNT) step_beams_kernel(const Step p) {
   __syncthreads();
   for (int i = threadIdx.x; i < p.K * W; i += SNT) {
     const int j = i / W, c = i % W;
-    if (blockIdx.x * W + c >= p.Dv) continue;
+    if (col + c >= p.Dv) continue;
     const float* x = red + j * 4 * W + c;
-    st_any(p.out, p.out_bf, ((n * p.K + j) * p.H + h) * p.Dv + blockIdx.x * W + c, (x[0] + x[W]) + (x[2 * W] + x[3 * W]));
+    st_any(p.out, p.out_bf, ((n * p.K + j) * p.H + h) * p.Dv + col + c, (x[0] + x[W]) + (x[2 * W] + x[3 * W]));
   }
 }
 
 template <int RPT>
 static int launch_step(cudaStream_t st, const Step& p, int64_t rows) {
   ProfScope ps("decay_step_kernel", st);
-  GLA_LAUNCHED(launch_overlapped(step_kernel<32, RPT>, dim3((unsigned)((p.Dv + 31) / 32), (unsigned)rows), dim3(SNT), 0, st, p));
+  GLA_LAUNCHED(launch_overlapped(step_kernel<32, RPT>, dim3((unsigned)((p.Dv + 31) / 32 * rows)), dim3(SNT), 0, st, p));
   return GLA_OK;
 }
 template <int W, bool KEYED>
@@ -188,7 +190,7 @@ static int launch_beams(cudaStream_t st, const Step& p, int64_t groups) {
   static SmemAttrOnce attr;
   GLA_TRY(attr.ensure(step_beams_kernel<W, KEYED>, 200 << 10));      // (32 beams of 256 features: 194 KB)
   ProfScope ps("step_beams_kernel", st);
-  GLA_LAUNCHED(launch_overlapped(step_beams_kernel<W, KEYED>, dim3((unsigned)((p.Dv + W - 1) / W), (unsigned)groups), dim3(SNT), smem, st, p));
+  GLA_LAUNCHED(launch_overlapped(step_beams_kernel<W, KEYED>, dim3((unsigned)((p.Dv + W - 1) / W * groups)), dim3(SNT), smem, st, p));
   return GLA_OK;
 }
 // Columns per block: as many as leave room for six blocks on an SM, so that one block's copies run beside another's steps
@@ -330,24 +332,25 @@ __global__ void __launch_bounds__(QNT) select_parts_kernel(const Select p) {
   __shared__ float wm[8];
   __shared__ double ws[8];
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
-  const int64_t row = blockIdx.y, V = p.V;
+  const int64_t row = blockIdx.x / p.parts, V = p.V;
+  const int own_part = blockIdx.x % p.parts;
   grid_dep_wait();
   grid_dep_launch();
-  u64* cand = p.cand + (row * p.parts + blockIdx.x) * p.M;
+  u64* cand = p.cand + (row * p.parts + own_part) * p.M;
   const float score = p.scores[row];
   const bool dead = !(score > -CUDART_INF_F), done = p.finished && p.finished[row];
   if (dead || done) {
     // a beam that has ended has one continuation, one without a score has none: the others rank by their number alone
     if (tid < p.M) {
       u64 x = 0;
-      if (blockIdx.x == 0) {
+      if (own_part == 0) {
         const bool one = done && !dead;
         const int64_t i = !one ? tid : tid == 0 ? p.pad : tid - 1 < p.pad ? tid - 1 : tid;
         if (i < V) x = key_of(one && tid == 0 ? 0.f : -CUDART_INF_F, (unsigned int)i);
       }
       cand[tid] = x;
     }
-    if (tid == 0) p.sums[row * p.parts + blockIdx.x] = blockIdx.x == 0 ? make_double2(0.0, 1.0) : make_double2(-CUDART_INF, 0.0);
+    if (tid == 0) p.sums[row * p.parts + own_part] = own_part == 0 ? make_double2(0.0, 1.0) : make_double2(-CUDART_INF, 0.0);
     return;
   }
   // A thread's logits are the same whatever a row's address, so that equal rows have equal sums to the last bit and their
@@ -356,7 +359,7 @@ __global__ void __launch_bounds__(QNT) select_parts_kernel(const Select p) {
   const char* base = (const char*)p.logits + row * V * ES;
   const auto w_of = [](int i) { return i / E; };                      // the access that logit i of a thread's tile came by
   const int shift = (int)((uintptr_t)base & 15) / ES;
-  const int64_t lo = blockIdx.x * p.part, hi = lo + p.part < V ? lo + p.part : V;
+  const int64_t lo = own_part * p.part, hi = lo + p.part < V ? lo + p.part : V;
   float s = 0.f;
   float v1 = -CUDART_INF_F, v2 = -CUDART_INF_F;      // the two largest (v1 is the running maximum), and the tiles that they came in
   int64_t t1 = lo, t2 = lo;
@@ -543,7 +546,7 @@ __global__ void __launch_bounds__(QNT) select_parts_kernel(const Select p) {
   if (tid == 0) {
     sum = 0.0;
     for (int w = 0; w < 8; ++w) sum += ws[w];
-    p.sums[row * p.parts + blockIdx.x] = make_double2(top, sum);
+    p.sums[row * p.parts + own_part] = make_double2(top, sum);
   }
 }
 
@@ -679,12 +682,14 @@ extern "C" {
 
 unsigned int gla_device_bad_parents(void) { return beam_bad_parents(); }
 
+constexpr int64_t GRID_MOST = 2147483647;
+
 static int step_check(int64_t B, int64_t H, int64_t Hk, int64_t Dk, int64_t Dv, int dtype, int out_dtype, const int32_t* parents, int64_t K) {
   if (B <= 0 || H <= 0 || Hk <= 0 || Dk <= 0 || Dv <= 0 || H % Hk) return GLA_ERR_BAD_DIMS;
   if (parents && (K <= 0 || B % K)) return GLA_ERR_BAD_DIMS;
   if ((dtype != GLA_F32 && dtype != GLA_BF16) || (out_dtype != GLA_F32 && out_dtype != GLA_BF16)) return GLA_ERR_UNSUPPORTED;
   if (Dk % 8 || Dv % 8 || Dk > 256 || Dv > 256 || (parents && K > 32)) return GLA_ERR_UNSUPPORTED;
-  if (B * H / (parents ? K : 1) > 65535) return GLA_ERR_TOO_LARGE;
+  if (B > GRID_MOST || B / (parents ? K : 1) * H > GRID_MOST / 64) return GLA_ERR_TOO_LARGE;      // (64 blocks of columns at most)
   return GLA_OK;
 }
 
@@ -755,7 +760,7 @@ static int select_check(int64_t N, int64_t K, int64_t V, int64_t M, int dtype, i
   if (N <= 0 || K <= 0 || V <= 0 || M <= 0 || M > K * V || pad < 0 || pad >= V) return GLA_ERR_BAD_DIMS;
   if (dtype != GLA_F32 && dtype != GLA_BF16) return GLA_ERR_UNSUPPORTED;
   if (K > 32 || M > 32) return GLA_ERR_UNSUPPORTED;
-  if (N * K > 65535 || V > 1 << 30) return GLA_ERR_TOO_LARGE;
+  if (N > GRID_MOST / 32 || V > 1 << 30) return GLA_ERR_TOO_LARGE;
   return GLA_OK;
 }
 static size_t select_bytes(int64_t N, int64_t K, int64_t M, int parts) {
@@ -786,7 +791,7 @@ int gla_beam_select(void* stream, int64_t N, int64_t K, int64_t V, int64_t M, in
   cudaStream_t st = (cudaStream_t)stream;
   {
     ProfScope ps("select_parts_kernel", st);
-    const dim3 grid((unsigned)p.parts, (unsigned)(N * K));
+    const dim3 grid((unsigned)(N * K * p.parts));
     GLA_LAUNCHED(launch_overlapped(p.bf ? beam::select_parts_kernel<true> : beam::select_parts_kernel<false>, grid, dim3(beam::QNT), 0, st, p));
   }
   ProfScope ps("select_beams_kernel", st);

@@ -10,13 +10,13 @@ namespace {
 // only offsets that rise lead to every run once, and every row is some sequence's or behind the last.  One block, since the running
 // maximum needs all before it; 3 us of a packed call.
 __device__ unsigned int g_bad_offsets = 0;      // sequences whose offsets had to be changed
-__global__ void __launch_bounds__(256) offsets_kernel(const int* cu, int64_t nseq, int T, int* clean) {
-  __shared__ int part[8];
+__global__ void __launch_bounds__(1024) offsets_kernel(const int* cu, int64_t nseq, int T, int* clean) {
+  __shared__ int part[32];
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   int carry = 0;
   grid_dep_wait();
   grid_dep_launch();
-  for (int64_t i0 = 0; i0 <= nseq; i0 += 256) {
+  for (int64_t i0 = 0; i0 <= nseq; i0 += 1024) {
     const int64_t i = i0 + tid;
     int x = 0;
     if (i > 0 && i <= nseq) {
@@ -32,7 +32,7 @@ __global__ void __launch_bounds__(256) offsets_kernel(const int* cu, int64_t nse
     if (lane == 31) part[warp] = x;
     __syncthreads();
     int all = carry;
-    for (int w = 0; w < 8; ++w) {
+    for (int w = 0; w < 32; ++w) {
       if (w < warp && part[w] > x) x = part[w];
       if (part[w] > all) all = part[w];
     }
@@ -381,7 +381,7 @@ int fwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const flo
   if (cu) {
     int* clean = (int*)(saved ? (char*)saved + saved_states(d) : (char*)ws + run_bytes(d, false));
     ProfScope ps("decay_offsets_kernel", st);
-    GLA_LAUNCHED(launch_overlapped(offsets_kernel, dim3(1), dim3(256), 0, st, cu, d.nseq, (int)d.T, clean));
+    GLA_LAUNCHED(launch_overlapped(offsets_kernel, dim3(1), dim3(1024), 0, st, cu, d.nseq, (int)d.T, clean));
     cu = clean;
   }
   if (fast(d)) return fast_fwd(st, d, cu, h0, g, gt, v, k, q, hf, out, saved, ws);
@@ -484,7 +484,8 @@ static int check(const Dims& d, int dtype, int hidden_dtype, const int* cu) {
   if ((d.nseq > 0) != (cu != nullptr) || (d.nseq > 0 && (d.B != 1 || d.T > 2147483647LL))) return GLA_ERR_BAD_DIMS;
   if ((dtype != GLA_F32 && dtype != GLA_BF16) || (hidden_dtype != GLA_F32 && hidden_dtype != dtype)) return GLA_ERR_UNSUPPORTED;
   if (d.Dk % 8 || d.Dv % 8 || d.Dk > 256 || d.Dv > 256) return GLA_ERR_UNSUPPORTED;
-  if (d.H > 65535 / 4 || d.seqs() > 65535 || d.T > (int64_t)1 << 40) return GLA_ERR_TOO_LARGE;
+  // (sequences are cut into runs only where they are fewer than the SMs)
+  if (d.H > 65535 / 4 || d.seqs() > 2147483647LL - 65536 || d.T > (int64_t)1 << 40) return GLA_ERR_TOO_LARGE;
   return GLA_OK;
 }
 

@@ -515,7 +515,7 @@ GLA_API int gla_sp_combine2(void* stream, int64_t R, int64_t rank, int64_t BH, i
  *   cu_seqlens[s + 1]) (DEVICE, int32, rising from 0, any length, 0 included); hidden is (nseq, H, Dk, Dv).  Tokens behind the last
  *   sequence give zeros.  Offsets that fall or leave [0, T] are held inside (the first is 0, each of the others at least the one
  *   before it and at most T) and counted (gla_device_bad_offsets).
- * Dk and Dv multiples of 8 up to 256; any T > 0; H a multiple of Hk.  `dtype` is that of value, key, query, out and their
+ * Dk and Dv multiples of 8 up to 256; any T > 0; H a multiple of Hk, at most 16383.  `dtype` is that of value, key, query, out and their
  * gradients; hidden_dtype that of hidden_init, hidden_final and their gradients: dtype or GLA_F32.  value, key, query, out and
  * gradients 16-byte aligned.
  * A forward that will be differentiated gets `saved` (gla_decay_saved_bytes), which the backward reads: final states in

@@ -350,3 +350,24 @@ def test_states_that_start_anywhere(cuda_device):
             assert b.data_ptr() % 16 and b.is_contiguous()
             assert torch.equal(step(a, g, v, k, q, parents=par), step(b, g, v, k, q, parents=par))
             assert torch.equal(a, b) and flat[0] == 0 and flat[-1] == 0
+
+
+def test_more_rows_than_a_grid_is_high(cuda_device):
+    """Batches of more than 65535 (request, head) or (request, beam) pairs equal the halves of them."""
+    from gla_jax_b200 import beam_select, decay_attention_step, decode_step
+    gen = torch.Generator(device=cuda_device).manual_seed(3)
+    n = lambda *s: torch.randn(*s, generator=gen, device=cuda_device)  # noqa: E731
+    B, H, D = 2 * 4120, 16, 32
+    for step, K in ((decay_attention_step, 1), (decay_attention_step, 2), (decode_step, 2)):
+        keyed = step is decode_step
+        state, g = n(B, H, D, D), -n(B, H, *([D] if keyed else [])).abs()
+        v, k, q = n(B, H, D), n(B, H, D), n(B, H, D)
+        par = torch.randint(0, K, (B // K, K), generator=gen, device=cuda_device, dtype=torch.int32) if K > 1 else None
+        a, b = state.clone(), state.clone()
+        out = step(a, g, v, k, q, parents=par)
+        for s in (slice(0, B // 2), slice(B // 2, B)):
+            part = step(b[s], g[s], v[s], k[s], q[s], parents=par[s.start // K:s.stop // K] if K > 1 else None)
+            assert torch.equal(part, out[s])
+        assert torch.equal(a, b)
+    logits, scores = n(35000, 2, 9), n(35000, 2)
+    same(beam_select(logits, scores), selected(logits, scores, 2))

@@ -104,3 +104,25 @@ def test_gates_gradient_before_a_value_or_key_that_is_not_finite(cuda_device, T,
                 assert not torch.isfinite(got[1][:, t + 1:, :heads]).any(), (t, what, bad)
                 if what == 2:
                     assert ((got[1][:, :, 1].double() - want[1][:, :, 1]).abs() <= lim[:, 1]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_more_sequences_than_a_grid_is_high(cuda_device, dtype):
+    """70,000 sequences of 0 to 3 tokens, as a batch and packed, equal the halves of them."""
+    from gla_jax_b200 import chunk_decay_attention, chunk_decay_attention_packed
+    n, half = 70000, 35000
+    xs = make(cuda_device, n, 2, 1, 1, 8, 8, dtype, dtype)
+    cots = [torch.randn_like(xs[0]), torch.randn_like(xs[2])]
+    got, grads = with_grads(chunk_decay_attention, xs, cots)
+    for s in (slice(0, half), slice(half, n)):
+        want, gw = with_grads(chunk_decay_attention, [x[s] for x in xs], [c[s] for c in cots])
+        assert all(torch.equal(a[s], b) for a, b in zip([*got, *grads], [*want, *gw]))
+    cu = [0, *(torch.arange(n) % 4).cumsum(0).tolist()]
+    xs, cots = packed(cuda_device, n, cu[-1], 1, 1, 8, 8, dtype)
+    got, grads = with_grads(lambda *a: chunk_decay_attention_packed(*a, cu), xs, cots)
+    for a, b in ((0, half), (half, n)):
+        s, t = slice(a, b), slice(cu[a], cu[b])
+        part = [x - cu[a] for x in cu[a:b + 1]]
+        want, gw = with_grads(lambda *y: chunk_decay_attention_packed(*y, part), [xs[0][s], *(x[t] for x in xs[1:])], [cots[0][s], cots[1][t]])
+        for i, (x, y) in enumerate(zip([*got, *grads], [*want, *gw])):
+            assert torch.equal(x[s if i in (0, 2) else t], y), i
