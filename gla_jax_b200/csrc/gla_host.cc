@@ -398,8 +398,9 @@ std::optional<std::tuple<Tensor, Tensor>> chunk_decay(const Tensor& h, const Ten
   const bool grad = wants_grad({&h, &g0, &v, &k, &q});
   Tensor g = g0;
   if (grad && !d.per_token && g0.requires_grad()) {
-    // the gradient of a decay that every token has is the sum over the tokens
-    g = v.dim() == 4 ? g0.expand({d.B, d.T, d.H}) : g0.expand({d.T, d.H});
+    // the gradient of a decay that every token has is the sum over the tokens, in float32 whatever its type
+    const Tensor wide = g0.to(torch::kFloat32);
+    g = v.dim() == 4 ? wide.expand({d.B, d.T, d.H}) : wide.expand({d.T, d.H});
     d.per_token = 1;
   }
   // (a node takes no undefined tensor)

@@ -126,3 +126,14 @@ def test_more_sequences_than_a_grid_is_high(cuda_device, dtype):
         want, gw = with_grads(lambda *y: chunk_decay_attention_packed(*y, part), [xs[0][s], *(x[t] for x in xs[1:])], [cots[0][s], cots[1][t]])
         for i, (x, y) in enumerate(zip([*got, *grads], [*want, *gw])):
             assert torch.equal(x[s if i in (0, 2) else t], y), i
+
+
+def test_bf16_decays_of_the_head_round_their_gradient_once(cuda_device):
+    from gla_jax_b200 import chunk_decay_attention
+    xs = make(cuda_device, 2, 500, 4, 4, 64, 64, torch.bfloat16, torch.bfloat16)
+    cots = [torch.randn_like(xs[0]), torch.randn_like(xs[2])]
+    xs[1] = torch.tensor([-0.5, -0.01, -0.1, -1.5], device=cuda_device, dtype=torch.bfloat16)
+    _, grads = with_grads(chunk_decay_attention, xs, cots)
+    xs[1] = xs[1].float()
+    _, want = with_grads(chunk_decay_attention, xs, cots)
+    assert grads[1].dtype == torch.bfloat16 and torch.equal(grads[1], want[1].bfloat16())
