@@ -210,7 +210,7 @@ struct Tensors {
   uint8_t* p[RT];
   int64_t bytes[RT];                   // of a row
   unsigned int start[RT + 1];          // first block of each tensor
-  int n, K, unit;                      // beams; bytes of an access
+  int n, K, count;                     // beams; whether this launch reports parents that are none
   const int* parents;
 };
 constexpr int MNT = 256;
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(MNT) reorder_kernel(const Tensors t) {
   const int64_t units = t.bytes[i] / (int64_t)sizeof(T), per = (units + MNT - 1) / MNT;
   const int64_t blk = blockIdx.x - t.start[i], n = blk / per, u = blk % per * MNT + threadIdx.x;
   T* base = reinterpret_cast<T*>(t.p[i]) + n * t.K * units + u;
-  const bool count = i == 0 && blk % per == 0 && threadIdx.x == 0;
+  const bool count = t.count && i == 0 && blk % per == 0 && threadIdx.x == 0;
   unsigned int taken = 0, moved = 0;
   for (int b = 0; b < t.K; ++b) {
     const int from = parent_of(t.parents, n, t.K, b, count);
@@ -727,13 +727,16 @@ int gla_reorder_states(void* stream, int64_t count, void* const* tensors, const 
     if (row_bytes[i] <= 0) return GLA_ERR_BAD_DIMS;
   }
   // tensors by the widest access that their address and rows allow, RT of them a launch
+  bool first = true;
   for (int unit = 16; unit; unit = unit == 16 ? 4 : unit == 4 ? 1 : 0) {
     beam::Tensors t{};
-    t.K = (int)beams; t.unit = unit; t.parents = parents;
+    t.K = (int)beams; t.parents = parents;
     unsigned int blocks = 0;
     const auto flush = [&]() -> int {
       if (!t.n) return GLA_OK;
       t.start[t.n] = blocks;
+      t.count = first;
+      first = false;
       const int s = unit == 16 ? beam::launch_reorder<uint4>((cudaStream_t)stream, t)
                     : unit == 4 ? beam::launch_reorder<uint32_t>((cudaStream_t)stream, t) : beam::launch_reorder<uint8_t>((cudaStream_t)stream, t);
       t.n = 0; blocks = 0;

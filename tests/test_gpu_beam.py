@@ -371,3 +371,19 @@ def test_more_rows_than_a_grid_is_high(cuda_device):
         assert torch.equal(a, b)
     logits, scores = n(35000, 2, 9), n(35000, 2)
     same(beam_select(logits, scores), selected(logits, scores, 2))
+
+
+def test_bad_parents_of_several_launches_are_counted_once(cuda_device):
+    """Tensors of 16-, 4- and 1-byte rows go in launches of their own, and no more than 64 in one."""
+    from gla_jax_b200 import check_device, reorder_states
+    from gla_jax_b200._lib import GlaError
+    check_device()
+    bad = torch.tensor([[0, 7], [-4, 1], [1, 0]], dtype=torch.int32, device=cuda_device)
+    states = [torch.randn(6, 8, device=cuda_device), torch.randn(6, 5, device=cuda_device), torch.ones(6, 3, device=cuda_device).bool()]
+    states += [torch.randn(6, 8, device=cuda_device) for _ in range(70)]
+    want = [torch.cat([s[:4], s[5:], s[4:5]]) for s in states]
+    reorder_states(states, bad)
+    assert all(torch.equal(a, b) for a, b in zip(states, want))
+    with pytest.raises(GlaError, match=" 2 parent"):
+        check_device()
+    check_device()
