@@ -77,7 +77,8 @@ def chunk_decay_attention_packed(hidden_init, log_decay, value, key, query, cu_s
         if value.is_cuda:
             cu = cu.to(torch.int32).to(value.device)
     elif cu.dtype != torch.int32:
-        cu = cu.to(torch.int32)
+        # (what 32 bits do not hold leaves [0, T] on the same side)
+        cu = (cu.clamp(-1, 2 ** 31 - 1) if cu.dtype == torch.int64 else cu).to(torch.int32)
     r = _lib.native().chunk_decay(hidden_init, log_decay, value, key, query, cu) if value.is_cuda else None
     if r is not None:
         return r

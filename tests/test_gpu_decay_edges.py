@@ -137,3 +137,17 @@ def test_bf16_decays_of_the_head_round_their_gradient_once(cuda_device):
     xs[1] = xs[1].float()
     _, want = with_grads(chunk_decay_attention, xs, cots)
     assert grads[1].dtype == torch.bfloat16 and torch.equal(grads[1], want[1].bfloat16())
+
+
+def test_offsets_beyond_32_bits_are_held_inside_too(cuda_device):
+    from gla_jax_b200 import check_device, chunk_decay_attention_packed
+    from gla_jax_b200._lib import GlaError
+    xs, _ = packed(cuda_device, 3, 600, 2, 1, 64, 64, torch.bfloat16)
+    check_device()
+    for offsets in ([0, 2 ** 32 + 100, 400, 600], [0, 100, -2 ** 32 + 300, 600], [0, 100, 400, 2 ** 40 + 600]):
+        want = chunk_decay_attention_packed(*xs, torch.tensor(held_inside(offsets, 600), device=cuda_device))
+        check_device()
+        got = chunk_decay_attention_packed(*xs, torch.tensor(offsets, device=cuda_device))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        with pytest.raises(GlaError):
+            check_device()
