@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
               s[u] = in ? __uint_as_float(x[c]) * w : 0.f;
               d[u] = in ? __uint_as_float(y[c]) * w : 0.f;
               if constexpr (GATE) {
-                m[c] = in ? s[u] * __uint_as_float(y[c]) * wm : 0.f;
+                m[c] = in ? s[u] * wm * __uint_as_float(y[c]) : 0.f;      // (s alone may be near the top)
                 rowsum += m[c];
               }
             }

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_decay import ALL_FINE, BF, F4, make, recurrence, with_grads
+from test_gpu_decay import ALL_FINE, BF, F4, check, make, recurrence, with_grads
 
 pytestmark = pytest.mark.gpu
 
@@ -151,3 +151,17 @@ def test_offsets_beyond_32_bits_are_held_inside_too(cuda_device):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         with pytest.raises(GlaError):
             check_device()
+
+
+@pytest.mark.parametrize("rate", [0.02, 0.3, 0.45])
+@pytest.mark.parametrize("D", [64, 128])
+def test_large_products_under_decay(cuda_device, rate, D):
+    """Scores up to 2^35 and products of values and cotangents up to 2^45: nothing between the inputs and the results, the gates'
+    gradient of their product among them, may overflow."""
+    from gla_jax_b200 import chunk_decay_attention
+    xs = make(cuda_device, 1, 260, 2, 2, D, D, torch.bfloat16, torch.float32)
+    xs[1] = torch.full_like(xs[1], -rate)
+    xs[2], xs[3], xs[4] = xs[2] * 2.0 ** 20, xs[3] * 2.0 ** 17, xs[4] * 2.0 ** 14
+    cots = [torch.randn_like(xs[0]), torch.randn_like(xs[2]) * 2.0 ** 20]
+    got, grads = with_grads(chunk_decay_attention, xs, cots)
+    check(xs, cots, got, grads, torch.bfloat16, torch.float32, rate)
