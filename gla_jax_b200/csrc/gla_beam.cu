@@ -658,7 +658,7 @@ __global__ void __launch_bounds__(BNT) select_beams_kernel(const Select p) {
 }
 
 // Parts of a row: enough blocks for the device (six per SM), few enough that a request's candidates fit.
-static void plan(int64_t rows, int64_t V, int K, int M, int bf, int* parts, int64_t* part) {
+static void plan(int64_t rows, int64_t V, int K, int M, int* parts, int64_t* part) {
   const int64_t tiles = (V + TILE - 1) / TILE;
   int64_t n = (6 * 148 + rows - 1) / rows;
   if (n > tiles) n = tiles;
@@ -773,7 +773,7 @@ static size_t select_bytes(int64_t N, int64_t K, int64_t M, int parts) {
 size_t gla_beam_select_workspace_bytes(int64_t N, int64_t K, int64_t V, int64_t M, int dtype) {
   if (select_check(N, K, V, M, dtype, 0) != GLA_OK) return 0;
   int parts; int64_t part;
-  beam::plan(N * K, V, (int)K, (int)M, dtype == GLA_BF16, &parts, &part);
+  beam::plan(N * K, V, (int)K, (int)M, &parts, &part);
   return select_bytes(N, K, M, parts);
 }
 
@@ -785,7 +785,7 @@ int gla_beam_select(void* stream, int64_t N, int64_t K, int64_t V, int64_t M, in
   if ((uintptr_t)logits % (dtype == GLA_BF16 ? 2 : 4)) return GLA_ERR_ALIGNMENT;
   beam::Select p{};
   p.logits = logits; p.scores = scores; p.finished = finished; p.V = V; p.K = (int)K; p.M = (int)M; p.bf = dtype == GLA_BF16; p.pad = pad_token;
-  beam::plan(N * K, V, p.K, p.M, p.bf, &p.parts, &p.part);
+  beam::plan(N * K, V, p.K, p.M, &p.parts, &p.part);
   if (!workspace || workspace_bytes < select_bytes(N, K, M, p.parts)) return GLA_ERR_WORKSPACE;
   if (!aligned16(workspace)) return GLA_ERR_ALIGNMENT;
   p.cand = (unsigned long long*)workspace;

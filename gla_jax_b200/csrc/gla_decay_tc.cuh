@@ -288,11 +288,10 @@ __device__ __forceinline__ bool check_rows(uint32_t tile, int nv) {
     }
   return (m & 0xffffu) >= 0x7f80u || (m >> 16) >= 0x7f80u;
 }
-// What is not finite in OA = P V, by sums over the tokens up to the row's own (UP = false) or from it on (UP): in the product,
-// zeros of P meet what is not finite in V, and 0 x inf is not a number, where the recurrence has it at its own token and after
-// (before) only.
+// What is not finite in OA = P V, by sums over the tokens up to the row's own: in the product, zeros of P meet what is not finite
+// in V, and 0 x inf is not a number, where the recurrence has it at its own token and after only.
 // P: this lane's row in tensor memory, 32 tokens in 16 columns at multiples of 32; 16 columns of V at a time.
-template <int DV, bool UP>
+template <int DV>
 __device__ __noinline__ void masked_sums(uint32_t tp, uint32_t to, uint32_t tv, int row, int qt) {
 #pragma unroll 1
   for (int c0 = qt * (DV / TC_COLS); c0 < (qt + 1) * (DV / TC_COLS); c0 += 16) {
@@ -313,7 +312,7 @@ __device__ __noinline__ void masked_sums(uint32_t tp, uint32_t to, uint32_t tv, 
         const uint32_t at = tv + (c0 >> 6) * 16384;
         const uint4 a = lds16(at + sw128_chunk(t, (c0 >> 3) & 7)), b = lds16(at + sw128_chunk(t, ((c0 >> 3) & 7) + 1));
         const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-        if (UP ? t >= row : t <= row)
+        if (t <= row)
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float2 v = pair_of(u[e]);
@@ -641,7 +640,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
         wait_for(ok, bar(B_PV), ph);             // (and Q S, which was issued before)
         tc_fence_after();
         const bool odd = was_odd(i), one = mild && !odd;
-        if (odd) masked_sums<DV, false>(tSC + lane_base, tOA + lane_base, uv, row, qt);
+        if (odd) masked_sums<DV>(tSC + lane_base, tOA + lane_base, uv, row, qt);
         const float wi = gs.wt[row].x, wp = mild ? wi : 1.f;
         const int64_t at = ((t0 + row) * p.H + h) * p.vd + HV * qt;      // (float32 outputs)
         const int64_t ra = p.r ? ((t0 + row) * (p.H / p.gr) + h / p.gr) * p.vd + HV * qt : 0;
