@@ -387,3 +387,61 @@ def test_bad_parents_of_several_launches_are_counted_once(cuda_device):
     with pytest.raises(GlaError, match=" 2 parent"):
         check_device()
     check_device()
+
+
+def _one_part(K, M, V, dtype):
+    """Tiles of 4096 logits in a part of a row: 1024 candidates a request are all that there is room for, so that 32 beams with 32
+    to select have a single part each."""
+    assert 1024 // (K * M) == 1
+    return -(-V // 4096)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_selection_one_after_the_other(cuda_device, dtype):
+    """A part of many tiles in which thirty of 256 threads hold all that is large: the bound is the lowest there is, and the logits
+    that reach it are more than the 1024 that the list holds, so that the M largest are found one after the other."""
+    from gla_jax_b200 import beam_select
+    N, K, V, M = 2, 32, 60001, 32
+    tiles = _one_part(K, M, V, dtype)
+    gen = torch.Generator(device=cuda_device).manual_seed(12)
+    x = torch.randn(N, K, V, generator=gen, device=cuda_device)
+    width = 8 if dtype == torch.bfloat16 else 4
+    owner = (torch.arange(V, device=cuda_device) // width) % 256
+    few = owner < 30
+    # (the bound is the 32nd of the threads' largest, so at most the second of the other threads' largest: below + 10)
+    assert tiles > 4 and int(few.sum()) > 1024
+    logits = torch.where(few, x.clamp(-4, 4) + 20, x.clamp(-4, 4)).to(dtype)
+    scores = -torch.arange(K, device=cuda_device).float().expand(N, K).contiguous()
+    same(beam_select(logits, scores, M), selected(logits, scores, M))
+    equal = torch.where(few, torch.full_like(x, 3.0), x.clamp(-2, 2)).to(dtype)           # all that is large is equal
+    same(beam_select(equal, scores, M), selected(equal, scores, M))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_selection_across_the_tiles_of_a_part(cuda_device, dtype):
+    """The two largest of a thread in an earlier, the same and a later tile, equal and unequal, and what else it met below them."""
+    from gla_jax_b200 import beam_select
+    N, K, V, M = 1, 32, 30011, 32
+    assert _one_part(K, M, V, dtype) == 8
+    gen = torch.Generator(device=cuda_device).manual_seed(13)
+    i = torch.arange(V, device=cuda_device)
+    scores = -3.0 * torch.arange(K, device=cuda_device).float().expand(N, K).contiguous()
+    noise = torch.rand(N, K, V, generator=gen, device=cuda_device)
+    ramp = (i.float() / 64).expand(N, K, V)
+    saw = ((i * 7919) % 251).float().expand(N, K, V)
+    coarse = torch.randint(0, 4, (N, K, V), generator=gen, device=cuda_device).float()
+    cases = [noise, ramp, ramp.flip(-1), saw, saw.flip(-1), coarse]
+    # one thread's places (token 4096 t + j of tile t): pairs of tiles hold its largest and second largest, in either order
+    for a, b in ((0, 0), (0, 3), (3, 0), (2, 7), (7, 2), (6, 6)):
+        for high, low in ((9.0, 8.0), (9.0, 9.0)):
+            y = noise.clone()
+            y[..., min(4096 * a + 2, V - 2)], y[..., min(4096 * b + 3, V - 1)] = high, low
+            y[..., 4096 * 4 + 1] = 7.0
+            cases.append(y)
+    masked = noise.clone()
+    masked[..., : 4096 * 5] = -math.inf
+    cases.append(masked)
+    for c, x in enumerate(cases):
+        x = x.contiguous().to(dtype)
+        for m in (M, 1, 5):
+            same(beam_select(x, scores, m), selected(x, scores, m))
