@@ -38,7 +38,7 @@ def beam_select(logits, scores, num_select: Optional[int] = None, finished=None,
             return r
     if not logits.is_cuda:
         raise RuntimeError("gla_jax_b200 operators need CUDA tensors; there is no CPU fallback")
-    if logits.dim() != 3 or tuple(scores.shape) != tuple(logits.shape[:2]) or logits.numel() == 0:
+    if logits.dim() != 3 or tuple(scores.shape) != tuple(logits.shape[:2]) or 0 in logits.shape[1:]:
         raise ValueError(f"beam_select: logits must be (N, K, V) and scores (N, K), got {tuple(logits.shape)}, {tuple(scores.shape)}")
     N, K, V = logits.shape
     if logits.dtype not in _DT or not scores.is_floating_point():
@@ -66,7 +66,7 @@ def reorder_states(states, parents) -> None:
         return
     if not parents.is_cuda or any(not s.is_cuda for s in states):
         raise RuntimeError("gla_jax_b200 operators need CUDA tensors; there is no CPU fallback")
-    if parents.dim() != 2 or parents.numel() == 0:
+    if parents.dim() != 2 or parents.shape[1] == 0:
         raise ValueError(f"reorder_states: parents must be (requests, beams), got {tuple(parents.shape)}")
     if parents.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"reorder_states: parents must be int32 or int64, got {parents.dtype}")

@@ -440,7 +440,7 @@ std::optional<Tensor> decay_step(Tensor state, const Tensor& g, const Tensor& v,
   return out;
 }
 bool reorder_states(const std::vector<Tensor>& states, const Tensor& parents) {
-  if (!parents.defined() || !here(parents) || parents.dim() != 2 || parents.numel() == 0) return false;
+  if (!parents.defined() || !here(parents) || parents.dim() != 2 || parents.size(1) == 0) return false;
   const auto par = parents_of(parents, parents.numel(), parents);
   if (!par.has_value()) return false;
   const int64_t rows = parents.numel();
@@ -457,6 +457,7 @@ bool reorder_states(const std::vector<Tensor>& states, const Tensor& parents) {
   }
   std::sort(spans.begin(), spans.end());
   for (size_t i = 1; i < spans.size(); ++i) if (spans[i].first < spans[i - 1].second) return false;
+  if (rows == 0) return true;
   check(gla_reorder_states(stream_of(parents), (int64_t)p.size(), p.data(), n.data(), parents.size(0), parents.size(1), (const int32_t*)ptr(*par)),
         "gla_reorder_states");
   return true;
@@ -468,11 +469,12 @@ std::optional<std::tuple<Tensor, Tensor, Tensor>> beam_select(const Tensor& logi
   if (scores.dim() != 2 || scores.size(0) != N || scores.size(1) != K || scores.device() != logits.device() || !scores.is_floating_point()) return std::nullopt;
   if (finished.has_value() && (finished->sizes() != scores.sizes() || finished->device() != logits.device() || finished->scalar_type() != torch::kBool))
     return std::nullopt;
-  if (N < 1 || M < 1 || K < 1 || V < 1 || M > K * V || pad < 0 || pad >= V || K > 32 || M > 32) return std::nullopt;
+  if (M < 1 || K < 1 || V < 1 || M > K * V || pad < 0 || pad >= V || K > 32 || M > 32) return std::nullopt;
   torch::NoGradGuard no_grad;
   Tensor x = logits.contiguous(), s = f32(scores), f = finished.has_value() ? finished->contiguous() : Tensor();
   Tensor best = torch::empty({N, M}, s.options().requires_grad(false)), tokens = torch::empty({N, M}, best.options().dtype(torch::kInt64)),
          parents = torch::empty({N, M}, best.options().dtype(torch::kInt32));
+  if (N == 0) return std::make_tuple(best, tokens, parents);
   const size_t n = gla_beam_select_workspace_bytes(N, K, V, M, dt_of(x));
   Tensor ws = bytes(x, n);
   check(gla_beam_select(stream_of(x), N, K, V, M, dt_of(x), ptr(x), (const float*)ptr(s), (const unsigned char*)ptr(f), pad, (float*)ptr(best),

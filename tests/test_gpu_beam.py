@@ -445,3 +445,17 @@ def test_selection_across_the_tiles_of_a_part(cuda_device, dtype):
         x = x.contiguous().to(dtype)
         for m in (M, 1, 5):
             same(beam_select(x, scores, m), selected(x, scores, m))
+
+
+def test_selection_and_moving_for_no_requests(cuda_device):
+    from gla_jax_b200 import beam_select, reorder_states
+    scores, tokens, parents = beam_select(torch.empty(0, 4, 50, device=cuda_device), torch.empty(0, 4, device=cuda_device), 3,
+                                          finished=torch.empty(0, 4, dtype=torch.bool, device=cuda_device))
+    assert scores.shape == tokens.shape == parents.shape == (0, 3) and (scores.dtype, tokens.dtype, parents.dtype) == (torch.float32, torch.int64, torch.int32)
+    reorder_states([torch.empty(0, 8, device=cuda_device)], torch.empty(0, 4, dtype=torch.int32, device=cuda_device))
+    with pytest.raises(ValueError):
+        beam_select(torch.empty(2, 0, 50, device=cuda_device), torch.empty(2, 0, device=cuda_device), 1)
+    with pytest.raises(ValueError):
+        beam_select(torch.empty(2, 4, 0, device=cuda_device), torch.empty(2, 4, device=cuda_device), 1)
+    with pytest.raises(ValueError):
+        reorder_states([torch.empty(0, 8, device=cuda_device)], torch.empty(2, 0, dtype=torch.int32, device=cuda_device))
