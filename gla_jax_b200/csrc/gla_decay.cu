@@ -95,16 +95,118 @@ __global__ void __launch_bounds__(256) share_sum_kernel(const float* x, T* out, 
   st_f(out, i, a.x); st_f(out, i + 1, a.y); st_f(out, i + 2, a.z); st_f(out, i + 3, a.w);
 }
 
-// dg_t = sum over i >= t of (q dq - k dk) + <S_T, dS_T>: a block per sequence and head, from the end, the running sum in
-// 64 bits.
-// The terms cancel over the sequence, while their errors (float32 products, some 2^-23 of each, cut off to one side) add up.
-// At the first token the sum has to be <S_0, dS_0>.  Where these states are float32, what it is off by is taken back, in
-// proportion to the magnitudes of the terms summed so far (2 x 250 tokens, 2 heads of 64: error 2.1e-6 of the norm without).
+// The pairs i >= t > j of a chunk of L tokens that gate t weighs, w_ij (q_i k_j)(do_i v_j) with float32 products: a block per chunk and
+// head, into dg.  Sums of all of a token's pairs, as q dq - k dk has them, would leave these as differences of two sums whose
+// errors then add up over the sequence (2 x 250 tokens, 2 heads of 64, gates of -3: 5e-6 of the norm against 6e-7; 2 us of 144).
+// It runs beside the walks, whose blocks are few where time is short: it reads nothing of theirs, and ends after them (so that what
+// follows in the stream finds both).
+template <typename T, int L>
+__global__ void __launch_bounds__(256) pairs_kernel(const Walk p, const T* dout, float* dg) {
+  constexpr int R = L / 16, W = 32;                    // rows and columns of a thread, features at a time
+  __shared__ float a[L][W + 1], b[L][W + 1], m[L][L + 1];
+  __shared__ double gate[L];
+  __shared__ float2 lam[L];
+  const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16, h = blockIdx.y;
+  // the chunk's first token, and the run's tokens from there on
+  int64_t t0, left;
+  if (!p.cu) {
+    const int64_t per = p.seg / L, i0 = blockIdx.x / per * p.seg % ((p.T + p.seg - 1) / p.seg * p.seg) + blockIdx.x % per * L;
+    t0 = blockIdx.x / per / ((p.T + p.seg - 1) / p.seg) * p.T + i0;
+    left = p.T - i0;
+  } else {
+    // sequence s, its run in cell c (see find_run) from token x on: chunks from number s + c + x / L on
+    int64_t l = 0, u = p.nseq - 1;
+    while (l < u) {
+      const int64_t s = (l + u + 1) / 2;
+      if (s + p.cu[s] / p.seg + p.cu[s] / L <= blockIdx.x) l = s; else u = s - 1;
+    }
+    const int64_t first = p.cu[l], end = p.cu[l + 1];
+    int64_t c = (blockIdx.x - l) / (1 + p.seg / L);
+    if (c < first / p.seg) c = first / p.seg;
+    const int64_t x = c * p.seg > first ? c * p.seg : first, hi = (c + 1) * p.seg < end ? (c + 1) * p.seg : end;
+    t0 = x + (blockIdx.x - l - c - x / L) * L;
+    left = hi - t0;
+  }
+  if (left <= 0) {
+    grid_dep_wait();
+    return;
+  }
+  const int nv = left < L ? (int)left : L;
+  if (tid < L) {
+    const float x = tid < nv ? p.g[(t0 + tid) * p.gt + h] : 0.f;
+    gate[tid] = (x < -200.f ? -200.f : x) * 1.4426950408889634;      // (as the walks take it)
+  }
+  __syncthreads();
+  if (tid < L) {
+    double v = 0.0;
+    for (int i = 0; i <= tid; ++i) v += gate[i];
+    const float hi = (float)v;
+    lam[tid] = make_float2(hi, (float)(v - hi));
+  }
+  float s[2][R][R] = {};
+  const int Hk = p.H / p.gk;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const int d = which ? p.vd : p.kd, heads = which ? p.H : Hk, at = which ? h : h / p.gk;
+    const T *x = which ? dout : (const T*)p.q, *y = which ? (const T*)p.v : (const T*)p.k;
+    for (int d0 = 0; d0 < d; d0 += W) {
+      __syncthreads();
+      for (int i = tid; i < L * W; i += 256) {
+        const int r = i / W, c = i % W;
+        const int64_t e = ((t0 + r) * heads + at) * d + d0 + c;
+        const bool in = r < nv && d0 + c < d;
+        a[r][c] = in ? ld_f(x, e) : 0.f;
+        b[r][c] = in ? ld_f(y, e) : 0.f;
+      }
+      __syncthreads();
+#pragma unroll 8
+      for (int c = 0; c < W; ++c) {
+        float u[R], v[R];
+#pragma unroll
+        for (int i = 0; i < R; ++i) { u[i] = a[ty + 16 * i][c]; v[i] = b[tx + 16 * i][c]; }
+#pragma unroll
+        for (int i = 0; i < R; ++i)
+#pragma unroll
+          for (int j = 0; j < R; ++j) s[which][i][j] = fmaf(u[i], v[j], s[which][i][j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int x = 0; x < R; ++x)
+#pragma unroll
+    for (int y = 0; y < R; ++y) {
+      const int i = ty + 16 * x, j = tx + 16 * y;
+      const float2 li = lam[i], lj = lam[j];
+      m[i][j] = j < i && i < nv ? s[0][x][y] * exp2f((li.x - lj.x) + (li.y - lj.y)) * s[1][x][y] : 0.f;
+    }
+  __syncthreads();
+  if (tid < L) {                                       // row i: m[i][t] = the sum over j < t
+    double sum = 0.0;
+    for (int j = 0; j < L; ++j) {
+      const float x = m[tid][j];
+      m[tid][j] = (float)sum;
+      sum += x;
+    }
+  }
+  __syncthreads();
+  if (tid < nv) {
+    double sum = 0.0;
+    for (int i = tid; i < nv; ++i) sum += m[i][tid];
+    dg[(t0 + tid) * p.H + h] = (float)sum;
+  }
+  grid_dep_wait();
+}
+
+// dg_t = the chunk's pairs (in dg) + sum over i >= t of (a_i - b_i) + <S_T, dS_T>: a block per sequence and head, from the end, the
+// running sum in 64 bits.
+// The errors of a and b (float32 products, some 2^-23 of each, cut off to one side) add up.  At the first token the sum has to be
+// <S_0, dS_0>: where these states are float32, what it is off by is taken back, in proportion to the magnitudes summed so far
+// (10 x 16384 tokens, 8 heads of 64, soft gates: 6e-7 to 2.3e-6 of the norm without, 5e-7 to 8e-7 with it).
 // A value or key that is not finite makes the sum not finite from there back, where dg reads neither: those tokens are summed
-// from the other end, dg_t = <S_0, dS_0> - sum over i < t.
+// from the other end, <S_0, dS_0> - sum over i < t.
 struct Gate {
-  const float *rq, *rk;             // [tiles][token][H]
-  int nq, nk;
+  const float *a, *b;               // [tiles][token][H]
+  int tiles;
   const int* cu;
   int64_t T, nseq, rows;
   int H;
@@ -117,6 +219,7 @@ struct Gate {
 __global__ void __launch_bounds__(512) gate_grad_kernel(const Gate p) {
   __shared__ double part[16];
   __shared__ double carry;
+  __shared__ unsigned long long bad;
   const int64_t s = blockIdx.x, h = blockIdx.y;
   const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32;
   int64_t a = s * p.T, b = a + p.T;
@@ -125,12 +228,13 @@ __global__ void __launch_bounds__(512) gate_grad_kernel(const Gate p) {
     if (s == p.nseq - 1)
       for (int64_t t = b + tid; t < p.T; t += 512) p.dg[t * p.H + h] = 0.f;
   }
-  const auto term = [&](int64_t t, double& size) {
+  double rate = 0.0;
+  const auto term = [&](int64_t t, double* size) {
     double x = 0.0, y = 0.0;
-    for (int i = 0; i < p.nq; ++i) x += p.rq[(i * p.rows + t) * p.H + h];
-    for (int i = 0; i < p.nk; ++i) y += p.rk[(i * p.rows + t) * p.H + h];
-    size = fabs(x) + fabs(y);
-    return x - y;
+    for (int i = 0; i < p.tiles; ++i) { x += p.a[(i * p.rows + t) * p.H + h]; y += p.b[(i * p.rows + t) * p.H + h]; }
+    const double m = fabs(x) + fabs(y);
+    if (size) *size = m;
+    return rate == 0.0 ? x - y : x - y - rate * m;
   };
   const auto total = [&](double x) {
 #pragma unroll
@@ -143,7 +247,7 @@ __global__ void __launch_bounds__(512) gate_grad_kernel(const Gate p) {
     return x;
   };
   const int64_t at0 = (s * p.H + h) * p.dd;
-  double dot = 0.0, off = 0.0, all = 0.0;
+  double dot = 0.0;
   for (int64_t e = tid; e < p.dd; e += 512) dot += (double)p.S[at0 + e] * ld_any(p.dS, !p.state_f32, at0 + e);
   dot = total(dot);
   const auto first = [&]() {
@@ -152,27 +256,22 @@ __global__ void __launch_bounds__(512) gate_grad_kernel(const Gate p) {
     return x;
   };
   if (p.state_f32) {
-    off = -first();
+    double off = -first(), all = 0.0;
     for (int64_t t = a + tid; t < b; t += 512) {
       double m;
-      off += term(t, m);
+      off += term(t, &m);
       all += m;
     }
     off = total(off) + dot;
     all = total(all);
+    // none where something is not finite, which has to stay with its tokens
+    if (all > 0.0 && isfinite(off / all)) rate = off / all;
   }
-  // per magnitude; none where something is not finite, which has to stay with its tokens
-  const double rate = p.state_f32 && all > 0.0 && isfinite(off / all) ? off / all : 0.0;
-  if (tid == 0) carry = dot;
+  if (tid == 0) { carry = dot; bad = 0; }
   __syncthreads();
   for (int64_t end = b; end > a; end -= 512) {
     const int64_t t = end - 1 - tid;
-    double x = 0.0;
-    if (t >= a) {
-      double m;
-      x = term(t, m);
-      if (rate != 0.0) x -= rate * m;
-    }
+    double x = t >= a ? term(t, nullptr) : 0.0;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const double y = __shfl_up_sync(0xffffffffu, x, d);
@@ -183,16 +282,20 @@ __global__ void __launch_bounds__(512) gate_grad_kernel(const Gate p) {
     double before = carry;
     for (int w = 0; w < warp; ++w) before += part[w];
     x += before;
-    if (t >= a) p.dg[t * p.H + h] = (float)x;
+    if (t >= a) {
+      if (isfinite(x)) p.dg[t * p.H + h] = (float)(x + p.dg[t * p.H + h]);
+      else atomicMax(&bad, (unsigned long long)(t - a + 1));
+    }
     __syncthreads();
     if (tid == 511) carry = x;
     __syncthreads();
   }
-  if (isfinite(carry)) return;
+  const int64_t back = a + (int64_t)bad;                            // tokens before it are still to be done
+  if (back == a) return;
   double before = total(first());
-  for (int64_t t0 = a; t0 < b; t0 += 512) {
+  for (int64_t t0 = a; t0 < back; t0 += 512) {
     const int64_t t = t0 + tid;
-    double m, x = t < b ? term(t, m) : 0.0;
+    double x = t < back ? term(t, nullptr) : 0.0;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const double y = __shfl_up_sync(0xffffffffu, x, d);
@@ -206,7 +309,7 @@ __global__ void __launch_bounds__(512) gate_grad_kernel(const Gate p) {
       if (w < warp) y -= part[w];
       before -= part[w];
     }
-    if (t < b && !isfinite(p.dg[t * p.H + h])) p.dg[t * p.H + h] = (float)y;
+    if (t < back) p.dg[t * p.H + h] = (float)(y + p.dg[t * p.H + h]);
     __syncthreads();
   }
 }
@@ -423,6 +526,20 @@ static int share_sum(cudaStream_t st, const Dims& d, const float* x, void* out) 
   GLA_CHECK_LAUNCH();
   return GLA_OK;
 }
+// (the runs are those of the walks for dq and dk)
+template <typename T, int L>
+static int pairs(cudaStream_t st, const Dims& d, const int* cu, const float* g, int64_t gt, const void* v, const void* k, const void* q,
+                 const void* dout, float* dg) {
+  Walk p{};
+  p.H = (int)d.H; p.T = d.T; p.nseq = d.seqs(); p.seg = d.seg(d.Dk); p.nslots = d.slots(p.seg);
+  p.g = g; p.gt = gt; p.cu = cu;
+  p.q = q; p.k = k; p.v = v; p.gk = (int)(d.H / d.Hk); p.kd = (int)d.Dk; p.vd = (int)d.Dv;
+  const int64_t chunks = cu ? p.nslots + (d.T + L - 1) / L : p.nslots * (p.seg / L);
+  if (chunks > 2147483647LL) return GLA_ERR_TOO_LARGE;
+  ProfScope ps("decay_pairs_kernel", st);
+  GLA_LAUNCHED(launch_overlapped(pairs_kernel<T, L>, dim3((unsigned)chunks, (unsigned)d.H), dim3(256), 0, st, p, (const T*)dout, dg));
+  return GLA_OK;
+}
 int bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const float* g, int64_t gt, const void* v, const void* k,
         const void* q, const void* saved, const void* dhf, const void* dout, void* dh, float* dg, void* dv, void* dk, void* dq, void* ws) {
   if (cu) cu = (const int*)((const char*)saved + saved_states(d));
@@ -462,8 +579,10 @@ int bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const flo
     GLA_TRY(run_walk(st, d, mode, t, ws, "decay_runs_kernel", "decay_dv_kernel"));
   }
   if (dg) {
+    const int s = d.bf ? pairs<bf16, Mode<M_FINE>::L>(st, d, cu, g, gt, v, k, q, dout, dg) : pairs<float, Mode<M_FULL>::L>(st, d, cu, g, gt, v, k, q, dout, dg);
+    if (s != GLA_OK) return s;
     Gate w{};
-    w.rq = rq; w.rk = rk; w.nq = w.nk = (int)((d.Dk + 127) / 128);
+    w.a = rq; w.b = rk; w.tiles = (int)((d.Dk + 127) / 128);
     w.cu = cu; w.T = d.T; w.nseq = d.seqs(); w.rows = d.rows(); w.H = (int)d.H;
     w.S = (const float*)saved; w.dS = dhf; w.S0 = h0; w.dS0 = dh; w.state_f32 = d.hid_f32; w.dd = d.Dk * d.Dv; w.dg = dg;
     ProfScope ps("decay_gate_grad_kernel", st);

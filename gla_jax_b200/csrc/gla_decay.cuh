@@ -15,7 +15,8 @@
 //   dq = walk(q: dO, k: v, v: k, state: S^T)           forwards
 //   dv = walk(q: k, k: q, v: dO, state: dS)            backwards in time, the gate of the next token at each step
 //   dk = walk(q: v, k: dO, v: q, state: dS^T)          backwards
-// and dg_t = sum_{i >= t} (q_i dq_i - k_i dk_i) + <S_T, dS_T>.
+// and dg_t = sum over i >= t > j of w_ij (q_i k_j)(do_i v_j), pairs of a chunk one by one, the others by what comes from outside it:
+//   dg_t = <S_T, dS_T> + sum over i >= t of (a_i - b_i) + the chunk's pairs,   a = q . (dq from before), b = k . (dk from behind)
 //
 // Types.  bf16 operands go to the tensor cores as they are, float32 ones as three bf16 planes (8 + 8 + 8 bits).  What the
 // kernel forms itself (scores, the state as an operand, weighted values) is split into as many planes as the mode says.
@@ -61,7 +62,7 @@ struct Walk {
   double* seg_total;                // [slot][H]: log2 of a run's decay
   void* out;                        // [token][H][vd]
   int out_f32;
-  const void* r;                    // rows multiplied with out's (float32) into rdot: [token][heads][vd]; may be NULL
+  const void* r;                    // rows multiplied into rdot with what comes from outside the chunk: [token][heads][vd]; may be NULL
   int gr;
   float* rdot;                      // [vt][token][H]
 };
@@ -220,6 +221,7 @@ __global__ void __launch_bounds__(NW * 32, KD <= 128 && MODE <= M_STATE ? 16 / N
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, gr = lane / 4, tq = lane % 4;
   const int h = blockIdx.y % p.H, vt = blockIdx.y / p.H;
   const int cbase = vt * Y::VT, cw = cbase + warp * 16;        // first value column of the block, of the warp
+  grid_dep_launch();
   const Run run = find_run(p, blockIdx.x);
   if constexpr (OUT) {
     if (run.zlo < run.zhi) {
@@ -249,8 +251,9 @@ __global__ void __launch_bounds__(NW * 32, KD <= 128 && MODE <= M_STATE ? 16 / N
   const int64_t len = run.hi - run.lo;
   const int dir = p.rev ? -1 : 1;
   double total = 0.0;                                          // of the run (warp 0)
-  for (int64_t c0 = 0; c0 < len; c0 += L) {
-    const int nv = len - c0 < L ? (int)(len - c0) : L;
+  // (chunks lie the same in both directions: a part of one comes first backwards)
+  int nv = p.rev ? (int)((len - 1) % L) + 1 : len < L ? (int)len : L;
+  for (int64_t c0 = 0; c0 < len; c0 += nv, nv = len - c0 < L ? (int)(len - c0) : L) {
     const int64_t t0 = run.base + (p.rev ? run.hi - 1 - c0 : run.lo + c0);     // token of row 0
     load_tile<MODE, KD, Y::LDK, Y::PK, NT>(sm + Y::K0, p.k, (t0 * Hk + h / p.gk) * p.kd, (int64_t)dir * Hk * p.kd, nv, p.kd);
     {
@@ -404,7 +407,7 @@ __global__ void __launch_bounds__(NW * 32, KD <= 128 && MODE <= M_STATE ? 16 / N
             for (int n = 0; n < 2; ++n) {
               const int c = cw + n * 8 + 2 * tq;
               if (c < p.vd) {
-                const float x = o[n][2 * half], y = o[n][2 * half + 1];
+                const float x = o[n][2 * half], y = o[n][2 * half + 1], bx = keep[n][2 * half], by = keep[n][2 * half + 1];
                 const int64_t at = (tok * p.H + h) * p.vd + c;
                 if (p.out_f32) *reinterpret_cast<float2*>((float*)p.out + at) = make_float2(x, y);
                 else *reinterpret_cast<uint32_t*>((bf16*)p.out + at) = pack_bf16x2(x, y);
@@ -413,7 +416,7 @@ __global__ void __launch_bounds__(NW * 32, KD <= 128 && MODE <= M_STATE ? 16 / N
                   float2 rv;
                   if constexpr (MODE == M_FULL) rv = __ldg((const float2*)((const float*)p.r + ra));
                   else rv = pair_of(__ldg((const unsigned int*)((const bf16*)p.r + ra)));
-                  dot[half] = fmaf(x, rv.x, fmaf(y, rv.y, dot[half]));
+                  dot[half] = fmaf(bx, rv.x, fmaf(by, rv.y, dot[half]));
                 }
               }
             }

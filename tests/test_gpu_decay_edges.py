@@ -165,3 +165,40 @@ def test_large_products_under_decay(cuda_device, rate, D):
     cots = [torch.randn_like(xs[0]), torch.randn_like(xs[2]) * 2.0 ** 20]
     got, grads = with_grads(chunk_decay_attention, xs, cots)
     check(xs, cots, got, grads, torch.bfloat16, torch.float32, rate)
+
+
+@pytest.mark.parametrize("shift", [-3.0, 0.0, 3.0])
+@pytest.mark.parametrize("size", [(2, 250, 2, 2, 64, 64), (1, 900, 4, 2, 128, 32), (1, 333, 2, 1, 24, 200)])
+def test_float32_gates_gradient_under_sharp_gates(cuda_device, size, shift):
+    """A gate's gradient is about the tokens that it weighs, however many others there are: pairs inside a chunk of 32 are summed as
+    they are, and the sums of what comes from outside a chunk, each of its own size, are off by some 2^-23 of theirs: 2^-20 of the
+    norm for up to 28 chunks, whose errors fall either way."""
+    from gla_jax_b200 import chunk_decay_attention
+    xs = make(cuda_device, *size, torch.float32, torch.float32, seed=21, shift=shift)
+    gen = torch.Generator(device=cuda_device).manual_seed(22)
+    cots = [torch.randn(x.shape, generator=gen, device=cuda_device) for x in (xs[0], xs[2])]
+    _, want = with_grads(recurrence, [x.double() for x in xs], [c.double() for c in cots])
+    _, got = with_grads(chunk_decay_attention, xs, cots)
+    for b in range(size[0]):
+        for h in range(size[2]):
+            err = (got[1][b, :, h].double() - want[1][b, :, h]).norm() / want[1][b, :, h].norm()
+            assert err <= 2.0 ** -20, (b, h, err.item())
+
+
+def test_float32_packed_gates_gradient_under_sharp_gates(cuda_device):
+    """The same for packed sequences, which are cut at cells of the axis, and whose chunks start at their first token."""
+    from gla_jax_b200 import chunk_decay_attention_packed
+    lens = [5, 0, 470, 1, 33, 0, 600, 64]
+    T = sum(lens) + 9
+    xs, cots = packed(cuda_device, len(lens), T, 2, 1, 64, 64, torch.float32, seed=23)
+    xs[1] = xs[1] - 2.0
+    cu = [0, *torch.tensor(lens).cumsum(0).tolist()]
+    _, got = with_grads(lambda *a: chunk_decay_attention_packed(*a, torch.tensor(cu, device=cuda_device)), xs, cots)
+    for s, (a, b) in enumerate(zip(cu, cu[1:])):
+        if a == b:
+            continue
+        one = [xs[0][s:s + 1], *(x[None, a:b] for x in xs[1:])]
+        _, want = with_grads(recurrence, [x.double() for x in one], [cots[0][s:s + 1].double(), cots[1][None, a:b].double()])
+        err = (got[1][a:b].double() - want[1][0]).norm() / want[1].norm()
+        assert err <= 2.0 ** -20, (s, err.item())
+    assert (got[1][cu[-1]:] == 0).all()
