@@ -392,9 +392,10 @@ static int run_walk(cudaStream_t st, const Dims& d, int mode, const Walk& p, voi
 // ---- bf16, head sizes up to 128: the walks of gla_decay_tc.cuh and gla_decay_tcb.cuh ---------------------------------------------------------
 static bool fast(const Dims& d) { return d.bf && d.Dk <= 128 && d.Dv <= 128; }
 static size_t state_bytes(const Dims& d, int64_t n) { return align_up((size_t)(n * d.H * d.Dk * d.Dv) * 4, 256); }
-// saved: final states in float32 | states that enter the runs (where sequences are cut) | offsets (where packed)
+// saved: final states in float32 | states that enter the runs (where sequences are cut) | offsets (where packed).  The first two for
+// the walks below only: the others' backward makes its own, with more digits than their forward has.
 static size_t saved_states(const Dims& d) {
-  return state_bytes(d, d.seqs()) + (fast(d) && d.cut(d.seg(128)) ? state_bytes(d, d.slots(d.seg(128))) : 0);
+  return fast(d) ? state_bytes(d, d.seqs()) + (d.cut(d.seg(128)) ? state_bytes(d, d.slots(d.seg(128))) : 0) : 0;
 }
 static size_t offset_bytes(const Dims& d) { return d.nseq ? align_up((size_t)(d.nseq + 1) * 4, 256) : 0; }
 size_t saved_bytes(const Dims& d) { return saved_states(d) + offset_bytes(d); }
@@ -493,7 +494,7 @@ int fwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const flo
   p.gq = p.gk = (int)(d.H / d.Hk); p.gv = 1;
   p.kd = (int)d.Dk; p.vd = (int)d.Dv;
   p.g = g; p.gt = gt; p.cu = cu;
-  p.init = h0; p.fin = hf; p.fin32 = (float*)saved; p.ik = d.Dv; p.ic = 1; p.init_f32 = p.fin_f32 = d.hid_f32;
+  p.init = h0; p.fin = hf; p.ik = d.Dv; p.ic = 1; p.init_f32 = p.fin_f32 = d.hid_f32;
   p.out = out; p.out_f32 = !d.bf;
   return run_walk(st, d, !d.bf ? M_FULL : d.hid_f32 ? M_STATE : M_ONE, p, ws, "decay_runs_kernel", "decay_walk_kernel");
 }
@@ -511,7 +512,8 @@ static size_t bwd_parts(const Dims& d, bool gate, size_t (&at)[5]) {
   at[1] = at[0] + dots;
   at[2] = at[1] + dots;
   at[3] = at[2] + (share > 1 ? align_up((size_t)(d.rows() * d.H * d.Dk) * 4, 256) : 0);
-  return at[3];
+  at[4] = at[3] + (gate ? state_bytes(d, d.seqs()) : 0);
+  return at[4];
 }
 size_t bwd_ws_bytes(const Dims& d, bool gate) {
   size_t at[5], fa[4];
@@ -546,7 +548,8 @@ int bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const flo
   if (fast(d)) return fast_bwd(st, d, cu, h0, g, gt, v, k, q, saved, dhf, dout, dh, dg, dv, dk, dq, ws);
   size_t at[5];
   bwd_parts(d, dg != nullptr, at);
-  float *rq = (float*)((char*)ws + at[0]), *rk = (float*)((char*)ws + at[1]), *wide = (float*)((char*)ws + at[2]);
+  float *rq = (float*)((char*)ws + at[0]), *rk = (float*)((char*)ws + at[1]), *wide = (float*)((char*)ws + at[2]),
+        *last = (float*)((char*)ws + at[3]);                    // the final states
   const int share = (int)(d.H / d.Hk), mode = d.bf ? M_FINE : M_FULL;
   Walks all{};
   Walk &p = all.w[0], &r = all.w[1], &t = all.w[2];
@@ -555,7 +558,7 @@ int bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const flo
   r = t = p;
   // dq, forwards over the states of the forward, transposed
   p.q = dout; p.k = v; p.v = k; p.gq = p.gk = 1; p.gv = share; p.kd = (int)d.Dv; p.vd = (int)d.Dk;
-  p.init = h0; p.ik = 1; p.ic = d.Dv;
+  p.init = h0; p.ik = 1; p.ic = d.Dv; p.fin32 = dg ? last : nullptr;
   p.out = share > 1 ? (void*)wide : dq; p.out_f32 = share > 1 || !d.bf;
   p.r = dg ? q : nullptr; p.gr = share; p.rdot = rq;
   // dk, backwards
@@ -584,7 +587,7 @@ int bwd(cudaStream_t st, const Dims& d, const int* cu, const void* h0, const flo
     Gate w{};
     w.a = rq; w.b = rk; w.tiles = (int)((d.Dk + 127) / 128);
     w.cu = cu; w.T = d.T; w.nseq = d.seqs(); w.rows = d.rows(); w.H = (int)d.H;
-    w.S = (const float*)saved; w.dS = dhf; w.S0 = h0; w.dS0 = dh; w.state_f32 = d.hid_f32; w.dd = d.Dk * d.Dv; w.dg = dg;
+    w.S = last; w.dS = dhf; w.S0 = h0; w.dS0 = dh; w.state_f32 = d.hid_f32; w.dd = d.Dk * d.Dv; w.dg = dg;
     ProfScope ps("decay_gate_grad_kernel", st);
     gate_grad_kernel<<<dim3((unsigned)w.nseq, (unsigned)d.H), 512, 0, st>>>(w);
     GLA_CHECK_LAUNCH();
@@ -656,11 +659,12 @@ int gla_decay_bwd(void* stream, int64_t B, int64_t T, int64_t H, int64_t Hk, int
                   const void* value, const void* key, const void* query, const void* saved, const void* dhidden_final,
                   const void* dout, void* dhidden_init, float* dlog_decay, void* dvalue, void* dkey, void* dquery, void* workspace,
                   size_t workspace_bytes) {
-  if (!hidden_init || !log_decay || !value || !key || !query || !dhidden_final || !dout || !saved || !dhidden_init || !dvalue || !dkey ||
+  if (!hidden_init || !log_decay || !value || !key || !query || !dhidden_final || !dout || !dhidden_init || !dvalue || !dkey ||
       !dquery)
     return GLA_ERR_NULL_POINTER;
   const Dims d = dims_of(B, T, H, Hk, Dk, Dv, dtype, hidden_dtype, nseq);
   GLA_TRY(decay::check(d, dtype, hidden_dtype, cu_seqlens));
+  if (!saved && decay::saved_bytes(d)) return GLA_ERR_NULL_POINTER;
   for (const void* p : {value, key, query, saved, dout, (const void*)dvalue, (const void*)dkey, (const void*)dquery})
     if (!aligned16(p)) return GLA_ERR_ALIGNMENT;
   const size_t need = decay::bwd_ws_bytes(d, dlog_decay != nullptr);

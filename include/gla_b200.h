@@ -518,9 +518,9 @@ GLA_API int gla_sp_combine2(void* stream, int64_t R, int64_t rank, int64_t BH, i
  * Dk and Dv multiples of 8 up to 256; any T > 0; H a multiple of Hk, at most 16383.  `dtype` is that of value, key, query, out and their
  * gradients; hidden_dtype that of hidden_init, hidden_final and their gradients: dtype or GLA_F32.  value, key, query, out and
  * gradients 16-byte aligned.
- * A forward that will be differentiated gets `saved` (gla_decay_saved_bytes), which the backward reads: final states in
- * float32, where few heads make the library cut sequences into runs the states that enter the runs, and the offsets as they
- * were used.  NULL otherwise.
+ * A forward that will be differentiated gets `saved` (gla_decay_saved_bytes, which may be 0), which the backward reads: in bf16 up to
+ * head size 128 final states in float32 and, where few heads make the library cut sequences into runs, the states that enter the
+ * runs; the offsets as they were used.  NULL otherwise.
  * bf16, head sizes up to 128: scores and the state as an operand are rounded to bf16 once, decayed values to two bf16
  * planes (three where hidden is float32; the state in two where dlog_decay is asked for); sums, states and decays in float32
  * and more.  bf16 beyond: one plane of each in the forward, two in the backward.  float32: three planes everywhere.

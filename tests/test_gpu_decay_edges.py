@@ -202,3 +202,20 @@ def test_float32_packed_gates_gradient_under_sharp_gates(cuda_device):
         err = (got[1][a:b].double() - want[1][0]).norm() / want[1].norm()
         assert err <= 2.0 ** -20, (s, err.item())
     assert (got[1][cu[-1]:] == 0).all()
+
+
+@pytest.mark.parametrize("size", [(1, 3000, 2, 2, 256, 64), (2, 1500, 40, 40, 64, 136), (1, 700, 1, 1, 136, 256), (1, 3000, 2, 2, 128, 64),
+                                  (2, 1500, 40, 40, 128, 128)])
+def test_gates_gradient_far_from_the_end(cuda_device, size):
+    """A cotangent of the final state reaches the gates of the last few tokens only, when memories are short: what the others get
+    besides is the error of the sum that starts at <S_T, dS_T>, whose parts are held in two bf16 planes and more (2^-16 each)."""
+    from gla_jax_b200 import chunk_decay_attention
+    xs = make(cuda_device, *size, torch.bfloat16, torch.bfloat16, seed=24, shift=0.0)
+    cots = [torch.randn_like(xs[0]), torch.zeros_like(xs[2])]
+    _, got = with_grads(chunk_decay_attention, xs, cots)
+    up = [x.double().requires_grad_(i == 1) for i, x in enumerate(xs)]
+    hf, _ = recurrence(*up)
+    want = torch.autograd.grad(hf, up[1], cots[0].double())[0]
+    far = got[1][:, : size[1] - 300].double()
+    assert want[:, : size[1] - 300].abs().max() < 1e-9
+    assert far.abs().max() <= 2.0 ** -13 * want.abs().max(), (far.abs().max().item(), want.abs().max().item())
