@@ -219,3 +219,41 @@ def test_gates_gradient_far_from_the_end(cuda_device, size):
     far = got[1][:, : size[1] - 300].double()
     assert want[:, : size[1] - 300].abs().max() < 1e-9
     assert far.abs().max() <= 2.0 ** -13 * want.abs().max(), (far.abs().max().item(), want.abs().max().item())
+
+
+@pytest.mark.parametrize("dtype,D,packs", [(torch.float32, 64, False), (torch.float32, 64, True), (torch.bfloat16, 136, True), (torch.bfloat16, 64, True)])
+def test_backward_in_a_graph_beside_another_stream(cuda_device, dtype, D, packs):
+    """Kernels that run beside others inside a call: captured, replayed with new inputs while another stream is at work."""
+    from gla_jax_b200 import chunk_decay_attention, chunk_decay_attention_packed
+    T = 700
+    cu = torch.tensor([0, 300, 301, 640], dtype=torch.int32, device=cuda_device)
+    sets = []
+    for seed in (31, 32):
+        if packs:
+            sets.append(packed(cuda_device, 3, T, 2, 1, D, D, dtype, seed=seed))
+        else:
+            xs = make(cuda_device, 2, T, 2, 1, D, D, dtype, dtype, seed=seed)
+            sets.append((xs, [torch.randn_like(xs[0]), torch.randn_like(xs[2])]))
+    f = (lambda *a: chunk_decay_attention_packed(*a, cu)) if packs else chunk_decay_attention
+    leaves, cots = [x.clone().requires_grad_(True) for x in sets[0][0]], [c.clone() for c in sets[0][1]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(f(*leaves), leaves, cots)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = f(*leaves)
+        grads = torch.autograd.grad(outs, leaves, cots)
+    want, gw = with_grads(f, *sets[1])
+    with torch.no_grad():
+        for a, b in zip([*leaves, *cots], [*sets[1][0], *sets[1][1]]):
+            a.copy_(b)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            other, go = with_grads(f, *sets[1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip([*outs, *grads], [*want, *gw]))
+        assert all(torch.equal(a, b) for a, b in zip([*other, *go], [*want, *gw]))
