@@ -25,8 +25,8 @@ def beam_select(logits, scores, num_select: Optional[int] = None, finished=None,
     """The ``num_select`` (default: the number of beams) best continuations of each request.
 
     ``logits`` (N, K, V) float32 or bfloat16, ``scores`` (N, K): log-probabilities of the beams so far, finite or ``-inf``.
-    Continuations rank by ``scores + log_softmax(logits)``, formed in 64 bits, the lowest (beam, token) first among equal
-    ones.  Returns the totals (N, M) in float32, tokens (N, M) int64 and parents (N, M) int32, best first.
+    Continuations rank by ``scores + log_softmax(logits)``, formed in 64 bits from float32 scores and sums of float32
+    exponentials, the lowest (beam, token) first among equal ones.  Returns the totals (N, M) in float32, tokens (N, M) int64 and parents (N, M) int32, best first.
 
     ``-inf`` or NaN masks a token; a beam without any token left, or with a score of ``-inf`` or NaN, offers totals of
     ``-inf``.  ``finished`` (N, K) bool: such a beam goes on with ``pad_token`` alone, at its score.  K and M are at most

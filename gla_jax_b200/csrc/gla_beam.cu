@@ -193,9 +193,9 @@ static int launch_beams(cudaStream_t st, const Step& p, int64_t groups) {
   GLA_LAUNCHED(launch_overlapped(step_beams_kernel<W, KEYED>, dim3((unsigned)((p.Dv + W - 1) / W * groups)), dim3(SNT), smem, st, p));
   return GLA_OK;
 }
-// Columns per block: as many as leave room for six blocks on an SM, so that one block's copies run beside another's steps
-// (16 requests of 4 beams, 16 heads of 128 x 64: 25.2 us with 32 columns and three blocks); below 16 the rows of a block no
-// longer fill 64 bytes.
+// Columns per block: as many as leave room for five or six blocks on an SM, so that one block's copies run beside another's steps
+// (16 requests of 4 beams, 16 heads of 128 x 64: 17 us with 16 columns, 25 with 32 and three blocks); below 16 the rows of a block no
+// longer fill 64 bytes.  Half the copy rate: 1.4 rounds of blocks, each of which loads, waits and then stores.
 template <bool KEYED>
 static int step_beams(cudaStream_t st, const Step& p, int64_t groups) {
   const int64_t col = (int64_t)p.K * (p.Dk + 31) / 32 * 32 * 4;      // bytes of a column
@@ -275,7 +275,9 @@ static int launch_reorder(cudaStream_t st, const Tensors& t) {
 // that a model leaves, but a sorted row may), the M largest are found one after the other.
 // Measured, 64 x 8 rows of 128000 bf16 logits, M = 16, the pass alone: lists in shared memory that are cut as they grow 136 us,
 // a sorted list per warp 312 us, the two largest with their places 79 us, this 57 us (the bytes at the copy rate: 17.5); both
-// kernels 70 us.  What bounds it: instructions, some ten a logit and an exponential, and the search at the end of each part.
+// kernels 70 us.  What bounds it: 64 registers leave room for four blocks on an SM, so that the 900 or so that have a live row come in
+// two rounds of 592, the second half empty (40 % of the warps there could be, instructions in 57 % of the cycles, HBM at 24 %), with
+// one tile of a part on its way.
 // A key is (order of the value, lowest index first), 0: none.
 typedef unsigned long long u64;
 __device__ __forceinline__ unsigned int order_of(float x) {
@@ -657,7 +659,7 @@ __global__ void __launch_bounds__(BNT) select_beams_kernel(const Select p) {
   }
 }
 
-// Parts of a row: enough blocks for the device (six per SM), few enough that a request's candidates fit.
+// Parts of a row: six blocks for each SM (four are resident, three in float32), few enough that a request's candidates fit.
 static void plan(int64_t rows, int64_t V, int K, int M, int* parts, int64_t* part) {
   const int64_t tiles = (V + TILE - 1) / TILE;
   int64_t n = (6 * 148 + rows - 1) / rows;

@@ -53,7 +53,8 @@ def chunk_decay_attention(hidden_init, log_decay, value, key, query) -> Tuple[to
     ``value`` (B, T, H, Dv), ``key`` and ``query`` (B, T, Hk, Dk) with ``H`` a multiple of ``Hk`` (value head ``h`` uses key
     head ``h // (H // Hk)``), ``hidden_init`` (B, H, Dk, Dv); without the batch axis everywhere, one sequence.
     ``log_decay`` (B, T, H), or (H,) for decays that do not depend on the token, is converted to float32; ``-inf`` resets the
-    state.  Head sizes are multiples of 8 up to 256, ``T`` is any.  float32 or bfloat16; ``hidden_init`` (and with it
+    state.  Head sizes are multiples of 8 up to 256, ``T`` is any, ``H`` up to 16383.  float32 or bfloat16 (products of a query
+    and a key below 2^62, as of a value and its cotangent); ``hidden_init`` (and with it
     ``hidden_final``) may be float32 beside bfloat16 arrays, for a state that ``decay_attention_step`` goes on with."""
     r = _lib.native().chunk_decay(hidden_init, log_decay, value, key, query, None)
     return r if r is not None else _refused("chunk_decay_attention", hidden_init, log_decay, value, key, query, False)

@@ -524,6 +524,10 @@ GLA_API int gla_sp_combine2(void* stream, int64_t R, int64_t rank, int64_t BH, i
  * bf16, head sizes up to 128: scores and the state as an operand are rounded to bf16 once, decayed values to two bf16
  * planes (three where hidden is float32; the state in two where dlog_decay is asked for); sums, states and decays in float32
  * and more.  bf16 beyond: one plane of each in the forward, two in the backward.  float32: three planes everywhere.
+ * Where a chunk's decay is mild its scores carry up to 2^64 of it on their way: bf16 calls up to head size 128 want products of a
+ * query and a key, in the backward of a value and its cotangent too, below 2^62.
+ * What is not finite stays with the tokens that read it (as not-a-number, where the recurrence may have an infinity), the gates'
+ * gradient between a query or cotangent that is not finite and a later value or key that is not excepted.
  * Backward: dlog_decay (B, T, H) float32 or NULL; dhidden_init as hidden_init.
  * Workspace: gla_decay_workspace_bytes for the forward without (what = 0) and with `saved` (1), the backward without (2)
  * and with dlog_decay (3); 0 bytes may be needed, or the sizes may be unsupported (the calls say which).
@@ -553,11 +557,12 @@ GLA_API int gla_decay_bwd(void* stream, int64_t B, int64_t T, int64_t H, int64_t
  *                          float32, value (B, H, Dv), key and query (B, Hk, Dk), out (B, H, Dv) in out_dtype.  With parents
  *                          (B = requests * beams) every row is stepped from its parent's state; the moves cost no pass.
  *   gla_decode_step_beams  gla_decode_step (a decay per key feature) with parents.
- *   gla_reorder_states     rows of `count` tensors (HOST arrays of device addresses and of bytes per row) moved to where
+ *                          Both: Dk and Dv as above; any number of rows.
+ *   gla_reorder_states     rows of `count` tensors (0 included; HOST arrays of device addresses and of bytes per row) moved to where
  *                          the parents say, in place; rows that stay are not touched.  The tensors must not overlap.
  *   gla_beam_select        logits (N, K, V) in dtype, scores (N, K) float32 (finite or -inf): the M best of each request's K V
  *                          totals scores[k] + log_softmax(logits[k])[v], largest first, the lowest (k, v) first among equal
- *                          ones; totals in 64 bits.  A logit of -inf or NaN is masked (a row of them has no continuation:
+ *                          ones; totals in 64 bits, from sums of float32 exponentials (2^-20).  A logit of -inf or NaN is masked (a row of them has no continuation:
  *                          totals of -inf), +inf counts as the largest finite number.  A beam with a score of -inf or NaN has totals of
  *                          -inf.  finished (N, K) bytes or NULL: such a beam continues with pad_token alone, at its score,
  *                          and its logits are not read.  out_scores (N, M) float32, tokens (N, M), parents (N, M).  K, M <= 32,
