@@ -19,8 +19,8 @@
 //
 // Roundings.  P and the state's image are one bf16 plane, as in this library's other chunk kernels: 2^-9 of each term, which leaves
 // outputs 2.3e-3 of their norm off, where their own rounding to bf16 is 1.7e-3.  Two planes of the state cost its second product and
-// the second stage of K: 8.2 us a chunk instead of 4.9, which only the gates' gradient is worth, whose terms cancel.  The state itself,
-// its sums and the gates' are in 32 bits and more.
+// the second stage of K: 8.2 us a chunk instead of 4.9, which only a backward with the gates' gradient is worth, whose terms cancel;
+// there P has two planes as well (3 % of the call).  The state itself, its sums and the gates' are in 32 bits and more.
 //
 // Tiles: 128 rows x 64 columns of bf16, 128-byte rows, 16-byte pieces at piece ^ (row % 8) (tc_ptx.cuh); D columns are D / 64
 // of them.  A copy brings 128 rows whatever the sequence's length: rows past its end are another sequence's or beyond the
@@ -296,8 +296,36 @@ __device__ __forceinline__ bool check_rows(uint32_t tile, int nv) {
 }
 // What is not finite in OA = P V, by sums over the tokens up to the row's own: in the product, zeros of P meet what is not finite
 // in V, and 0 x inf is not a number, where the recurrence has it at its own token and after only.
-// P: this lane's row in tensor memory, 32 tokens in 16 columns at multiples of 32; 16 columns of V at a time.
-template <int DV>
+// P: this lane's row in tensor memory, 16 tokens in 8 columns at multiples of 16, the second of two planes (NP) behind; 16 columns of
+// V at a time.
+template <int NP>
+__device__ __forceinline__ void load_scores(uint32_t a, float (&s)[16]) {
+  uint32_t pk[8], pl[8];
+  tmem_ld8(a, pk);
+  if constexpr (NP == 2) tmem_ld8(a + 8, pl);
+  tmem_ld_wait();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float2 y = pair_of(pk[j]), z = NP == 2 ? pair_of(pl[j]) : make_float2(0.f, 0.f);
+    s[2 * j] = y.x + z.x;
+    s[2 * j + 1] = y.y + z.y;
+  }
+}
+// 16 scores of a row in their place, over what they were made of
+template <int NP>
+__device__ __forceinline__ void store_scores(uint32_t a, const float (&s)[16]) {
+  uint32_t r[NP == 2 ? 16 : 8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint32_t z[NP];
+    planes<NP>(s[2 * j], s[2 * j + 1], z);
+#pragma unroll
+    for (int n = 0; n < NP; ++n) r[8 * n + j] = z[n];
+  }
+  if constexpr (NP == 2) tmem_st16(a, r);
+  else tmem_st8(a, r);
+}
+template <int DV, int NP>
 __device__ __noinline__ void masked_sums(uint32_t tp, uint32_t to, uint32_t tv, int row, int qt) {
 #pragma unroll 1
   for (int c0 = qt * (DV / TC_COLS); c0 < (qt + 1) * (DV / TC_COLS); c0 += 16) {
@@ -306,15 +334,13 @@ __device__ __noinline__ void masked_sums(uint32_t tp, uint32_t to, uint32_t tv, 
     for (int e = 0; e < 16; ++e) o[e] = 0.f;
 #pragma unroll 1
     for (int k = 0; k < 8; ++k) {
-      uint32_t pk[8];
+      float p[16];
       __syncwarp();
-      tmem_ld8(tp + 32 * (k >> 1) + 8 * (k & 1), pk);
-      tmem_ld_wait();
+      load_scores<NP>(tp + 16 * k, p);
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int t = 16 * k + j;
-        const float2 y = pair_of(pk[j / 2]);
-        const float pj = j % 2 ? y.y : y.x;
+        const float pj = p[j];
         const uint32_t at = tv + (c0 >> 6) * 16384;
         const uint4 a = lds16(at + sw128_chunk(t, (c0 >> 3) & 7)), b = lds16(at + sw128_chunk(t, ((c0 >> 3) & 7) + 1));
         const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
@@ -362,7 +388,7 @@ struct TcWalk {
   Walk w;
 };
 
-// NU: planes of the weighted keys; NS: planes of the state as an operand
+// NU: planes of the weighted keys; NS: planes of the state as an operand and of the scores
 template <int DK, int DV, int NU, int NS, bool OUT>
 __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_constant__ TcWalk a) {
   using Y = TLay<DK, DV, NU, NS, OUT>;
@@ -452,7 +478,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
           const bool one = gates[i & 1].low <= MILD && !p.r && !was_odd(i);         // (on top of Q S)
           const uint32_t to = one ? tOI : tOA;
 #pragma unroll
-          for (int s = 0; s < 8; ++s) umma_ts(to, tSC + 32 * (s >> 1) + 8 * (s & 1), desc_advance(dV, s * 2048), i_pv, one || s > 0);
+          for (int n = NS - 1; n >= 0; --n)
+#pragma unroll
+            for (int s = 0; s < 8; ++s) umma_ts(to, tSC + 16 * s + 8 * n, desc_advance(dV, s * 2048), i_pv, one || n < NS - 1 || s > 0);
           umma_commit(bar(B_PV));
         }
         const uint32_t lst = Y::NL == 2 ? (i & 1) * (NU - 1) * Y::TK : 0;
@@ -581,10 +609,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
 #pragma unroll 1
         for (int sb = qt * (8 / TC_COLS); sb < (qt + 1) * (8 / TC_COLS); ++sb) {
           const int grp = sb >> 1;          // columns 16 sb + [0, 16), of the group of 32
-          uint32_t pk[8];
+          float s[16];
           if (grp > q4) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) pk[e] = 0u;
+            for (int e = 0; e < 16; ++e) s[e] = 0.f;
           } else {
             uint32_t x[16];
             tmem_ld16(tSC + lane_base + 16 * sb, x);
@@ -597,26 +625,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float4 c = cf[e];
-                const float y0 = 4 * e <= last ? __uint_as_float(x[4 * e]) * (rf * c.x) : 0.f;
-                const float y1 = 4 * e + 1 <= last ? __uint_as_float(x[4 * e + 1]) * (rf * c.y) : 0.f;
-                const float y2 = 4 * e + 2 <= last ? __uint_as_float(x[4 * e + 2]) * (rf * c.z) : 0.f;
-                const float y3 = 4 * e + 3 <= last ? __uint_as_float(x[4 * e + 3]) * (rf * c.w) : 0.f;
-                pk[2 * e] = pack_bf16x2(y0, y1);
-                pk[2 * e + 1] = pack_bf16x2(y2, y3);
+                s[4 * e] = 4 * e <= last ? __uint_as_float(x[4 * e]) * (rf * c.x) : 0.f;
+                s[4 * e + 1] = 4 * e + 1 <= last ? __uint_as_float(x[4 * e + 1]) * (rf * c.y) : 0.f;
+                s[4 * e + 2] = 4 * e + 2 <= last ? __uint_as_float(x[4 * e + 2]) * (rf * c.z) : 0.f;
+                s[4 * e + 3] = 4 * e + 3 <= last ? __uint_as_float(x[4 * e + 3]) * (rf * c.w) : 0.f;
               }
             } else {
               const float2 li = gs.lam[row];
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 const float4 l = *reinterpret_cast<const float4*>(&gs.lam[16 * sb + 2 * e]);
-                const float x0 = 2 * e <= last ? __uint_as_float(x[2 * e]) * decay_of(li, make_float2(l.x, l.y)) : 0.f;
-                const float x1 = 2 * e + 1 <= last ? __uint_as_float(x[2 * e + 1]) * decay_of(li, make_float2(l.z, l.w)) : 0.f;
-                pk[e] = pack_bf16x2(x0, x1);
+                s[2 * e] = 2 * e <= last ? __uint_as_float(x[2 * e]) * decay_of(li, make_float2(l.x, l.y)) : 0.f;
+                s[2 * e + 1] = 2 * e + 1 <= last ? __uint_as_float(x[2 * e + 1]) * decay_of(li, make_float2(l.z, l.w)) : 0.f;
               }
             }
           }
           // P over this thread's own part of SC, which it has read up to here
-          tmem_st8(tSC + lane_base + 32 * grp + 8 * (sb & 1), pk);
+          store_scores<NS>(tSC + lane_base + 16 * sb, s);
         }
         tmem_st_wait();
       }
@@ -646,7 +671,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
         wait_for(ok, bar(B_PV), ph);             // (and Q S, which was issued before)
         tc_fence_after();
         const bool odd = was_odd(i), one = mild && !odd;
-        if (odd) masked_sums<DV>(tSC + lane_base, tOA + lane_base, uv, row, qt);
+        if (odd) masked_sums<DV, NS>(tSC + lane_base, tOA + lane_base, uv, row, qt);
         const float wi = gs.wt[row].x, wp = mild ? wi : 1.f;
         const int64_t at = ((t0 + row) * p.H + h) * p.vd + HV * qt;      // (float32 outputs)
         const int64_t ra = p.r ? ((t0 + row) * (p.H / p.gr) + h / p.gr) * p.vd + HV * qt : 0;

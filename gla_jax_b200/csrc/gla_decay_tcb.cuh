@@ -11,10 +11,10 @@
 // products are done by then.
 //   dg_t = sum over i >= t of (r_i + a_i - c_i - b_i) + <the state that leaves the run, its gradient>
 //   M_ji = P_ji DT_ji in float32, r its column and c its row sums;  a = q . (dq from before the chunk), b = k . (dk from behind it)
-// with the products of dS in two planes where this is asked for: the sum is over the whole run and its terms cancel.  A value or key
+// from operands in two planes: the sum is over the whole run and its terms cancel.  A value or key
 // that is not finite makes it not finite from there back, where dg reads neither: those tokens are summed from the other end,
 //   dg_t = <the state that enters the run, its gradient> - sum over i < t of (r_i + a_i - c_i - b_i)
-// P and E are one bf16 plane, and so is the image of dS without the gates' gradient (as in the forward).
+// With the gates' gradient P, E and the image of dS are two bf16 planes, else one (as in the forward).
 // Bounded as the forward is: 4 x 4096 tokens of 6 heads, 128 x 128: 77 us; 8191 packed tokens, 16 heads of 128 x 64 with the
 // gates' gradient: 174 us; n chunks of 128 x 128: 24 + 9.5 n us, with the gates' gradient 33 + 11.9 n.
 #pragma once
@@ -53,7 +53,7 @@ enum TbBar { C_LOAD = 0, C_ST = 1, C_I = 2, C_DV = 3, C_U = 4, C_P = 5, C_W = 6,
 
 // o (a row of tensor memory, D / TC_COLS columns from the worker's first) += sum over i >= row of P_i V_i, for a chunk in which V holds
 // something that is not finite (see masked_sums)
-template <int D>
+template <int D, int NP>
 __device__ __noinline__ void masked_add(uint32_t tp, uint32_t to, uint32_t tv, int row, int qt) {
 #pragma unroll 1
   for (int c0 = qt * (D / TC_COLS); c0 < (qt + 1) * (D / TC_COLS); c0 += 16) {
@@ -63,15 +63,13 @@ __device__ __noinline__ void masked_add(uint32_t tp, uint32_t to, uint32_t tv, i
     tmem_ld_wait();
 #pragma unroll 1
     for (int k = 0; k < 8; ++k) {
-      uint32_t pk[8];
+      float p[16];
       __syncwarp();
-      tmem_ld8(tp + 32 * (k >> 1) + 8 * (k & 1), pk);
-      tmem_ld_wait();
+      load_scores<NP>(tp + 16 * k, p);
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int t = 16 * k + j;
-        const float2 y = pair_of(pk[j / 2]);
-        const float pj = j % 2 ? y.y : y.x;
+        const float pj = p[j];
         const uint32_t at = tv + (c0 >> 6) * 16384;
         const uint4 a = lds16(at + sw128_chunk(t, (c0 >> 3) & 7)), b = lds16(at + sw128_chunk(t, ((c0 >> 3) & 7) + 1));
         const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
@@ -248,9 +246,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(odd) : "r"(bar(C_ODD) + 4 * (i & 1)) : "memory");
         if (odd != (uint32_t)(i + 1)) {
 #pragma unroll
-          for (int s = 0; s < 8; ++s) umma_ts(tIV, tST + 32 * (s >> 1) + 8 * (s & 1), desc_advance(mO, s * 2048), idesc_bf16(128, DV, 0, 1), 1);
+          for (int s = 0; s < 8 * NS; ++s) umma_ts(tIV, tST + 16 * (s & 7) + 8 * (s >> 3), desc_advance(mO, (s & 7) * 2048), idesc_bf16(128, DV, 0, 1), 1);
 #pragma unroll
-          for (int s = 0; s < 8; ++s) umma_ts(tIK, tDT + 32 * (s >> 1) + 8 * (s & 1), desc_advance(mQ, s * 2048), idesc_bf16(128, DK, 0, 1), 1);
+          for (int s = 0; s < 8 * NS; ++s) umma_ts(tIK, tDT + 16 * (s & 7) + 8 * (s >> 3), desc_advance(mQ, (s & 7) * 2048), idesc_bf16(128, DK, 0, 1), 1);
         }
         umma_commit(bar(C_DV));
         wait_for(ok, bar(C_W), ph);
@@ -383,10 +381,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
 #pragma unroll 1
       for (int sb = qt * (8 / TC_COLS); sb < (qt + 1) * (8 / TC_COLS); ++sb) {
         const int grp = sb >> 1;             // columns (tokens i) 16 sb + [0, 16), of the group of 32
-        uint32_t pk[8], ek[8];
+        float s[16], d[16];
         if (grp < q4) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) pk[e] = ek[e] = 0u;
+          for (int e = 0; e < 16; ++e) s[e] = d[e] = 0.f;
           if (GATE && lane < 16) sum[128 * q4 + 16 * sb + lane] = 0.f;
         } else {
           uint32_t x[16], y[16];
@@ -401,30 +399,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
           const int first = own ? lane - 16 * (sb & 1) : 0, end = nv - 16 * sb;           // columns that count
           const float wm = mild ? wj : 1.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            float s[2], d[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              const int c = 2 * e + u;
-              const float w = sharp ? decay_of(gs.lam[16 * sb + c], lj) : rf[16 * sb + c] * cf;
-              const bool in = c >= first && c < end;
-              s[u] = in ? __uint_as_float(x[c]) * w : 0.f;
-              d[u] = in ? __uint_as_float(y[c]) * w : 0.f;
-              if constexpr (GATE) {
-                m[c] = in ? s[u] * wm * __uint_as_float(y[c]) : 0.f;      // (s alone may be near the top)
-                rowsum += m[c];
-              }
+          for (int c = 0; c < 16; ++c) {
+            const float w = sharp ? decay_of(gs.lam[16 * sb + c], lj) : rf[16 * sb + c] * cf;
+            const bool in = c >= first && c < end;
+            s[c] = in ? __uint_as_float(x[c]) * w : 0.f;
+            d[c] = in ? __uint_as_float(y[c]) * w : 0.f;
+            if constexpr (GATE) {
+              m[c] = in ? s[c] * wm * __uint_as_float(y[c]) : 0.f;      // (s alone may be near the top)
+              rowsum += m[c];
             }
-            pk[e] = pack_bf16x2(s[0], s[1]);
-            ek[e] = pack_bf16x2(d[0], d[1]);
           }
           if constexpr (GATE) {
             const float t = lane_sums(m, lane);
             if (lane < 16) sum[128 * q4 + 16 * sb + lane] = t;
           }
         }
-        tmem_st8(tST + lane_base + 32 * grp + 8 * (sb & 1), pk);
-        tmem_st8(tDT + lane_base + 32 * grp + 8 * (sb & 1), ek);
+        store_scores<NS>(tST + lane_base + 16 * sb, s);
+        store_scores<NS>(tDT + lane_base + 16 * sb, d);
       }
       if (GATE) sum[512 + 128 * qt + row] = rowsum;
       bool odd = check_rows<DV>(base + Y::O0, nv);
@@ -473,8 +464,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
       odd = workers_or(odd);              // (and K and V are done with)
       if (odd) {
         tc_fence_after();
-        masked_add<DV>(tST + lane_base, tIV + lane_base, base + Y::O0, row, qt);
-        masked_add<DK>(tDT + lane_base, tIK + lane_base, base + Y::Q0, row, qt);
+        masked_add<DV, NS>(tST + lane_base, tIV + lane_base, base + Y::O0, row, qt);
+        masked_add<DK, NS>(tDT + lane_base, tIK + lane_base, base + Y::Q0, row, qt);
         tc_fence_before();
         if (tid == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(bar(C_ODD) + 4 * (i & 1)), "r"(i + 1) : "memory");
       }

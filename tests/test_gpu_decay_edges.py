@@ -257,3 +257,18 @@ def test_backward_in_a_graph_beside_another_stream(cuda_device, dtype, D, packs)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip([*outs, *grads], [*want, *gw]))
         assert all(torch.equal(a, b) for a, b in zip([*other, *go], [*want, *gw]))
+
+
+@pytest.mark.parametrize("size", [(2, 84, 3, 3, 8, 128), (3, 557, 2, 2, 32, 32), (1, 841, 1, 1, 80, 32), (2, 112, 3, 3, 112, 32), (1, 274, 2, 1, 24, 32)])
+def test_bf16_gradients_of_few_terms(cuda_device, size):
+    """Sums of few terms under sharp gates, where a term rounded to bf16 shows: with the gates' gradient every operand is in two
+    planes, and the one rounding is the result's."""
+    from gla_jax_b200 import chunk_decay_attention
+    for seed in range(12):
+        xs = make(cuda_device, *size, torch.bfloat16, torch.bfloat16, seed=seed)
+        gen = torch.Generator(device=cuda_device).manual_seed(seed)
+        u = torch.rand(xs[1].shape, generator=gen, device=cuda_device)
+        xs[1] = (-u * 0.3, -u * 5.0, torch.where(u < 0.5, 0.0, -3.0 * u), torch.where(u < 0.05, -1e4, -0.1 * u))[seed % 4].contiguous()
+        cots = [torch.randn(x.shape, generator=gen, device=cuda_device).to(x.dtype) for x in (xs[0], xs[2])]
+        got, grads = with_grads(chunk_decay_attention, xs, cots)
+        check(xs, cots, got, grads, torch.bfloat16, torch.bfloat16, (size, seed))
