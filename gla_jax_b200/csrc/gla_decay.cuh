@@ -282,7 +282,8 @@ __global__ void __launch_bounds__(NW * 32, KD <= 128 && MODE <= M_STATE ? 16 / N
         const double y = __shfl_up_sync(0xffffffffu, inc, d);
         if (lane >= d) inc += y;
       }
-      const double all = __shfl_sync(0xffffffffu, inc, 31), before = inc - sum;
+      // (not inc - sum, which is lost for all of a lane's rows where one gate is not a number)
+      const double all = __shfl_sync(0xffffffffu, inc, 31), left = __shfl_up_sync(0xffffffffu, inc, 1), before = lane ? left : 0.0;
       total += all;
 #pragma unroll
       for (int i = 0; i < R; ++i) {

@@ -526,8 +526,9 @@ GLA_API int gla_sp_combine2(void* stream, int64_t R, int64_t rank, int64_t BH, i
  * and more.  bf16 beyond: one plane of each in the forward, two in the backward.  float32: three planes everywhere.
  * Where a chunk's decay is mild its scores carry up to 2^64 of it on their way: bf16 calls up to head size 128 want products of a
  * query and a key, in the backward of a value and its cotangent too, below 2^62.
- * What is not finite stays with the tokens that read it (as not-a-number, where the recurrence may have an infinity), the gates'
- * gradient between a query or cotangent that is not finite and a later value or key that is not excepted.
+ * What is not finite stays with the tokens that read it (as not-a-number, where the recurrence may have an infinity), with two
+ * exceptions in the backward: a gate that is not a number reaches the gradients of its whole chunk, and of the gates between a query
+ * or cotangent that is not finite and a later value or key that is not the gradient is not either.
  * Backward: dlog_decay (B, T, H) float32 or NULL; dhidden_init as hidden_init.
  * Workspace: gla_decay_workspace_bytes for the forward without (what = 0) and with `saved` (1), the backward without (2)
  * and with dlog_decay (3); 0 bytes may be needed, or the sizes may be unsupported (the calls say which).

@@ -272,3 +272,19 @@ def test_bf16_gradients_of_few_terms(cuda_device, size):
         cots = [torch.randn(x.shape, generator=gen, device=cuda_device).to(x.dtype) for x in (xs[0], xs[2])]
         got, grads = with_grads(chunk_decay_attention, xs, cots)
         check(xs, cots, got, grads, torch.bfloat16, torch.bfloat16, (size, seed))
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.float32, 64), (torch.bfloat16, 136)])
+def test_outputs_before_a_gate_that_is_not_a_number(cuda_device, dtype, D):
+    from gla_jax_b200 import chunk_decay_attention
+    xs = make(cuda_device, 1, 200, 2, 2, D, D, dtype, dtype)
+    want = chunk_decay_attention(*xs)
+    for t in (1, 46, 47, 63, 64, 130):
+        ys = [x.clone() for x in xs]
+        ys[1][0, t, 0] = math.nan
+        hf, out = chunk_decay_attention(*ys)
+        # (the weights of a chunk are made in another way where its sums are not finite: a rounding of scores and result may differ)
+        unit = want[1][:, :t].double().abs() + want[1][:, :t].double().abs().mean()
+        assert ((out[:, :t].double() - want[1][:, :t].double()).abs() <= (2.0 ** -5 if dtype == torch.bfloat16 else 2.0 ** -16) * unit).all(), t
+        assert torch.equal(out[:, :, 1], want[1][:, :, 1]) and torch.equal(hf[:, 1], want[0][:, 1])
+        assert torch.isnan(out[:, t:, 0]).all() and torch.isnan(hf[:, 0]).all()
