@@ -296,8 +296,9 @@ __device__ __forceinline__ bool check_rows(uint32_t tile, int nv) {
 }
 // What is not finite in OA = P V, by sums over the tokens up to the row's own: in the product, zeros of P meet what is not finite
 // in V, and 0 x inf is not a number, where the recurrence has it at its own token and after only.
-// P: this lane's row in tensor memory, 16 tokens in 8 columns at multiples of 16, the second of two planes (NP) behind; 16 columns of
-// V at a time.
+// P: this lane's row in tensor memory, 16 tokens in 8 columns, the second of two planes (NP) in the 8 behind; 16 columns of V at a time.
+template <int NP>
+__device__ __forceinline__ constexpr int score_at(int s) { return NP == 1 ? 32 * (s >> 1) + 8 * (s & 1) : 16 * s; }      // of tokens 16 s on
 template <int NP>
 __device__ __forceinline__ void load_scores(uint32_t a, float (&s)[16]) {
   uint32_t pk[8], pl[8];
@@ -311,17 +312,16 @@ __device__ __forceinline__ void load_scores(uint32_t a, float (&s)[16]) {
     s[2 * j + 1] = y.y + z.y;
   }
 }
-// 16 scores of a row in their place, over what they were made of
+// scores 2 j and 2 j + 1 of 16, and all of them to their place, over what they were made of
 template <int NP>
-__device__ __forceinline__ void store_scores(uint32_t a, const float (&s)[16]) {
-  uint32_t r[NP == 2 ? 16 : 8];
+__device__ __forceinline__ void set_scores(uint32_t (&r)[8 * NP], int j, float x, float y) {
+  uint32_t z[NP];
+  planes<NP>(x, y, z);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    uint32_t z[NP];
-    planes<NP>(s[2 * j], s[2 * j + 1], z);
-#pragma unroll
-    for (int n = 0; n < NP; ++n) r[8 * n + j] = z[n];
-  }
+  for (int n = 0; n < NP; ++n) r[8 * n + j] = z[n];
+}
+template <int NP>
+__device__ __forceinline__ void store_scores(uint32_t a, const uint32_t (&r)[8 * NP]) {
   if constexpr (NP == 2) tmem_st16(a, r);
   else tmem_st8(a, r);
 }
@@ -336,7 +336,7 @@ __device__ __noinline__ void masked_sums(uint32_t tp, uint32_t to, uint32_t tv, 
     for (int k = 0; k < 8; ++k) {
       float p[16];
       __syncwarp();
-      load_scores<NP>(tp + 16 * k, p);
+      load_scores<NP>(tp + score_at<NP>(k), p);
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int t = 16 * k + j;
@@ -480,7 +480,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
 #pragma unroll
           for (int n = NS - 1; n >= 0; --n)
 #pragma unroll
-            for (int s = 0; s < 8; ++s) umma_ts(to, tSC + 16 * s + 8 * n, desc_advance(dV, s * 2048), i_pv, one || n < NS - 1 || s > 0);
+            for (int s = 0; s < 8; ++s) umma_ts(to, tSC + score_at<NS>(s) + 8 * n, desc_advance(dV, s * 2048), i_pv, one || n < NS - 1 || s > 0);
           umma_commit(bar(B_PV));
         }
         const uint32_t lst = Y::NL == 2 ? (i & 1) * (NU - 1) * Y::TK : 0;
@@ -609,10 +609,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
 #pragma unroll 1
         for (int sb = qt * (8 / TC_COLS); sb < (qt + 1) * (8 / TC_COLS); ++sb) {
           const int grp = sb >> 1;          // columns 16 sb + [0, 16), of the group of 32
-          float s[16];
+          uint32_t s[8 * NS];
           if (grp > q4) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) s[e] = 0.f;
+            for (int e = 0; e < 8 * NS; ++e) s[e] = 0u;
           } else {
             uint32_t x[16];
             tmem_ld16(tSC + lane_base + 16 * sb, x);
@@ -625,23 +625,26 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_walk_kernel(const __grid_con
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
                 const float4 c = cf[e];
-                s[4 * e] = 4 * e <= last ? __uint_as_float(x[4 * e]) * (rf * c.x) : 0.f;
-                s[4 * e + 1] = 4 * e + 1 <= last ? __uint_as_float(x[4 * e + 1]) * (rf * c.y) : 0.f;
-                s[4 * e + 2] = 4 * e + 2 <= last ? __uint_as_float(x[4 * e + 2]) * (rf * c.z) : 0.f;
-                s[4 * e + 3] = 4 * e + 3 <= last ? __uint_as_float(x[4 * e + 3]) * (rf * c.w) : 0.f;
+                const float y0 = 4 * e <= last ? __uint_as_float(x[4 * e]) * (rf * c.x) : 0.f;
+                const float y1 = 4 * e + 1 <= last ? __uint_as_float(x[4 * e + 1]) * (rf * c.y) : 0.f;
+                const float y2 = 4 * e + 2 <= last ? __uint_as_float(x[4 * e + 2]) * (rf * c.z) : 0.f;
+                const float y3 = 4 * e + 3 <= last ? __uint_as_float(x[4 * e + 3]) * (rf * c.w) : 0.f;
+                set_scores<NS>(s, 2 * e, y0, y1);
+                set_scores<NS>(s, 2 * e + 1, y2, y3);
               }
             } else {
               const float2 li = gs.lam[row];
 #pragma unroll
               for (int e = 0; e < 8; ++e) {
                 const float4 l = *reinterpret_cast<const float4*>(&gs.lam[16 * sb + 2 * e]);
-                s[2 * e] = 2 * e <= last ? __uint_as_float(x[2 * e]) * decay_of(li, make_float2(l.x, l.y)) : 0.f;
-                s[2 * e + 1] = 2 * e + 1 <= last ? __uint_as_float(x[2 * e + 1]) * decay_of(li, make_float2(l.z, l.w)) : 0.f;
+                const float x0 = 2 * e <= last ? __uint_as_float(x[2 * e]) * decay_of(li, make_float2(l.x, l.y)) : 0.f;
+                const float x1 = 2 * e + 1 <= last ? __uint_as_float(x[2 * e + 1]) * decay_of(li, make_float2(l.z, l.w)) : 0.f;
+                set_scores<NS>(s, e, x0, x1);
               }
             }
           }
           // P over this thread's own part of SC, which it has read up to here
-          store_scores<NS>(tSC + lane_base + 16 * sb, s);
+          store_scores<NS>(tSC + lane_base + score_at<NS>(sb), s);
         }
         tmem_st_wait();
       }

@@ -65,7 +65,7 @@ __device__ __noinline__ void masked_add(uint32_t tp, uint32_t to, uint32_t tv, i
     for (int k = 0; k < 8; ++k) {
       float p[16];
       __syncwarp();
-      load_scores<NP>(tp + 16 * k, p);
+      load_scores<NP>(tp + score_at<NP>(k), p);
 #pragma unroll
       for (int j = 0; j < 16; ++j) {
         const int t = 16 * k + j;
@@ -246,9 +246,9 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(odd) : "r"(bar(C_ODD) + 4 * (i & 1)) : "memory");
         if (odd != (uint32_t)(i + 1)) {
 #pragma unroll
-          for (int s = 0; s < 8 * NS; ++s) umma_ts(tIV, tST + 16 * (s & 7) + 8 * (s >> 3), desc_advance(mO, (s & 7) * 2048), idesc_bf16(128, DV, 0, 1), 1);
+          for (int s = 0; s < 8 * NS; ++s) umma_ts(tIV, tST + score_at<NS>(s & 7) + 8 * (s >> 3), desc_advance(mO, (s & 7) * 2048), idesc_bf16(128, DV, 0, 1), 1);
 #pragma unroll
-          for (int s = 0; s < 8 * NS; ++s) umma_ts(tIK, tDT + 16 * (s & 7) + 8 * (s >> 3), desc_advance(mQ, (s & 7) * 2048), idesc_bf16(128, DK, 0, 1), 1);
+          for (int s = 0; s < 8 * NS; ++s) umma_ts(tIK, tDT + score_at<NS>(s & 7) + 8 * (s >> 3), desc_advance(mQ, (s & 7) * 2048), idesc_bf16(128, DK, 0, 1), 1);
         }
         umma_commit(bar(C_DV));
         wait_for(ok, bar(C_W), ph);
@@ -381,10 +381,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
 #pragma unroll 1
       for (int sb = qt * (8 / TC_COLS); sb < (qt + 1) * (8 / TC_COLS); ++sb) {
         const int grp = sb >> 1;             // columns (tokens i) 16 sb + [0, 16), of the group of 32
-        float s[16], d[16];
+        uint32_t pk[8 * NS], ek[8 * NS];
         if (grp < q4) {
 #pragma unroll
-          for (int e = 0; e < 16; ++e) s[e] = d[e] = 0.f;
+          for (int e = 0; e < 8 * NS; ++e) pk[e] = ek[e] = 0u;
           if (GATE && lane < 16) sum[128 * q4 + 16 * sb + lane] = 0.f;
         } else {
           uint32_t x[16], y[16];
@@ -399,23 +399,30 @@ __global__ void __launch_bounds__(TC_THREADS, 1) tc_back_kernel(const __grid_con
           const int first = own ? lane - 16 * (sb & 1) : 0, end = nv - 16 * sb;           // columns that count
           const float wm = mild ? wj : 1.f;
 #pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const float w = sharp ? decay_of(gs.lam[16 * sb + c], lj) : rf[16 * sb + c] * cf;
-            const bool in = c >= first && c < end;
-            s[c] = in ? __uint_as_float(x[c]) * w : 0.f;
-            d[c] = in ? __uint_as_float(y[c]) * w : 0.f;
-            if constexpr (GATE) {
-              m[c] = in ? s[c] * wm * __uint_as_float(y[c]) : 0.f;      // (s alone may be near the top)
-              rowsum += m[c];
+          for (int e = 0; e < 8; ++e) {
+            float s[2], d[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int c = 2 * e + u;
+              const float w = sharp ? decay_of(gs.lam[16 * sb + c], lj) : rf[16 * sb + c] * cf;
+              const bool in = c >= first && c < end;
+              s[u] = in ? __uint_as_float(x[c]) * w : 0.f;
+              d[u] = in ? __uint_as_float(y[c]) * w : 0.f;
+              if constexpr (GATE) {
+                m[c] = in ? s[u] * wm * __uint_as_float(y[c]) : 0.f;      // (s alone may be near the top)
+                rowsum += m[c];
+              }
             }
+            set_scores<NS>(pk, e, s[0], s[1]);
+            set_scores<NS>(ek, e, d[0], d[1]);
           }
           if constexpr (GATE) {
             const float t = lane_sums(m, lane);
             if (lane < 16) sum[128 * q4 + 16 * sb + lane] = t;
           }
         }
-        store_scores<NS>(tST + lane_base + 16 * sb, s);
-        store_scores<NS>(tDT + lane_base + 16 * sb, d);
+        store_scores<NS>(tST + lane_base + score_at<NS>(sb), pk);
+        store_scores<NS>(tDT + lane_base + score_at<NS>(sb), ek);
       }
       if (GATE) sum[512 + 128 * qt + row] = rowsum;
       bool odd = check_rows<DV>(base + Y::O0, nv);
