@@ -288,3 +288,21 @@ def test_outputs_before_a_gate_that_is_not_a_number(cuda_device, dtype, D):
         assert ((out[:, :t].double() - want[1][:, :t].double()).abs() <= (2.0 ** -5 if dtype == torch.bfloat16 else 2.0 ** -16) * unit).all(), t
         assert torch.equal(out[:, :, 1], want[1][:, :, 1]) and torch.equal(hf[:, 1], want[0][:, 1])
         assert torch.isnan(out[:, t:, 0]).all() and torch.isnan(hf[:, 0]).all()
+
+
+def test_gates_gradient_over_a_long_uncut_sequence(cuda_device):
+    """80 sequences, so that none is cut, of 16384 tokens.  The running sum adds up the errors of its terms: 2^-17 of each from operands
+    in two planes, falling either way, the terms being of the gradient's own size: 2^-17 sqrt(16384) = 2^-10 of its norm, whatever
+    the gates' memory."""
+    from gla_jax_b200 import chunk_decay_attention
+    T, D = 16384, 64
+    xs = make(cuda_device, 80, T, 1, 1, D, D, torch.bfloat16, torch.bfloat16, seed=41, shift=5.0)
+    gen = torch.Generator(device=cuda_device).manual_seed(42)
+    cots = [torch.randn(x.shape, generator=gen, device=cuda_device).to(x.dtype) for x in (xs[0], xs[2])]
+    _, got = with_grads(chunk_decay_attention, xs, cots)
+    for s in (0, 79):
+        one = [x[s:s + 1].double().requires_grad_(i == 1) for i, x in enumerate(xs)]
+        want = torch.autograd.grad(recurrence(*one), one[1], [c[s:s + 1].double() for c in cots])[0][0, :, 0]
+        for part in (slice(0, T // 4), slice(T - T // 4, T), slice(0, T)):
+            err = (got[1][s, part, 0].double() - want[part]).norm() / want[part].norm()
+            assert err <= 2.0 ** -10, (s, part, err.item())
