@@ -10,17 +10,17 @@
 // copies left them.
 //
 // What bounds it (4 x 4096 tokens of 6 heads, 128 x 128, runs of 768 tokens: 47 us a walk with outputs, 22 us one of sums).  A walk of
-// n chunks takes 20 + 4.9 n us (144 blocks, n from 1 to 32, caches cold).  A chunk's 9000 cycles are its phases in a row, since
+// n chunks takes 21 + 4.8 n us (144 blocks, n from 1 to 32, caches cold).  A chunk's 9000 cycles are its phases in a row, since
 // each needs the one before: scores 1900, weights 1100, the check of the values 600, a wait for the products 1100, outputs and
 // their stores 3000, the state 600.  No unit is at work for a third of them (tensor cores 19 %, accesses to shared memory 17 %, HBM
-// 24 %), and there is room for one block per SM only.  The 20 us are what comes before the first chunk, the entering state read in
+// 24 %), and there is room for one block per SM only.  The 21 us are what comes before the first chunk, the entering state read in
 // strides among it, and after the last.  Measured besides: sixteen workers the same; eight for the scores and eight for outputs
 // and state side by side 49 to 57 us.
 //
 // Roundings.  P and the state's image are one bf16 plane, as in this library's other chunk kernels: 2^-9 of each term, which leaves
 // outputs 2.3e-3 of their norm off, where their own rounding to bf16 is 1.7e-3.  Two planes of the state cost its second product and
-// the second stage of K: 8.2 us a chunk instead of 4.9, which only a backward with the gates' gradient is worth, whose terms cancel;
-// there P has two planes as well (3 % of the call).  The state itself, its sums and the gates' are in 32 bits and more.
+// the second stage of K: 8.2 us a chunk instead of 4.8, which only a backward with the gates' gradient is worth, whose terms cancel;
+// there P has two planes as well (9.0 us a chunk).  The state itself, its sums and the gates' are in 32 bits and more.
 //
 // Tiles: 128 rows x 64 columns of bf16, 128-byte rows, 16-byte pieces at piece ^ (row % 8) (tc_ptx.cuh); D columns are D / 64
 // of them.  A copy brings 128 rows whatever the sequence's length: rows past its end are another sequence's or beyond the

@@ -16,7 +16,7 @@
 //   dg_t = <the state that enters the run, its gradient> - sum over i < t of (r_i + a_i - c_i - b_i)
 // With the gates' gradient P, E and the image of dS are two bf16 planes, else one (as in the forward).
 // Bounded as the forward is: 4 x 4096 tokens of 6 heads, 128 x 128: 77 us; 8191 packed tokens, 16 heads of 128 x 64 with the
-// gates' gradient: 174 us; n chunks of 128 x 128: 24 + 9.5 n us, with the gates' gradient 33 + 11.9 n.
+// gates' gradient: 177 us; n chunks of 128 x 128: 19 + 9.8 n us, with the gates' gradient 26 + 12.4 n.
 #pragma once
 #include "gla_decay_tc.cuh"
 

@@ -558,7 +558,7 @@ GLA_API int gla_decay_bwd(void* stream, int64_t B, int64_t T, int64_t H, int64_t
  *                          float32, value (B, H, Dv), key and query (B, Hk, Dk), out (B, H, Dv) in out_dtype.  With parents
  *                          (B = requests * beams) every row is stepped from its parent's state; the moves cost no pass.
  *   gla_decode_step_beams  gla_decode_step (a decay per key feature) with parents.
- *                          Both: Dk and Dv as above; any number of rows.
+ *                          Both: Dk and Dv as above; up to 33 million (row, head) pairs, (request, head) with parents.
  *   gla_reorder_states     rows of `count` tensors (0 included; HOST arrays of device addresses and of bytes per row) moved to where
  *                          the parents say, in place; rows that stay are not touched.  The tensors must not overlap.
  *   gla_beam_select        logits (N, K, V) in dtype, scores (N, K) float32 (finite or -inf): the M best of each request's K V

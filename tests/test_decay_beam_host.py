@@ -67,3 +67,23 @@ def test_no_states_to_move(lib):
     assert lib.gla_reorder_states(None, 0, None, None, 2, 4, p) == 0
     assert lib.gla_reorder_states(None, 0, None, None, 2, 4, None) == 1
     assert lib.gla_reorder_states(None, 1, p, None, 2, 4, p) == 1
+
+
+def test_what_a_packed_call_and_a_backward_keep(lib):
+    """Offsets travel in the workspace of a forward alone and in `saved` of one that is differentiated; what has no other state to
+    keep (float32, head sizes beyond 128) may go without `saved`."""
+    p, big = ctypes.c_void_p(4096), 1 << 40
+    ws = lambda *a: lib.gla_decay_workspace_bytes(*a)  # noqa: E731
+    assert ws(1, 8, 2, 2, 64, 64, 1, 1, 3, 0) >= 16 and ws(1, 8, 2, 2, 64, 64, 1, 1, 3, 1) == 0
+    assert lib.gla_decay_saved_bytes(1, 8, 2, 2, 64, 64, 0, 0, 0) == lib.gla_decay_saved_bytes(1, 8, 2, 2, 256, 64, 1, 1, 0) == 0
+    assert lib.gla_decay_saved_bytes(1, 8, 2, 2, 64, 64, 0, 0, 3) >= 16
+    assert lib.gla_decay_saved_bytes(1, 8, 2, 2, 64, 64, 1, 1, 3) >= 3 * 2 * 64 * 64 * 4 + 16
+    assert ws(1, 8, 2, 2, 64, 64, 0, 0, 0, 3) >= 2 * 64 * 64 * 4 + ws(1, 8, 2, 2, 64, 64, 0, 0, 0, 2)
+    bwd = lambda dt, nseq, cu, saved, n=big: lib.gla_decay_bwd(  # noqa: E731
+        None, 1, 8, 2, 2, 64, 64, dt, dt, nseq, cu, p, p, 1, p, p, p, saved, p, p, p, p, p, p, p, p, n)
+    assert bwd(1, 0, None, None) == 1 and bwd(0, 1, p, None) == 1
+    assert bwd(0, 0, None, None, 16) == 5 and bwd(1, 0, None, ctypes.c_void_p(4100)) == 4
+    step = lambda B, H, parents=None, beams=1: lib.gla_decay_step(None, B, H, H, 64, 64, 1, None, p, p, p, p, p, 1, parents, beams)  # noqa: E731
+    assert step(1 << 20, 16) == 1                    # (a null state is all that is wrong)
+    sizes = lambda B, H: lib.gla_decay_step(None, B, H, H, 64, 64, 1, p, p, p, p, p, p, 1, None, 1)  # noqa: E731
+    assert sizes(1 << 32, 1) == sizes(1 << 22, 16) == 8
