@@ -324,8 +324,8 @@ int sm_count() {
 
 // Tokens of a run.  A walk has a block per run, head and tile of value columns; with fewer blocks than the device has
 // SMs sequences are cut into runs, at the price of reading k and v twice and of two launches more
-// (1155 tokens of 16 heads, 128 x 128: 46 us in runs of 384, 40 in runs of 256).  With blocks for half the SMs or more nothing is cut:
-// twice the blocks would halve the time in the chunks at most, and pay a second pass.
+// (1155 tokens of 16 heads, 128 x 128: 46 us in runs of 384, 40 in runs of 256).  With blocks for half the SMs or more nothing is
+// cut, whatever the lengths of packed sequences, which the host does not know.
 int64_t run_tokens(int64_t T, int64_t nseq, int64_t H, int64_t vd, bool packed) {
   const int64_t blocks = H * ((vd + 127) / 128) * nseq, want = (int64_t)sm_count();
   int64_t n = packed ? want / (H * ((vd + 127) / 128)) : want / blocks;      // runs: of the packed axis, of each sequence
