@@ -523,7 +523,7 @@ GLA_API int gla_sp_combine2(void* stream, int64_t R, int64_t rank, int64_t BH, i
  * runs; the offsets as they were used.  NULL otherwise.
  * bf16, head sizes up to 128: scores and the state as an operand are rounded to bf16 once, decayed values to two bf16
  * planes (three where hidden is float32; scores and the state in two in a backward with dlog_decay); sums, states and decays in float32
- * and more.  bf16 beyond: one plane of each in the forward, two in the backward.  float32: three planes everywhere.
+ * and more.  bf16 beyond: the same, all in two planes in a backward.  float32: three planes everywhere.
  * Where a chunk's decay is mild its scores carry up to 2^64 of it on their way: bf16 calls up to head size 128 want products of a
  * query and a key, in the backward of a value and its cotangent too, below 2^62.
  * What is not finite stays with the tokens that read it (as not-a-number, where the recurrence may have an infinity), with two

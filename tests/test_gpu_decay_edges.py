@@ -306,3 +306,16 @@ def test_gates_gradient_over_a_long_uncut_sequence(cuda_device):
         for part in (slice(0, T // 4), slice(T - T // 4, T), slice(0, T)):
             err = (got[1][s, part, 0].double() - want[part]).norm() / want[part].norm()
             assert err <= 2.0 ** -10, (s, part, err.item())
+
+
+@pytest.mark.parametrize("size", [(1, 700, 2, 2, 256, 64), (2, 300, 2, 1, 64, 136), (1, 900, 1, 1, 136, 256), (3, 500, 40, 40, 128, 136),
+                                  (1, 700, 2, 2, 128, 128)])
+def test_bf16_states_leave_with_their_own_rounding(cuda_device, size):
+    """The state is summed from terms in two planes and more (2^-16 each), so that what it is off by as it leaves in bf16 is its
+    rounding: that of the exact state, but for those that fall the other way."""
+    from gla_jax_b200 import chunk_decay_attention
+    xs = make(cuda_device, *size, torch.bfloat16, torch.bfloat16, seed=51, shift=4.0)
+    hf, _ = chunk_decay_attention(*xs)
+    want, _ = recurrence(*(x.double() for x in xs))
+    own = (want.bfloat16().double() - want).norm()
+    assert (hf.double() - want).norm() <= 1.05 * own, ((hf.double() - want).norm() / want.norm()).item()
